@@ -602,6 +602,108 @@ int r3d_host_write_delta_frames(const char *const *velodyne_paths, const char *c
 int r3d_host_append_text_files(const char *const *src, const char *const *dst, const char *const *extra, int32_t n,
                                int32_t threads);
 
+/* =====================================================================================
+ * From a finished batch to a training step on its points.  None of this is in the reference, which
+ * leaves training to other programs: the scenes of r3d_batch_finish stay in HBM, in the pages of a pool,
+ * and what a step needs of them is made on the device from lengths that only the device knows.
+ * Same conventions as above: device pointers, no allocation, no synchronisation, capturable.
+ * Outputs are written whole; an output must not overlap an input unless it says so.
+ * ===================================================================================== */
+/* types of values */
+#define R3D_T_F32 0
+#define R3D_T_BF16 1
+#define R3D_T_F16 2
+#define R3D_T_F64 3
+#define R3D_T_I32 4
+#define R3D_T_I64 5
+
+/* Block tables from lengths.  Row i of a table [n_rows][max_blocks] lists the blocks (of block_size points) that hold scene
+ * i's points, -1 behind them; held[i] = points the row is for now; free_blocks[0 .. n_free[0]) = a stack of the blocks that
+ * belong to no row (n_blocks in all).  The call makes row i ready for lengths[i] points, as if one row after the other:
+ *   first every row with more blocks than ceil(lengths[i] / block_size) gives back the ones behind those (pushed in their
+ *   order), then every row with fewer pops the rest from the end of the stack.  The first row whose blocks are not there and
+ *   every later growing row keep what they had, and so does a row whose length is negative or beyond its table.
+ * held_out[i] = lengths[i] where served, held[i] elsewhere; status (nullable) is set to R3D_S_CAPACITY where a row was not
+ * served or a block is both free and held, else to 0.  free_out is -1 from n_free_out[0] on.  Needs max_blocks * block_size < 2^31. */
+size_t r3d_block_tables_workspace_bytes(int64_t n_rows);
+int r3d_block_tables(const int32_t *lengths, int64_t n_rows, int32_t block_size, int32_t max_blocks, const int32_t *tables,
+                     const int32_t *held, const int32_t *free_blocks, int64_t n_blocks, const int32_t *n_free, int32_t *tables_out,
+                     int32_t *held_out, int32_t *free_out, int32_t *n_free_out, int32_t *status, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* Where the points of some scenes stand, one after the other.  Sequence i is row rows[i] (nullable: row i) with lengths[row]
+ * points (0 for a row that is not there or a negative length; never more than its table has room for); offsets [n_seq + 1] =
+ * exclusive sums.  Point p of the sequence, token t = offsets[i] + p:
+ *   slots[t] = tables[row][p / block_size] * block_size + p % block_size, -1 where the table has no block;
+ *   tables null: one block a row (a batch's slabs, block_size = cap): slots[t] = row * block_size + p;
+ *   sequence[t] = i.
+ * -1 in both behind the last token, up to capacity; tokens beyond capacity are left out (offsets tell).  A row may be listed twice.
+ * slots and sequence 16-byte aligned. */
+int r3d_slot_map(const int32_t *lengths, int64_t n_lengths, const int32_t *tables, int32_t block_size, int32_t max_blocks,
+                 const int32_t *rows, int64_t n_seq, int64_t capacity, int64_t *offsets, int64_t *slots, int32_t *sequence,
+                 void *stream);
+
+/* Rows moved through maps: for t < n, row src_slots[t] (nullable: t) of every array goes to row dst_slots[t] (nullable: t).
+ * Without dst_slots a row whose source is outside [0, n_src) is filled with zeros; with them nothing is written for a source
+ * outside [0, n_src) or a destination outside [0, n_dst): rows that no slot names stay as they were.  Destinations must be
+ * distinct (of two equal ones either row may win, unit by unit).  arrays: HOST array, strides and widths in bytes. */
+#define R3D_MAX_ROW_ARRAYS 4
+typedef struct r3d_rows_t {
+  const void *src;
+  void *dst;
+  int64_t src_stride, dst_stride, row_bytes;
+} r3d_rows_t;
+int r3d_move_rows(const r3d_rows_t *arrays, int32_t n_arrays, const int64_t *src_slots, const int64_t *dst_slots, int64_t n,
+                  int64_t n_src, int64_t n_dst, void *stream);
+
+/* Rotary positions with several axes.  Axis a has sections[a] pairs; pair number j of axis a turns by
+ * pos[t][a] * base^(-j / sections[a]).  The pairs of all axes, R in all, stand one after the other: pair i is the elements
+ * (i, i + R) of a head, or (2i, 2i + 1) where interleaved; elements from 2R on are copied.  x[0] / x[1]: queries and keys
+ * [tokens][heads[w]][dim] (heads[1] = 0: none), strides in elements, the last axis dense; y dense.  backward: the angles
+ * negated (the gradient).  Angles in double, sine and cosine of what is left of a turn in float. */
+#define R3D_ROTARY_MAX_AXES 8
+typedef struct r3d_rotary_t {
+  const void *x[2];
+  void *y[2];
+  int64_t token_stride[2], head_stride[2];
+  int64_t tokens;
+  int32_t heads[2];
+  int32_t dim, type, interleaved, backward;
+  int32_t axes, sections[R3D_ROTARY_MAX_AXES];
+  int32_t pos_type;
+  const void *pos;
+  int64_t pos_token_stride, pos_axis_stride;
+  double base;
+} r3d_rotary_t;
+int r3d_rotary(const r3d_rotary_t *d, void *stream);
+
+/* Softmax cross entropy of a linear head over v classes, in pieces of the classes, without keeping the n x v logits:
+ *   logits = x w^T + bias;  loss_i = log sum exp logits_i - logits_i[target_i]
+ * x [n] rows of ld_x elements, w [v] rows of ld_w, bias [v] (nullable), all of `type`; targets of target_type.  A point whose
+ * target is ignore_index has loss 0 and gradient 0, and what its features hold reaches no sum; one whose target is no class has
+ * loss NaN.  loss: float [n] (R3D_CE_NONE) or [1] (sum, mean over the points that count; 0 where none does).
+ * The forward call fills idx, place, tgt (int32 [n] each), lse2 (float [n]) and counted (16 bytes), which the backward call of
+ * the same descriptor reads.  backward: grad = float [n] or
+ * [1]; dx [n][d], dw [v][d], db [v] dense, of `type`, each nullable.  piece: classes whose logit gradients are held at a time
+ * (0: as many as 256 MB take). */
+#define R3D_CE_NONE 0
+#define R3D_CE_SUM 1
+#define R3D_CE_MEAN 2
+typedef struct r3d_linear_ce_t {
+  const void *x, *w, *bias, *target;
+  int64_t ld_x, ld_w, n, v, d, ignore_index, piece;
+  int32_t type, target_type, reduction, reserved;
+  int32_t *idx, *place, *tgt;
+  float *lse2;
+  void *counted;
+  float *loss;
+  const float *grad;
+  void *dx, *dw, *db;
+} r3d_linear_ce_t;
+size_t r3d_linear_ce_workspace_bytes(const r3d_linear_ce_t *d, int32_t backward);
+int r3d_linear_ce_forward(const r3d_linear_ce_t *d, void *workspace, size_t workspace_bytes, void *stream);
+int r3d_linear_ce_backward(const r3d_linear_ce_t *d, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,5 +19,8 @@ from . import places  # noqa: F401
 from .places import PlaceScene, find_places  # noqa: F401
 from .placed import PlacedInserter  # noqa: F401
 from .rich_map import build_rich_map  # noqa: F401
+from .scene_pool import ScenePool, block_tables, put_rows, slot_map, take_rows  # noqa: F401
+from .point_ops import linear_cross_entropy, rotary_positions  # noqa: F401
 
-__all__ = ["SceneBatch", "augment_batch", "run_sharded", "shard_indices", "AugmentPipeline", "Frame", "run_sharded_files", "Real3DAug", "synth", "R3DError", "places", "PlaceScene", "find_places", "PlacedInserter", "build_rich_map", "affinity"]
+__all__ = ["SceneBatch", "augment_batch", "run_sharded", "shard_indices", "AugmentPipeline", "Frame", "run_sharded_files", "Real3DAug", "synth", "R3DError", "places", "PlaceScene", "find_places", "PlacedInserter", "build_rich_map", "affinity",
+           "ScenePool", "block_tables", "slot_map", "take_rows", "put_rows", "rotary_positions", "linear_cross_entropy"]

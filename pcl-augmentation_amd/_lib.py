@@ -80,6 +80,34 @@ class PlaceQuery(C.Structure):
     ]
 
 
+class Rows(C.Structure):
+    """Mirror of r3d_rows_t."""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_stride", C.c_int64), ("dst_stride", C.c_int64), ("row_bytes", C.c_int64)]
+
+
+T_F32, T_BF16, T_F16, T_F64, T_I32, T_I64 = range(6)
+MAX_ROW_ARRAYS, ROTARY_MAX_AXES, ROTARY_MAX_PAIRS = 4, 8, 256
+CE_NONE, CE_SUM, CE_MEAN = 0, 1, 2
+
+
+class Rotary(C.Structure):
+    """Mirror of r3d_rotary_t."""
+    _fields_ = [("x", C.c_void_p * 2), ("y", C.c_void_p * 2), ("token_stride", C.c_int64 * 2), ("head_stride", C.c_int64 * 2),
+                ("tokens", C.c_int64), ("heads", C.c_int32 * 2), ("dim", C.c_int32), ("type", C.c_int32), ("interleaved", C.c_int32),
+                ("backward", C.c_int32), ("axes", C.c_int32), ("sections", C.c_int32 * ROTARY_MAX_AXES), ("pos_type", C.c_int32),
+                ("pos", C.c_void_p), ("pos_token_stride", C.c_int64), ("pos_axis_stride", C.c_int64), ("base", C.c_double)]
+
+
+class LinearCE(C.Structure):
+    """Mirror of r3d_linear_ce_t."""
+    _fields_ = [("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("target", C.c_void_p),
+                ("ld_x", C.c_int64), ("ld_w", C.c_int64), ("n", C.c_int64), ("v", C.c_int64), ("d", C.c_int64),
+                ("ignore_index", C.c_int64), ("piece", C.c_int64),
+                ("type", C.c_int32), ("target_type", C.c_int32), ("reduction", C.c_int32), ("reserved", C.c_int32),
+                ("idx", C.c_void_p), ("place", C.c_void_p), ("tgt", C.c_void_p), ("lse2", C.c_void_p), ("counted", C.c_void_p),
+                ("loss", C.c_void_p), ("grad", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("db", C.c_void_p)]
+
+
 PLACE_ROTATIONS, PLACE_SURFACE_CAP, PLACE_MAX_OK_LABELS = 360, 128, 32
 PS_SURFACE_OVERFLOW, PS_NONFINITE, PS_BAD_DESCRIPTOR = 1, 2, 4
 PQ_POINTWISE_ROTATION, PQ_MAP_NEEDS_POINT, PQ_COLLIDE_LABEL, PQ_COLLIDE_ABOVE, PQ_SCENE_SLAB, PQ_ORIG_SLAB = 1, 2, 4, 8, 16, 32
@@ -149,6 +177,14 @@ _SIGNATURES = {
     "r3d_find_possible_places": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_int32,
                                            C.POINTER(C.c_double), C.c_int32, _P, _P, _P, _P, _P, C.c_int32, _P,
                                            _P, C.c_size_t, _P]),
+    "r3d_block_tables_workspace_bytes": (C.c_size_t, [C.c_int64]),
+    "r3d_block_tables": (C.c_int, [_P, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, C.c_int64, _P, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
+    "r3d_slot_map": (C.c_int, [_P, C.c_int64, _P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, _P, _P, _P, _P]),
+    "r3d_move_rows": (C.c_int, [C.POINTER(Rows), C.c_int32, _P, _P, C.c_int64, C.c_int64, C.c_int64, _P]),
+    "r3d_rotary": (C.c_int, [C.POINTER(Rotary), _P]),
+    "r3d_linear_ce_workspace_bytes": (C.c_size_t, [C.POINTER(LinearCE), C.c_int32]),
+    "r3d_linear_ce_forward": (C.c_int, [C.POINTER(LinearCE), _P, C.c_size_t, _P]),
+    "r3d_linear_ce_backward": (C.c_int, [C.POINTER(LinearCE), _P, C.c_size_t, _P]),
 }
 EXPORTS = tuple(_SIGNATURES)
 

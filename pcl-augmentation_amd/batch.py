@@ -477,6 +477,16 @@ class SceneBatch:
         _lib.check(self.lib.r3d_batch_finish(C.byref(self.desc), cp, int(check_cols or 5), _lib.stream_ptr()),
                    "r3d_batch_finish")
 
+    @_lib.on_own_device
+    def replace_result(self, s, xyzi, label):
+        """After ``finish``: the merged cloud of scene ``s`` is this one (host arrays), e.g. what Level 1 made of a frame."""
+        torch, n = self.torch, len(xyzi)
+        if n > self.cap or len(label) != n:
+            raise ValueError(f"scene {s}: {n} points and {len(label)} labels for a capacity of {self.cap}")
+        self.out_xyzi[s, :n] = torch.from_numpy(np.ascontiguousarray(xyzi, dtype=np.float32)).to(self.device)
+        self.out_label[s, :n] = torch.from_numpy(np.ascontiguousarray(label).astype(np.uint32).view(np.int32)).to(self.device)
+        self.n_out[s] = n
+
     def count_pairs(self, on=True):
         """Descriptor bit 4096: the insert kernels count per pair (pairs, chunks listed, parked, committed from a record) --
         atomics of every pair on a few addresses, hence off unless somebody reads them (``debug_counters``)."""
@@ -613,7 +623,7 @@ def level2_takes(rows, cols):
 
 
 def augment_batch(scenes, candidates, min_points, rows=_lib.NUMROW, cols=_lib.NUMCOLUMN, device="cuda:0",
-                  check_cols=5, reuse=None, debug=0):
+                  check_cols=5, reuse=None, debug=0, pool=None, pool_scenes=None):
     """Run whole frames through the insert loop on one GPU.
 
     scenes[s] = (xyzi float32 [n,4], label uint32 [n]); candidates[s][k] = ordered list of M x 5
@@ -621,9 +631,14 @@ def augment_batch(scenes, candidates, min_points, rows=_lib.NUMROW, cols=_lib.NU
     reaches min_points[s][k] points is merged, insertion.py:449-526).  Returns
     (results, accepted) with results as ``SceneBatch.results`` and accepted[s][k] = index of the
     accepted candidate or -1.  ``reuse``: optional dict in which the ``SceneBatch`` is kept between
-    calls (keyed by B) instead of being allocated every time.
+    calls (keyed by B) instead of being allocated every time.  ``pool``: a ``ScenePool`` of the same GPU which takes the
+    finished scenes where they stand, as scenes ``pool_scenes`` (default 0 .. B-1); nothing is downloaded then, results is None.
     """
     B = len(scenes)
+    if pool is not None and not level2_takes(rows, cols):
+        raise ValueError("augment_batch: a pool takes scenes from the batched path only, which this range image is not for")
+    if pool is not None:
+        pool.check_scenes(pool_scenes, B)
     if not level2_takes(rows, cols):
         # a range image the batched kernels are not built for (columns that are no multiple of 32: the bit images are rows of
         # 32-pixel words; 2^24 pixels and more; edge tables beyond the projection kernel's LDS): every frame through the
@@ -663,13 +678,22 @@ def augment_batch(scenes, candidates, min_points, rows=_lib.NUMROW, cols=_lib.NU
     redo = [int(s) for s in np.nonzero(status)[0] if _lib.needs_level1(status[s])]
     if redo:
         batch.status[torch_index(batch, redo)] = 0
-    results = batch.results()
+    if pool is None:
+        results = batch.results()
+    else:
+        batch.raise_on_status()
+        results = [None] * B
     if redo:
         from . import level1
         for s in redo:
             results[s], accepted[s] = level1.augment_scene(scenes[s][0], scenes[s][1], candidates[s], min_points[s], rows, cols,
                                                            device, check_cols)
+            if pool is not None:
+                batch.replace_result(s, *results[s][:2])
         batch.last_level1 = SceneBatch.last_level1 = redo
+    if pool is not None:
+        pool.add(batch, pool_scenes)
+        return None, accepted
     return results, accepted
 
 

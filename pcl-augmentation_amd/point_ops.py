@@ -1,0 +1,234 @@
+"""What a training step on the points of resident scenes needs beside the scenes themselves (``scene_pool``): rotary positions
+over the axes of a point or a pixel, and the softmax cross entropy of a linear head over the labels, with their gradients.
+Tensors on the GPU in and out, on the current stream; no CPU fallback (include/real3daug_hip.h, r3d_rotary, r3d_linear_ce_*).
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+import functools
+
+from . import _lib
+
+_REDUCTIONS = {"none": _lib.CE_NONE, "sum": _lib.CE_SUM, "mean": _lib.CE_MEAN}
+
+
+@functools.lru_cache(maxsize=None)
+def _types():
+    import torch
+    return ({torch.float32: _lib.T_F32, torch.bfloat16: _lib.T_BF16, torch.float16: _lib.T_F16},
+            {torch.int32: _lib.T_I32, torch.int64: _lib.T_I64, torch.float32: _lib.T_F32, torch.float64: _lib.T_F64})
+
+
+def on_device_of(what, *tensors):
+    """The device of these tensors made current (a null context where it is already); refuses tensors that are not on one GPU."""
+    import torch
+    device = tensors[0].device
+    if device.type != "cuda":
+        _lib.require_gpu()
+        raise _lib.R3DError(f"{what}: the tensors must be on a GPU, got {device}")
+    for t in tensors[1:]:
+        if t.device != device:
+            raise ValueError(f"{what}: tensors on {device} and {t.device}")
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _value_type(what, t):
+    kind = _types()[0].get(t.dtype)
+    if kind is None:
+        raise TypeError(f"{what}: float32, bfloat16 or float16, got {t.dtype}")
+    return kind
+
+
+# ---- rotary positions -------------------------------------------------------------------------------------------------
+def _turn(tensors, positions, sections, base, interleaved, backward):
+    """One launch over up to two [tokens, heads, dim] tensors (None: none); returns dense ones."""
+    import torch
+    d = _lib.Rotary()
+    outs = []
+    for w, x in enumerate(tensors):
+        if x is None or x.shape[1] == 0:
+            d.heads[w] = 0
+            outs.append(None if x is None else torch.empty_like(x))
+            continue
+        if x.stride(2) != 1:
+            x = x.contiguous()
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        outs.append(y)
+        d.x[w], d.y[w] = x.data_ptr(), y.data_ptr()
+        d.token_stride[w], d.head_stride[w] = x.stride(0), x.stride(1)
+        d.heads[w], d.tokens, d.dim, d.type = x.shape[1], x.shape[0], x.shape[2], _types()[0][x.dtype]
+        tensors = tensors[:w] + (x,) + tensors[w + 1:]      # (kept until the launch)
+    if d.heads[0] + d.heads[1] == 0 or d.tokens == 0:
+        return outs
+    d.interleaved, d.backward, d.axes, d.base = int(interleaved), int(backward), len(sections), base
+    d.sections[:len(sections)] = sections
+    d.pos_type, d.pos = _types()[1][positions.dtype], positions.data_ptr()
+    d.pos_token_stride, d.pos_axis_stride = positions.stride()
+    with on_device_of("rotary_positions", *[t for t in tensors if t is not None], positions):
+        _lib.check(_lib.load().r3d_rotary(C.byref(d), _lib.stream_ptr()), "r3d_rotary")
+    return outs
+
+
+@functools.lru_cache(maxsize=None)
+def _rotary_function():
+    import torch
+    from torch.autograd.function import once_differentiable
+
+    class RotaryPositions(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, query, key, positions, sections, base, interleaved):
+            ctx.save_for_backward(positions)
+            ctx.how = sections, base, interleaved
+            return tuple(_turn((query, key), positions, sections, base, interleaved, False))
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, grad_query, grad_key):
+            # a rotation: the gradient is turned back
+            need = [g if n else None for g, n in zip((grad_query, grad_key), ctx.needs_input_grad)]
+            got = _turn(tuple(need), ctx.saved_tensors[0], *ctx.how, True)
+            return got[0], got[1], None, None, None, None
+
+    return RotaryPositions
+
+
+def rotary_positions(query, positions, sections, key=None, base=10000.0, style="half"):
+    """Rotary positions with several axes: ``query`` [tokens, heads, dim] (and ``key`` with heads of its own) turned by the
+    positions of their tokens.
+
+    positions [tokens, axes]: whole numbers (scan, row, column of a pixel) or floats (x, y, z of a point, in the units the base
+    is meant for; a slice of packed rows, ``xyzi[:, :3]``, is taken as it lies); sections: pairs of every axis.  Pair j of an
+    axis with s pairs turns by ``position * base ** (-j / s)``; the pairs of the axes stand one after the other, R in all
+    (at most 256, 2 R <= dim): pair i is the elements (i, i + R) of a head (``style="half"``) or (2i, 2i + 1)
+    (``"interleaved"``), elements from 2 R on stay.  Angles are taken in double, products in 32 bits, one rounding.
+    Returns (query, key), key None where none was given; differentiable in both, once."""
+    import torch
+    if query.dim() != 3 or (key is not None and key.dim() != 3):
+        raise ValueError("rotary_positions: query and key must be [tokens, heads, dim]")
+    if style not in ("half", "interleaved"):
+        raise ValueError("rotary_positions: style is 'half' or 'interleaved'")
+    sections = tuple(int(s) for s in sections)
+    if not 1 <= len(sections) <= _lib.ROTARY_MAX_AXES or min(sections) < 0:
+        raise ValueError(f"rotary_positions: 1 to {_lib.ROTARY_MAX_AXES} sections of zero or more pairs")
+    if positions.dim() != 2 or positions.shape != (query.shape[0], len(sections)):
+        raise ValueError(f"rotary_positions: positions must be [{query.shape[0]}, {len(sections)}], got {tuple(positions.shape)}")
+    if positions.dtype not in _types()[1]:
+        raise TypeError(f"rotary_positions: positions are int32, int64, float32 or float64, got {positions.dtype}")
+    if positions.requires_grad:
+        raise ValueError("rotary_positions: positions have no gradient here (detach them)")
+    _value_type("rotary_positions", query)
+    if key is not None and (key.dtype != query.dtype or key.shape[0] != query.shape[0] or key.shape[2] != query.shape[2]):
+        raise ValueError("rotary_positions: key must have query's tokens, dim and type")
+    if sum(sections) > _lib.ROTARY_MAX_PAIRS or 2 * sum(sections) > query.shape[2]:
+        raise ValueError(f"rotary_positions: {sum(sections)} pairs do not fit a head of {query.shape[2]} (at most {_lib.ROTARY_MAX_PAIRS} pairs)")
+    if query.shape[2] % 2 or query.shape[2] > 4096:
+        raise ValueError("rotary_positions: the size of a head must be even and at most 4096")
+    if max(query.shape[1], 0 if key is None else key.shape[1]) > 65536:
+        raise ValueError("rotary_positions: at most 65536 heads")
+    base = float(base)
+    if not base > 0.0 or base == float("inf"):
+        raise ValueError("rotary_positions: base must be positive and finite")
+    on_device_of("rotary_positions", query, positions, *(() if key is None else (key,)))
+    return _rotary_function().apply(query, key, positions, sections, base, style == "interleaved")
+
+
+# ---- softmax cross entropy of a linear head ------------------------------------------------------------------------------
+@functools.lru_cache(maxsize=None)
+def _loss_function():
+    import torch
+    from torch.autograd.function import once_differentiable
+
+    def descriptor(x, weight, bias, target, state, how):
+        d = _lib.LinearCE()
+        n = x.shape[0]
+        d.x, d.w, d.bias, d.target = x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), target.data_ptr()
+        d.ld_x, d.ld_w = x.stride(0), weight.stride(0)
+        d.n, d.v, d.d = n, weight.shape[0], x.shape[1]
+        d.ignore_index, d.reduction, d.piece = how
+        d.type, d.target_type = _types()[0][x.dtype], _types()[1][target.dtype]
+        at = state.data_ptr()
+        d.counted, d.idx, d.place, d.tgt, d.lse2 = at, at + 16, at + 16 + 4 * n, at + 16 + 8 * n, at + 16 + 12 * n
+        return d
+
+    def workspace(lib, d, backward, device):
+        size = lib.r3d_linear_ce_workspace_bytes(C.byref(d), backward)
+        if size == 0:
+            _lib.check(_lib.E_ARG, "r3d_linear_ce_workspace_bytes")
+        return torch.empty(size, dtype=torch.uint8, device=device)
+
+    class LinearCrossEntropy(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, weight, bias, target, how):
+            n = x.shape[0]
+            with on_device_of("linear_cross_entropy", x):
+                lib = _lib.load()
+                state = torch.empty(4 + 4 * n, dtype=torch.int32, device=x.device)
+                loss = torch.empty(n if how[1] == _lib.CE_NONE else (), dtype=torch.float32, device=x.device)
+                d = descriptor(x, weight, bias, target, state, how)
+                d.loss = loss.data_ptr()
+                ws = workspace(lib, d, 0, x.device)
+                _lib.check(lib.r3d_linear_ce_forward(C.byref(d), ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "r3d_linear_ce_forward")
+            ctx.save_for_backward(x, weight, bias, target, state)
+            ctx.how = how
+            return loss
+
+        @staticmethod
+        @once_differentiable
+        def backward(ctx, grad):
+            x, weight, bias, target, state = ctx.saved_tensors
+            need = ctx.needs_input_grad
+            with on_device_of("linear_cross_entropy", x):
+                lib = _lib.load()
+                d = descriptor(x, weight, bias, target, state, ctx.how)
+                grad = grad.to(torch.float32).contiguous()
+                d.grad = grad.data_ptr()
+                outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and n else None
+                        for t, n in zip((x, weight, bias), need)]
+                d.dx, d.dw, d.db = (0 if o is None else o.data_ptr() for o in outs)
+                ws = workspace(lib, d, 1, x.device)
+                _lib.check(lib.r3d_linear_ce_backward(C.byref(d), ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "r3d_linear_ce_backward")
+            return outs[0], outs[1], outs[2], None, None
+
+    return LinearCrossEntropy
+
+
+def _rows_dense(t):
+    """[n, d] with the last axis dense and rows that do not overlap."""
+    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean", piece=0):
+    """Softmax cross entropy of the logits ``x @ weight.T + bias`` without ever holding them: x [..., features] (float32,
+    bfloat16 or float16), weight [classes, features] and bias [classes] of the same type, target [...] int32 / int64.
+
+    Points whose target is ``ignore_index`` have loss and gradient 0, whatever their features are; a target that is no class makes
+    the loss NaN.  reduction: "mean" over the points that count (0 where none does), "sum" or "none" ([...]); the loss is
+    float32.  Differentiable once in x, weight and bias; the backward pass makes the logits' gradients ``piece`` classes at a time
+    (0: as many as 256 MB hold).  The same inputs give the same bits."""
+    import torch
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"linear_cross_entropy: x [..., features] and weight [classes, features], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    _value_type("linear_cross_entropy", x)
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise TypeError("linear_cross_entropy: x, weight and bias must have one type")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"linear_cross_entropy: bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: target must be {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    if target.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"linear_cross_entropy: target is int32 or int64, got {target.dtype}")
+    if reduction not in _REDUCTIONS:
+        raise ValueError("linear_cross_entropy: reduction is 'none', 'sum' or 'mean'")
+    if int(piece) < 0:
+        raise ValueError("linear_cross_entropy: piece must not be negative")
+    if target.numel() > 2 ** 31 - 1025 or weight.shape[0] > 2 ** 31 - 1025 or weight.shape[1] > 1 << 20:
+        raise ValueError("linear_cross_entropy: too large (2^31 points, 2^31 classes, 2^20 features)")
+    on_device_of("linear_cross_entropy", x, weight, target, *(() if bias is None else (bias,)))
+    if target.numel() == 0:      # nothing to sum; the gradients are zeros
+        none = (x.sum() + weight.sum() * 0 + (0 if bias is None else bias.sum() * 0)).float() * 0
+        return none if reduction != "none" else none.expand(target.shape) + torch.zeros(target.shape, device=x.device)
+    how = (int(ignore_index), _REDUCTIONS[reduction], int(piece))
+    loss = _loss_function().apply(_rows_dense(x.reshape(-1, x.shape[-1])), _rows_dense(weight), None if bias is None else bias.contiguous(),
+                                  target.reshape(-1).contiguous(), how)
+    return loss.reshape(target.shape) if reduction == "none" else loss

@@ -1,0 +1,288 @@
+"""Augmented scenes that stay in HBM: a pool of pages, block tables made on the GPU from the lengths a finished batch holds, slot
+maps, and the points of the scenes a training step asks for, packed (include/real3daug_hip.h: r3d_block_tables, r3d_slot_map,
+r3d_move_rows).  288 GB take every augmented frame of a training split (20 bytes a point); a culled or grown scene takes
+the pages it needs.  Tensors on the GPU in and out, on the current stream, no host round trip; no CPU fallback.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+from . import _lib
+from .point_ops import on_device_of
+
+
+class BlockTables(NamedTuple):
+    tables: object       # int32 [rows, max_blocks]: the blocks of every row, -1 behind them
+    held: object         # int32 [rows]: points every row is for
+    free_blocks: object  # int32 [blocks]: the stack of blocks that belong to no row, -1 behind them
+    n_free: object       # int32 [1]
+    status: object       # int32 [1]: 0, or _lib.S_CAPACITY where a row was not served
+
+
+class SlotMap(NamedTuple):
+    offsets: object   # int64 [sequences + 1]: first token of every sequence
+    slots: object     # int64 [capacity]: where the token's point stands, -1 behind the last one
+    sequence: object  # int32 [capacity]: which sequence it is of, -1 behind the last one
+
+
+def _whole(what, name, t, dtype, dims):
+    if t.dtype != dtype or t.dim() != dims or not t.is_contiguous():
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of {dims} axes, got {t.dtype} {tuple(t.shape)}")
+
+
+def block_tables(lengths, block_size, tables, held, free_blocks, n_free):
+    """Block tables for new lengths: row i made ready for ``lengths[i]`` points from the blocks it has (``tables[i]``, for
+    ``held[i]`` points) and the stack of free ones.
+
+    As if row after row: rows with more blocks than ``ceil(lengths[i] / block_size)`` give back the ones behind (pushed in order),
+    then rows with fewer pop the rest from the end of the stack.  The first row whose blocks are not there and every later growing
+    row keep what they had, and so does a row with a negative length or one beyond its table: ``held`` tells, and
+    ``status`` is not 0.  All int32: lengths, held [rows], tables [rows, max_blocks], free_blocks [blocks], n_free [1].
+    Returns new tensors (``BlockTables``); the inputs stay as they are."""
+    import torch
+    what = "block_tables"
+    for name, t, dims in (("lengths", lengths, 1), ("tables", tables, 2), ("held", held, 1), ("free_blocks", free_blocks, 1), ("n_free", n_free, 1)):
+        _whole(what, name, t, torch.int32, dims)
+    rows, most = tables.shape
+    if lengths.shape[0] != rows or held.shape[0] != rows or n_free.shape[0] != 1:
+        raise ValueError(f"{what}: lengths and held must be [{rows}], n_free [1]")
+    if rows < 1 or most < 1 or free_blocks.shape[0] < 1:
+        raise ValueError(f"{what}: no rows or no blocks")
+    block_size = int(block_size)
+    if block_size < 1 or block_size * most >= 2 ** 31:
+        raise ValueError(f"{what}: block_size must be positive and block_size * max_blocks below 2^31")
+    with on_device_of(what, lengths, tables, held, free_blocks, n_free):
+        lib = _lib.load()
+        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=lengths.device)  # noqa: E731
+        out = BlockTables(new(rows, most), new(rows), new(free_blocks.shape[0]), new(1), new(1))
+        ws = torch.empty(lib.r3d_block_tables_workspace_bytes(rows), dtype=torch.uint8, device=lengths.device)
+        _lib.check(lib.r3d_block_tables(lengths.data_ptr(), rows, block_size, most, tables.data_ptr(), held.data_ptr(), free_blocks.data_ptr(),
+                                        free_blocks.shape[0], n_free.data_ptr(), out.tables.data_ptr(), out.held.data_ptr(),
+                                        out.free_blocks.data_ptr(), out.n_free.data_ptr(), out.status.data_ptr(), ws.data_ptr(), ws.numel(),
+                                        _lib.stream_ptr()), "r3d_block_tables")
+    return out
+
+
+def slot_map(lengths, block_size, tables=None, rows=None, capacity=None):
+    """Where the points of some scenes stand, one after the other (``SlotMap``): sequence i is row ``rows[i]`` (int32; None: every
+    row in order) with ``lengths[row]`` points (int32), point p of it stands at ``tables[row, p // block_size] * block_size +
+    p % block_size``.  tables None: one block a row, e.g. the slabs of a batch with ``block_size = batch.cap``.  ``capacity``: tokens
+    there is room for (None: read from the device, which waits for it); tokens beyond it are left out, ``offsets`` tell."""
+    import torch
+    what = "slot_map"
+    _whole(what, "lengths", lengths, torch.int32, 1)
+    if tables is not None:
+        _whole(what, "tables", tables, torch.int32, 2)
+        if tables.shape[0] != lengths.shape[0] or tables.shape[1] < 1:
+            raise ValueError(f"{what}: tables must have a row for each of the {lengths.shape[0]} lengths, and a column")
+    if rows is not None:
+        _whole(what, "rows", rows, torch.int32, 1)
+    block_size, most = int(block_size), 1 if tables is None else tables.shape[1]
+    if lengths.shape[0] < 1 or block_size < 1 or block_size * most >= 2 ** 31:
+        raise ValueError(f"{what}: no rows, or block_size not positive, or block_size * max_blocks not below 2^31")
+    if capacity is not None and int(capacity) < 0:
+        raise ValueError(f"{what}: capacity must not be negative")
+    with on_device_of(what, lengths, *[t for t in (tables, rows) if t is not None]):
+        lib = _lib.load()
+        if capacity is None:
+            each = lengths.clamp(0, block_size * most)
+            if rows is not None:
+                there = (rows >= 0) & (rows < lengths.shape[0])
+                each = torch.where(there, each[rows.clamp(0, lengths.shape[0] - 1).long()], 0)
+            capacity = int(each.sum(dtype=torch.int64))
+        n, capacity = lengths.shape[0] if rows is None else rows.shape[0], int(capacity)
+        out = SlotMap(torch.empty(n + 1, dtype=torch.int64, device=lengths.device), torch.empty(capacity, dtype=torch.int64, device=lengths.device),
+                      torch.empty(capacity, dtype=torch.int32, device=lengths.device))
+        # (an empty tensor has no address; nothing is written where capacity is 0)
+        slots, sequence = (t.data_ptr() if capacity else out.offsets.data_ptr() for t in out[1:])
+        _lib.check(lib.r3d_slot_map(lengths.data_ptr(), lengths.shape[0], 0 if tables is None else tables.data_ptr(), block_size, most,
+                                    0 if rows is None else rows.data_ptr(), n, capacity, out.offsets.data_ptr(), slots, sequence,
+                                    _lib.stream_ptr()), "r3d_slot_map")
+    return out
+
+
+def _slots(what, name, slots):
+    import torch
+    _whole(what, name, slots, torch.int64, 1)
+
+
+def _move(what, sources, dests, src_slots, dst_slots, n):
+    arrays = (_lib.Rows * len(sources))()
+    for a, s, t in zip(arrays, sources, dests):
+        size = s.element_size()
+        width = size
+        for e in s.shape[1:]:
+            width *= e
+        a.src, a.dst, a.row_bytes = s.data_ptr(), t.data_ptr(), width
+        a.src_stride, a.dst_stride = (s.stride(0) * size if s.shape[0] > 1 else width), (t.stride(0) * size if t.shape[0] > 1 else width)
+    _lib.check(_lib.load().r3d_move_rows(arrays, len(sources), 0 if src_slots is None else src_slots.data_ptr(),
+                                         0 if dst_slots is None else dst_slots.data_ptr(), n, sources[0].shape[0], dests[0].shape[0],
+                                         _lib.stream_ptr()), "r3d_move_rows")
+
+
+def _rows_of(what, name, tensors, like=None):
+    """Tensors [rows, ...] with a row in one piece, the same number of rows each."""
+    tensors = tuple(tensors)
+    if not 1 <= len(tensors) <= _lib.MAX_ROW_ARRAYS:
+        raise ValueError(f"{what}: 1 to {_lib.MAX_ROW_ARRAYS} {name}")
+    for t in tensors:
+        if t.dim() < 1 or t.shape[0] != tensors[0].shape[0]:
+            raise ValueError(f"{what}: {name} must have the same number of rows")
+        if t.requires_grad:
+            raise ValueError(f"{what}: no gradient passes through moved rows (detach them)")
+        width = 1
+        for e, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if e != 1 and s != width:
+                raise ValueError(f"{what}: a row of {name} must lie in one piece")
+            width *= e
+        if width == 0:
+            raise ValueError(f"{what}: empty rows")
+    return tensors
+
+
+def take_rows(slots, sources):
+    """Rows of up to four tensors by their slots, in one pass: ``out[k][t] = sources[k][slots[t]]``, zeros where the slot is
+    outside the source (a map's -1).  slots int64 [n] (``SlotMap.slots``); sources [rows, ...] of any type, a row in one piece.
+    Returns a tuple of dense tensors.  Not differentiable: for data, not for features."""
+    import torch
+    what = "take_rows"
+    _slots(what, "slots", slots)
+    sources = _rows_of(what, "sources", sources)
+    n = slots.shape[0]
+    with on_device_of(what, slots, *sources):
+        outs = tuple(torch.empty((n,) + t.shape[1:], dtype=t.dtype, device=t.device) for t in sources)
+        if n:
+            if sources[0].shape[0] == 0:
+                return tuple(o.zero_() for o in outs)
+            _move(what, sources, outs, slots, None, n)
+    return outs
+
+
+def put_rows(slots, rows, dests, source_slots=None):
+    """The other way, in place: ``dests[k][slots[t]] = rows[k][t]`` -- or ``rows[k][source_slots[t]]`` -- for up to four pairs of
+    tensors in one pass.  Nothing is written where either slot is outside (a map's -1): rows that no slot names stay as they
+    were.  The slots must be distinct; which of two equal ones wins is not defined.  Returns dests."""
+    what = "put_rows"
+    _slots(what, "slots", slots)
+    rows, dests = _rows_of(what, "rows", rows), _rows_of(what, "dests", dests)
+    if len(rows) != len(dests) or any(r.dtype != d.dtype or r.shape[1:] != d.shape[1:] for r, d in zip(rows, dests)):
+        raise ValueError(f"{what}: rows and dests must match in number, type and shape of a row")
+    n = slots.shape[0]
+    if source_slots is not None:
+        _slots(what, "source_slots", source_slots)
+        if source_slots.shape[0] != n:
+            raise ValueError(f"{what}: as many source_slots as slots")
+    elif rows[0].shape[0] < n:
+        raise ValueError(f"{what}: {n} slots for {rows[0].shape[0]} rows")
+    for d in dests:
+        if d.shape[0] > 1 and d.stride(0) < d[0].numel():
+            raise ValueError(f"{what}: the rows of dests overlap")
+    with on_device_of(what, slots, *rows, *dests, *(() if source_slots is None else (source_slots,))):
+        if n and rows[0].shape[0] and dests[0].shape[0]:
+            _move(what, rows, dests, source_slots, slots, n)
+    return dests
+
+
+class PackedScenes(NamedTuple):
+    xyzi: object      # float32 [tokens, 4]
+    label: object     # int32 [tokens], the bits of the batch's uint32 labels
+    offsets: object   # int64 [scenes + 1]
+    sequence: object  # int32 [tokens]: number within the request, -1 behind the last point
+    slots: object     # int64 [tokens]
+
+
+class ScenePool:
+    """Up to ``max_scenes`` augmented scenes resident on one GPU, in ``n_blocks`` pages of ``block_size`` points.
+
+    ``add(batch)`` takes the scenes of a finished ``SceneBatch`` where they stand, ``packed(scenes)`` returns the points of the
+    scenes a step asks for; neither waits for the device (but see ``packed``)."""
+
+    def __init__(self, max_scenes, max_points, n_blocks=None, block_size=2048, device="cuda:0"):
+        torch = _lib.require_gpu()
+        max_scenes, max_points, block_size = int(max_scenes), int(max_points), int(block_size)
+        if max_scenes < 1 or max_points < 1 or block_size < 1:
+            raise ValueError("ScenePool: max_scenes, max_points and block_size must be positive")
+        most = -(-max_points // block_size)
+        if most * block_size >= 2 ** 31:
+            raise ValueError("ScenePool: a scene must have fewer than 2^31 points")
+        n_blocks = max_scenes * most if n_blocks is None else int(n_blocks)
+        if not 1 <= n_blocks < 2 ** 31:
+            raise ValueError("ScenePool: n_blocks must be positive and below 2^31")
+        self.block_size, self.max_scenes, self.max_points, self.device = block_size, max_scenes, most * block_size, torch.device(device)
+        with _lib.on(self.device):
+            self.xyzi = torch.zeros((n_blocks * block_size, 4), dtype=torch.float32, device=self.device)
+            self.label = torch.zeros((n_blocks * block_size,), dtype=torch.int32, device=self.device)
+            i32 = dict(dtype=torch.int32, device=self.device)
+            self.blocks = BlockTables(torch.full((max_scenes, most), -1, **i32), torch.zeros(max_scenes, **i32),
+                                      torch.arange(n_blocks - 1, -1, -1, **i32), torch.full((1,), n_blocks, **i32), torch.zeros(1, **i32))
+
+    def _rows(self, scenes):
+        import torch
+        if isinstance(scenes, torch.Tensor):
+            scenes = scenes.tolist()
+        scenes = [int(s) for s in scenes]
+        if any(not 0 <= s < self.max_scenes for s in scenes):
+            raise ValueError(f"ScenePool: scenes are numbered 0 to {self.max_scenes - 1}")
+        return scenes
+
+    @property
+    def lengths(self):
+        """Points of every scene (int32 [max_scenes], on the device; 0: no scene)."""
+        return self.blocks.held
+
+    @_lib.on_own_device
+    def resize(self, lengths):
+        """New lengths for all scenes (int32 [max_scenes] on the device): pages given back and taken (``block_tables``).  What a
+        scene's first points are stays; new ones are whatever the page held."""
+        b = self.blocks
+        self.blocks = block_tables(lengths, self.block_size, b.tables, b.held, b.free_blocks, b.n_free)
+
+    def check_scenes(self, scenes, n):
+        """The distinct scene numbers of a batch of n (None: 0 .. n-1); raises where they are not that."""
+        scenes = list(range(n)) if scenes is None else self._rows(scenes)
+        if len(scenes) != n or len(set(scenes)) != n or n > self.max_scenes:
+            raise ValueError(f"ScenePool: {n} distinct scene numbers below {self.max_scenes}")
+        return scenes
+
+    @_lib.on_own_device
+    def add(self, batch, scenes=None):
+        """The merged clouds of a finished batch (``SceneBatch.finish``) become scenes ``scenes`` (distinct numbers, one per scene of
+        the batch; default 0 .. B-1), replacing what was there.  A scene the pool has no room for keeps its old points.
+        Returns an int32 tensor [B] on the device: 1 where the scene was taken."""
+        import torch
+        scenes = self.check_scenes(scenes, batch.B)
+        if batch.device != self.device and (batch.device.type, batch.device.index or 0) != (self.device.type, self.device.index or 0):
+            raise ValueError(f"ScenePool.add: the batch is on {batch.device}, the pool on {self.device}")
+        rows = torch.tensor(scenes, dtype=torch.int32, device=self.device)
+        self.resize(self.blocks.held.index_copy(0, rows.long(), batch.n_out))
+        taken = self.blocks.held[rows.long()] == batch.n_out
+        new = torch.where(taken, batch.n_out, 0)
+        capacity = batch.B * batch.cap
+        at = slot_map(torch.zeros_like(self.blocks.held).index_copy_(0, rows.long(), new), self.block_size, self.blocks.tables, rows, capacity)
+        put_rows(at.slots, (batch.out_xyzi.view(-1, 4), batch.out_label.view(-1)), (self.xyzi, self.label),
+                 source_slots=slot_map(new, batch.cap, capacity=capacity).slots)
+        return taken.to(torch.int32)
+
+    @_lib.on_own_device
+    def remove(self, scenes):
+        """These scenes' pages are free again."""
+        import torch
+        rows = torch.tensor(self._rows(scenes), dtype=torch.int64, device=self.device)
+        self.resize(self.blocks.held.index_fill(0, rows, 0))
+
+    @_lib.on_own_device
+    def packed(self, scenes, capacity=None):
+        """The points and labels of these scenes (any order, repeats allowed), one scene after the other (``PackedScenes``).
+        ``capacity``: room for that many points, zeros behind the last one (None: exactly as many as there are, which
+        reads the lengths back)."""
+        import torch
+        rows = torch.tensor(self._rows(scenes), dtype=torch.int32, device=self.device)
+        m = slot_map(self.blocks.held, self.block_size, self.blocks.tables, rows, capacity)
+        xyzi, label = take_rows(m.slots, (self.xyzi, self.label))
+        return PackedScenes(xyzi, label, m.offsets, m.sequence, m.slots)
+
+    def raise_on_status(self):
+        """Waits for the device; raises where the last ``add`` / ``resize`` did not find room for a scene."""
+        if int(self.blocks.status.item()):
+            raise _lib.R3DError("ScenePool: no room for a scene (out of pages, or more points than max_points)")

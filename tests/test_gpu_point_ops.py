@@ -1,0 +1,380 @@
+"""Rotary positions and the cross entropy of a linear head against their definitions in 64 bits, with bounds that follow from
+the types: a rounding to a type with step eps is off by eps / 2 of the value at most."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+E = 2.0 ** -24      # half a step of float32
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ---- rotary positions ----------------------------------------------------------------------------------------------------
+def rotate64(x, pos, sections, base, style, sign=1.0):
+    """(value, bound): the rotation in 64 bits, and how far a kernel may be off that holds the angle's fraction of a turn in 32
+    bits (pi E of angle), takes sine and cosine within two steps (4 E), multiplies and adds in 32 bits (2 E) and rounds once."""
+    x64 = x.detach().double().cpu()
+    freq = torch.cat([base ** (-torch.arange(s, dtype=torch.float64) / s) for s in sections if s]) if sum(sections) else torch.zeros(0, dtype=torch.float64)
+    axis = [a for a, s in enumerate(sections) for _ in range(s)]
+    angle = (pos.double().cpu()[:, axis] * freq)[:, None, :]
+    c, s = torch.cos(angle), torch.sin(angle) * sign
+    r = len(axis)
+    i1, i2 = (slice(0, r), slice(r, 2 * r)) if style == "half" else (slice(0, 2 * r, 2), slice(1, 2 * r, 2))
+    y, size = x64.clone(), torch.zeros_like(x64)
+    y[..., i1], y[..., i2] = x64[..., i1] * c - x64[..., i2] * s, x64[..., i2] * c + x64[..., i1] * s
+    size[..., i1] = size[..., i2] = x64[..., i1].abs() + x64[..., i2].abs()
+    # the position times turns per unit: 2^-52 of the angle, and what the whole turns take of it
+    lost = torch.zeros_like(x64)
+    lost[..., i1] = lost[..., i2] = (angle.abs() * 2.0 ** -51).expand(-1, x64.shape[1], -1)
+    tiny = torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
+    return y, size * (10 * E + lost) + torch.finfo(x.dtype).eps / 2 * y.abs() + tiny
+
+
+def near(got, want, bound):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape
+    off = (got - want).abs() - bound
+    assert not torch.isnan(off).any() and off.max().item() <= 0, (off.max().item(), (got - want).abs().max().item())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("style", ["half", "interleaved"])
+@pytest.mark.parametrize("tokens,heads,kv,dim,sections,pos", [
+    (1, 1, 0, 2, (1,), "i32"), (7, 3, 1, 10, (2, 3), "f32"), (65, 4, 4, 48, (8, 8, 8), "f32"), (300, 8, 2, 64, (10, 10, 10), "i64"),
+    (33, 1, 1, 130, (5, 0, 7, 9), "f64"), (1030, 2, 1, 96, (48,), "i32"), (5, 40, 8, 256, (32, 32, 64), "i32"), (3, 2, 0, 8, (0,), "f32"),
+    (2, 70, 70, 512, (256,), "f32")])
+def test_rotary(pkg, dtype, style, tokens, heads, kv, dim, sections, pos):
+    g = gen(tokens * 31 + dim)
+    q = torch.randn((tokens, heads, dim), generator=g).to(dtype).cuda().requires_grad_()
+    k = torch.randn((tokens, kv, dim), generator=g).to(dtype).cuda().requires_grad_() if kv else None
+    kind = {"i32": torch.int32, "i64": torch.int64, "f32": torch.float32, "f64": torch.float64}[pos]
+    p = (torch.randn((tokens, len(sections)), generator=g) * 50).to(kind).cuda()
+    a, b = pkg.rotary_positions(q, p, sections, key=k, base=500.0, style=style)
+    assert a.dtype == dtype and (b is None) == (k is None)
+    for x, y in ((q, a), (k, b)):
+        if x is None:
+            continue
+        near(y, *rotate64(x, p, sections, 500.0, style))
+        up = torch.randn(y.shape, generator=g).to(dtype).cuda()
+        back, = torch.autograd.grad(y, x, up, retain_graph=True)
+        near(back, *rotate64(up, p, sections, 500.0, style, -1.0))
+
+
+def test_rotary_gradient_against_differences(pkg):
+    g = gen(5)
+    x = torch.randn((9, 2, 12), generator=g).cuda().requires_grad_()
+    p, up = torch.randn((9, 2), generator=g).cuda() * 7, torch.randn((9, 2, 12), generator=g).cuda()
+    f = lambda v: (pkg.rotary_positions(v, p, (3, 2))[0].double() * up.double()).sum()  # noqa: E731
+    got, = torch.autograd.grad(f(x), x)
+    for t, h, e in ((0, 0, 0), (3, 1, 4), (8, 0, 11), (5, 1, 9)):
+        step = torch.zeros_like(x)
+        step[t, h, e] = 0.5
+        # the map is linear: a difference of any length is exact but for 32-bit rounding of both sides, over a step of 1
+        want = (f((x + step).detach()) - f((x - step).detach())).item()
+        assert abs(got[t, h, e].item() - want) <= 64 * E * (up[t, h].abs().sum().item() * (x[t, h].abs().max().item() + 1))
+
+
+def test_rotary_far_positions(pkg):
+    p = torch.tensor([[0], [1], [161279], [2 ** 31 - 1], [-2 ** 31]], dtype=torch.int32)
+    x = torch.randn((5, 1, 64), generator=gen(1))
+    y, _ = pkg.rotary_positions(x.cuda(), p.cuda(), (32,))
+    near(y, *rotate64(x, p, (32,), 10000.0, "half"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rotary_takes_strides(pkg, dtype):
+    g = gen(3)
+    fused = torch.randn((50, 6, 24), generator=g).to(dtype).cuda()
+    rows = torch.randn((50, 4), generator=g).cuda() * 20      # points: x y z are a slice
+    q, k = fused[:, :4], fused[:, 4:5]
+    a, b = pkg.rotary_positions(q, rows[:, :3], (4, 4, 3), key=k)
+    near(a, *rotate64(q, rows[:, :3], (4, 4, 3), 10000.0, "half"))
+    near(b, *rotate64(k, rows[:, :3], (4, 4, 3), 10000.0, "half"))
+    turned = fused[:, :4].transpose(1, 2).contiguous().transpose(1, 2)      # the last axis is not dense
+    near(pkg.rotary_positions(turned, rows[:, :3], (4, 4, 3))[0], *rotate64(q, rows[:, :3], (4, 4, 3), 10000.0, "half"))
+    by_head = fused[:, :4].transpose(0, 1).contiguous().transpose(0, 1)      # heads outside
+    near(pkg.rotary_positions(by_head, rows[:, :3], (4, 4, 3), style="interleaved")[0], *rotate64(q, rows[:, :3], (4, 4, 3), 10000.0, "interleaved"))
+    odd = fused.reshape(-1)[2:2 + 49 * 144].reshape(49, 6, 24)      # 4 (or 8) byte alignment
+    near(pkg.rotary_positions(odd, rows[1:, 1:3], (4, 4))[0], *rotate64(odd, rows[1:, 1:3], (4, 4), 10000.0, "half"))
+    wide = fused[:1].expand(50, 6, 24)      # one row for all tokens
+    near(pkg.rotary_positions(wide, rows[:, :1], (12,))[0], *rotate64(wide, rows[:, :1], (12,), 10000.0, "half"))
+
+
+def test_rotary_of_nothing_and_not_a_number(pkg):
+    q = torch.zeros((0, 2, 8), device="cuda", requires_grad=True)
+    y, k = pkg.rotary_positions(q, torch.zeros((0, 1), device="cuda"), (4,))
+    assert y.shape == (0, 2, 8) and k is None
+    assert torch.autograd.grad(y.sum(), q)[0].shape == (0, 2, 8)
+    x = torch.ones((2, 1, 8), device="cuda")
+    x[0, 0, 7] = float("inf")      # behind the pairs: copied, touches nothing
+    y, _ = pkg.rotary_positions(x, torch.tensor([[0.5], [float("nan")]], device="cuda"), (3,))
+    assert torch.isfinite(y[0, 0, :7]).all() and y[0, 0, 7] == float("inf")
+    assert torch.isnan(y[1, 0, :6]).all() and (y[1, 0, 6:] == 1).all()
+
+
+# ---- cross entropy -------------------------------------------------------------------------------------------------------
+def check_loss(pkg, n, v, d, dtype, bias=True, ignore=-100, reduction="mean", piece=0, target_type=torch.int64, share=0.2, spread=1.0, x=None, w=None,
+               b="make", target=None, up=None, seed=0):
+    """Loss and gradients against the definition in 64 bits, within the bounds of a kernel that sums in 32 bits and rounds dl to the
+    inputs' type: a logit is off by e_l = (features + 16) E of the sum of its absolute products, a probability by twice that
+    and 2^-20 (the exponent's base-2 argument, of at most 16 here, rounded to 32 bits), relative to itself."""
+    g = gen(seed + n * 7 + v * 3 + d)
+    if x is None:
+        x = torch.randn((n, d), generator=g).to(dtype)
+    if w is None:
+        w = (torch.randn((v, d), generator=g) * spread * 2 / math.sqrt(d)).to(dtype)
+    if isinstance(b, str):
+        b = torch.randn((v,), generator=g).to(dtype) if bias else None
+    if target is None:
+        target = torch.randint(0, v, (n,), generator=g)
+        target[torch.rand((n,), generator=g) < share] = ignore
+    target = target.to(target_type)
+    if up is None:
+        up = torch.rand((n,), generator=g) * 3 - 1 if reduction == "none" else torch.tensor(2.5)
+    ins = [None if t is None else t.cuda().requires_grad_() for t in (x, w, b)]
+    loss = pkg.linear_cross_entropy(ins[0], ins[1], target.cuda(), bias=ins[2], ignore_index=ignore, reduction=reduction, piece=piece)
+    assert loss.dtype == F32
+    leaves = [t for t in ins if t is not None]
+    got = torch.autograd.grad(loss, leaves, up.cuda())
+    # ---- the definition, over the points that count
+    x64, w64 = x.double(), w.double()
+    b64 = torch.zeros(v, dtype=torch.float64) if b is None else b.double()
+    keep = torch.nonzero(target.long() != ignore)[:, 0]
+    xs, ts = x64[keep], target.long()[keep]
+    logits = xs @ w64.t() + b64
+    finite_b = torch.where(b64.abs() < 1e4, b64, 0)      # (masked classes take part in nothing)
+    e_l = ((d + 16) * E * (xs.abs() @ w64.abs().t() + finite_b.abs() + 1)).amax(1, keepdim=True) if len(keep) else torch.zeros((0, 1), dtype=torch.float64)
+    lse = torch.logsumexp(logits, 1, keepdim=True)
+    each = lse[:, 0] - logits[torch.arange(len(keep)), ts]
+    each_tol = 2 * e_l[:, 0] + 8 * E * (lse[:, 0].abs() + each.abs()) + 1e-30
+    full, full_tol = torch.zeros(n, dtype=torch.float64), torch.zeros(n, dtype=torch.float64)
+    full[keep], full_tol[keep] = each, each_tol
+    count = max(1, len(keep)) if reduction == "mean" else 1
+    if reduction == "none":
+        near(loss, full, full_tol)
+        weight = up.double()[keep][:, None]
+    else:
+        near(loss, full.sum() / count, full_tol.sum() / count + 2 * E * (full.abs().sum() / count))
+        weight = up.double() / count * torch.ones((len(keep), 1), dtype=torch.float64)
+    p = torch.exp(logits - lse)
+    dl = p.clone()
+    dl[torch.arange(len(keep)), ts] -= 1
+    u = torch.finfo(dtype).eps / 2
+    # float32 is held in planes (2^-25) and multiplied without the products below 2^-24 (three of them)
+    u_dl = 2.0 ** -22 if dtype == F32 else u
+    dl_tol = weight.abs() * (p * (2 * e_l + 2.0 ** -20) + u_dl * dl.abs())
+    if dtype == F16:      # steps below the smallest normal number, 2^15 down, of the largest weight
+        dl_tol = dl_tol + weight.abs().max() * 2.0 ** -40 if len(keep) else dl_tol
+    if dtype == F32:      # the third plane of the smallest values
+        dl_tol = dl_tol + weight.abs() * 2.0 ** -126
+    dl = dl * weight
+    tiny = torch.finfo(dtype).smallest_normal * (1 if dtype != F16 else torch.finfo(dtype).eps)
+    dx, dx_tol = torch.zeros((n, d), dtype=torch.float64), torch.zeros((n, d), dtype=torch.float64)
+    dx[keep] = dl @ w64
+    sums = lambda k: (k + 64) * E  # noqa: E731  (additions of a sum in 32 bits, its splits among them)
+    dx_tol[keep] = dl_tol @ w64.abs() + sums(v) * (dl.abs() @ w64.abs()) + (2.0 ** -22 * (dl.abs() @ w64.abs()) if dtype == F32 else 0)
+    near(got[0], dx, dx_tol + u * dx.abs() * (1 + 2.0 ** -8) + tiny)
+    dw = dl.t() @ xs
+    size = dl.abs().t() @ xs.abs()
+    near(got[1], dw, dl_tol.t() @ xs.abs() + sums(n) * size + (2.0 ** -22 * size if dtype == F32 else 0) + u * dw.abs() * (1 + 2.0 ** -8) + tiny)
+    if b is not None:
+        db = dl.sum(0)
+        near(got[2], db, dl_tol.sum(0) + sums(n) * dl.abs().sum(0) + u * db.abs() * (1 + 2.0 ** -8) + tiny)
+    return loss, got
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,v,d", [(1, 1, 1), (1, 2, 8), (3, 20, 64), (127, 129, 67), (128, 128, 64), (129, 20, 96), (257, 260, 128), (500, 33, 30),
+                                   (64, 1000, 192), (40, 3001, 16), (2, 700, 513)])
+def test_loss_sizes(pkg, dtype, n, v, d):
+    check_loss(pkg, n, v, d, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("bias,target_type,ignore", [(True, torch.int32, 0), (False, torch.int64, -100)])
+def test_loss_reductions(pkg, dtype, reduction, bias, target_type, ignore):
+    check_loss(pkg, 300, 50, 64, dtype, bias, ignore, reduction, target_type=target_type)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("piece", [1, 128, 256, 100000])
+def test_loss_pieces(pkg, dtype, piece):
+    check_loss(pkg, 200, 777, 64, dtype, piece=piece)
+    check_loss(pkg, 700, 300, 40, dtype, piece=piece, reduction="none")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_loss_large_logits(pkg, dtype):
+    check_loss(pkg, 200, 300, 64, dtype, spread=30.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v,d,share", [(5000, 20, 32, 0.1), (3000, 260, 128, 0.85), (1500, 5000, 64, 0.0), (20, 20000, 128, 0.2)])
+def test_loss_larger(pkg, dtype, n, v, d, share):
+    check_loss(pkg, n, v, d, dtype, share=share)
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_loss_where_no_point_counts(pkg, reduction):
+    loss, got = check_loss(pkg, 150, 20, 64, BF16, target=torch.full((150,), -100), reduction=reduction)
+    assert not loss.any() and not any(t.any() for t in got)
+
+
+def test_loss_ignored_features_reach_nothing(pkg):
+    g = gen(8)
+    for dtype, d in ((BF16, 64), (BF16, 50), (F32, 64)):
+        x, target = torch.randn((400, d), generator=g).to(dtype), torch.randint(0, 30, (400,), generator=g)
+        out = torch.rand((400,), generator=g) < 0.3
+        target[out] = -100
+        a = check_loss(pkg, 400, 30, d, dtype, x=x, target=target)
+        x = x.clone()
+        x[out] = float("nan")
+        ins = x.cuda().requires_grad_()
+        w = (torch.randn((30, d), generator=gen(400 * 7 + 30 * 3 + d)) * 2 / math.sqrt(d)).to(dtype)
+        w = w.cuda().requires_grad_()
+        loss = pkg.linear_cross_entropy(ins, w, target.cuda(), reduction="sum")
+        dx, dw = torch.autograd.grad(loss, (ins, w))
+        assert torch.isfinite(loss) and torch.isfinite(dx).all() and torch.isfinite(dw).all() and not dx[out.cuda()].any()
+        assert a is not None
+
+
+def test_loss_masked_classes(pkg):
+    """Classes masked by a bias of -inf or the type's lowest value have probability 0; a row that keeps only its own class, loss 0."""
+    for dtype in (F32, BF16, F16):
+        for low in (float("-inf"), torch.finfo(dtype).min):
+            b = torch.zeros(200, dtype=dtype)
+            b[50:] = low
+            target = torch.arange(90) % 50
+            check_loss(pkg, 90, 200, 64, dtype, b=b, target=target)
+    b = torch.full((40,), float("-inf"), dtype=BF16)
+    b[7] = 0
+    loss, got = check_loss(pkg, 30, 40, 64, BF16, b=b, target=torch.full((30,), 7), reduction="none")
+    assert loss.abs().max() <= 1e-5 and not got[0].any()
+    # the target itself masked: infinite, as the definition says; every class masked: no number
+    x, w = torch.randn((3, 64), generator=gen(1)).cuda(), torch.randn((40, 64), generator=gen(2)).cuda()
+    loss = pkg.linear_cross_entropy(x, w, torch.tensor([3, 7, 8]).cuda(), bias=b.float().cuda(), reduction="none")
+    assert loss[0] == float("inf") and loss[1] == 0 and loss[2] == float("inf")
+    loss = pkg.linear_cross_entropy(x, w, torch.tensor([3, 7, 8]).cuda(), bias=torch.full((40,), float("-inf")).cuda(), reduction="none")
+    assert torch.isnan(loss).all()
+
+
+def test_loss_targets_that_are_no_class(pkg):
+    x, w = torch.randn((4, 64), generator=gen(1)).cuda().requires_grad_(), torch.randn((20, 64), generator=gen(2)).cuda().requires_grad_()
+    loss = pkg.linear_cross_entropy(x, w, torch.tensor([3, 20, -1, 2 ** 40]).cuda(), reduction="none")
+    assert torch.isfinite(loss[0]) and torch.isnan(loss[1:]).all()
+    dx, = torch.autograd.grad(loss, x, torch.ones(4, device="cuda"))
+    assert torch.isfinite(dx[0]).all() and torch.isnan(dx[1:]).all()
+
+
+def test_loss_layouts(pkg):
+    g = gen(4)
+    for dtype in (BF16, F32):
+        base, wide = torch.randn((90, 3, 70), generator=g).to(dtype).cuda(), torch.randn((128, 50), generator=g).to(dtype).cuda()
+        target = torch.randint(0, 50, (90, 3), generator=g).cuda()
+        for x, w, t in ((base[:, :, 3:67], wide[:64].t(), target), (base[:, 1, :64], wide.t()[:, 10:74], target[:, 1]),
+                        (base[:1, :1, :64].expand(90, 3, 64), wide.t()[:, :64], target), (base[0, 0, :64], wide.t()[:, :64], target[0, 0])):
+            x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+            loss = pkg.linear_cross_entropy(x, w, t, reduction="sum")
+            dx, dw = torch.autograd.grad(loss, (x, w))
+            x2, w2 = x.detach().contiguous().requires_grad_(), w.detach().contiguous().requires_grad_()
+            l2 = pkg.linear_cross_entropy(x2, w2, t.contiguous(), reduction="sum")
+            ex, ew = torch.autograd.grad(l2, (x2, w2))
+            assert torch.equal(loss, l2) and torch.equal(dx, ex) and torch.equal(dw, ew) and dx.shape == x.shape
+    # a head shared by two losses: the gradients add up
+    w = wide.t()[:, :64].detach().contiguous().requires_grad_()
+    x = base[:, 0, :64].contiguous()
+    one = lambda a, t: torch.autograd.grad(pkg.linear_cross_entropy(a, w, t), w)[0]  # noqa: E731
+    both, = torch.autograd.grad(pkg.linear_cross_entropy(x, w, target[:, 0]) + pkg.linear_cross_entropy(x * 2, w, target[:, 1]), w)
+    assert torch.equal(both, one(x, target[:, 0]) + one(x * 2, target[:, 1]))
+
+
+def test_loss_parts_of_the_gradient(pkg):
+    g = gen(6)
+    x, w, b = torch.randn((70, 64), generator=g).cuda(), torch.randn((30, 64), generator=g).cuda(), torch.randn((30,), generator=g).cuda()
+    t = torch.randint(0, 30, (70,), generator=g).cuda()
+    ins = [v.clone().requires_grad_() for v in (x, w, b)]
+    want = torch.autograd.grad(pkg.linear_cross_entropy(ins[0], ins[1], t, bias=ins[2]), ins)
+    for k in range(3):
+        some = [v.clone().requires_grad_(i == k) for i, v in enumerate((x, w, b))]
+        got, = torch.autograd.grad(pkg.linear_cross_entropy(some[0], some[1], t, bias=some[2]), some[k])
+        assert torch.equal(got, want[k])
+    assert not pkg.linear_cross_entropy(x, w, t).requires_grad
+    # backward twice through one forward
+    loss = pkg.linear_cross_entropy(ins[0], ins[1], t, bias=ins[2])
+    for _ in range(2):
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(loss, ins, retain_graph=True), want))
+
+
+def test_loss_of_no_points(pkg):
+    w = torch.randn((30, 64), device="cuda").requires_grad_()
+    x = torch.zeros((0, 64), device="cuda").requires_grad_()
+    t = torch.zeros(0, dtype=torch.int64, device="cuda")
+    for reduction, shape in (("mean", ()), ("sum", ()), ("none", (0,))):
+        loss = pkg.linear_cross_entropy(x, w, t, reduction=reduction)
+        assert loss.shape == shape and not loss.any()
+        dx, dw = torch.autograd.grad(loss.sum(), (x, w))
+        assert dx.shape == (0, 64) and not dw.any()
+
+
+def test_loss_gradient_against_differences(pkg):
+    g = gen(9)
+    x, w, b = (torch.randn(s, generator=g).cuda().requires_grad_() for s in ((12, 16), (9, 16), (9,)))
+    t = torch.randint(0, 9, (12,), generator=g).cuda()
+    f = lambda *a: pkg.linear_cross_entropy(a[0], a[1], t, bias=a[2], reduction="sum").item()  # noqa: E731
+    got = torch.autograd.grad(pkg.linear_cross_entropy(x, w, t, bias=b, reduction="sum"), (x, w, b))
+    h = 2.0 ** -6
+    for k, at in ((0, (3, 5)), (0, (11, 15)), (1, (0, 0)), (1, (8, 7)), (2, (4,))):
+        up, down = [v.detach().clone() for v in (x, w, b)], [v.detach().clone() for v in (x, w, b)]
+        up[k][at] += h
+        down[k][at] -= h
+        # third derivative of the loss below 30 (|w|, |x| < 4) times h^2 / 6; the sum's rounding over 2 h
+        assert abs(got[k][at].item() - (f(*up) - f(*down)) / (2 * h)) <= 30 * h * h / 6 + 200 * E / h
+
+
+def test_operators_on_another_stream_and_in_a_graph(pkg):
+    g = gen(11)
+    q = torch.randn((260, 2, 32), generator=g).to(BF16).cuda()
+    pos = torch.randn((260, 3), generator=g).cuda() * 9
+    w = torch.randn((21, 64), generator=g).to(BF16).cuda()
+    t = torch.randint(0, 21, (260,), generator=g).cuda()
+
+    def step(q, w):
+        y, _ = pkg.rotary_positions(q, pos, (5, 5, 5))
+        loss = pkg.linear_cross_entropy(y.flatten(1), w, t, ignore_index=0)
+        return (loss, *torch.autograd.grad(loss, (q, w)))
+
+    def eager(q, w):
+        return [v.detach().clone() for v in step(q.detach().clone().requires_grad_(), w.detach().clone().requires_grad_())]
+
+    want = eager(q, w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = eager(q, w)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # two graphs of the same step over leaves of their own, replayed in turn with new values and eager work between
+    graphs = []
+    for _ in range(2):
+        a, b = q.clone().requires_grad_(), w.clone().requires_grad_()
+        with torch.cuda.stream(side):
+            step(a, b)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step(a, b)
+        graphs.append((graph, a, b, out))
+    for k in range(4):
+        for graph, a, b, out in graphs:
+            with torch.no_grad():
+                a.copy_(torch.randn(q.shape, generator=g).to(BF16))
+                b.copy_(torch.randn(w.shape, generator=g).to(BF16))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(out, eager(a, b))), k

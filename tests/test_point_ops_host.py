@@ -1,0 +1,139 @@
+"""Refusals of the pool's and the training step's operators: arguments are looked at before the GPU is (not gpu)."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def test_c_entries_refuse_without_a_gpu(pkg):
+    L, lib = pkg._lib, pkg._lib.load()
+    assert lib.r3d_block_tables_workspace_bytes(0) == 0 and lib.r3d_block_tables_workspace_bytes(1000) >= 4 * 2 * 8
+    assert lib.r3d_block_tables(*[None] * 1, 4, 16, 2, *[None] * 3, 8, *[None] * 7, 0, None) == L.E_ARG
+    assert b"block_tables" in lib.r3d_last_error()
+    p = C.cast(C.create_string_buffer(64), C.c_void_p).value // 16 * 16
+    bad = [(p, 0, 16, 2), (p, 4, 0, 2), (p, 4, 16, 0), (p, 4, 1 << 30, 4), (p, -1, 16, 2)]
+    for lengths, rows, block, most in bad:
+        assert lib.r3d_block_tables(lengths, rows, block, most, p, p, p, 8, p, p + 16, p + 16, p + 16, p + 16, None, p, 1 << 20, None) == L.E_ARG
+    assert lib.r3d_block_tables(p, 4, 16, 2, p, p, p, 8, p, p, p + 16, p + 16, p + 16, None, p, 1 << 20, None) == L.E_ARG      # in place
+    assert lib.r3d_block_tables(p, 4, 16, 2, p, p, p, 8, p, p + 16, p + 16, p + 16, p + 16, None, p, 8, None) == L.E_WORKSPACE
+    assert lib.r3d_slot_map(None, 4, None, 16, 1, None, 4, 10, p, p, p, None) == L.E_ARG
+    assert lib.r3d_slot_map(p, 4, None, 16, 1, None, 5, 10, p, p, p, None) == L.E_ARG       # five sequences of four rows
+    assert lib.r3d_slot_map(p, 4, None, 16, 1, None, 4, -1, p, p, p, None) == L.E_ARG
+    assert lib.r3d_slot_map(p, 4, p, 1 << 30, 4, None, 4, 10, p, p, p, None) == L.E_ARG
+    assert lib.r3d_slot_map(p, 4, None, 16, 1, None, 4, 10, p, p + 8, p, None) == L.E_ARG    # alignment
+    rows = (L.Rows * 1)(L.Rows(p, p, 16, 16, 16))
+    assert lib.r3d_move_rows(None, 1, None, None, 1, 1, 1, None) == L.E_ARG
+    assert lib.r3d_move_rows(rows, 5, None, None, 1, 1, 1, None) == L.E_ARG
+    assert lib.r3d_move_rows(rows, 1, None, None, 4, 3, 4, None) == L.E_ARG
+    assert lib.r3d_move_rows(rows, 1, None, None, 4, 4, 3, None) == L.E_ARG
+    assert lib.r3d_move_rows((L.Rows * 1)(L.Rows(p, p, 16, 8, 16)), 1, None, None, 1, 1, 1, None) == L.E_ARG
+    assert lib.r3d_rotary(None, None) == L.E_ARG
+    d = L.Rotary(tokens=4, dim=8, axes=1, base=10.0, pos_type=L.T_F32)
+    d.heads[0], d.sections[0] = 1, 4
+    assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG and b"positions" in lib.r3d_last_error()
+    d.sections[0] = 5
+    assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG and b"pairs" in lib.r3d_last_error()
+    d.sections[0], d.base = 4, -1.0
+    assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG
+    e = L.LinearCE(n=4, v=3, d=8, ld_x=8, ld_w=8, type=L.T_F32, target_type=L.T_I64, reduction=L.CE_MEAN)
+    assert lib.r3d_linear_ce_workspace_bytes(C.byref(e), 0) > 0 and lib.r3d_linear_ce_workspace_bytes(C.byref(e), 1) > 0
+    assert lib.r3d_linear_ce_forward(C.byref(e), None, 0, None) == L.E_ARG
+    assert lib.r3d_linear_ce_backward(C.byref(e), None, 0, None) == L.E_ARG
+    for name, value in (("n", 0), ("v", 0), ("d", 0), ("ld_x", 7), ("type", L.T_F64), ("target_type", L.T_F32), ("reduction", 3), ("piece", -1)):
+        old = getattr(e, name)
+        setattr(e, name, value)
+        assert lib.r3d_linear_ce_workspace_bytes(C.byref(e), 0) == 0, name
+        setattr(e, name, old)
+
+
+def test_descriptors_match_the_header(pkg):
+    L = pkg._lib
+    assert C.sizeof(L.Rows) == 2 * 8 + 3 * 8
+    assert C.sizeof(L.Rotary) == 4 * 8 + 4 * 8 + 8 + 2 * 4 + 4 * 4 + 4 + 8 * 4 + 4 + 8 + 2 * 8 + 8
+    assert C.sizeof(L.LinearCE) == 4 * 8 + 7 * 8 + 4 * 4 + 10 * 8
+
+
+def test_block_tables_refuses(pkg):
+    t = torch.full((4, 3), -1, dtype=torch.int32)
+    good = [i32(1, 2, 3, 4), 16, t, i32(0, 0, 0, 0), i32(*range(12)), i32(12)]
+    for at, value in ((0, i32(1, 2)), (0, i32(1, 2, 3, 4).long()), (1, 0), (1, 1 << 30), (2, t[:, ::2]), (2, t.reshape(-1)), (3, i32(1)),
+                      (4, i32()), (5, i32(1, 2))):
+        args = list(good)
+        args[at] = value
+        with pytest.raises(ValueError):
+            pkg.block_tables(*args)
+    if not torch.cuda.is_available():
+        with pytest.raises(pkg.R3DError):
+            pkg.block_tables(*good)
+
+
+def test_slot_map_refuses(pkg):
+    n, t = i32(5, 6), torch.zeros((2, 2), dtype=torch.int32)
+    for args, kw in (((n.long(), 4), {}), ((n, 0), {}), ((n, 4), {"tables": t[:1]}), ((n, 4), {"tables": t.t()}), ((n, 1 << 30), {"tables": t}),
+                     ((n, 4), {"rows": torch.tensor([0])}), ((n, 4), {"capacity": -1}), ((i32(), 4), {})):
+        with pytest.raises(ValueError):
+            pkg.slot_map(*args, **kw)
+    if not torch.cuda.is_available():
+        with pytest.raises(pkg.R3DError):
+            pkg.slot_map(n, 4, capacity=8)
+
+
+def test_rows_refuse(pkg):
+    s, x = torch.zeros(3, dtype=torch.int64), torch.zeros((5, 4))
+    with pytest.raises(ValueError):
+        pkg.take_rows(s.int(), (x,))
+    with pytest.raises(ValueError):
+        pkg.take_rows(s, ())
+    with pytest.raises(ValueError):
+        pkg.take_rows(s, (x,) * 5)
+    with pytest.raises(ValueError):
+        pkg.take_rows(s, (x, x[:3]))
+    with pytest.raises(ValueError):
+        pkg.take_rows(s, (torch.zeros((4, 5)).t(),))
+    with pytest.raises(ValueError):
+        pkg.take_rows(s, (x.clone().requires_grad_(),))
+    with pytest.raises(ValueError):
+        pkg.put_rows(s, (x,), (x.double(),))
+    with pytest.raises(ValueError):
+        pkg.put_rows(s, (x[:2],), (x,))
+    with pytest.raises(ValueError):
+        pkg.put_rows(s, (x,), (x,), source_slots=s[:2])
+    with pytest.raises(ValueError):
+        pkg.put_rows(s, (x,), (x[:1].expand(5, 4),))
+    if not torch.cuda.is_available():
+        with pytest.raises(pkg.R3DError):
+            pkg.take_rows(s, (x,))
+
+
+def test_rotary_refuses(pkg):
+    q, p = torch.zeros((6, 2, 16)), torch.zeros((6, 2))
+    for args, kw in (((q[0], p, (4, 4)), {}), ((q, p, (4,)), {}), ((q, p[:5], (4, 4)), {}), ((q, p, (4, 5)), {}), ((q, p, (4, -1)), {}),
+                     ((q, p, (4, 4)), {"style": "other"}), ((q, p, (4, 4)), {"base": 0.0}), ((q, p, (4, 4)), {"base": float("inf")}),
+                     ((q, p, (4, 4)), {"key": q.half()}), ((q, p, (4, 4)), {"key": q[:5]}), ((q, p.clone().requires_grad_(), (4, 4)), {}),
+                     ((torch.zeros((6, 2, 15)), p, (2, 2)), {}), ((torch.zeros((6, 1, 1024)), p, (200, 200)), {})):
+        with pytest.raises(ValueError):
+            pkg.rotary_positions(*args, **kw)
+    for args in ((q.double(), p, (4, 4)), (q, p.to(torch.int16), (4, 4))):
+        with pytest.raises(TypeError):
+            pkg.rotary_positions(*args)
+    if not torch.cuda.is_available():
+        with pytest.raises(pkg.R3DError):
+            pkg.rotary_positions(q, p, (4, 4))
+
+
+def test_linear_cross_entropy_refuses(pkg):
+    x, w, t = torch.zeros((6, 8)), torch.zeros((5, 8)), torch.zeros(6, dtype=torch.int64)
+    for args, kw in (((x, w[:, :7], t), {}), ((x, w[:0], t), {}), ((x, w, t[:5]), {}), ((x, w, t), {"bias": torch.zeros(4)}),
+                     ((x, w, t), {"reduction": "average"}), ((x, w, t), {"piece": -1}), ((x, w[0], t), {})):
+        with pytest.raises(ValueError):
+            pkg.linear_cross_entropy(*args, **kw)
+    for args, kw in (((x, w.half(), t), {}), ((x.double(), w.double(), t), {}), ((x, w, t.float()), {}), ((x, w, t), {"bias": torch.zeros(5).half()})):
+        with pytest.raises(TypeError):
+            pkg.linear_cross_entropy(*args, **kw)
+    if not torch.cuda.is_available():
+        with pytest.raises(pkg.R3DError):
+            pkg.linear_cross_entropy(x, w, t)
