@@ -23,9 +23,6 @@ namespace {
 using namespace r3d;
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr int kPairs = 6;      // (plane of A, plane of B) of a split product, largest last dropped: m*l, l*l < 2^-24
-__device__ constexpr int kPlaneA[kPairs] = {0, 0, 1, 1, 0, 2}, kPlaneB[kPairs] = {0, 1, 0, 1, 2, 0};
-
 struct Counted {      // the points that count, on the device
   int32_t n;          // how many
   float share;        // 1 / n for a mean (0 where none counts), 1 else
@@ -123,6 +120,7 @@ struct PackArgs {
   int64_t ld, rows, width, ld_out, plane;      // width: of the source; ld_out a multiple of 64
   const int32_t *idx;
   const Counted *counted;      // rows: how many of them, where given
+  int32_t vector;              // rows begin at multiples of 16 bytes
 };
 
 __device__ __forceinline__ __bf16 toward_zero(float v) {      // (rounding up the largest floats would give infinities)
@@ -135,16 +133,42 @@ __device__ __forceinline__ void split3(float v, __bf16 &h, __bf16 &m, __bf16 &l)
   l = (__bf16)(r - (float)m);
 }
 
+template <class T>
+struct alignas(16) Piece {
+  T v[8];
+};
+
+// A thread makes a piece of 8 values of a row.
 template <class S, class T, int kPlanes>
 __global__ __launch_bounds__(256) void k_ce_pack(PackArgs a) {
-  const int64_t rows = a.counted ? a.counted->n : a.rows, all = rows * a.ld_out;
-  const S *src = static_cast<const S *>(a.src);
-  T *dst = static_cast<T *>(a.dst);
+  const int64_t rows = a.counted ? a.counted->n : a.rows;
+  const unsigned each = (unsigned)(a.ld_out / 8);
+  const int64_t all = rows * each;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / a.ld_out, c = i - r * a.ld_out;
-    const S v = c < a.width ? src[(a.idx ? a.idx[r] : r) * a.ld + c] : (S)0.0f;
-    if constexpr (kPlanes == 3) split3(v, dst[i], dst[i + a.plane], dst[i + 2 * a.plane]);
-    else dst[i] = v;
+    const int64_t r = all <= UINT32_MAX ? (unsigned)i / each : i / each;
+    const int64_t c = (i - r * each) * 8;
+    const S *src = static_cast<const S *>(a.src) + (a.idx ? a.idx[r] : r) * a.ld + c;
+    S v[8];
+    if (c + 8 <= a.width && a.vector) {
+      typedef S s4 __attribute__((ext_vector_type(16 / sizeof(S))));
+#pragma unroll
+      for (int k = 0; k < (int)sizeof(S) / 2; ++k) {
+        const s4 w = reinterpret_cast<const s4 *>(src)[k];
+#pragma unroll
+        for (int e = 0; e < 16 / (int)sizeof(S); ++e) v[k * (16 / sizeof(S)) + e] = w[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c + e < a.width ? src[e] : (S)0.0f;
+    }
+    Piece<T> out[kPlanes];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (kPlanes == 3) split3(v[e], out[0].v[e], out[1].v[e], out[2].v[e]);
+      else out[0].v[e] = v[e];
+    }
+#pragma unroll
+    for (int k = 0; k < kPlanes; ++k) *reinterpret_cast<Piece<T> *>(static_cast<T *>(a.dst) + k * a.plane + r * a.ld_out + c) = out[k];
   }
 }
 
@@ -161,58 +185,17 @@ struct Product {
   int32_t planes;
 };
 
-// acc += the k-blocks [kb0, kb1) of one 128 x 128 tile.  Ends with a barrier: LDS is free.
-template <class T, bool kACols, bool kBCols>
-__device__ __forceinline__ void product_tile(const Product &p, int64_t m0, int64_t n0, int64_t rows_a, int64_t rows_b, int64_t cols_a,
-                                             int64_t cols_b, int64_t kb0, int64_t kb1, T *lds, f32x16 (&acc)[2][2]) {
-  const int wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  const int pairs = p.planes == 3 ? kPairs : 1;
-  const int64_t n_kb = kb1 - kb0, steps = n_kb * pairs;
-  if (steps <= 0) return;
-  RowLoader<T> ra, rb;
-  ColLoader<T> ca, cb;
-  if constexpr (kACols) ca.tile(m0, cols_a); else ra.tile(p.a, m0, rows_a);
-  if constexpr (kBCols) cb.tile(n0, cols_b); else rb.tile(p.b, n0, rows_b);
-  int64_t kb = kb0;
-  int pair = 0;
-  if constexpr (kACols) ca.look(p.a, kb * kTileK, rows_a);
-  if constexpr (kBCols) cb.look(p.b, kb * kTileK, rows_b);
-  auto issue = [&](int buf) {
-    T *la = lds + buf * 2 * kOperandElems, *lb = la + kOperandElems;
-    const int64_t oa = (int64_t)kPlaneA[pair] * p.a.plane, ob = (int64_t)kPlaneB[pair] * p.b.plane;
-    if constexpr (kACols) ca.issue(p.a, la, oa); else ra.issue(la, oa + kb * kTileK);
-    if constexpr (kBCols) cb.issue(p.b, lb, ob); else rb.issue(lb, ob + kb * kTileK);
-    if (++kb == kb1) {
-      kb = kb0;
-      ++pair;
-    }
-    if constexpr (kACols) ca.look(p.a, kb * kTileK, rows_a);
-    if constexpr (kBCols) cb.look(p.b, kb * kTileK, rows_b);
-  };
-  issue(0);
-  __syncthreads();
-  for (int64_t s = 0; s < steps; ++s) {
-    const int buf = (int)(s & 1);
-    if (s + 1 < steps) issue(buf ^ 1);
-    const T *la = lds + buf * 2 * kOperandElems;
-    mma_block<T, kACols, kBCols>(la, la + kOperandElems, wm, wn, acc);
-    __syncthreads();
-  }
-}
-
-__device__ __forceinline__ void clear(f32x16 (&acc)[2][2]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+// Tiles in groups of 8 in n, so that the workgroups that run at a time share their rows of both operands.
+__device__ __forceinline__ void tile_of(int64_t id, int64_t mtiles, int64_t ntiles, int64_t &mt, int64_t &nt) {
+  const int64_t group = id / (8 * mtiles), first = group * 8, wide = ntiles - first < 8 ? ntiles - first : 8, in = id - group * 8 * mtiles;
+  mt = in / wide;
+  nt = first + in - mt * wide;
 }
 
 struct LseArgs {
   Product p;      // a: W [V], b: x [points]
-  int64_t v, kb, n_rows_x;      // n_rows_x: rows of x's storage
-  int32_t vtiles, splits, packed;
+  int64_t v, kb, ntiles;
+  int32_t vtiles, splits;
   const float *bias2;
   const int32_t *tgt;
   const Counted *counted;
@@ -220,38 +203,53 @@ struct LseArgs {
   int64_t n_pad;
 };
 
-// Maximum and sum of 2^(logit * log2 e) over a split of the classes for 128 points.  The classes are the rows of C, so a lane
-// holds 32 classes of each of its two points: the statistics of a tile stay in its registers, lanes and waves are joined once
-// at the end.
-template <class T>
-__global__ __launch_bounds__(kMmaThreads, 2) void k_ce_lse(LseArgs a) {
-  __shared__ __attribute__((aligned(128))) T lds[4 * kOperandElems];
+// Maximum and sum of 2^(logit * log2 e) over a split of the classes for the points of a tile.  The classes are the rows of C, so
+// a lane holds 16 FM classes of each of its FN points: the statistics of a tile stay in its registers, lanes and waves are
+// joined once at the end.
+template <class T, class S>
+__global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
+  __shared__ __attribute__((aligned(128))) T lds[2 * S::buffer];
   const int nc = a.counted->n;
-  const int64_t n0 = (int64_t)(blockIdx.x / a.splits) * kTileN;
-  const int split = blockIdx.x % a.splits;
+  const int64_t id = xcd_order(blockIdx.x, gridDim.x);
+  const int split = (int)(id / a.ntiles);
+  const int64_t n0 = (id - split * a.ntiles) * S::BN;
   if (n0 >= nc) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  int64_t col[2];
-  int tgt[2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+  float m[S::FN], l[S::FN];
+  int tgt[S::FN];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    col[j] = n0 + wn * 64 + j * 32 + (lane & 31);
-    tgt[j] = col[j] < nc ? a.tgt[col[j]] : -1;
+  for (int j = 0; j < S::FN; ++j) {
+    const int64_t col = n0 + (wn * S::FN + j) * 32 + (lane & 31);
+    m[j] = -INFINITY;
+    l[j] = 0.0f;
+    tgt[j] = col < nc ? a.tgt[col] : -1;
   }
   const int vt0 = (int)((int64_t)a.vtiles * split / a.splits), vt1 = (int)((int64_t)a.vtiles * (split + 1) / a.splits);
+  Stream<T, S, Lies::Rows, Lies::Rows> st;
+  st.a = a.p.a;
+  st.b = a.p.b;
+  st.rows_a = st.rows_b = 0;
+  st.range(0, a.kb, a.p.planes);
+  st.lb.tile(st.b, n0, nc);
+  st.la.tile(st.a, (int64_t)vt0 * S::BM, a.v);
+  st.issue(lds, 0);
+  __syncthreads();
   for (int vt = vt0; vt < vt1; ++vt) {
-    f32x16 acc[2][2];
+    f32x16 acc[S::FM][S::FN];
+    float none[S::FM];
     clear(acc);
-    product_tile<T, false, false>(a.p, (int64_t)vt * kTileM, n0, a.v, nc, 0, 0, 0, a.kb, lds, acc);
+    st.template run<false>(lds, acc, none, false, [&] {
+      if (vt + 1 < vt1) st.la.tile(st.a, (int64_t)(vt + 1) * S::BM, a.v);
+      return vt + 1 < vt1;
+    });
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int vb = vt * kTileM + wm * 64 + i * 32;
+    for (int i = 0; i < S::FM; ++i) {
+      const int vb = vt * S::BM + (wm * S::FM + i) * 32;
       float b[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) b[r] = a.bias2[vb + mma_row(r)];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < S::FN; ++j) {
         float t[16], top = m[j];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -268,29 +266,33 @@ __global__ __launch_bounds__(kMmaThreads, 2) void k_ce_lse(LseArgs a) {
         if (__any(d >= 0 && d < 32)) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (d == mma_row(r)) a.hit[col[j]] = t[r];
+            if (d == mma_row(r)) a.hit[n0 + (wn * S::FN + j) * 32 + (lane & 31)] = t[r];
         }
       }
     }
   }
   // a logit that is NaN leaves the maximum as it was and the sum NaN
-  float *s_m = reinterpret_cast<float *>(lds), *s_l = s_m + 2 * kTileN;
+  float *s_m = reinterpret_cast<float *>(lds), *s_l = s_m + S::WM * S::BN;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < S::FN; ++j) {
     const float om = __shfl_xor(m[j], 32), ol = __shfl_xor(l[j], 32), top = fmaxf(m[j], om), base = top == -INFINITY ? 0.0f : top;
     const float sum = l[j] * __builtin_amdgcn_exp2f(m[j] - base) + ol * __builtin_amdgcn_exp2f(om - base);
     if (lane < 32) {
-      const int at = wm * kTileN + wn * 64 + j * 32 + lane;
+      const int at = wm * S::BN + (wn * S::FN + j) * 32 + lane;
       s_m[at] = top;
       s_l[at] = sum;
     }
   }
   __syncthreads();
-  if (threadIdx.x < kTileN) {
-    const float m0 = s_m[threadIdx.x], m1 = s_m[kTileN + threadIdx.x], top = fmaxf(m0, m1), base = top == -INFINITY ? 0.0f : top;
-    const int64_t at = split * a.n_pad + n0 + threadIdx.x;
-    a.part_m[at] = top;
-    a.part_l[at] = s_l[threadIdx.x] * __builtin_amdgcn_exp2f(m0 - base) + s_l[kTileN + threadIdx.x] * __builtin_amdgcn_exp2f(m1 - base);
+  for (int c = threadIdx.x; c < S::BN; c += S::threads) {
+    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < S::WM; ++w) top = fmaxf(top, s_m[w * S::BN + c]);
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < S::WM; ++w) sum += s_l[w * S::BN + c] * __builtin_amdgcn_exp2f(s_m[w * S::BN + c] - base);
+    a.part_m[split * a.n_pad + n0 + c] = top;
+    a.part_l[split * a.n_pad + n0 + c] = sum;
   }
 }
 
@@ -390,37 +392,53 @@ __global__ __launch_bounds__(256) void k_ce_weight(WeightArgs a) {
 
 struct DlArgs {
   Product p;
-  int64_t v, kb;
-  int64_t piece0, piece, dl_plane;      // first class of the piece, its width in the workspace (a multiple of 128)
-  int32_t vtiles;
-  float held;      // 2^15 for float16
+  int64_t v, kb, ntiles;
+  int64_t piece0, dl_plane, n_pad;      // first class of the piece
+  int32_t vtiles, width;                // width: classes of the piece, a multiple of 64
+  float held;                           // 2^15 for float16
   const float *bias2, *lse2, *weight;
   const int32_t *tgt;
   const Counted *counted;
-  void *dl;        // [planes][points][piece]
+  void *dl;        // [planes][width / 8][n_pad][8]
 };
 
-template <class T, int kPlanes>
-__global__ __launch_bounds__(kMmaThreads, 2) void k_ce_dl(DlArgs a) {
-  __shared__ __attribute__((aligned(128))) T lds[4 * kOperandElems];
+// dl of a piece of the classes.  A lane holds 4 neighbouring classes of a point and its partner 32 lanes on the next 4: a swap
+// makes pieces of 8, and 32 lanes write 512 contiguous bytes.
+template <class T, class S, int kPlanes>
+__global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
+  __shared__ __attribute__((aligned(128))) T lds[2 * S::buffer];
   const int nc = a.counted->n;
-  const int64_t n0 = (int64_t)(blockIdx.x / a.vtiles) * kTileN;
-  const int vt = blockIdx.x % a.vtiles;
+  int64_t vt, nt;
+  tile_of(xcd_order(blockIdx.x, gridDim.x), a.vtiles, a.ntiles, vt, nt);
+  const int64_t n0 = nt * S::BN;
   if (n0 >= nc) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-  f32x16 acc[2][2];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+  f32x16 acc[S::FM][S::FN];
+  float none[S::FM];
   clear(acc);
-  product_tile<T, false, false>(a.p, a.piece0 + (int64_t)vt * kTileM, n0, a.v, nc, 0, 0, 0, a.kb, lds, acc);
+  {
+    Stream<T, S, Lies::Rows, Lies::Rows> st;
+    st.a = a.p.a;
+    st.b = a.p.b;
+    st.rows_a = st.rows_b = 0;
+    st.range(0, a.kb, a.p.planes);
+    st.la.tile(st.a, a.piece0 + vt * S::BM, a.v);
+    st.lb.tile(st.b, n0, nc);
+    st.issue(lds, 0);
+    __syncthreads();
+    st.template run<false>(lds, acc, none, false, [] { return false; });
+  }
   T *dl = static_cast<T *>(a.dl);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t col = n0 + wn * 64 + j * 32 + (lane & 31);
+  for (int j = 0; j < S::FN; ++j) {
+    const int64_t col = n0 + (wn * S::FN + j) * 32 + (lane & 31);
     const bool in = col < nc;
     const int tgt = in ? a.tgt[col] : -1;
-    const float lse2 = in ? a.lse2[col] : 0.0f, weight = a.weight[col] * a.held;
+    const float lse2 = in ? a.lse2[col] : 0.0f, weight = in ? a.weight[col] * a.held : 0.0f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int local = vt * kTileM + wm * 64 + i * 32;
+    for (int i = 0; i < S::FM; ++i) {
+      const int local = (int)vt * S::BM + (wm * S::FM + i) * 32;
+      if (local >= a.width) continue;
       const int64_t vb = a.piece0 + local;
       const int64_t d = tgt - vb;
       float p[16];
@@ -430,90 +448,124 @@ __global__ __launch_bounds__(kMmaThreads, 2) void k_ce_dl(DlArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] -= d == mma_row(r) ? 1.0f : 0.0f;
       }
+      typedef T t4 __attribute__((ext_vector_type(4)));
+      typedef unsigned u2 __attribute__((ext_vector_type(2)));
+      typedef unsigned u4 __attribute__((ext_vector_type(4)));
+      t4 q[4][kPlanes];
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        typedef T t4 __attribute__((ext_vector_type(4)));
-        t4 q[3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float w = in ? p[r + e] * weight : 0.0f;
-          if constexpr (kPlanes == 3) {
-            T h, mm, l;
-            split3(w, h, mm, l);
-            q[0][e] = h;
-            q[1][e] = mm;
-            q[2][e] = l;
-          } else {
-            q[0][e] = (T)w;
-          }
+      for (int r = 0; r < 16; ++r) {
+        const float w = in ? p[r] * weight : 0.0f;
+        if constexpr (kPlanes == 3) {
+          T h, mm, l;
+          split3(w, h, mm, l);
+          q[r >> 2][0][r & 3] = h;
+          q[r >> 2][1][r & 3] = mm;
+          q[r >> 2][2][r & 3] = l;
+        } else {
+          q[r >> 2][0][r & 3] = (T)w;
         }
-#pragma unroll
-        for (int k = 0; k < kPlanes; ++k) *reinterpret_cast<t4 *>(dl + k * a.dl_plane + col * a.piece + local + mma_row(r)) = q[k];
       }
+#pragma unroll
+      for (int k = 0; k < kPlanes; ++k)
+#pragma unroll
+        for (int h = 0; h < 4; h += 2) {
+          const u2 even = __builtin_bit_cast(u2, q[h][k]), odd = __builtin_bit_cast(u2, q[h + 1][k]);
+          const auto s0 = __builtin_amdgcn_permlane32_swap(even[0], odd[0], false, false);
+          const auto s1 = __builtin_amdgcn_permlane32_swap(even[1], odd[1], false, false);
+          const u4 out = {s0[0], s1[0], s0[1], s1[1]};
+          const int64_t piece = local / 8 + h + (lane >> 5);
+          *reinterpret_cast<u4 *>(dl + k * a.dl_plane + (piece * a.n_pad + col) * 8) = out;
+        }
     }
   }
 }
 
 struct OutArgs {
   Product p;
-  int64_t m, n, k_rows_a, k_rows_b;      // k_rows: storage rows of a "columns" operand
-  int64_t cols_a, cols_b, kb;
-  int32_t m_counted, k_counted;          // the dimension is the points: take it from the device
+  int64_t m, n, kb;                      // m: rows of the result, n: columns that are written
+  int64_t limit_a, limit_b, rows_b;      // columns of the operands, rows of b
+  int32_t points;                        // 0: m and the rest as given; 1: m is the points that count; 2: k is
   int32_t mtiles, ntiles, splits, add;
   const Counted *counted;
-  float *out;                            // [splits][m_pad][ld]
+  float *out;                            // [splits][m_pad][ld], or null:
   int64_t ld, split_stride;
-  float *row_sum;                        // [splits][m_pad]: sums over k of A, or null
+  void *final_out;                       // the result itself, rows through idx where given
+  const int32_t *idx;
+  const float *scale;
+  float unheld;
+  float *row_sum;                        // [splits][sum_stride]: sums over k of A, or null
+  int64_t sum_stride;
 };
 
-template <class T>
-__device__ __forceinline__ float sum8(typename Mma<T>::v8 v, float s) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s += (float)v[i];
-  return s;
-}
-
-// The products with dl: dx = dl W (A rows, B columns) and dW = dl^T x (both columns), in 32 bits into the workspace.
-template <class T, bool kACols>
-__global__ __launch_bounds__(kMmaThreads, 2) void k_ce_out(OutArgs a) {
-  __shared__ __attribute__((aligned(128))) T lds[4 * kOperandElems];
+// The products with dl: dx = dl W and dW = dl^T x (with db, the sums of dl's columns, which pass by), into 32-bit sums in the
+// workspace or, where nothing is left to add, to the result.
+template <class V, class T, class S, Lies LA>
+__global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
+  __shared__ __attribute__((aligned(128))) T lds[2 * S::buffer];
   const int nc = a.counted->n;
-  const int tiles = a.mtiles * a.ntiles, tile = blockIdx.x % tiles, split = blockIdx.x / tiles;
-  const int64_t m0 = (int64_t)(tile / a.ntiles) * kTileM, n0 = (int64_t)(tile % a.ntiles) * kTileN;
-  const int64_t m = a.m_counted ? nc : a.m, kb = a.k_counted ? (nc + kTileK - 1) / kTileK : a.kb;
+  const int64_t id = xcd_order(blockIdx.x, gridDim.x), tiles = (int64_t)a.mtiles * a.ntiles;
+  const int split = (int)(id / tiles);
+  int64_t mt, nt;
+  tile_of(id - split * tiles, a.mtiles, a.ntiles, mt, nt);
+  const int64_t m0 = mt * S::BM, n0 = nt * S::BN;
+  const int64_t m = a.points == 1 ? nc : a.m, kb = a.points == 2 ? (nc + kTileK - 1) / kTileK : a.kb;
   if (m0 >= m) return;
-  const int64_t kb0 = kb * split / a.splits, kb1 = kb * (split + 1) / a.splits;
-  f32x16 acc[2][2];
+  constexpr bool kSums = LA == Lies::PiecesCols;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+  const bool sums = kSums && a.row_sum && nt == 0 && wn == 0;
+  f32x16 acc[S::FM][S::FN];
+  float row_sum[S::FM];
   clear(acc);
-  product_tile<T, kACols, true>(a.p, m0, n0, kACols ? a.k_rows_a : m, a.k_counted ? nc : a.k_rows_b, a.cols_a, a.cols_b, kb0, kb1, lds, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < S::FM; ++i) row_sum[i] = 0.0f;
+  const int64_t kb0 = kb * split / a.splits, kb1 = kb * (split + 1) / a.splits;
+  if (kb1 > kb0) {
+    Stream<T, S, LA, Lies::Cols> st;
+    st.a = a.p.a;
+    st.b = a.p.b;
+    st.rows_a = 0;
+    st.rows_b = a.points == 2 ? nc : a.rows_b;
+    st.la.tile(st.a, m0, a.points == 1 ? nc : a.limit_a);
+    st.lb.tile(st.b, n0, a.limit_b);
+    st.range(kb0, kb1, a.p.planes);
+    st.issue(lds, 0);
+    __syncthreads();
+    st.template run<kSums>(lds, acc, row_sum, sums, [] { return false; });
+  }
+  const float scale = a.final_out ? *a.scale * a.unheld : 1.0f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t n = n0 + wn * 64 + j * 32 + (lane & 31);
-      if (n >= a.n) continue;
+  for (int i = 0; i < S::FM; ++i) {
+    if (kSums && sums) {
+      const float s = row_sum[i] + __shfl_xor(row_sum[i], 32);
+      const int64_t row = m0 + (wm * S::FM + i) * 32 + lane;
+      if (lane < 32 && row < m) a.row_sum[split * a.sum_stride + row] = s;
+    }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t row = m0 + wm * 64 + i * 32 + mma_row(r);
-        float *at = a.out + split * a.split_stride + row * a.ld + n;
-        if (row < m) *at = a.add ? *at + acc[i][j][r] : acc[i][j][r];
+    for (int r = 0; r < 16; ++r) {
+      const int64_t row = m0 + (wm * S::FM + i) * 32 + mma_row(r);
+      if (row >= m) continue;
+      const int64_t to = a.final_out && a.idx ? a.idx[row] : row;
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) {
+        const int64_t n = n0 + (wn * S::FN + j) * 32 + (lane & 31);
+        if (n >= a.n) continue;
+        if (a.final_out) {
+          static_cast<V *>(a.final_out)[to * a.ld + n] = (V)(acc[i][j][r] * scale);
+        } else {
+          float *at = a.out + split * a.split_stride + row * a.ld + n;
+          *at = a.add ? *at + acc[i][j][r] : acc[i][j][r];
+        }
       }
     }
+  }
 }
 
-// db: the columns of dl summed over the points, a thread per class and slice of the points.
-template <class T, int kPlanes>
-__global__ __launch_bounds__(256) void k_ce_db(const T *dl, int64_t piece, int64_t plane, const Counted *counted, int32_t slices, float *out) {
-  const int nc = counted->n;
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= piece) return;
-  const int64_t lo = (int64_t)nc * blockIdx.y / slices, hi = (int64_t)nc * (blockIdx.y + 1) / slices;
-  float sum = 0.0f;
-  for (int64_t n = lo; n < hi; ++n)
-#pragma unroll
-    for (int k = 0; k < kPlanes; ++k) sum += (float)dl[k * plane + n * piece + c];
-  out[blockIdx.y * piece + c] = sum;
+// Rows of the points that do not count.
+template <class V>
+__global__ __launch_bounds__(256) void k_ce_zero(V *dx, int64_t n, int64_t d, const int32_t *place) {
+  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += (int64_t)gridDim.x * 4)
+    if (place[r] < 0)
+      for (int64_t c = threadIdx.x & 63; c < d; c += 64) dx[r * d + c] = (V)0.0f;
 }
 
 struct FinishArgs {
@@ -526,32 +578,80 @@ struct FinishArgs {
   void *out;
 };
 
-// Splits joined, the factor put back, one rounding.
-template <class S>
+// Splits joined, the factor put back, one rounding.  A thread makes kVec neighbouring values.
+template <class V, int kVec>
 __global__ __launch_bounds__(256) void k_ce_finish(FinishArgs a) {
+  typedef float fv __attribute__((ext_vector_type(kVec)));
+  struct alignas(kVec * sizeof(V)) Out {
+    V v[kVec];
+  };
   const float scale = *a.scale * a.unheld;
-  const int64_t all = a.rows * a.width;
+  const unsigned each = (unsigned)(a.width / kVec);
+  const int64_t all = a.rows * each;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / a.width, c = i - r * a.width, at = a.place ? a.place[r] : r;
-    float sum = 0.0f;
+    const int64_t r = all <= UINT32_MAX ? (unsigned)i / each : i / each;
+    const int64_t c = (i - r * each) * kVec, at = a.place ? a.place[r] : r;
+    float sum[kVec];
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) sum[e] = 0.0f;
     if (at >= 0) {
-      for (int s = 0; s < a.splits; ++s) sum += a.acc[s * a.split_stride + at * a.ld + c];
-      sum *= scale;
+      const float *from = a.acc + at * a.ld + c;
+#pragma unroll 8
+      for (int s = 0; s < a.splits; ++s) {
+        if constexpr (kVec == 1) {
+          sum[0] += from[s * a.split_stride];
+        } else {
+          const fv v = *reinterpret_cast<const fv *>(from + s * a.split_stride);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) sum[e] += v[e];
+        }
+      }
     }
-    static_cast<S *>(a.out)[r * a.ld_out + c] = (S)sum;
+    Out out;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) out.v[e] = (V)(at >= 0 ? sum[e] * scale : 0.0f);
+    *reinterpret_cast<Out *>(static_cast<V *>(a.out) + r * a.ld_out + c) = out;
   }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kPieceBytes = 256ll << 20;      // what a piece's dl may take: the last-level cache's size
+constexpr int kCus = 256;
 
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+int64_t tiles_of(int64_t m, int64_t n, int64_t bm, int64_t bn) { return (up(m, bm) / bm) * (up(n, bn) / bn); }
+
+// Parts in which the long axis of a product is cut: enough workgroups for the chip, and no last round that leaves most of it
+// idle; at least four k-blocks each.
+int cut(int64_t tiles, int64_t slots, int64_t most) {
+  if (most < 1) most = 1;
+  int best = 1;
+  double best_share = 0.0;
+  for (int64_t s = 1; s <= most && s <= 1024; ++s) {
+    const int64_t all = tiles * s, rounds = (all + slots - 1) / slots;
+    const double share = (double)all / (double)(rounds * slots);
+    if (share > best_share * 1.05) {
+      best = (int)s;
+      best_share = share;
+    }
+    if (all >= 4 * slots) break;
+  }
+  return best;
+}
+
+// A product's tiles: large ones where they fill the chip and waste no more than a quarter over small ones at the edges.
+bool large_tiles(int64_t m, int64_t n, int64_t most_splits) {
+  const int64_t big = tiles_of(m, n, Big::BM, Big::BN), small = tiles_of(m, n, Small::BM, Small::BN);
+  return big * most_splits >= kCus && big * 4 * 4 <= small * 5;
+}
 
 struct Plan {
   bool direct;      // the operands are multiplied where they lie
   int planes, type_bytes;
   int64_t dp, n_pad, v_pad, piece;
-  int lse_splits, dx_splits, dw_splits, db_slices, top_parts, groups;
+  bool lse_big, dl_big, dx_big, dw_big;
+  int lse_splits, dx_splits, dw_splits, top_parts, groups;
+  bool dx_final, dw_final;      // nothing to add: straight into the result
   // workspace
   int32_t *part;
   void *xp, *wp;
@@ -570,14 +670,9 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   p.type_bytes = d.type == R3D_T_F32 ? 4 : 2;
   p.direct = p.planes == 1 && d.d % kTileK == 0 && d.ld_x % 8 == 0 && d.ld_w % 8 == 0 && aligned16(d.x) && aligned16(d.w);
   p.dp = up(d.d, kTileK);
-  p.n_pad = up(d.n, kTileN);
-  p.v_pad = up(d.v, kTileM);
+  p.n_pad = up(d.n, Big::BN);
+  p.v_pad = up(d.v, Big::BM);
   p.groups = (int)((d.n + kCountRows - 1) / kCountRows);
-  const int64_t ntiles = p.n_pad / kTileN, vtiles = p.v_pad / kTileM;
-  auto splits = [](int64_t tiles, int64_t most) {      // about two workgroups a CU
-    int64_t s = (512 + tiles - 1) / tiles;
-    return (int)(s < 1 ? 1 : s > most ? (most < 1 ? 1 : most) : s);
-  };
   Carver c(workspace);
   p.bias2 = c.take<float>(p.v_pad);
   if (!p.direct) {
@@ -585,28 +680,36 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     p.wp = c.take<uint16_t>((size_t)p.planes * p.v_pad * p.dp);
   }
   if (!backward) {
-    p.lse_splits = splits(ntiles, vtiles);
+    p.lse_big = large_tiles(d.v, d.n, 1);
+    const int64_t bm = p.lse_big ? Big::BM : Small::BM, bn = p.lse_big ? Big::BN : Small::BN;
+    p.lse_splits = cut(up(d.n, bn) / bn, kCus * (p.lse_big ? 1 : 2), up(d.v, bm) / bm);
     p.part = c.take<int32_t>(p.groups);
     p.part_m = c.take<float>((size_t)p.lse_splits * p.n_pad);
     p.part_l = c.take<float>((size_t)p.lse_splits * p.n_pad);
     p.hit = c.take<float>(p.n_pad);
     p.sums = c.take<double>((d.n + 255) / 256);
   } else {
-    int64_t piece = d.piece > 0 ? up(d.piece, kTileM) : kPieceBytes / (p.n_pad * 2 * p.planes) / kTileM * kTileM;
-    if (piece < kTileM) piece = kTileM;
-    p.piece = piece < p.v_pad ? piece : p.v_pad;
-    const int64_t dtiles = (p.dp + kTileN - 1) / kTileN;
-    p.dx_splits = splits(ntiles * dtiles, p.piece / kTileK / 4);
-    p.dw_splits = splits(p.piece / kTileM * dtiles, p.n_pad / kTileK / 4);
-    p.db_slices = splits((p.piece + 255) / 256, (d.n + 63) / 64);
+    const int64_t v64 = up(d.v, kTileK);
+    int64_t piece = d.piece > 0 ? up(d.piece, kTileK) : kPieceBytes / (p.n_pad * 2 * p.planes) / Big::BM * Big::BM;
+    if (piece < Small::BM) piece = Small::BM;
+    p.piece = piece < v64 ? piece : v64;
+    p.dl_big = large_tiles(p.piece, d.n, 1);
+    const int64_t kx = p.piece / kTileK / 4, kw = p.n_pad / kTileK / 4;
+    p.dx_big = large_tiles(d.n, p.dp, kx);
+    p.dw_big = large_tiles(p.piece, p.dp, kw);
+    auto tiles = [&](int64_t m, int64_t n, bool big) { return big ? tiles_of(m, n, Big::BM, Big::BN) : tiles_of(m, n, Small::BM, Small::BN); };
+    p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus * (p.dx_big ? 1 : 2), kx);
+    p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus * (p.dw_big ? 1 : 2), kw);
+    p.dx_final = p.dx_splits == 1 && p.piece >= d.v;
+    p.dw_final = p.dw_splits == 1;
     p.top_parts = (int)(d.n < 256 * 256 ? (d.n + 255) / 256 : 256);
     p.top = c.take<float>(p.top_parts);
     p.scale = c.take<float>(1);
     p.weight = c.take<float>(p.n_pad);
     p.dl = c.take<uint16_t>((size_t)p.planes * p.n_pad * p.piece);
-    p.accx = c.take<float>((size_t)p.dx_splits * p.n_pad * p.dp);
-    p.accw = c.take<float>((size_t)p.dw_splits * p.piece * p.dp);
-    p.accb = c.take<float>((size_t)p.db_slices * p.piece);
+    if (!p.dx_final) p.accx = c.take<float>((size_t)p.dx_splits * p.n_pad * p.dp);
+    p.accw = c.take<float>((size_t)(p.dw_final && d.dw ? 0 : p.dw_splits) * p.piece * p.dp);
+    p.accb = c.take<float>((size_t)p.dw_splits * p.piece);
   }
   p.bytes = c.off;
   return p;
@@ -625,7 +728,7 @@ int check(const r3d_linear_ce_t *d) {
 
 template <class S, class T, int kPlanes>
 void pack(const PackArgs &a, int64_t rows, hipStream_t st) {
-  hipLaunchKernelGGL((k_ce_pack<S, T, kPlanes>), dim3(blocks_for(rows * a.ld_out, 1024, 8192)), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((k_ce_pack<S, T, kPlanes>), dim3(blocks_for(rows * a.ld_out, 2048, 8192)), dim3(256), 0, st, a);
 }
 
 // The operands as the products take them: in place, or packed into the workspace.
@@ -637,10 +740,18 @@ void operands(const r3d_linear_ce_t &d, const Plan &p, const Counted *counted, h
     w = Operand{d.w, d.ld_w, 0, nullptr};
     return;
   }
-  pack<S, T, kPlanes>(PackArgs{d.x, p.xp, d.ld_x, d.n, d.d, p.dp, p.n_pad * p.dp, d.idx, counted}, d.n, st);
-  pack<S, T, kPlanes>(PackArgs{d.w, p.wp, d.ld_w, d.v, d.d, p.dp, p.v_pad * p.dp, nullptr, nullptr}, d.v, st);
+  const int size = (int)sizeof(S);
+  pack<S, T, kPlanes>(PackArgs{d.x, p.xp, d.ld_x, d.n, d.d, p.dp, p.n_pad * p.dp, d.idx, counted, aligned16(d.x) && d.ld_x * size % 16 == 0}, d.n, st);
+  pack<S, T, kPlanes>(PackArgs{d.w, p.wp, d.ld_w, d.v, d.d, p.dp, p.v_pad * p.dp, nullptr, nullptr, aligned16(d.w) && d.ld_w * size % 16 == 0}, d.v, st);
   x = Operand{p.xp, p.dp, p.n_pad * p.dp, nullptr};
   w = Operand{p.wp, p.dp, p.v_pad * p.dp, nullptr};
+}
+
+template <class T, class S>
+void lse(LseArgs a, const Plan &p, int64_t n, int64_t v, hipStream_t st) {
+  a.ntiles = up(n, S::BN) / S::BN;
+  a.vtiles = (int)(up(v, S::BM) / S::BM);
+  hipLaunchKernelGGL((k_ce_lse<T, S>), dim3((unsigned)(a.ntiles * p.lse_splits)), dim3(S::threads), 0, st, a);
 }
 
 template <class S, class T, int kPlanes>
@@ -654,7 +765,6 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   la.p.planes = kPlanes;
   la.v = d.v;
   la.kb = p.dp / kTileK;
-  la.vtiles = (int)(p.v_pad / kTileM);
   la.splits = p.lse_splits;
   la.bias2 = p.bias2;
   la.tgt = d.tgt;
@@ -663,13 +773,36 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   la.part_l = p.part_l;
   la.hit = p.hit;
   la.n_pad = p.n_pad;
-  hipLaunchKernelGGL(k_ce_lse<T>, dim3((unsigned)(p.n_pad / kTileN * p.lse_splits)), dim3(kMmaThreads), 0, st, la);
+  if (p.lse_big) lse<T, Big>(la, p, d.n, d.v, st);
+  else lse<T, Small>(la, p, d.n, d.v, st);
   CombineArgs ca{p.part_m, p.part_l, p.hit, d.tgt, d.place, counted, d.lse2, d.reduction == R3D_CE_NONE ? d.loss : nullptr, d.loss, p.sums, d.n, p.n_pad,
                  p.lse_splits};
   const int blocks = (int)((d.n + 255) / 256);
   hipLaunchKernelGGL(k_ce_join, dim3(blocks), dim3(256), 0, st, ca);
   if (d.reduction != R3D_CE_NONE)
     hipLaunchKernelGGL(k_ce_mean, dim3(1), dim3(256), 0, st, p.sums, (int64_t)blocks, counted, d.reduction == R3D_CE_MEAN ? 1 : 0, d.loss);
+}
+
+template <class T, class S, int kPlanes>
+void dl_piece(DlArgs a, int64_t n, hipStream_t st) {
+  a.ntiles = up(n, S::BN) / S::BN;
+  a.vtiles = (int)(up(a.width, S::BM) / S::BM);
+  hipLaunchKernelGGL((k_ce_dl<T, S, kPlanes>), dim3((unsigned)(a.ntiles * a.vtiles)), dim3(S::threads), 0, st, a);
+}
+
+template <class V, class T, class S, Lies LA>
+void out_product(OutArgs a, int64_t m, int64_t n, hipStream_t st) {
+  a.mtiles = (int)(up(m, S::BM) / S::BM);
+  a.ntiles = (int)(up(n, S::BN) / S::BN);
+  hipLaunchKernelGGL((k_ce_out<V, T, S, LA>), dim3((unsigned)((int64_t)a.mtiles * a.ntiles * a.splits)), dim3(S::threads), 0, st, a);
+}
+
+template <class V>
+void finish(const FinishArgs &a, hipStream_t st) {
+  const bool four = a.width % 4 == 0 && a.ld % 4 == 0 && a.ld_out % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(V))) == 0;
+  const int64_t threads = a.rows * a.width / (four ? 4 : 1);
+  if (four) hipLaunchKernelGGL((k_ce_finish<V, 4>), dim3(blocks_for(threads, 256, 8192)), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((k_ce_finish<V, 1>), dim3(blocks_for(threads, 256, 8192)), dim3(256), 0, st, a);
 }
 
 template <class S, class T, int kPlanes>
@@ -681,19 +814,17 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
                      WeightArgs{d.grad, p.top, each ? 1 : 0, p.top_parts, d.idx, counted, p.scale, p.weight, p.n_pad});
   Operand x, w;
   operands<S, T, kPlanes>(d, p, counted, st, x, w);
-  const float held = d.type == R3D_T_F16 ? 32768.0f : 1.0f;
-  const int64_t dtiles = (p.dp + kTileN - 1) / kTileN;
-  for (int64_t v0 = 0; v0 < p.v_pad; v0 += p.piece) {
-    const int64_t wide_v = p.piece < p.v_pad - v0 ? p.piece : p.v_pad - v0;      // (a multiple of 128)
-    const int64_t real_v = wide_v < d.v - v0 ? wide_v : d.v - v0;
+  const float held = d.type == R3D_T_F16 ? 32768.0f : 1.0f, unheld = 1.0f / held;
+  for (int64_t v0 = 0; v0 < d.v; v0 += p.piece) {
+    const int64_t real_v = p.piece < d.v - v0 ? p.piece : d.v - v0, width = up(real_v, kTileK);
     DlArgs da{};
     da.p = Product{w, x, kPlanes};
     da.v = d.v;
     da.kb = p.dp / kTileK;
     da.piece0 = v0;
-    da.piece = p.piece;
     da.dl_plane = p.n_pad * p.piece;
-    da.vtiles = (int)(wide_v / kTileM);
+    da.n_pad = p.n_pad;
+    da.width = (int)width;
     da.held = held;
     da.bias2 = p.bias2;
     da.lse2 = d.lse2;
@@ -701,61 +832,64 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     da.tgt = d.tgt;
     da.counted = counted;
     da.dl = p.dl;
-    hipLaunchKernelGGL((k_ce_dl<T, kPlanes>), dim3((unsigned)(p.n_pad / kTileN * da.vtiles)), dim3(kMmaThreads), 0, st, da);
-    const Operand dl{p.dl, p.piece, p.n_pad * p.piece, nullptr};
+    if (p.dl_big) dl_piece<T, Big, kPlanes>(da, d.n, st);
+    else dl_piece<T, Small, kPlanes>(da, d.n, st);
+    const Operand dl{p.dl, p.n_pad, p.n_pad * p.piece, nullptr};
     if (d.dx) {
       Operand wv = w;      // the rows of this piece
       wv.p = static_cast<const char *>(w.p) + v0 * w.ld * 2;
       OutArgs oa{};
       oa.p = Product{dl, wv, kPlanes};
-      oa.n = p.dp;
-      oa.k_rows_b = real_v;
-      oa.cols_b = p.dp;
-      oa.kb = wide_v / kTileK;
-      oa.m_counted = 1;
-      oa.mtiles = (int)(p.n_pad / kTileM);
-      oa.ntiles = (int)dtiles;
+      oa.n = p.dx_final ? d.d : p.dp;
+      oa.kb = width / kTileK;
+      oa.limit_b = p.dp;
+      oa.rows_b = real_v;
+      oa.points = 1;
       oa.splits = p.dx_splits;
       oa.add = v0 > 0;
       oa.counted = counted;
       oa.out = p.accx;
-      oa.ld = p.dp;
+      oa.ld = p.dx_final ? d.d : p.dp;
       oa.split_stride = p.n_pad * p.dp;
-      hipLaunchKernelGGL((k_ce_out<T, false>), dim3((unsigned)(oa.mtiles * dtiles * oa.splits)), dim3(kMmaThreads), 0, st, oa);
+      oa.final_out = p.dx_final ? d.dx : nullptr;
+      oa.idx = d.idx;
+      oa.scale = p.scale;
+      oa.unheld = unheld;
+      if (p.dx_big) out_product<S, T, Big, Lies::PiecesRows>(oa, d.n, p.dp, st);
+      else out_product<S, T, Small, Lies::PiecesRows>(oa, d.n, p.dp, st);
     }
-    if (d.dw) {
+    if (d.dw || d.db) {
+      const bool straight = p.dw_final && d.dw;
       OutArgs oa{};
       oa.p = Product{dl, x, kPlanes};
-      oa.m = wide_v;
-      oa.n = p.dp;
-      oa.k_rows_a = p.n_pad;
-      oa.k_counted = 1;
-      oa.cols_a = p.piece;
-      oa.cols_b = p.dp;
-      oa.mtiles = (int)(wide_v / kTileM);
-      oa.ntiles = (int)dtiles;
+      oa.m = straight ? real_v : width;
+      oa.n = straight ? d.d : p.dp;
+      oa.limit_a = width;
+      oa.limit_b = p.dp;
+      oa.points = 2;
       oa.splits = p.dw_splits;
       oa.counted = counted;
       oa.out = p.accw;
-      oa.ld = p.dp;
+      oa.ld = straight ? d.d : p.dp;
       oa.split_stride = p.piece * p.dp;
-      hipLaunchKernelGGL((k_ce_out<T, true>), dim3((unsigned)(oa.mtiles * dtiles * oa.splits)), dim3(kMmaThreads), 0, st, oa);
-      FinishArgs fa{p.accw, p.dp, p.piece * p.dp, real_v, d.d, d.d, p.dw_splits, 1.0f / held, nullptr, p.scale,
-                    static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes};
-      hipLaunchKernelGGL(k_ce_finish<S>, dim3(blocks_for(real_v * d.d, 1024, 8192)), dim3(256), 0, st, fa);
-    }
-    if (d.db) {
-      hipLaunchKernelGGL((k_ce_db<T, kPlanes>), dim3((unsigned)((wide_v + 255) / 256), p.db_slices), dim3(256), 0, st,
-                         static_cast<const T *>(p.dl), p.piece, p.n_pad * p.piece, counted, p.db_slices, p.accb);
-      FinishArgs fa{p.accb, 1, p.piece, real_v, 1, 1, p.db_slices, 1.0f / held, nullptr, p.scale,
-                    static_cast<char *>(d.db) + v0 * p.type_bytes};
-      hipLaunchKernelGGL(k_ce_finish<S>, dim3(blocks_for(real_v, 256, 8192)), dim3(256), 0, st, fa);
+      oa.final_out = straight ? static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes : nullptr;
+      oa.scale = p.scale;
+      oa.unheld = unheld;
+      oa.row_sum = d.db ? p.accb : nullptr;
+      oa.sum_stride = p.piece;
+      if (p.dw_big) out_product<S, T, Big, Lies::PiecesCols>(oa, width, p.dp, st);
+      else out_product<S, T, Small, Lies::PiecesCols>(oa, width, p.dp, st);
+      if (d.dw && !straight)
+        finish<S>(FinishArgs{p.accw, p.dp, p.piece * p.dp, real_v, d.d, d.d, p.dw_splits, unheld, nullptr, p.scale,
+                             static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes}, st);
+      if (d.db)
+        finish<S>(FinishArgs{p.accb, 1, p.piece, real_v, 1, 1, p.dw_splits, unheld, nullptr, p.scale, static_cast<char *>(d.db) + v0 * p.type_bytes}, st);
     }
   }
-  if (d.dx) {
-    FinishArgs fa{p.accx, p.dp, p.n_pad * p.dp, d.n, d.d, d.d, p.dx_splits, 1.0f / held, d.place, p.scale, d.dx};
-    hipLaunchKernelGGL(k_ce_finish<S>, dim3(blocks_for(d.n * d.d, 1024, 8192)), dim3(256), 0, st, fa);
-  }
+  if (d.dx && p.dx_final)
+    hipLaunchKernelGGL(k_ce_zero<S>, dim3(blocks_for(d.n, 4, 2048)), dim3(256), 0, st, static_cast<S *>(d.dx), d.n, d.d, d.place);
+  else if (d.dx)
+    finish<S>(FinishArgs{p.accx, p.dp, p.n_pad * p.dp, d.n, d.d, d.d, p.dx_splits, unheld, d.place, p.scale, d.dx}, st);
 }
 }  // namespace
 
