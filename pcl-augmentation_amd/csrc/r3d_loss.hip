@@ -208,7 +208,7 @@ struct LseArgs {
 // joined once at the end.
 template <class T, class S>
 __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
-  __shared__ __attribute__((aligned(128))) T lds[2 * S::buffer];
+  __shared__ __attribute__((aligned(128))) T lds[kBuffers * S::buffer];
   const int nc = a.counted->n;
   const int64_t id = xcd_order(blockIdx.x, gridDim.x);
   const int split = (int)(id / a.ntiles);
@@ -228,20 +228,21 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
   Stream<T, S, Lies::Rows, Lies::Rows> st;
   st.a = a.p.a;
   st.b = a.p.b;
-  st.rows_a = st.rows_b = 0;
-  st.range(0, a.kb, a.p.planes);
+  st.rows_b = 0;
   st.lb.tile(st.b, n0, nc);
   st.la.tile(st.a, (int64_t)vt0 * S::BM, a.v);
-  st.issue(lds, 0);
-  __syncthreads();
+  int ahead = vt0;      // the tile that is being loaded
+  auto more = [&] {
+    if (++ahead >= vt1) return false;
+    st.la.tile(st.a, (int64_t)ahead * S::BM, a.v);
+    return true;
+  };
+  if (vt1 > vt0) st.begin(lds, 0, (int)a.kb, a.p.planes, more);
   for (int vt = vt0; vt < vt1; ++vt) {
     f32x16 acc[S::FM][S::FN];
     float none[S::FM];
     clear(acc);
-    st.template run<false>(lds, acc, none, false, [&] {
-      if (vt + 1 < vt1) st.la.tile(st.a, (int64_t)(vt + 1) * S::BM, a.v);
-      return vt + 1 < vt1;
-    });
+    st.template run<false>(lds, acc, none, false, more);
 #pragma unroll
     for (int i = 0; i < S::FM; ++i) {
       const int vb = vt * S::BM + (wm * S::FM + i) * 32;
@@ -271,6 +272,7 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
       }
     }
   }
+  st.end();
   // a logit that is NaN leaves the maximum as it was and the sum NaN
   float *s_m = reinterpret_cast<float *>(lds), *s_l = s_m + S::WM * S::BN;
 #pragma unroll
@@ -406,7 +408,7 @@ struct DlArgs {
 // makes pieces of 8, and 32 lanes write 512 contiguous bytes.
 template <class T, class S, int kPlanes>
 __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
-  __shared__ __attribute__((aligned(128))) T lds[2 * S::buffer];
+  __shared__ __attribute__((aligned(128))) T lds[kBuffers * S::buffer];
   const int nc = a.counted->n;
   int64_t vt, nt;
   tile_of(xcd_order(blockIdx.x, gridDim.x), a.vtiles, a.ntiles, vt, nt);
@@ -420,13 +422,13 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
     Stream<T, S, Lies::Rows, Lies::Rows> st;
     st.a = a.p.a;
     st.b = a.p.b;
-    st.rows_a = st.rows_b = 0;
-    st.range(0, a.kb, a.p.planes);
+    st.rows_b = 0;
     st.la.tile(st.a, a.piece0 + vt * S::BM, a.v);
     st.lb.tile(st.b, n0, nc);
-    st.issue(lds, 0);
-    __syncthreads();
-    st.template run<false>(lds, acc, none, false, [] { return false; });
+    auto more = [] { return false; };
+    st.begin(lds, 0, (int)a.kb, a.p.planes, more);
+    st.template run<false>(lds, acc, none, false, more);
+    st.end();
   }
   T *dl = static_cast<T *>(a.dl);
 #pragma unroll
@@ -501,7 +503,7 @@ struct OutArgs {
 // workspace or, where nothing is left to add, to the result.
 template <class V, class T, class S, Lies LA>
 __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
-  __shared__ __attribute__((aligned(128))) T lds[2 * S::buffer];
+  __shared__ __attribute__((aligned(128))) T lds[kBuffers * S::buffer];
   const int nc = a.counted->n;
   const int64_t id = xcd_order(blockIdx.x, gridDim.x), tiles = (int64_t)a.mtiles * a.ntiles;
   const int split = (int)(id / tiles);
@@ -523,14 +525,13 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
     Stream<T, S, LA, Lies::Cols> st;
     st.a = a.p.a;
     st.b = a.p.b;
-    st.rows_a = 0;
-    st.rows_b = a.points == 2 ? nc : a.rows_b;
+    st.rows_b = (int)(a.points == 2 ? nc : a.rows_b);
     st.la.tile(st.a, m0, a.points == 1 ? nc : a.limit_a);
     st.lb.tile(st.b, n0, a.limit_b);
-    st.range(kb0, kb1, a.p.planes);
-    st.issue(lds, 0);
-    __syncthreads();
-    st.template run<kSums>(lds, acc, row_sum, sums, [] { return false; });
+    auto more = [] { return false; };
+    st.begin(lds, (int)kb0, (int)kb1, a.p.planes, more);
+    st.template run<kSums>(lds, acc, row_sum, sums, more);
+    st.end();
   }
   const float scale = a.final_out ? *a.scale * a.unheld : 1.0f;
 #pragma unroll
@@ -617,6 +618,7 @@ __global__ __launch_bounds__(256) void k_ce_finish(FinishArgs a) {
 // ---- host ------------------------------------------------------------------------------------------------------------------
 constexpr int64_t kPieceBytes = 256ll << 20;      // what a piece's dl may take: the last-level cache's size
 constexpr int kCus = 256;
+constexpr int kPadK = 64;      // operands are padded to whole cache lines along k
 
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t tiles_of(int64_t m, int64_t n, int64_t bm, int64_t bn) { return (up(m, bm) / bm) * (up(n, bn) / bn); }
@@ -668,8 +670,8 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   Plan p{};
   p.planes = d.type == R3D_T_F32 ? 3 : 1;
   p.type_bytes = d.type == R3D_T_F32 ? 4 : 2;
-  p.direct = p.planes == 1 && d.d % kTileK == 0 && d.ld_x % 8 == 0 && d.ld_w % 8 == 0 && aligned16(d.x) && aligned16(d.w);
-  p.dp = up(d.d, kTileK);
+  p.direct = p.planes == 1 && d.d % kPadK == 0 && d.ld_x % 8 == 0 && d.ld_w % 8 == 0 && aligned16(d.x) && aligned16(d.w);
+  p.dp = up(d.d, kPadK);
   p.n_pad = up(d.n, Big::BN);
   p.v_pad = up(d.v, Big::BM);
   p.groups = (int)((d.n + kCountRows - 1) / kCountRows);
@@ -689,12 +691,12 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     p.hit = c.take<float>(p.n_pad);
     p.sums = c.take<double>((d.n + 255) / 256);
   } else {
-    const int64_t v64 = up(d.v, kTileK);
-    int64_t piece = d.piece > 0 ? up(d.piece, kTileK) : kPieceBytes / (p.n_pad * 2 * p.planes) / Big::BM * Big::BM;
+    const int64_t v64 = up(d.v, kPadK);
+    int64_t piece = d.piece > 0 ? up(d.piece, kPadK) : kPieceBytes / (p.n_pad * 2 * p.planes) / Big::BM * Big::BM;
     if (piece < Small::BM) piece = Small::BM;
     p.piece = piece < v64 ? piece : v64;
     p.dl_big = large_tiles(p.piece, d.n, 1);
-    const int64_t kx = p.piece / kTileK / 4, kw = p.n_pad / kTileK / 4;
+    const int64_t kx = p.piece / 256, kw = p.n_pad / 256;
     p.dx_big = large_tiles(d.n, p.dp, kx);
     p.dw_big = large_tiles(p.piece, p.dp, kw);
     auto tiles = [&](int64_t m, int64_t n, bool big) { return big ? tiles_of(m, n, Big::BM, Big::BN) : tiles_of(m, n, Small::BM, Small::BN); };
@@ -718,7 +720,7 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
 int check(const r3d_linear_ce_t *d) {
   if (!d) return fail(R3D_E_ARG, "linear_ce: null descriptor");
   if (d->n <= 0 || d->v <= 0 || d->d <= 0 || d->n > INT32_MAX - 1024 || d->v > INT32_MAX - 1024 || d->d > (1 << 20) || d->ld_x < d->d || d->ld_w < d->d ||
-      d->piece < 0)
+      d->ld_x > INT32_MAX || d->ld_w > INT32_MAX || d->piece < 0)
     return fail(R3D_E_ARG, "linear_ce: bad size");
   if (d->type != R3D_T_F32 && d->type != R3D_T_BF16 && d->type != R3D_T_F16) return fail(R3D_E_ARG, "linear_ce: type");
   if (d->target_type != R3D_T_I32 && d->target_type != R3D_T_I64) return fail(R3D_E_ARG, "linear_ce: type of the targets");
@@ -816,7 +818,7 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   operands<S, T, kPlanes>(d, p, counted, st, x, w);
   const float held = d.type == R3D_T_F16 ? 32768.0f : 1.0f, unheld = 1.0f / held;
   for (int64_t v0 = 0; v0 < d.v; v0 += p.piece) {
-    const int64_t real_v = p.piece < d.v - v0 ? p.piece : d.v - v0, width = up(real_v, kTileK);
+    const int64_t real_v = p.piece < d.v - v0 ? p.piece : d.v - v0, width = up(real_v, kPadK);
     DlArgs da{};
     da.p = Product{w, x, kPlanes};
     da.v = d.v;

@@ -1,6 +1,6 @@
 // Matrix products on the matrix cores (gfx950), for the fused kernels of r3d_loss.hip.
 //
-// C[m][n] = sum_k A(m,k) B(n,k) in tiles of BM x BN x 64, every wave FM x FN blocks of v_mfma_f32_32x32x16.  How an operand lies:
+// C[m][n] = sum_k A(m,k) B(n,k) in tiles of BM x BN x 32, every wave FM x FN blocks of v_mfma_f32_32x32x16.  How an operand lies:
 //   Rows    A[m][k], k contiguous
 //   Cols    A[k][m], m contiguous
 //   Pieces  in pieces of 8 values, piece-major: value (r, c) at ((c / 8) * rows + r) * 8 + c % 8 -- what a product that is an
@@ -15,7 +15,9 @@
 
 namespace r3d {
 
-constexpr int kTileK = 64;
+constexpr int kTileK = 32;      // k of a block: what one barrier is for
+constexpr int kAhead = 3;       // blocks on their way to LDS beside the one that is multiplied (a block takes 0.4 us, HBM up to 1)
+constexpr int kBuffers = kAhead + 1;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // Tile and waves.  A wave's share of 128 x 64 reads 0.75 of the 128 bytes a clock that LDS gives while the matrix cores are
@@ -50,40 +52,43 @@ struct Operand {
   const int32_t *idx;
 };
 
-typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) void lds_void;
 
-__device__ __forceinline__ void load_lds16(const void *g, void *lds_wave_base) {
-  __builtin_amdgcn_global_load_lds((global_void *)g, (lds_void *)lds_wave_base, 16, 0, 0);
+// 16 bytes a lane from `g` to LDS, lanes in one line from the wave's base `to`.  Written out, because the compiler waits for all
+// of the builtin's loads before every ds_read_b64_tr_b16 that follows, whichever buffer it reads; nothing but LDS is written, and
+// wait_loads() stands between a load and the reads of what it brought.  (One wait state between m0 and its use.)
+__device__ __forceinline__ void load_lds16(const void *g, unsigned to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(g) : "m0", "memory");
 }
 
-// A thread's part of an operand tile of R rows (or columns) x 64 k: `per` pieces of 16 bytes, piece number i * threads + thread.
+// A thread's part of an operand tile of R rows (or columns) x kTileK: `per` pieces of 16 bytes, piece number i * threads + thread,
+// from pointers that move from k-block to k-block.
 template <class T, Lies L, int R, int kThreads>
 struct Loader {
   static constexpr int per = R * kTileK / 8 / kThreads;
-  const T *at[per];      // Rows, Pieces: where the thread's pieces of the current tile begin
-  int64_t row[per];      // Cols: rows of the next k-block, looked up one block ahead
-  int col;
+  static constexpr int row_lanes = R / 8, rows_wave = 64 / row_lanes;      // Cols: lanes to a row, rows to a wave's load
+  const T *at[per];
+  int col;      // Cols: first column of the thread's pieces
 
-  // first: first row (Rows, PiecesRows) or column of the tile; limit: how many there are.  What lies behind is read from the last
-  // one, any finite or infinite values: its results are not used.
+  // The tile's first k-block.  first: first row (Rows, PiecesRows) or column of the tile; limit: how many there are.  What lies
+  // behind is read from the last one, whatever it holds: its results are not used.
   __device__ __forceinline__ void tile(const Operand &o, int64_t first, int64_t limit) {
 #pragma unroll
     for (int i = 0; i < per; ++i) {
       const int c = i * kThreads + threadIdx.x;
       if constexpr (L == Lies::Rows) {
-        const int r = c >> 3;
+        const int r = c >> 2;
         int64_t n = first + r;
         n = n < limit ? n : limit - 1;
         if (o.idx) n = o.idx[n];
-        at[i] = static_cast<const T *>(o.p) + n * o.ld + (((c & 7) ^ ((r >> 1) & 7)) << 3);
+        at[i] = static_cast<const T *>(o.p) + n * o.ld + (((c & 3) ^ ((r >> 2) & 3)) << 3);
       } else if constexpr (L == Lies::PiecesRows) {
-        const int r = c % R, q = c / R;      // LDS: [8 pieces of k][R rows]
+        const int r = c % R, q = c / R;      // LDS: [4 pieces of k][R rows]
         int64_t n = first + r;
         n = n < limit ? n : limit - 1;
         at[i] = static_cast<const T *>(o.p) + (q * o.ld + n) * 8;
       } else if constexpr (L == Lies::PiecesCols) {
-        const int k = c & 63, q = c >> 6;    // LDS: [R / 8 pieces of m][64 k], k in fours at k ^ 4 (q & 3)
+        const int k = c & 31, q = c >> 5;    // LDS: [R / 8 pieces of m][32 k], k in fours at k ^ 4 (q & 3)
         int64_t p = first / 8 + q;
         p = p < limit / 8 ? p : limit / 8 - 1;
         at[i] = static_cast<const T *>(o.p) + (p * o.ld + (k ^ ((q & 3) << 2))) * 8;
@@ -95,27 +100,42 @@ struct Loader {
       col = (int)(m + 8 <= limit ? m : limit - 8);
     }
   }
-  // Cols: the rows of k-block kb.
-  __device__ __forceinline__ void look(const Operand &o, int64_t kb, int64_t rows) {
+  // Elements from one k-block to the next.
+  static __device__ __forceinline__ int64_t step(const Operand &o) {
+    return L == Lies::Rows ? kTileK : L == Lies::PiecesRows ? (kTileK / 8) * o.ld * 8 : L == Lies::PiecesCols ? kTileK * 8 : 0;
+  }
+  __device__ __forceinline__ void move(int64_t elements) {
+    if constexpr (L != Lies::Cols) {
+#pragma unroll
+      for (int i = 0; i < per; ++i) at[i] += elements;
+    }
+  }
+  // Cols: the rows of k-block kb.  Their numbers come by scalar loads -- a vector load would have to wait for every load to LDS
+  // that was issued before it.
+  __device__ __forceinline__ void look(const Operand &o, int kb, int rows, int64_t plane) {
     if constexpr (L == Lies::Cols) {
+      const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = (threadIdx.x & 63) / row_lanes;
+      const T *base = static_cast<const T *>(o.p) + plane;
 #pragma unroll
       for (int i = 0; i < per; ++i) {
-        int64_t r = kb * kTileK + (i * kThreads + threadIdx.x) / (R / 8);
-        r = r < rows ? r : rows - 1;
-        row[i] = o.idx ? o.idx[r] : r;
+        const int first = kb * kTileK + (i * (kThreads / 64) + wave) * rows_wave;
+        int row = first + mine < rows ? first + mine : rows - 1;
+        if (o.idx) {
+          const auto *idx = (const __attribute__((address_space(4))) int32_t *)o.idx;
+          int32_t n[rows_wave];
+#pragma unroll
+          for (int e = 0; e < rows_wave; ++e) n[e] = idx[first + e < rows ? first + e : rows - 1];
+          row = n[0];
+#pragma unroll
+          for (int e = 1; e < rows_wave; ++e) row = mine == e ? n[e] : row;
+        }
+        at[i] = base + ((uint64_t)(uint32_t)row * (uint32_t)o.ld + (uint32_t)col);
       }
     }
   }
-  __device__ __forceinline__ void issue(const Operand &o, T *lds, int64_t kb, int64_t plane) const {
-    const int wave = threadIdx.x >> 6;
+  __device__ __forceinline__ void issue(unsigned to) const {
 #pragma unroll
-    for (int i = 0; i < per; ++i) {
-      T *to = lds + (i * kThreads + wave * 64) * 8;
-      if constexpr (L == Lies::Rows) load_lds16(at[i] + plane + kb * kTileK, to);
-      else if constexpr (L == Lies::PiecesRows) load_lds16(at[i] + plane + kb * 8 * o.ld * 8, to);
-      else if constexpr (L == Lies::PiecesCols) load_lds16(at[i] + plane + kb * kTileK * 8, to);
-      else load_lds16(static_cast<const T *>(o.p) + plane + row[i] * o.ld + col, to);
-    }
+    for (int i = 0; i < per; ++i) load_lds16(at[i], to + i * kThreads * 16);
   }
 };
 
@@ -125,7 +145,7 @@ __device__ __forceinline__ typename Mma<T>::v8 fragment(const T *lds, int r0, in
   const int lane = threadIdx.x & 63;
   if constexpr (L == Lies::Rows || L == Lies::PiecesRows) {
     const int r = r0 + (lane & 31), q = kk * 2 + (lane >> 5);
-    const T *at = L == Lies::Rows ? lds + r * kTileK + ((q ^ ((r >> 1) & 7)) << 3) : lds + (q * R + r) * 8;
+    const T *at = L == Lies::Rows ? lds + r * kTileK + ((q ^ ((r >> 2) & 3)) << 3) : lds + (q * R + r) * 8;
     return *reinterpret_cast<const typename Mma<T>::v8 *>(at);
   } else {
     typedef short s4 __attribute__((ext_vector_type(4)));
@@ -136,8 +156,8 @@ __device__ __forceinline__ typename Mma<T>::v8 fragment(const T *lds, int r0, in
       lo_at = lds + k * R + ((q ^ ((k & 3) << 2)) << 3) + (c & 7);
       hi_at = lo_at + 4 * R;
     } else {
-      lo_at = lds + (q * 64 + (k ^ ((q & 3) << 2))) * 8 + (c & 7);
-      hi_at = lds + (q * 64 + ((k + 4) ^ ((q & 3) << 2))) * 8 + (c & 7);
+      lo_at = lds + (q * kTileK + (k ^ ((q & 3) << 2))) * 8 + (c & 7);
+      hi_at = lds + (q * kTileK + ((k + 4) ^ ((q & 3) << 2))) * 8 + (c & 7);
     }
     const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)lo_at);
     const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)hi_at);
@@ -156,60 +176,89 @@ __device__ __forceinline__ float sum8(typename Mma<T>::v8 v, float s) {
 constexpr int kPairs = 6;
 __device__ constexpr int kPlaneA[kPairs] = {0, 0, 1, 1, 0, 2}, kPlaneB[kPairs] = {0, 1, 0, 1, 2, 0};
 
-// A stream of k-blocks through two LDS buffers: the next block is on its way while the current one is multiplied.
+// Waits until at most `left` of the wave's loads are on their way, then for the other waves.
+template <int left>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(left) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// A stream of k-blocks through kBuffers LDS buffers: kAhead blocks are on their way while one is multiplied.  One barrier a
+// block: behind it the block is there for all waves, and all of them are done with the one before, whose buffer the next load
+// takes.  The stream goes on over the tiles of a workgroup (`more`): their loads do not wait for a tile's end.
 template <class T, class S, Lies LA, Lies LB>
 struct Stream {
   Operand a, b;
   Loader<T, LA, S::BM, S::threads> la;
   Loader<T, LB, S::BN, S::threads> lb;
-  int64_t rows_a, rows_b;      // rows of Cols operands
-  int64_t kb, kb0, kb1;
-  int pair, pairs, buf;
+  static constexpr int loads = Loader<T, LA, S::BM, S::threads>::per + Loader<T, LB, S::BN, S::threads>::per;
+  int rows_b;                  // rows of a Cols operand
+  int kb, kb0, kb1;
+  int pair, pairs, get, put;   // buffers: the next to multiply, the next to fill
+  bool dry;                    // nothing left to load
+  unsigned base;               // LDS address of the wave's part of buffer 0
 
-  __device__ __forceinline__ void range(int64_t first, int64_t end, int planes) {
-    kb0 = first;
+  // k-blocks [first, end) of every tile (at least one); the loaders hold the first tile.
+  template <class More>
+  __device__ __forceinline__ void begin(T *lds, int first, int end, int planes, More &&more) {
+    kb = kb0 = first;
     kb1 = end;
     pairs = planes == 3 ? kPairs : 1;
-    buf = 0;
-    rewind();
+    get = put = pair = 0;
+    dry = false;
+    base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_void *)lds + (threadIdx.x >> 6) * 1024);
+    la.move(first * la.step(a));
+    lb.move(first * lb.step(b));
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) issue(more);
   }
-  __device__ __forceinline__ void rewind() {
-    kb = kb0;
-    pair = 0;
-    la.look(a, kb, rows_a);
-    lb.look(b, kb, rows_b);
-  }
-  __device__ __forceinline__ void issue(T *lds, int to) {
-    la.issue(a, lds + to * S::buffer, kb, kPlaneA[pair] * a.plane);
-    lb.issue(b, lds + to * S::buffer + S::a_elems, kb, kPlaneB[pair] * b.plane);
-    if (++kb == kb1) {
-      kb = kb0;
-      ++pair;
+  // The next block on its way; at the end of a tile `more()` sets A's loader for the next one and says whether there is one.
+  // Without one the last block is loaded again: the count of loads on their way stays what wait_loads() takes it for.
+  template <class More>
+  __device__ __forceinline__ void issue(More &&more) {
+    lb.look(b, kb, rows_b, kPlaneB[pair] * b.plane);
+    const unsigned to = base + put * (S::buffer * (unsigned)sizeof(T));
+    la.issue(to);
+    lb.issue(to + S::a_elems * (unsigned)sizeof(T));
+    put = (put + 1) % kBuffers;
+    if (dry) return;
+    if (++kb < kb1) {
+      la.move(la.step(a));
+      lb.move(lb.step(b));
+      return;
     }
-    la.look(a, kb, rows_a);
-    lb.look(b, kb, rows_b);
+    const int was = pair;
+    if (++pair == pairs) {
+      pair = 0;
+      if (!more()) {
+        dry = true;
+        pair = was;
+        kb = kb1 - 1;
+        return;
+      }
+      la.move(kb0 * la.step(a));
+    } else {
+      la.move((kb0 + 1 - kb1) * la.step(a) + (kPlaneA[pair] - kPlaneA[was]) * a.plane);
+    }
+    lb.move((kb0 + 1 - kb1) * lb.step(b) + (kPlaneB[pair] - kPlaneB[was]) * b.plane);
+    kb = kb0;
   }
-  // acc += all k-blocks of the tile whose first block is in the current buffer; `next()` is called while the last block is
-  // multiplied and says whether there is another tile, whose loaders it has set.  kSums: row_sum += sums over k of A,
-  // where `sums`.
-  template <bool kSums, class Next>
-  __device__ __forceinline__ void run(T *lds, f32x16 (&acc)[S::FM][S::FN], float (&row_sum)[S::FM], bool sums, Next &&next) {
+  // acc += all k-blocks of a tile.  kSums: row_sum += sums over k of A, where `sums`.
+  template <bool kSums, class More>
+  __device__ __forceinline__ void run(T *lds, f32x16 (&acc)[S::FM][S::FN], float (&row_sum)[S::FM], bool sums, More &&more) {
     const int wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-    const int64_t steps = (kb1 - kb0) * pairs;
-    int at_pair = 0;
-    int64_t pair_end = kb1 - kb0;
-    for (int64_t s = 0; s < steps; ++s) {
+    const int steps = (kb1 - kb0) * pairs;
+    int at_pair = 0, pair_end = kb1 - kb0;
+    for (int s = 0; s < steps; ++s) {
       if (s == pair_end) {
         ++at_pair;
         pair_end += kb1 - kb0;
       }
-      if (s + 1 < steps) {
-        issue(lds, buf ^ 1);
-      } else if (next()) {
-        rewind();
-        issue(lds, buf ^ 1);
-      }
-      const T *pa = lds + buf * S::buffer, *pb = pa + S::a_elems;
+      wait_loads<(kAhead - 1) * loads>();
+      issue(more);
+      const T *pa = lds + get * S::buffer, *pb = pa + S::a_elems;
+      get = (get + 1) % kBuffers;
       typename Mma<T>::v8 fa[2][S::FM], fb[2][S::FN];
       auto read = [&](int kk, int into) {
 #pragma unroll
@@ -230,10 +279,10 @@ struct Stream {
           for (int i = 0; i < S::FM; ++i) row_sum[i] = sum8<T>(fa[kk & 1][i], row_sum[i]);
         }
       }
-      __syncthreads();
-      buf ^= 1;
     }
   }
+  // Before LDS is used for anything else, and before the workgroup ends: nothing on its way to it.
+  __device__ __forceinline__ void end() { wait_loads<0>(); }
 };
 
 template <int FM, int FN>
