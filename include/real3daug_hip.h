@@ -685,7 +685,7 @@ int r3d_rotary(const r3d_rotary_t *d, void *stream);
  * The forward call fills idx, place, tgt (int32 [n] each), lse2 (float [n]) and counted (16 bytes), which the backward call of
  * the same descriptor reads.  backward: grad = float [n] or
  * [1]; dx [n][d], dw [v][d], db [v] dense, of `type`, each nullable.  piece: classes whose logit gradients are held at a time
- * (0: as many as 256 MB take). */
+ * (0: as many as 512 MB take). */
 #define R3D_CE_NONE 0
 #define R3D_CE_SUM 1
 #define R3D_CE_MEAN 2

@@ -208,7 +208,7 @@ struct LseArgs {
 // joined once at the end.
 template <class T, class S>
 __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
-  __shared__ __attribute__((aligned(128))) T lds[kBuffers * S::buffer];
+  __shared__ __attribute__((aligned(128))) T lds[S::buffers * S::buffer];
   const int nc = a.counted->n;
   const int64_t id = xcd_order(blockIdx.x, gridDim.x);
   const int split = (int)(id / a.ntiles);
@@ -408,7 +408,7 @@ struct DlArgs {
 // makes pieces of 8, and 32 lanes write 512 contiguous bytes.
 template <class T, class S, int kPlanes>
 __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
-  __shared__ __attribute__((aligned(128))) T lds[kBuffers * S::buffer];
+  __shared__ __attribute__((aligned(128))) T lds[S::buffers * S::buffer];
   const int nc = a.counted->n;
   int64_t vt, nt;
   tile_of(xcd_order(blockIdx.x, gridDim.x), a.vtiles, a.ntiles, vt, nt);
@@ -503,7 +503,7 @@ struct OutArgs {
 // workspace or, where nothing is left to add, to the result.
 template <class V, class T, class S, Lies LA>
 __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
-  __shared__ __attribute__((aligned(128))) T lds[kBuffers * S::buffer];
+  __shared__ __attribute__((aligned(128))) T lds[S::buffers * S::buffer];
   const int nc = a.counted->n;
   const int64_t id = xcd_order(blockIdx.x, gridDim.x), tiles = (int64_t)a.mtiles * a.ntiles;
   const int split = (int)(id / tiles);
@@ -542,20 +542,27 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
       if (lane < 32 && row < m) a.row_sum[split * a.sum_stride + row] = s;
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int64_t row = m0 + (wm * S::FM + i) * 32 + mma_row(r);
-      if (row >= m) continue;
-      const int64_t to = a.final_out && a.idx ? a.idx[row] : row;
+    for (int j = 0; j < S::FN; ++j) {
+      const int64_t n = n0 + (wn * S::FN + j) * 32 + (lane & 31), row0 = m0 + (wm * S::FM + i) * 32;
+      if (n >= a.n) continue;
+      if (a.final_out) {
 #pragma unroll
-      for (int j = 0; j < S::FN; ++j) {
-        const int64_t n = n0 + (wn * S::FN + j) * 32 + (lane & 31);
-        if (n >= a.n) continue;
-        if (a.final_out) {
-          static_cast<V *>(a.final_out)[to * a.ld + n] = (V)(acc[i][j][r] * scale);
-        } else {
-          float *at = a.out + split * a.split_stride + row * a.ld + n;
-          *at = a.add ? *at + acc[i][j][r] : acc[i][j][r];
+        for (int r = 0; r < 16; ++r) {
+          const int64_t row = row0 + mma_row(r);
+          if (row < m) static_cast<V *>(a.final_out)[(a.idx ? a.idx[row] : row) * a.ld + n] = (V)(acc[i][j][r] * scale);
         }
+      } else {
+        float *at = a.out + split * a.split_stride + row0 * a.ld + n;
+        if (a.add) {      // (all loads before the first store: one at a time they are 128 latencies)
+          float old[16];
+#pragma unroll
+          for (int r = 0; r < 16; ++r) old[r] = row0 + mma_row(r) < m ? at[mma_row(r) * a.ld] : 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] += old[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (row0 + mma_row(r) < m) at[mma_row(r) * a.ld] = acc[i][j][r];
       }
     }
   }
@@ -616,7 +623,8 @@ __global__ __launch_bounds__(256) void k_ce_finish(FinishArgs a) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-constexpr int64_t kPieceBytes = 256ll << 20;      // what a piece's dl may take: the last-level cache's size
+// What a piece's dl may take.  8192 points x 161280 classes x 512: 8.8 ms with 64 MB, 7.1 with 256, 6.7 with 512, 6.4 with all 2.6 GB.
+constexpr int64_t kPieceBytes = 512ll << 20;
 constexpr int kCus = 256;
 constexpr int kPadK = 64;      // operands are padded to whole cache lines along k
 
@@ -684,7 +692,7 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   if (!backward) {
     p.lse_big = large_tiles(d.v, d.n, 1);
     const int64_t bm = p.lse_big ? Big::BM : Small::BM, bn = p.lse_big ? Big::BN : Small::BN;
-    p.lse_splits = cut(up(d.n, bn) / bn, kCus * (p.lse_big ? 1 : 2), up(d.v, bm) / bm);
+    p.lse_splits = cut(up(d.n, bn) / bn, kCus * (p.lse_big ? Big::per_cu : Small::per_cu), up(d.v, bm) / bm);
     p.part = c.take<int32_t>(p.groups);
     p.part_m = c.take<float>((size_t)p.lse_splits * p.n_pad);
     p.part_l = c.take<float>((size_t)p.lse_splits * p.n_pad);
@@ -695,13 +703,15 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     int64_t piece = d.piece > 0 ? up(d.piece, kPadK) : kPieceBytes / (p.n_pad * 2 * p.planes) / Big::BM * Big::BM;
     if (piece < Small::BM) piece = Small::BM;
     p.piece = piece < v64 ? piece : v64;
+    if (d.piece == 0) p.piece = up((v64 + (v64 + p.piece - 1) / p.piece - 1) / ((v64 + p.piece - 1) / p.piece), Big::BM);      // pieces of one size
+    if (p.piece > v64) p.piece = v64;
     p.dl_big = large_tiles(p.piece, d.n, 1);
     const int64_t kx = p.piece / 256, kw = p.n_pad / 256;
     p.dx_big = large_tiles(d.n, p.dp, kx);
     p.dw_big = large_tiles(p.piece, p.dp, kw);
     auto tiles = [&](int64_t m, int64_t n, bool big) { return big ? tiles_of(m, n, Big::BM, Big::BN) : tiles_of(m, n, Small::BM, Small::BN); };
-    p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus * (p.dx_big ? 1 : 2), kx);
-    p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus * (p.dw_big ? 1 : 2), kw);
+    p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus * (p.dx_big ? Big::per_cu : Small::per_cu), kx);
+    p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus * (p.dw_big ? Big::per_cu : Small::per_cu), kw);
     p.dx_final = p.dx_splits == 1 && p.piece >= d.v;
     p.dw_final = p.dw_splits == 1;
     p.top_parts = (int)(d.n < 256 * 256 ? (d.n + 255) / 256 : 256);

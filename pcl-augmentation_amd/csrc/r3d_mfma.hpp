@@ -16,19 +16,20 @@
 namespace r3d {
 
 constexpr int kTileK = 32;      // k of a block: what one barrier is for
-constexpr int kAhead = 3;       // blocks on their way to LDS beside the one that is multiplied (a block takes 0.4 us, HBM up to 1)
-constexpr int kBuffers = kAhead + 1;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // Tile and waves.  A wave's share of 128 x 64 reads 0.75 of the 128 bytes a clock that LDS gives while the matrix cores are
 // busy, one of 64 x 64 all of them; a tile of 256 x 256 takes 32 bytes a clock and CU out of L2, one of 128 x 128 64.
-template <int BM_, int BN_, int WM_, int WN_>
+// ahead: blocks on their way to LDS beside the one that is multiplied (a block takes 0.4 us, HBM up to 1).  256 x 128 with two
+// workgroups a CU, the one's products beside the other's exponentials, was no faster (1.56 ms against 1.47, 8192 x 161280 x 512).
+template <int BM_, int BN_, int WM_, int WN_, int ahead_, int per_cu_>
 struct Shape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, threads = 64 * WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
   static constexpr int a_elems = BM * kTileK, b_elems = BN * kTileK, buffer = a_elems + b_elems;
+  static constexpr int ahead = ahead_, buffers = ahead + 1, per_cu = per_cu_;
 };
-using Big = Shape<256, 256, 2, 4>;
-using Small = Shape<128, 128, 2, 2>;
+using Big = Shape<256, 256, 2, 4, 3, 1>;
+using Small = Shape<128, 128, 2, 2, 3, 2>;
 
 enum class Lies { Rows, Cols, PiecesRows, PiecesCols };
 
@@ -184,7 +185,7 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
 }
 
-// A stream of k-blocks through kBuffers LDS buffers: kAhead blocks are on their way while one is multiplied.  One barrier a
+// A stream of k-blocks through LDS buffers: S::ahead blocks are on their way while one is multiplied.  One barrier a
 // block: behind it the block is there for all waves, and all of them are done with the one before, whose buffer the next load
 // takes.  The stream goes on over the tiles of a workgroup (`more`): their loads do not wait for a tile's end.
 template <class T, class S, Lies LA, Lies LB>
@@ -211,7 +212,7 @@ struct Stream {
     la.move(first * la.step(a));
     lb.move(first * lb.step(b));
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) issue(more);
+    for (int i = 0; i < S::ahead; ++i) issue(more);
   }
   // The next block on its way; at the end of a tile `more()` sets A's loader for the next one and says whether there is one.
   // Without one the last block is loaded again: the count of loads on their way stays what wait_loads() takes it for.
@@ -221,7 +222,7 @@ struct Stream {
     const unsigned to = base + put * (S::buffer * (unsigned)sizeof(T));
     la.issue(to);
     lb.issue(to + S::a_elems * (unsigned)sizeof(T));
-    put = (put + 1) % kBuffers;
+    put = (put + 1) % S::buffers;
     if (dry) return;
     if (++kb < kb1) {
       la.move(la.step(a));
@@ -244,41 +245,51 @@ struct Stream {
     lb.move((kb0 + 1 - kb1) * lb.step(b) + (kPlaneB[pair] - kPlaneB[was]) * b.plane);
     kb = kb0;
   }
-  // acc += all k-blocks of a tile.  kSums: row_sum += sums over k of A, where `sums`.
+  // acc += all k-blocks of a tile.  kSums: row_sum += sums over k of A, where `sums`.  A fragment is read one k-step before it is
+  // multiplied, over the blocks' borders too: the reads after a barrier would else hold up the matrix cores of all waves at once.
   template <bool kSums, class More>
   __device__ __forceinline__ void run(T *lds, f32x16 (&acc)[S::FM][S::FN], float (&row_sum)[S::FM], bool sums, More &&more) {
     const int wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
     const int steps = (kb1 - kb0) * pairs;
     int at_pair = 0, pair_end = kb1 - kb0;
+    typename Mma<T>::v8 fa[2][S::FM], fb[2][S::FN];
+    auto read = [&](int kk, int into) {
+      const T *pa = lds + get * S::buffer, *pb = pa + S::a_elems;
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i) fa[into][i] = fragment<T, LA, S::BM>(pa, (wm * S::FM + i) * 32, kk);
+#pragma unroll
+      for (int j = 0; j < S::FN; ++j) fb[into][j] = fragment<T, LB, S::BN>(pb, (wn * S::FN + j) * 32, kk);
+    };
+    auto multiply = [&](int from) {
+#pragma unroll
+      for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) acc[i][j] = Mma<T>::mma(fa[from][i], fb[from][j], acc[i][j]);
+      if (kSums && sums && kPlaneB[at_pair] == 0) {      // (every plane of A once)
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i) row_sum[i] = sum8<T>(fa[from][i], row_sum[i]);
+      }
+    };
+    static_assert(kTileK == 32, "two k-steps a block");
+    wait_loads<(S::ahead - 1) * loads>();
+    read(0, 0);
     for (int s = 0; s < steps; ++s) {
       if (s == pair_end) {
         ++at_pair;
         pair_end += kb1 - kb0;
       }
-      wait_loads<(kAhead - 1) * loads>();
+      read(1, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(0);
+      __builtin_amdgcn_sched_barrier(0);
+      // the next block is there, and all waves are done with the one before this one: its buffer is filled
+      wait_loads<(S::ahead - 2) * loads>();
       issue(more);
-      const T *pa = lds + get * S::buffer, *pb = pa + S::a_elems;
-      get = (get + 1) % kBuffers;
-      typename Mma<T>::v8 fa[2][S::FM], fb[2][S::FN];
-      auto read = [&](int kk, int into) {
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i) fa[into][i] = fragment<T, LA, S::BM>(pa, (wm * S::FM + i) * 32, kk);
-#pragma unroll
-        for (int j = 0; j < S::FN; ++j) fb[into][j] = fragment<T, LB, S::BN>(pb, (wn * S::FN + j) * 32, kk);
-      };
-      read(0, 0);
-#pragma unroll
-      for (int kk = 0; kk < kTileK / 16; ++kk) {
-        if (kk + 1 < kTileK / 16) read(kk + 1, (kk + 1) & 1);
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i)
-#pragma unroll
-          for (int j = 0; j < S::FN; ++j) acc[i][j] = Mma<T>::mma(fa[kk & 1][i], fb[kk & 1][j], acc[i][j]);
-        if (kSums && sums && kPlaneB[at_pair] == 0) {      // (every plane of A once)
-#pragma unroll
-          for (int i = 0; i < S::FM; ++i) row_sum[i] = sum8<T>(fa[kk & 1][i], row_sum[i]);
-        }
-      }
+      get = (get + 1) % S::buffers;
+      if (s + 1 < steps) read(0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   // Before LDS is used for anything else, and before the workgroup ends: nothing on its way to it.
