@@ -15,19 +15,12 @@
 // each, all 24) and multiplied as the six products that reach beyond 2^-24: 2.5 PFLOP/s of bfloat16 in six are more than the
 // 0.16 of float32.
 #include "r3d_host.hpp"
-#include "r3d_mfma.hpp"
+#include "r3d_loss.hpp"
 
 #include <cmath>
 
 namespace {
 using namespace r3d;
-
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-struct Counted {      // the points that count, on the device
-  int32_t n;          // how many
-  float share;        // 1 / n for a mean (0 where none counts), 1 else
-  float pad[2];
-};
 
 template <class T>
 __device__ __forceinline__ float wide(T v) { return (float)v; }
@@ -122,16 +115,6 @@ struct PackArgs {
   const Counted *counted;      // rows: how many of them, where given
   int32_t vector;              // rows begin at multiples of 16 bytes
 };
-
-__device__ __forceinline__ __bf16 toward_zero(float v) {      // (rounding up the largest floats would give infinities)
-  return __builtin_bit_cast(__bf16, (unsigned short)(__builtin_bit_cast(unsigned, v) >> 16));
-}
-__device__ __forceinline__ void split3(float v, __bf16 &h, __bf16 &m, __bf16 &l) {
-  h = toward_zero(v);
-  const float r = v - (float)h;
-  m = toward_zero(r);
-  l = (__bf16)(r - (float)m);
-}
 
 template <class T>
 struct alignas(16) Piece {
@@ -352,7 +335,7 @@ __global__ __launch_bounds__(256) void k_ce_mean(const double *sums, int64_t n, 
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------------
-// The factor that is taken out of dl: the one weight of a sum or a mean, the largest weight of single points.
+// The factor that is taken out of dl: the one weight of a sum or a mean; for float16 the largest weight of single points.
 __global__ __launch_bounds__(256) void k_ce_top(const float *grad, int64_t n, const int32_t *place, float *part) {
   __shared__ float s[4];
   float top = 0.0f;
@@ -821,9 +804,10 @@ template <class S, class T, int kPlanes>
 void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   const Counted *counted = static_cast<const Counted *>(d.counted);
   const bool each = d.reduction == R3D_CE_NONE;
-  if (each) hipLaunchKernelGGL(k_ce_top, dim3(p.top_parts), dim3(256), 0, st, d.grad, d.n, d.place, p.top);
+  const int parts = each && d.type == R3D_T_F16 ? p.top_parts : 0;
+  if (parts) hipLaunchKernelGGL(k_ce_top, dim3(parts), dim3(256), 0, st, d.grad, d.n, d.place, p.top);
   hipLaunchKernelGGL(k_ce_weight, dim3(blocks_for(p.n_pad, 256, 1 << 30)), dim3(256), 0, st,
-                     WeightArgs{d.grad, p.top, each ? 1 : 0, p.top_parts, d.idx, counted, p.scale, p.weight, p.n_pad});
+                     WeightArgs{d.grad, p.top, each ? 1 : 0, parts, d.idx, counted, p.scale, p.weight, p.n_pad});
   Operand x, w;
   operands<S, T, kPlanes>(d, p, counted, st, x, w);
   const float held = d.type == R3D_T_F16 ? 32768.0f : 1.0f, unheld = 1.0f / held;
@@ -907,7 +891,8 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
 
 extern "C" size_t r3d_linear_ce_workspace_bytes(const r3d_linear_ce_t *d, int32_t backward_pass) {
   if (check(d) != R3D_OK) return 0;
-  return plan(*d, backward_pass != 0, nullptr).bytes;
+  const size_t few = few_bytes(*d, backward_pass != 0);
+  return few ? few : plan(*d, backward_pass != 0, nullptr).bytes;
 }
 
 extern "C" int r3d_linear_ce_forward(const r3d_linear_ce_t *d, void *workspace, size_t workspace_bytes, void *stream) {
@@ -915,9 +900,15 @@ extern "C" int r3d_linear_ce_forward(const r3d_linear_ce_t *d, void *workspace, 
   if (rc != R3D_OK) return rc;
   if (!d->x || !d->w || !d->target || !d->idx || !d->place || !d->tgt || !d->lse2 || !d->counted || !d->loss || !workspace)
     return fail(R3D_E_ARG, "linear_ce_forward: null pointer");
-  const Plan p = plan(*d, false, workspace);
-  if (workspace_bytes < p.bytes) return fail(R3D_E_WORKSPACE, "linear_ce_forward: workspace too small");
+  if (workspace_bytes < r3d_linear_ce_workspace_bytes(d, 0)) return fail(R3D_E_WORKSPACE, "linear_ce_forward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (few_bytes(*d, false)) {
+    rc = few_forward(*d, workspace, st);
+    if (rc != R3D_OK) return rc;
+    R3D_LAUNCHED("linear_ce forward kernels, few classes");
+    return R3D_OK;
+  }
+  const Plan p = plan(*d, false, workspace);
   if (d->type == R3D_T_F32) forward<float, __bf16, 3>(*d, p, st);
   else if (d->type == R3D_T_BF16) forward<__bf16, __bf16, 1>(*d, p, st);
   else forward<_Float16, _Float16, 1>(*d, p, st);
@@ -930,9 +921,15 @@ extern "C" int r3d_linear_ce_backward(const r3d_linear_ce_t *d, void *workspace,
   if (rc != R3D_OK) return rc;
   if (!d->x || !d->w || !d->idx || !d->place || !d->tgt || !d->lse2 || !d->counted || !d->grad || !workspace)
     return fail(R3D_E_ARG, "linear_ce_backward: null pointer");
-  const Plan p = plan(*d, true, workspace);
-  if (workspace_bytes < p.bytes) return fail(R3D_E_WORKSPACE, "linear_ce_backward: workspace too small");
+  if (workspace_bytes < r3d_linear_ce_workspace_bytes(d, 1)) return fail(R3D_E_WORKSPACE, "linear_ce_backward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (few_bytes(*d, true)) {
+    rc = few_backward(*d, workspace, st);
+    if (rc != R3D_OK) return rc;
+    R3D_LAUNCHED("linear_ce backward kernels, few classes");
+    return R3D_OK;
+  }
+  const Plan p = plan(*d, true, workspace);
   if (d->type == R3D_T_F32) backward<float, __bf16, 3>(*d, p, st);
   else if (d->type == R3D_T_BF16) backward<__bf16, __bf16, 1>(*d, p, st);
   else backward<_Float16, _Float16, 1>(*d, p, st);

@@ -1,0 +1,34 @@
+// What the two files of the linear head's cross entropy share (r3d_loss.hip: any sizes; r3d_loss_few.hip: few classes).
+#pragma once
+
+#include "r3d_mfma.hpp"
+
+#include "../../include/real3daug_hip.h"
+
+namespace r3d {
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+struct Counted {      // the points that count, on the device
+  int32_t n;          // how many
+  float share;        // 1 / n for a mean (0 where none counts), 1 else
+  float pad[2];
+};
+
+__device__ __forceinline__ __bf16 toward_zero(float v) {      // (rounding up the largest floats would give infinities)
+  return __builtin_bit_cast(__bf16, (unsigned short)(__builtin_bit_cast(unsigned, v) >> 16));
+}
+// The three planes of 8 bits of a float: v = h + m + l to 2^-25.
+__device__ __forceinline__ void split3(float v, __bf16 &h, __bf16 &m, __bf16 &l) {
+  h = toward_zero(v);
+  const float r = v - (float)h;
+  m = toward_zero(r);
+  l = (__bf16)(r - (float)m);
+}
+
+// Few classes: workspace (0: not this head), the two passes.
+size_t few_bytes(const r3d_linear_ce_t &d, bool backward);
+int few_forward(const r3d_linear_ce_t &d, void *workspace, hipStream_t st);
+int few_backward(const r3d_linear_ce_t &d, void *workspace, hipStream_t st);
+
+}  // namespace r3d
