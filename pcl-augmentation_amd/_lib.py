@@ -231,6 +231,13 @@ def stream_ptr():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def raw_stream(index):
+    """The current stream of device ``index`` as an integer: what ``stream_ptr`` says, a few microseconds earlier (no stream
+    object is made) -- for calls whose kernels are shorter than that."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def on(device):
     """Context manager that makes `device` (a torch.device, string, index or CUDA tensor) the current
     one: every library call must run with the device of its pointers current."""

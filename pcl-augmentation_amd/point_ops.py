@@ -13,6 +13,9 @@ from . import _lib
 _REDUCTIONS = {"none": _lib.CE_NONE, "sum": _lib.CE_SUM, "mean": _lib.CE_MEAN}
 
 
+_HERE = contextlib.nullcontext()
+
+
 @functools.lru_cache(maxsize=None)
 def _types():
     import torch
@@ -23,14 +26,14 @@ def _types():
 def on_device_of(what, *tensors):
     """The device of these tensors made current (a null context where it is already); refuses tensors that are not on one GPU."""
     import torch
-    device = tensors[0].device
-    if device.type != "cuda":
+    index = tensors[0].get_device()
+    if index < 0:
         _lib.require_gpu()
-        raise _lib.R3DError(f"{what}: the tensors must be on a GPU, got {device}")
+        raise _lib.R3DError(f"{what}: the tensors must be on a GPU, got {tensors[0].device}")
     for t in tensors[1:]:
-        if t.device != device:
-            raise ValueError(f"{what}: tensors on {device} and {t.device}")
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        if t.get_device() != index:
+            raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def _value_type(what, t):
@@ -65,8 +68,8 @@ def _turn(tensors, positions, sections, base, interleaved, backward):
     d.sections[:len(sections)] = sections
     d.pos_type, d.pos = _types()[1][positions.dtype], positions.data_ptr()
     d.pos_token_stride, d.pos_axis_stride = positions.stride()
-    with on_device_of("rotary_positions", *[t for t in tensors if t is not None], positions):
-        _lib.check(_lib.load().r3d_rotary(C.byref(d), _lib.stream_ptr()), "r3d_rotary")
+    with on_device_of("rotary_positions", positions):
+        _lib.check(_lib.load().r3d_rotary(C.byref(d), _lib.raw_stream(positions.get_device())), "r3d_rotary")
     return outs
 
 
@@ -139,23 +142,18 @@ def _loss_function():
     import torch
     from torch.autograd.function import once_differentiable
 
-    def descriptor(x, weight, bias, target, state, how):
-        d = _lib.LinearCE()
-        n = x.shape[0]
+    def follow(d, x, weight, bias, target, state):
+        """The descriptor's tensors (in the backward pass: as they come back from where they were kept)."""
+        n, at = d.n, state.data_ptr()
         d.x, d.w, d.bias, d.target = x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), target.data_ptr()
-        d.ld_x, d.ld_w = x.stride(0), weight.stride(0)
-        d.n, d.v, d.d = n, weight.shape[0], x.shape[1]
-        d.ignore_index, d.reduction, d.piece = how
-        d.type, d.target_type = _types()[0][x.dtype], _types()[1][target.dtype]
-        at = state.data_ptr()
         d.counted, d.idx, d.place, d.tgt, d.lse2 = at, at + 16, at + 16 + 4 * n, at + 16 + 8 * n, at + 16 + 12 * n
-        return d
+        d.ld_x, d.ld_w = x.stride(0), weight.stride(0)
 
     def workspace(lib, d, backward, device):
         size = lib.r3d_linear_ce_workspace_bytes(C.byref(d), backward)
         if size == 0:
             _lib.check(_lib.E_ARG, "r3d_linear_ce_workspace_bytes")
-        return torch.empty(size, dtype=torch.uint8, device=device)
+        return torch.empty(size, dtype=torch.uint8, device=device), size
 
     class LinearCrossEntropy(torch.autograd.Function):
         @staticmethod
@@ -165,12 +163,14 @@ def _loss_function():
                 lib = _lib.load()
                 state = torch.empty(4 + 4 * n, dtype=torch.int32, device=x.device)
                 loss = torch.empty(n if how[1] == _lib.CE_NONE else (), dtype=torch.float32, device=x.device)
-                d = descriptor(x, weight, bias, target, state, how)
-                d.loss = loss.data_ptr()
-                ws = workspace(lib, d, 0, x.device)
-                _lib.check(lib.r3d_linear_ce_forward(C.byref(d), ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "r3d_linear_ce_forward")
+                types = _types()
+                d = _lib.LinearCE(n=n, v=weight.shape[0], d=x.shape[1], ignore_index=how[0], reduction=how[1], piece=how[2],
+                                  type=types[0][x.dtype], target_type=types[1][target.dtype], loss=loss.data_ptr())
+                follow(d, x, weight, bias, target, state)
+                ws, size = workspace(lib, d, 0, x.device)
+                _lib.check(lib.r3d_linear_ce_forward(C.byref(d), ws.data_ptr(), size, _lib.raw_stream(x.get_device())), "r3d_linear_ce_forward")
             ctx.save_for_backward(x, weight, bias, target, state)
-            ctx.how = how
+            ctx.descriptor = d
             return loss
 
         @staticmethod
@@ -180,15 +180,16 @@ def _loss_function():
             need = ctx.needs_input_grad
             with on_device_of("linear_cross_entropy", x):
                 lib = _lib.load()
-                d = descriptor(x, weight, bias, target, state, ctx.how)
+                d = _lib.LinearCE.from_buffer_copy(ctx.descriptor)      # (two backward passes may run at once)
+                follow(d, x, weight, bias, target, state)
                 grad = grad.to(torch.float32).contiguous()
                 d.grad = grad.data_ptr()
-                outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and n else None
-                        for t, n in zip((x, weight, bias), need)]
-                d.dx, d.dw, d.db = (0 if o is None else o.data_ptr() for o in outs)
-                ws = workspace(lib, d, 1, x.device)
-                _lib.check(lib.r3d_linear_ce_backward(C.byref(d), ws.data_ptr(), ws.numel(), _lib.stream_ptr()), "r3d_linear_ce_backward")
-            return outs[0], outs[1], outs[2], None, None
+                new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+                dx, dw, db = (new(x) if need[0] else None, new(weight) if need[1] else None, new(bias) if need[2] else None)
+                d.dx, d.dw, d.db = (0 if o is None else o.data_ptr() for o in (dx, dw, db))
+                ws, size = workspace(lib, d, 1, x.device)
+                _lib.check(lib.r3d_linear_ce_backward(C.byref(d), ws.data_ptr(), size, _lib.raw_stream(x.get_device())), "r3d_linear_ce_backward")
+            return dx, dw, db, None, None
 
     return LinearCrossEntropy
 
@@ -229,6 +230,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
         none = (x.sum() + weight.sum() * 0 + (0 if bias is None else bias.sum() * 0)).float() * 0
         return none if reduction != "none" else none.expand(target.shape) + torch.zeros(target.shape, device=x.device)
     how = (int(ignore_index), _REDUCTIONS[reduction], int(piece))
-    loss = _loss_function().apply(_rows_dense(x.reshape(-1, x.shape[-1])), _rows_dense(weight), None if bias is None else bias.contiguous(),
-                                  target.reshape(-1).contiguous(), how)
+    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    loss = _loss_function().apply(_rows_dense(flat), _rows_dense(weight), None if bias is None else bias.contiguous(),
+                                  (target if target.dim() == 1 else target.reshape(-1)).contiguous(), how)
     return loss.reshape(target.shape) if reduction == "none" else loss

@@ -60,7 +60,7 @@ def block_tables(lengths, block_size, tables, held, free_blocks, n_free):
         _lib.check(lib.r3d_block_tables(lengths.data_ptr(), rows, block_size, most, tables.data_ptr(), held.data_ptr(), free_blocks.data_ptr(),
                                         free_blocks.shape[0], n_free.data_ptr(), out.tables.data_ptr(), out.held.data_ptr(),
                                         out.free_blocks.data_ptr(), out.n_free.data_ptr(), out.status.data_ptr(), ws.data_ptr(), ws.numel(),
-                                        _lib.stream_ptr()), "r3d_block_tables")
+                                        _lib.raw_stream(lengths.get_device())), "r3d_block_tables")
     return out
 
 
@@ -98,7 +98,7 @@ def slot_map(lengths, block_size, tables=None, rows=None, capacity=None):
         slots, sequence = (t.data_ptr() if capacity else out.offsets.data_ptr() for t in out[1:])
         _lib.check(lib.r3d_slot_map(lengths.data_ptr(), lengths.shape[0], 0 if tables is None else tables.data_ptr(), block_size, most,
                                     0 if rows is None else rows.data_ptr(), n, capacity, out.offsets.data_ptr(), slots, sequence,
-                                    _lib.stream_ptr()), "r3d_slot_map")
+                                    _lib.raw_stream(lengths.get_device())), "r3d_slot_map")
     return out
 
 
@@ -118,7 +118,7 @@ def _move(what, sources, dests, src_slots, dst_slots, n):
         a.src_stride, a.dst_stride = (s.stride(0) * size if s.shape[0] > 1 else width), (t.stride(0) * size if t.shape[0] > 1 else width)
     _lib.check(_lib.load().r3d_move_rows(arrays, len(sources), 0 if src_slots is None else src_slots.data_ptr(),
                                          0 if dst_slots is None else dst_slots.data_ptr(), n, sources[0].shape[0], dests[0].shape[0],
-                                         _lib.stream_ptr()), "r3d_move_rows")
+                                         _lib.raw_stream(sources[0].get_device())), "r3d_move_rows")
 
 
 def _rows_of(what, name, tensors, like=None):
