@@ -682,25 +682,26 @@ int r3d_rotary(const r3d_rotary_t *d, void *stream);
  * x [n] rows of ld_x elements, w [v] rows of ld_w, bias [v] (nullable), all of `type`; targets of target_type.  A point whose
  * target is ignore_index has loss 0 and gradient 0, and what its features hold reaches no sum; one whose target is no class has
  * loss NaN.  loss: float [n] (R3D_CE_NONE) or [1] (sum, mean over the points that count; 0 where none does).
- * The forward call fills idx, place, tgt (int32 [n] each), lse2 (float [n]) and counted (16 bytes), which the backward call of
- * the same descriptor reads.  backward: grad = float [n] or
- * [1]; dx [n][d], dw [v][d], db [v] dense, of `type`, each nullable.  piece: classes whose logit gradients are held at a time
- * (0: as many as 512 MB take). */
+ * The forward call fills `state` (R3D_CE_BYTES_STATE bytes: which points count, their statistics, what had to be packed), which
+ * the backward call of the same descriptor reads and leaves as it is.  backward: grad = float [n] or [1]; dx [n][d], dw [v][d],
+ * db [v] dense, of `type`, each nullable.  piece: classes whose logit gradients are held at a time (0: as many as 512 MB take).
+ * r3d_linear_ce_bytes: of the state and of the two calls' workspaces, for the descriptor as it will be passed (0: bad descriptor). */
 #define R3D_CE_NONE 0
 #define R3D_CE_SUM 1
 #define R3D_CE_MEAN 2
+#define R3D_CE_BYTES_STATE 0
+#define R3D_CE_BYTES_FORWARD 1
+#define R3D_CE_BYTES_BACKWARD 2
 typedef struct r3d_linear_ce_t {
   const void *x, *w, *bias, *target;
   int64_t ld_x, ld_w, n, v, d, ignore_index, piece;
   int32_t type, target_type, reduction, reserved;
-  int32_t *idx, *place, *tgt;
-  float *lse2;
-  void *counted;
+  void *state;
   float *loss;
   const float *grad;
   void *dx, *dw, *db;
 } r3d_linear_ce_t;
-size_t r3d_linear_ce_workspace_bytes(const r3d_linear_ce_t *d, int32_t backward);
+size_t r3d_linear_ce_bytes(const r3d_linear_ce_t *d, int32_t which);
 int r3d_linear_ce_forward(const r3d_linear_ce_t *d, void *workspace, size_t workspace_bytes, void *stream);
 int r3d_linear_ce_backward(const r3d_linear_ce_t *d, void *workspace, size_t workspace_bytes, void *stream);
 

@@ -88,6 +88,7 @@ class Rows(C.Structure):
 T_F32, T_BF16, T_F16, T_F64, T_I32, T_I64 = range(6)
 MAX_ROW_ARRAYS, ROTARY_MAX_AXES, ROTARY_MAX_PAIRS = 4, 8, 256
 CE_NONE, CE_SUM, CE_MEAN = 0, 1, 2
+CE_BYTES_STATE, CE_BYTES_FORWARD, CE_BYTES_BACKWARD = 0, 1, 2
 
 
 class Rotary(C.Structure):
@@ -104,8 +105,7 @@ class LinearCE(C.Structure):
                 ("ld_x", C.c_int64), ("ld_w", C.c_int64), ("n", C.c_int64), ("v", C.c_int64), ("d", C.c_int64),
                 ("ignore_index", C.c_int64), ("piece", C.c_int64),
                 ("type", C.c_int32), ("target_type", C.c_int32), ("reduction", C.c_int32), ("reserved", C.c_int32),
-                ("idx", C.c_void_p), ("place", C.c_void_p), ("tgt", C.c_void_p), ("lse2", C.c_void_p), ("counted", C.c_void_p),
-                ("loss", C.c_void_p), ("grad", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("db", C.c_void_p)]
+                ("state", C.c_void_p), ("loss", C.c_void_p), ("grad", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("db", C.c_void_p)]
 
 
 PLACE_ROTATIONS, PLACE_SURFACE_CAP, PLACE_MAX_OK_LABELS = 360, 128, 32
@@ -182,7 +182,7 @@ _SIGNATURES = {
     "r3d_slot_map": (C.c_int, [_P, C.c_int64, _P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, _P, _P, _P, _P]),
     "r3d_move_rows": (C.c_int, [C.POINTER(Rows), C.c_int32, _P, _P, C.c_int64, C.c_int64, C.c_int64, _P]),
     "r3d_rotary": (C.c_int, [C.POINTER(Rotary), _P]),
-    "r3d_linear_ce_workspace_bytes": (C.c_size_t, [C.POINTER(LinearCE), C.c_int32]),
+    "r3d_linear_ce_bytes": (C.c_size_t, [C.POINTER(LinearCE), C.c_int32]),
     "r3d_linear_ce_forward": (C.c_int, [C.POINTER(LinearCE), _P, C.c_size_t, _P]),
     "r3d_linear_ce_backward": (C.c_int, [C.POINTER(LinearCE), _P, C.c_size_t, _P]),
 }

@@ -22,52 +22,44 @@
 namespace {
 using namespace r3d;
 
-template <class T>
-__device__ __forceinline__ float wide(T v) { return (float)v; }
+// ---- which points count, and the operands --------------------------------------------------------------------------------
+constexpr int kStartThreads = 1024, kStartRows = 4 * kStartThreads;
+constexpr int kOneGroup = 16384;      // points one workgroup numbers by itself (in 10 us; two launches over many take 8)
 
-// ---- which points count -------------------------------------------------------------------------------------------------
-constexpr int kCountRows = 1024;
+// A side of the products: rows padded to whole k-blocks, split into planes where the type is wider.
+struct PackArgs {
+  const void *src;
+  void *dst;
+  int64_t ld, rows, width, ld_out, plane;      // width: of the source; ld_out a multiple of 64
+  int32_t vector;                              // rows begin at multiples of 16 bytes
+  int32_t blocks;
+};
 
-struct IndexArgs {
-  const void *target;
+struct StartArgs {
+  const void *target, *bias;
   int64_t n, v, ignore;
   int32_t wide_target, mean;
   int32_t *part, *idx, *place, *tgt;      // idx: point of a number, place: number of a point or -1, tgt: its class or -1 (not a class)
   Counted *counted;
+  float *bias2;                           // in units of log 2, -inf behind the last class: those count for nothing anywhere
+  int64_t v_pad;
+  int32_t groups, bias_blocks;
+  PackArgs pack[2];
 };
 
-__device__ __forceinline__ int64_t target_of(const IndexArgs &a, int64_t i) {
+__device__ __forceinline__ int64_t target_of(const StartArgs &a, int64_t i) {
   return a.wide_target ? static_cast<const int64_t *>(a.target)[i] : static_cast<const int32_t *>(a.target)[i];
 }
 
-__global__ __launch_bounds__(256) void k_ce_count(IndexArgs a) {
-  __shared__ int s[4];
-  int c = 0;
-  const int64_t first = (int64_t)blockIdx.x * kCountRows + threadIdx.x * 4;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) c += first + j < a.n && target_of(a, first + j) != a.ignore;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) c += __shfl_xor(c, d);
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = c;
-  __syncthreads();
-  if (threadIdx.x == 0) a.part[blockIdx.x] = s[0] + s[1] + s[2] + s[3];
-}
-
-__global__ __launch_bounds__(256) void k_ce_index(IndexArgs a) {
-  __shared__ int s[4], s_before[4], s_all[4];
+// Numbers the points [first, first + kStartRows) that count from `at` on; returns the next number.  s: 16 words.
+__device__ __forceinline__ int number_rows(const StartArgs &a, int64_t first, int at, int *s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int before = 0, all = 0;
-  for (int b = threadIdx.x; b < (int)gridDim.x; b += 256) {
-    const int v = a.part[b];
-    all += v;
-    before += b < (int)blockIdx.x ? v : 0;
-  }
-  const int64_t first = (int64_t)blockIdx.x * kCountRows + threadIdx.x * 4;
+  const int64_t mine0 = first + threadIdx.x * 4;
   int64_t t[4];
   int mine = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    t[j] = first + j < a.n ? target_of(a, first + j) : a.ignore;
+    t[j] = mine0 + j < a.n ? target_of(a, mine0 + j) : a.ignore;
     mine += t[j] != a.ignore;
   }
   int run = mine;
@@ -76,45 +68,33 @@ __global__ __launch_bounds__(256) void k_ce_index(IndexArgs a) {
     const int o = __shfl_up(run, d);
     if (lane >= d) run += o;
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    before += __shfl_xor(before, d);
-    all += __shfl_xor(all, d);
-  }
   if (lane == 63) s[wave] = run;
-  if (lane == 0) {
-    s_before[wave] = before;
-    s_all[wave] = all;
+  __syncthreads();
+  int to = at + run - mine, end = at;
+#pragma unroll
+  for (int w = 0; w < kStartThreads / 64; ++w) {
+    to += w < wave ? s[w] : 0;
+    end += s[w];
   }
   __syncthreads();
-  int at = run - mine + s_before[0] + s_before[1] + s_before[2] + s_before[3];
-  for (int w = 0; w < wave; ++w) at += s[w];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    if (first + j >= a.n) break;
+    if (mine0 + j >= a.n) break;
     const bool counts = t[j] != a.ignore;
-    a.place[first + j] = counts ? at : -1;
+    a.place[mine0 + j] = counts ? to : -1;
     if (counts) {
-      a.idx[at] = (int32_t)(first + j);
-      a.tgt[at++] = t[j] >= 0 && t[j] < a.v ? (int32_t)t[j] : -1;
+      a.idx[to] = (int32_t)(mine0 + j);
+      a.tgt[to++] = t[j] >= 0 && t[j] < a.v ? (int32_t)t[j] : -1;
     }
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    const int n = s_all[0] + s_all[1] + s_all[2] + s_all[3];
-    a.counted->n = n;
-    a.counted->share = !a.mean ? 1.0f : n ? 1.0f / (float)n : 0.0f;
-  }
+  return end;
 }
 
-// ---- operands: rows of whole k-blocks, split into planes where the type is wider -------------------------------------------
-struct PackArgs {
-  const void *src;
-  void *dst;
-  int64_t ld, rows, width, ld_out, plane;      // width: of the source; ld_out a multiple of 64
-  const int32_t *idx;
-  const Counted *counted;      // rows: how many of them, where given
-  int32_t vector;              // rows begin at multiples of 16 bytes
-};
+__device__ __forceinline__ void put_counted(const StartArgs &a, int n) {
+  a.counted->n = n;
+  a.counted->share = !a.mean ? 1.0f : n ? 1.0f / (float)n : 0.0f;
+  a.counted->ticket = 0;
+}
 
 template <class T>
 struct alignas(16) Piece {
@@ -123,14 +103,13 @@ struct alignas(16) Piece {
 
 // A thread makes a piece of 8 values of a row.
 template <class S, class T, int kPlanes>
-__global__ __launch_bounds__(256) void k_ce_pack(PackArgs a) {
-  const int64_t rows = a.counted ? a.counted->n : a.rows;
+__device__ __forceinline__ void pack_rows(const PackArgs &a, int block) {
   const unsigned each = (unsigned)(a.ld_out / 8);
-  const int64_t all = rows * each;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+  const int64_t all = a.rows * each;
+  for (int64_t i = (int64_t)block * kStartThreads + threadIdx.x; i < all; i += (int64_t)a.blocks * kStartThreads) {
     const int64_t r = all <= UINT32_MAX ? (unsigned)i / each : i / each;
     const int64_t c = (i - r * each) * 8;
-    const S *src = static_cast<const S *>(a.src) + (a.idx ? a.idx[r] : r) * a.ld + c;
+    const S *src = static_cast<const S *>(a.src) + r * a.ld + c;
     S v[8];
     if (c + 8 <= a.width && a.vector) {
       typedef S s4 __attribute__((ext_vector_type(16 / sizeof(S))));
@@ -155,11 +134,70 @@ __global__ __launch_bounds__(256) void k_ce_pack(PackArgs a) {
   }
 }
 
-// The bias in units of log 2, -inf behind the last class: those count for nothing anywhere.
-template <class S>
-__global__ __launch_bounds__(256) void k_ce_bias(const S *bias, float *out, int64_t v, int64_t v_all) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < v_all) out[i] = i >= v ? -INFINITY : bias ? wide(bias[i]) * kLog2e : 0.0f;
+// Everything the products need, in one launch: the points that count numbered (or, where they are many, counted by groups), the
+// bias, the operands packed.
+template <class S, class T, int kPlanes>
+__global__ __launch_bounds__(kStartThreads) void k_ce_start(StartArgs a) {
+  __shared__ int s[kStartThreads / 64];
+  int block = blockIdx.x;
+  if (block < a.groups) {
+    if (a.n <= kOneGroup) {
+      int at = 0;
+      for (int64_t first = 0; first < a.n; first += kStartRows) at = number_rows(a, first, at, s);
+      if (threadIdx.x == 0) put_counted(a, at);
+      return;
+    }
+    int c = 0;
+    const int64_t first = (int64_t)block * kStartRows + threadIdx.x * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c += first + j < a.n && target_of(a, first + j) != a.ignore;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) c += __shfl_xor(c, d);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = c;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      c = 0;
+      for (int w = 0; w < kStartThreads / 64; ++w) c += s[w];
+      a.part[block] = c;
+    }
+    return;
+  }
+  block -= a.groups;
+  if (block < a.bias_blocks) {
+    const int64_t i = (int64_t)block * kStartThreads + threadIdx.x;
+    if (i < a.v_pad) a.bias2[i] = i >= a.v ? -INFINITY : a.bias ? (float)static_cast<const S *>(a.bias)[i] * kLog2e : 0.0f;
+    return;
+  }
+  block -= a.bias_blocks;
+  if (block < a.pack[0].blocks) pack_rows<S, T, kPlanes>(a.pack[0], block);
+  else pack_rows<S, T, kPlanes>(a.pack[1], block - a.pack[0].blocks);
+}
+
+__global__ __launch_bounds__(kStartThreads) void k_ce_index(StartArgs a) {
+  __shared__ int s[kStartThreads / 64], s_before[kStartThreads / 64], s_all[kStartThreads / 64];
+  int before = 0, all = 0;
+  for (int b = threadIdx.x; b < a.groups; b += kStartThreads) {
+    const int v = a.part[b];
+    all += v;
+    before += b < (int)blockIdx.x ? v : 0;
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    before += __shfl_xor(before, d);
+    all += __shfl_xor(all, d);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    s_before[threadIdx.x >> 6] = before;
+    s_all[threadIdx.x >> 6] = all;
+  }
+  __syncthreads();
+  before = all = 0;
+  for (int w = 0; w < kStartThreads / 64; ++w) {
+    before += s_before[w];
+    all += s_all[w];
+  }
+  number_rows(a, (int64_t)blockIdx.x * kStartRows, before, s);
+  if (blockIdx.x == 0 && threadIdx.x == 0) put_counted(a, all);
 }
 
 // ---- products --------------------------------------------------------------------------------------------------------------
@@ -281,26 +319,37 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
   }
 }
 
-struct CombineArgs {
+struct JoinArgs {
   const float *part_m, *part_l, *hit;
   const int32_t *tgt, *place;
-  const Counted *counted;
+  Counted *counted;
   float *lse2, *each, *loss;
   double *sums;
   int64_t n, n_pad;
-  int32_t splits;
+  int32_t splits, mean;
 };
 
-// The splits joined; the loss of every point (each) or the sums of 256 of them.  Over the points as the caller numbers them.
-__global__ __launch_bounds__(256) void k_ce_join(CombineArgs a) {
+__device__ __forceinline__ double group_sum(double d, double *s) {
+#pragma unroll
+  for (int k = 32; k; k >>= 1) d += __shfl_xor(d, k);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = d;
+  __syncthreads();
+  return s[0] + s[1] + s[2] + s[3];
+}
+
+// The splits joined; the loss of every point (each), or their sum: every workgroup leaves that of its 256 points, the last one
+// adds them up, always in the same order.  Over the points as the caller numbers them.
+__global__ __launch_bounds__(256) void k_ce_join(JoinArgs a) {
+  __shared__ double s[4];
+  __shared__ int s_last;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int at = i < a.n ? a.place[i] : -1;
   float loss = 0.0f;
   if (at >= 0) {
     float top = -INFINITY, sum = 0.0f;
-    for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_m[s * a.n_pad + at]);
+    for (int k = 0; k < a.splits; ++k) top = fmaxf(top, a.part_m[k * a.n_pad + at]);
     const float base = top == -INFINITY ? 0.0f : top;
-    for (int s = 0; s < a.splits; ++s) sum += a.part_l[s * a.n_pad + at] * __builtin_amdgcn_exp2f(a.part_m[s * a.n_pad + at] - base);
+    for (int k = 0; k < a.splits; ++k) sum += a.part_l[k * a.n_pad + at] * __builtin_amdgcn_exp2f(a.part_m[k * a.n_pad + at] - base);
     const bool fine = a.tgt[at] >= 0;      // a target that is no class: NaN, and so are its gradients
     const float lse2 = fine ? top + __builtin_amdgcn_logf(sum) : NAN;
     a.lse2[at] = lse2;
@@ -310,27 +359,22 @@ __global__ __launch_bounds__(256) void k_ce_join(CombineArgs a) {
     if (i < a.n) a.each[i] = loss;
     return;
   }
-  __shared__ double s[4];
-  double d = loss;
-#pragma unroll
-  for (int k = 32; k; k >>= 1) d += __shfl_xor(d, k);
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = d;
-  __syncthreads();
-  if (threadIdx.x == 0) a.sums[blockIdx.x] = s[0] + s[1] + s[2] + s[3];
-}
-
-__global__ __launch_bounds__(256) void k_ce_mean(const double *sums, int64_t n, const Counted *counted, int32_t mean, float *loss) {
-  __shared__ double s[4];
-  double d = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 256) d += sums[i];
-#pragma unroll
-  for (int k = 32; k; k >>= 1) d += __shfl_xor(d, k);
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = d;
-  __syncthreads();
+  const double mine = group_sum(loss, s);
   if (threadIdx.x == 0) {
-    d = s[0] + s[1] + s[2] + s[3];
-    const int c = counted->n;
-    *loss = (float)(mean && c ? d / c : d);
+    a.sums[blockIdx.x] = mine;
+    __threadfence();
+    s_last = atomicAdd(&a.counted->ticket, 1) == (int)gridDim.x - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!s_last) return;
+  double d = 0.0;
+  for (int64_t b = threadIdx.x; b < gridDim.x; b += 256) d += __hip_atomic_load(&a.sums[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  d = group_sum(d, s);
+  if (threadIdx.x == 0) {
+    const int c = a.counted->n;
+    *a.loss = (float)(a.mean && c ? d / c : d);
   }
 }
 
@@ -351,13 +395,15 @@ __global__ __launch_bounds__(256) void k_ce_top(const float *grad, int64_t n, co
 struct WeightArgs {
   const float *grad, *part;
   int32_t each, parts;
-  const int32_t *idx;
+  const int32_t *idx, *place;
   const Counted *counted;
   float *scale;       // [1] the factor taken out of dl
-  float *weight;      // of every point in the line, at most 1; 0 up to n_pad
-  int64_t n_pad;
+  float *weight;      // of every point in the line, at most 1 where a factor is taken out; 0 up to n_pad
+  int64_t n, n_pad, d;
+  void *dx;           // rows of the points that do not count become zeros here, where nothing else writes them
 };
 
+template <class V>
 __global__ __launch_bounds__(256) void k_ce_weight(WeightArgs a) {
   const int nc = a.counted->n;
   float scale;
@@ -373,6 +419,16 @@ __global__ __launch_bounds__(256) void k_ce_weight(WeightArgs a) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i < a.n_pad) a.weight[i] = i >= nc ? 0.0f : a.each ? a.grad[a.idx[i]] / scale : 1.0f;
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.scale = scale;
+  if (!a.dx) return;
+  // a wave's 64 points: those that do not count one after the other
+  const int64_t first = (int64_t)blockIdx.x * 256 + (threadIdx.x & ~63);
+  uint64_t out = __ballot(i < a.n && a.place[i < a.n ? i : 0] < 0);
+  V *dx = static_cast<V *>(a.dx);
+  while (out) {
+    const int64_t row = first + __builtin_ctzll(out);
+    out &= out - 1;
+    for (int64_t c = threadIdx.x & 63; c < a.d; c += 64) dx[row * a.d + c] = (V)0.0f;
+  }
 }
 
 struct DlArgs {
@@ -551,57 +607,69 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
   }
 }
 
-// Rows of the points that do not count.
-template <class V>
-__global__ __launch_bounds__(256) void k_ce_zero(V *dx, int64_t n, int64_t d, const int32_t *place) {
-  for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < n; r += (int64_t)gridDim.x * 4)
-    if (place[r] < 0)
-      for (int64_t c = threadIdx.x & 63; c < d; c += 64) dx[r * d + c] = (V)0.0f;
-}
-
-struct FinishArgs {
+struct Finish {
   const float *acc;
-  int64_t ld, split_stride, rows, width, ld_out;
-  int32_t splits;
-  float unheld;      // 2^-15 for float16
+  int64_t ld, split_stride, rows, width;      // ld a multiple of 4
+  int32_t splits, vector;                     // vector: four values of the result can be stored at once
   const int32_t *place;
-  const float *scale;
   void *out;
 };
+struct FinishArgs {
+  Finish of[3];
+  const float *scale;
+  float unheld;      // 2^-15 for float16
+};
 
-// Splits joined, the factor put back, one rounding.  A thread makes kVec neighbouring values.
-template <class V, int kVec>
-__global__ __launch_bounds__(256) void k_ce_finish(FinishArgs a) {
-  typedef float fv __attribute__((ext_vector_type(kVec)));
-  struct alignas(kVec * sizeof(V)) Out {
-    V v[kVec];
+// Splits joined, the factor put back, one rounding; gridDim.y results.  A thread makes four neighbouring values; where there are
+// many splits the four waves of a workgroup share them.
+template <class V>
+__global__ __launch_bounds__(256) void k_ce_finish(FinishArgs all) {
+  typedef float f4 __attribute__((ext_vector_type(4)));
+  struct alignas(4 * sizeof(V)) Out {
+    V v[4];
   };
-  const float scale = *a.scale * a.unheld;
-  const unsigned each = (unsigned)(a.width / kVec);
-  const int64_t all = a.rows * each;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = all <= UINT32_MAX ? (unsigned)i / each : i / each;
-    const int64_t c = (i - r * each) * kVec, at = a.place ? a.place[r] : r;
-    float sum[kVec];
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) sum[e] = 0.0f;
+  __shared__ f4 s[4][64];
+  const Finish a = all.of[blockIdx.y];
+  const float scale = *all.scale * all.unheld;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, slices = a.splits >= 8 ? 4 : 1;
+  const unsigned each = (unsigned)((a.width + 3) / 4);
+  const int64_t count = a.rows * each, step = (int64_t)gridDim.x * (256 / slices);
+  for (int64_t i0 = (int64_t)blockIdx.x * (256 / slices); i0 < count; i0 += step) {
+    const int64_t i = i0 + (slices == 4 ? lane : (int)threadIdx.x);
+    const int64_t r = count <= UINT32_MAX ? (unsigned)i / each : i / each;
+    const int64_t c = (i - r * each) * 4;
+    const int64_t at = i >= count ? -1 : a.place ? a.place[r] : r;
+    f4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     if (at >= 0) {
       const float *from = a.acc + at * a.ld + c;
 #pragma unroll 8
-      for (int s = 0; s < a.splits; ++s) {
-        if constexpr (kVec == 1) {
-          sum[0] += from[s * a.split_stride];
-        } else {
-          const fv v = *reinterpret_cast<const fv *>(from + s * a.split_stride);
+      for (int k = slices == 4 ? wave : 0; k < a.splits; k += slices) {
+        const f4 v = *reinterpret_cast<const f4 *>(from + k * a.split_stride);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) sum[e] += v[e];
-        }
+        for (int e = 0; e < 4; ++e) sum[e] += v[e];
       }
     }
+    if (slices == 4) {
+      s[wave][lane] = sum;
+      __syncthreads();
+      const f4 t[4] = {s[0][lane], s[1][lane], s[2][lane], s[3][lane]};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] = t[0][e] + t[1][e] + t[2][e] + t[3][e];
+      __syncthreads();
+      if (wave) continue;
+    }
+    if (i >= count) continue;
     Out out;
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) out.v[e] = (V)(at >= 0 ? sum[e] * scale : 0.0f);
-    *reinterpret_cast<Out *>(static_cast<V *>(a.out) + r * a.ld_out + c) = out;
+    for (int e = 0; e < 4; ++e) out.v[e] = (V)(at >= 0 ? sum[e] * scale : 0.0f);
+    V *to = static_cast<V *>(a.out) + r * a.width + c;
+    if (a.vector) {
+      *reinterpret_cast<Out *>(to) = out;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (c + e < a.width) to[e] = out.v[e];
+    }
   }
 }
 
@@ -645,10 +713,15 @@ struct Plan {
   bool lse_big, dl_big, dx_big, dw_big;
   int lse_splits, dx_splits, dw_splits, top_parts, groups;
   bool dx_final, dw_final;      // nothing to add: straight into the result
+  // kept from the forward to the backward pass
+  Counted *counted;
+  int32_t *idx, *place, *tgt;
+  float *lse2, *bias2;
+  void *xp, *wp;
+  size_t state_bytes;
   // workspace
   int32_t *part;
-  void *xp, *wp;
-  float *bias2, *part_m, *part_l, *hit;
+  float *part_m, *part_l, *hit;
   double *sums;
   float *top, *scale, *weight, *accx, *accw, *accb;
   void *dl;
@@ -665,13 +738,20 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   p.dp = up(d.d, kPadK);
   p.n_pad = up(d.n, Big::BN);
   p.v_pad = up(d.v, Big::BM);
-  p.groups = (int)((d.n + kCountRows - 1) / kCountRows);
-  Carver c(workspace);
-  p.bias2 = c.take<float>(p.v_pad);
+  p.groups = d.n <= kOneGroup ? 1 : (int)((d.n + kStartRows - 1) / kStartRows);
+  Carver k(d.state);
+  p.counted = k.take<Counted>(1);
+  p.idx = k.take<int32_t>(d.n);
+  p.place = k.take<int32_t>(d.n);
+  p.tgt = k.take<int32_t>(d.n);
+  p.lse2 = k.take<float>(d.n);
+  p.bias2 = k.take<float>(p.v_pad);
   if (!p.direct) {
-    p.xp = c.take<uint16_t>((size_t)p.planes * p.n_pad * p.dp);
-    p.wp = c.take<uint16_t>((size_t)p.planes * p.v_pad * p.dp);
+    p.xp = k.take<uint16_t>((size_t)p.planes * d.n * p.dp);
+    p.wp = k.take<uint16_t>((size_t)p.planes * d.v * p.dp);
   }
+  p.state_bytes = k.off;
+  Carver c(workspace);
   if (!backward) {
     p.lse_big = large_tiles(d.v, d.n, 1);
     const int64_t bm = p.lse_big ? Big::BM : Small::BM, bn = p.lse_big ? Big::BN : Small::BN;
@@ -721,25 +801,15 @@ int check(const r3d_linear_ce_t *d) {
   return R3D_OK;
 }
 
-template <class S, class T, int kPlanes>
-void pack(const PackArgs &a, int64_t rows, hipStream_t st) {
-  hipLaunchKernelGGL((k_ce_pack<S, T, kPlanes>), dim3(blocks_for(rows * a.ld_out, 2048, 8192)), dim3(256), 0, st, a);
+// The operands as the products take them: in place, or as the forward pass has packed them.
+void operands(const r3d_linear_ce_t &d, const Plan &p, Operand &x, Operand &w) {
+  x = p.direct ? Operand{d.x, d.ld_x, 0, p.idx} : Operand{p.xp, p.dp, d.n * p.dp, p.idx};
+  w = p.direct ? Operand{d.w, d.ld_w, 0, nullptr} : Operand{p.wp, p.dp, d.v * p.dp, nullptr};
 }
 
-// The operands as the products take them: in place, or packed into the workspace.
-template <class S, class T, int kPlanes>
-void operands(const r3d_linear_ce_t &d, const Plan &p, const Counted *counted, hipStream_t st, Operand &x, Operand &w) {
-  hipLaunchKernelGGL(k_ce_bias<S>, dim3(blocks_for(p.v_pad, 256, 1 << 30)), dim3(256), 0, st, static_cast<const S *>(d.bias), p.bias2, d.v, p.v_pad);
-  if (p.direct) {
-    x = Operand{d.x, d.ld_x, 0, d.idx};
-    w = Operand{d.w, d.ld_w, 0, nullptr};
-    return;
-  }
-  const int size = (int)sizeof(S);
-  pack<S, T, kPlanes>(PackArgs{d.x, p.xp, d.ld_x, d.n, d.d, p.dp, p.n_pad * p.dp, d.idx, counted, aligned16(d.x) && d.ld_x * size % 16 == 0}, d.n, st);
-  pack<S, T, kPlanes>(PackArgs{d.w, p.wp, d.ld_w, d.v, d.d, p.dp, p.v_pad * p.dp, nullptr, nullptr, aligned16(d.w) && d.ld_w * size % 16 == 0}, d.v, st);
-  x = Operand{p.xp, p.dp, p.n_pad * p.dp, nullptr};
-  w = Operand{p.wp, p.dp, p.v_pad * p.dp, nullptr};
+PackArgs pack_args(const Plan &p, const void *src, void *dst, int64_t ld, int64_t rows, int64_t width) {
+  const bool vector = aligned16(src) && ld * p.type_bytes % 16 == 0;
+  return PackArgs{src, dst, ld, rows, width, p.dp, rows * p.dp, vector, blocks_for(rows * p.dp / 8, kStartThreads * 2, 1024)};
 }
 
 template <class T, class S>
@@ -751,31 +821,48 @@ void lse(LseArgs a, const Plan &p, int64_t n, int64_t v, hipStream_t st) {
 
 template <class S, class T, int kPlanes>
 void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
-  Counted *counted = static_cast<Counted *>(d.counted);
-  IndexArgs ia{d.target, d.n, d.v, d.ignore_index, d.target_type == R3D_T_I64, d.reduction == R3D_CE_MEAN, p.part, d.idx, d.place, d.tgt, counted};
-  hipLaunchKernelGGL(k_ce_count, dim3(p.groups), dim3(256), 0, st, ia);
-  hipLaunchKernelGGL(k_ce_index, dim3(p.groups), dim3(256), 0, st, ia);
+  const bool mean = d.reduction == R3D_CE_MEAN;
+  StartArgs sa{};
+  sa.target = d.target;
+  sa.bias = d.bias;
+  sa.n = d.n;
+  sa.v = d.v;
+  sa.ignore = d.ignore_index;
+  sa.wide_target = d.target_type == R3D_T_I64;
+  sa.mean = mean;
+  sa.part = p.part;
+  sa.idx = p.idx;
+  sa.place = p.place;
+  sa.tgt = p.tgt;
+  sa.counted = p.counted;
+  sa.bias2 = p.bias2;
+  sa.v_pad = p.v_pad;
+  sa.groups = p.groups;
+  sa.bias_blocks = blocks_for(p.v_pad, kStartThreads, 1 << 30);
+  if (!p.direct) {
+    sa.pack[0] = pack_args(p, d.w, p.wp, d.ld_w, d.v, d.d);
+    sa.pack[1] = pack_args(p, d.x, p.xp, d.ld_x, d.n, d.d);
+  }
+  hipLaunchKernelGGL((k_ce_start<S, T, kPlanes>), dim3(sa.groups + sa.bias_blocks + sa.pack[0].blocks + sa.pack[1].blocks), dim3(kStartThreads), 0, st, sa);
+  if (p.groups > 1) hipLaunchKernelGGL(k_ce_index, dim3(p.groups), dim3(kStartThreads), 0, st, sa);
   LseArgs la{};
-  operands<S, T, kPlanes>(d, p, counted, st, la.p.b, la.p.a);
+  operands(d, p, la.p.b, la.p.a);
   la.p.planes = kPlanes;
   la.v = d.v;
   la.kb = p.dp / kTileK;
   la.splits = p.lse_splits;
   la.bias2 = p.bias2;
-  la.tgt = d.tgt;
-  la.counted = counted;
+  la.tgt = p.tgt;
+  la.counted = p.counted;
   la.part_m = p.part_m;
   la.part_l = p.part_l;
   la.hit = p.hit;
   la.n_pad = p.n_pad;
   if (p.lse_big) lse<T, Big>(la, p, d.n, d.v, st);
   else lse<T, Small>(la, p, d.n, d.v, st);
-  CombineArgs ca{p.part_m, p.part_l, p.hit, d.tgt, d.place, counted, d.lse2, d.reduction == R3D_CE_NONE ? d.loss : nullptr, d.loss, p.sums, d.n, p.n_pad,
-                 p.lse_splits};
-  const int blocks = (int)((d.n + 255) / 256);
-  hipLaunchKernelGGL(k_ce_join, dim3(blocks), dim3(256), 0, st, ca);
-  if (d.reduction != R3D_CE_NONE)
-    hipLaunchKernelGGL(k_ce_mean, dim3(1), dim3(256), 0, st, p.sums, (int64_t)blocks, counted, d.reduction == R3D_CE_MEAN ? 1 : 0, d.loss);
+  JoinArgs ja{p.part_m, p.part_l, p.hit, p.tgt, p.place, p.counted, p.lse2, d.reduction == R3D_CE_NONE ? d.loss : nullptr, d.loss, p.sums, d.n, p.n_pad,
+              p.lse_splits, mean};
+  hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((d.n + 255) / 256)), dim3(256), 0, st, ja);
 }
 
 template <class T, class S, int kPlanes>
@@ -793,26 +880,40 @@ void out_product(OutArgs a, int64_t m, int64_t n, hipStream_t st) {
 }
 
 template <class V>
-void finish(const FinishArgs &a, hipStream_t st) {
-  const bool four = a.width % 4 == 0 && a.ld % 4 == 0 && a.ld_out % 4 == 0 && (reinterpret_cast<uintptr_t>(a.out) % (4 * sizeof(V))) == 0;
-  const int64_t threads = a.rows * a.width / (four ? 4 : 1);
-  if (four) hipLaunchKernelGGL((k_ce_finish<V, 4>), dim3(blocks_for(threads, 256, 8192)), dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((k_ce_finish<V, 1>), dim3(blocks_for(threads, 256, 8192)), dim3(256), 0, st, a);
+Finish finish_of(const float *acc, int64_t ld, int64_t split_stride, int64_t rows, int64_t width, int splits, const int32_t *place, void *out) {
+  const bool vector = width % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(V)) == 0;
+  return Finish{acc, ld, split_stride, rows, width, splits, vector, place, out};
+}
+
+template <class V>
+void finish(const Finish *of, int n, const Plan &p, float unheld, hipStream_t st) {
+  FinishArgs a{};
+  a.scale = p.scale;
+  a.unheld = unheld;
+  int64_t most = 0;
+  for (int i = 0; i < n; ++i) {
+    a.of[i] = of[i];
+    const int64_t threads = of[i].rows * ((of[i].width + 3) / 4) * (of[i].splits >= 8 ? 4 : 1);
+    if (threads > most) most = threads;
+  }
+  if (n) hipLaunchKernelGGL(k_ce_finish<V>, dim3(blocks_for(most, 256, 8192), n), dim3(256), 0, st, a);
 }
 
 template <class S, class T, int kPlanes>
 void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
-  const Counted *counted = static_cast<const Counted *>(d.counted);
   const bool each = d.reduction == R3D_CE_NONE;
   const int parts = each && d.type == R3D_T_F16 ? p.top_parts : 0;
-  if (parts) hipLaunchKernelGGL(k_ce_top, dim3(parts), dim3(256), 0, st, d.grad, d.n, d.place, p.top);
-  hipLaunchKernelGGL(k_ce_weight, dim3(blocks_for(p.n_pad, 256, 1 << 30)), dim3(256), 0, st,
-                     WeightArgs{d.grad, p.top, each ? 1 : 0, parts, d.idx, counted, p.scale, p.weight, p.n_pad});
+  if (parts) hipLaunchKernelGGL(k_ce_top, dim3(parts), dim3(256), 0, st, d.grad, d.n, p.place, p.top);
+  hipLaunchKernelGGL(k_ce_weight<S>, dim3((unsigned)(p.n_pad / 256)), dim3(256), 0, st,
+                     WeightArgs{d.grad, p.top, each ? 1 : 0, parts, p.idx, p.place, p.counted, p.scale, p.weight, d.n, p.n_pad, d.d,
+                                p.dx_final ? d.dx : nullptr});
   Operand x, w;
-  operands<S, T, kPlanes>(d, p, counted, st, x, w);
+  operands(d, p, x, w);
   const float held = d.type == R3D_T_F16 ? 32768.0f : 1.0f, unheld = 1.0f / held;
   for (int64_t v0 = 0; v0 < d.v; v0 += p.piece) {
     const int64_t real_v = p.piece < d.v - v0 ? p.piece : d.v - v0, width = up(real_v, kPadK);
+    Finish of[3];
+    int n_of = 0;
     DlArgs da{};
     da.p = Product{w, x, kPlanes};
     da.v = d.v;
@@ -823,10 +924,10 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     da.width = (int)width;
     da.held = held;
     da.bias2 = p.bias2;
-    da.lse2 = d.lse2;
+    da.lse2 = p.lse2;
     da.weight = p.weight;
-    da.tgt = d.tgt;
-    da.counted = counted;
+    da.tgt = p.tgt;
+    da.counted = p.counted;
     da.dl = p.dl;
     if (p.dl_big) dl_piece<T, Big, kPlanes>(da, d.n, st);
     else dl_piece<T, Small, kPlanes>(da, d.n, st);
@@ -843,16 +944,17 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       oa.points = 1;
       oa.splits = p.dx_splits;
       oa.add = v0 > 0;
-      oa.counted = counted;
+      oa.counted = p.counted;
       oa.out = p.accx;
       oa.ld = p.dx_final ? d.d : p.dp;
       oa.split_stride = p.n_pad * p.dp;
       oa.final_out = p.dx_final ? d.dx : nullptr;
-      oa.idx = d.idx;
+      oa.idx = p.idx;
       oa.scale = p.scale;
       oa.unheld = unheld;
       if (p.dx_big) out_product<S, T, Big, Lies::PiecesRows>(oa, d.n, p.dp, st);
       else out_product<S, T, Small, Lies::PiecesRows>(oa, d.n, p.dp, st);
+      if (!p.dx_final && v0 + p.piece >= d.v) of[n_of++] = finish_of<S>(p.accx, p.dp, p.n_pad * p.dp, d.n, d.d, p.dx_splits, p.place, d.dx);
     }
     if (d.dw || d.db) {
       const bool straight = p.dw_final && d.dw;
@@ -864,7 +966,7 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       oa.limit_b = p.dp;
       oa.points = 2;
       oa.splits = p.dw_splits;
-      oa.counted = counted;
+      oa.counted = p.counted;
       oa.out = p.accw;
       oa.ld = straight ? d.d : p.dp;
       oa.split_stride = p.piece * p.dp;
@@ -876,42 +978,36 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       if (p.dw_big) out_product<S, T, Big, Lies::PiecesCols>(oa, width, p.dp, st);
       else out_product<S, T, Small, Lies::PiecesCols>(oa, width, p.dp, st);
       if (d.dw && !straight)
-        finish<S>(FinishArgs{p.accw, p.dp, p.piece * p.dp, real_v, d.d, d.d, p.dw_splits, unheld, nullptr, p.scale,
-                             static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes}, st);
-      if (d.db)
-        finish<S>(FinishArgs{p.accb, 1, p.piece, real_v, 1, 1, p.dw_splits, unheld, nullptr, p.scale, static_cast<char *>(d.db) + v0 * p.type_bytes}, st);
+        of[n_of++] = finish_of<S>(p.accw, p.dp, p.piece * p.dp, real_v, d.d, p.dw_splits, nullptr, static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes);
+      if (d.db) of[n_of++] = finish_of<S>(p.accb, p.piece, p.piece, 1, real_v, p.dw_splits, nullptr, static_cast<char *>(d.db) + v0 * p.type_bytes);
     }
+    finish<S>(of, n_of, p, unheld, st);
   }
-  if (d.dx && p.dx_final)
-    hipLaunchKernelGGL(k_ce_zero<S>, dim3(blocks_for(d.n, 4, 2048)), dim3(256), 0, st, static_cast<S *>(d.dx), d.n, d.d, d.place);
-  else if (d.dx)
-    finish<S>(FinishArgs{p.accx, p.dp, p.n_pad * p.dp, d.n, d.d, d.d, p.dx_splits, unheld, d.place, p.scale, d.dx}, st);
 }
 }  // namespace
 
-extern "C" size_t r3d_linear_ce_workspace_bytes(const r3d_linear_ce_t *d, int32_t backward_pass) {
-  if (check(d) != R3D_OK) return 0;
-  const size_t few = few_bytes(*d, backward_pass != 0);
-  return few ? few : plan(*d, backward_pass != 0, nullptr).bytes;
+extern "C" size_t r3d_linear_ce_bytes(const r3d_linear_ce_t *d, int32_t which) {
+  if (check(d) != R3D_OK || which < R3D_CE_BYTES_STATE || which > R3D_CE_BYTES_BACKWARD) return 0;
+  if (few_takes(*d)) return few_bytes(*d, which);
+  const Plan p = plan(*d, which == R3D_CE_BYTES_BACKWARD, nullptr);
+  return which == R3D_CE_BYTES_STATE ? p.state_bytes : p.bytes;
 }
 
 extern "C" int r3d_linear_ce_forward(const r3d_linear_ce_t *d, void *workspace, size_t workspace_bytes, void *stream) {
   int rc = check(d);
   if (rc != R3D_OK) return rc;
-  if (!d->x || !d->w || !d->target || !d->idx || !d->place || !d->tgt || !d->lse2 || !d->counted || !d->loss || !workspace)
-    return fail(R3D_E_ARG, "linear_ce_forward: null pointer");
-  if (workspace_bytes < r3d_linear_ce_workspace_bytes(d, 0)) return fail(R3D_E_WORKSPACE, "linear_ce_forward: workspace too small");
+  if (!d->x || !d->w || !d->target || !d->state || !d->loss || !workspace) return fail(R3D_E_ARG, "linear_ce_forward: null pointer");
+  if (workspace_bytes < r3d_linear_ce_bytes(d, R3D_CE_BYTES_FORWARD)) return fail(R3D_E_WORKSPACE, "linear_ce_forward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (few_bytes(*d, false)) {
+  if (few_takes(*d)) {
     rc = few_forward(*d, workspace, st);
     if (rc != R3D_OK) return rc;
-    R3D_LAUNCHED("linear_ce forward kernels, few classes");
-    return R3D_OK;
+  } else {
+    const Plan p = plan(*d, false, workspace);
+    if (d->type == R3D_T_F32) forward<float, __bf16, 3>(*d, p, st);
+    else if (d->type == R3D_T_BF16) forward<__bf16, __bf16, 1>(*d, p, st);
+    else forward<_Float16, _Float16, 1>(*d, p, st);
   }
-  const Plan p = plan(*d, false, workspace);
-  if (d->type == R3D_T_F32) forward<float, __bf16, 3>(*d, p, st);
-  else if (d->type == R3D_T_BF16) forward<__bf16, __bf16, 1>(*d, p, st);
-  else forward<_Float16, _Float16, 1>(*d, p, st);
   R3D_LAUNCHED("linear_ce forward kernels");
   return R3D_OK;
 }
@@ -919,20 +1015,18 @@ extern "C" int r3d_linear_ce_forward(const r3d_linear_ce_t *d, void *workspace, 
 extern "C" int r3d_linear_ce_backward(const r3d_linear_ce_t *d, void *workspace, size_t workspace_bytes, void *stream) {
   int rc = check(d);
   if (rc != R3D_OK) return rc;
-  if (!d->x || !d->w || !d->idx || !d->place || !d->tgt || !d->lse2 || !d->counted || !d->grad || !workspace)
-    return fail(R3D_E_ARG, "linear_ce_backward: null pointer");
-  if (workspace_bytes < r3d_linear_ce_workspace_bytes(d, 1)) return fail(R3D_E_WORKSPACE, "linear_ce_backward: workspace too small");
+  if (!d->x || !d->w || !d->target || !d->state || !d->grad || !workspace) return fail(R3D_E_ARG, "linear_ce_backward: null pointer");
+  if (workspace_bytes < r3d_linear_ce_bytes(d, R3D_CE_BYTES_BACKWARD)) return fail(R3D_E_WORKSPACE, "linear_ce_backward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (few_bytes(*d, true)) {
+  if (few_takes(*d)) {
     rc = few_backward(*d, workspace, st);
     if (rc != R3D_OK) return rc;
-    R3D_LAUNCHED("linear_ce backward kernels, few classes");
-    return R3D_OK;
+  } else {
+    const Plan p = plan(*d, true, workspace);
+    if (d->type == R3D_T_F32) backward<float, __bf16, 3>(*d, p, st);
+    else if (d->type == R3D_T_BF16) backward<__bf16, __bf16, 1>(*d, p, st);
+    else backward<_Float16, _Float16, 1>(*d, p, st);
   }
-  const Plan p = plan(*d, true, workspace);
-  if (d->type == R3D_T_F32) backward<float, __bf16, 3>(*d, p, st);
-  else if (d->type == R3D_T_BF16) backward<__bf16, __bf16, 1>(*d, p, st);
-  else backward<_Float16, _Float16, 1>(*d, p, st);
   R3D_LAUNCHED("linear_ce backward kernels");
   return R3D_OK;
 }

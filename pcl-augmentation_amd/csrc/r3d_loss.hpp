@@ -12,7 +12,8 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 struct Counted {      // the points that count, on the device
   int32_t n;          // how many
   float share;        // 1 / n for a mean (0 where none counts), 1 else
-  float pad[2];
+  int32_t ticket;     // workgroups that have left their part of a sum
+  int32_t pad;
 };
 
 __device__ __forceinline__ __bf16 toward_zero(float v) {      // (rounding up the largest floats would give infinities)
@@ -26,8 +27,9 @@ __device__ __forceinline__ void split3(float v, __bf16 &h, __bf16 &m, __bf16 &l)
   l = (__bf16)(r - (float)m);
 }
 
-// Few classes: workspace (0: not this head), the two passes.
-size_t few_bytes(const r3d_linear_ce_t &d, bool backward);
+// Few classes: whether a head is that, the bytes of R3D_CE_BYTES_*, the two passes.
+bool few_takes(const r3d_linear_ce_t &d);
+size_t few_bytes(const r3d_linear_ce_t &d, int32_t which);
 int few_forward(const r3d_linear_ce_t &d, void *workspace, hipStream_t st);
 int few_backward(const r3d_linear_ce_t &d, void *workspace, hipStream_t st);
 

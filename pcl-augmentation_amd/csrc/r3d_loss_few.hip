@@ -551,9 +551,15 @@ FewArgs few_args(const r3d_linear_ce_t &d, const FewPlan &p) {
 
 namespace r3d {
 
-size_t few_bytes(const r3d_linear_ce_t &d, bool backward) {
+bool few_takes(const r3d_linear_ce_t &d) {
   FewPlan p;
-  return few_plan(d, p) ? few_space(p, backward, nullptr).bytes : 0;
+  return few_plan(d, p);
+}
+
+size_t few_bytes(const r3d_linear_ce_t &d, int32_t which) {
+  FewPlan p;
+  few_plan(d, p);
+  return which == R3D_CE_BYTES_STATE ? sizeof(Counted) : few_space(p, which == R3D_CE_BYTES_BACKWARD, nullptr).bytes;
 }
 
 int few_forward(const r3d_linear_ce_t &d, void *workspace, hipStream_t st) {
@@ -566,7 +572,7 @@ int few_forward(const r3d_linear_ce_t &d, void *workspace, hipStream_t st) {
   a.counts = s.counts;
   const int rc = by_type<false>(d, a, p, st);
   if (rc != R3D_OK) return rc;
-  hipLaunchKernelGGL(k_few_mean, dim3(1), dim3(256), 0, st, s.sums, s.counts, p.groups, d.reduction, d.loss, static_cast<Counted *>(d.counted));
+  hipLaunchKernelGGL(k_few_mean, dim3(1), dim3(256), 0, st, s.sums, s.counts, p.groups, d.reduction, d.loss, static_cast<Counted *>(d.state));
   return R3D_OK;
 }
 
@@ -578,7 +584,7 @@ int few_backward(const r3d_linear_ce_t &d, void *workspace, hipStream_t st) {
   const bool half = d.type == R3D_T_F16;
   a.grad = d.grad;
   a.grad_each = d.reduction == R3D_CE_NONE;
-  a.counted = static_cast<const Counted *>(d.counted);
+  a.counted = static_cast<const Counted *>(d.state);
   a.top = s.top;
   a.parts = a.grad_each && half ? blocks_for(d.n, 256, kTopParts) : 0;
   a.held = half ? 32768.0f : 1.0f;

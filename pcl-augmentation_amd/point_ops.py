@@ -133,7 +133,9 @@ def rotary_positions(query, positions, sections, key=None, base=10000.0, style="
     if not base > 0.0 or base == float("inf"):
         raise ValueError("rotary_positions: base must be positive and finite")
     on_device_of("rotary_positions", query, positions, *(() if key is None else (key,)))
-    return _rotary_function().apply(query, key, positions, sections, base, style == "interleaved")
+    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+        return _rotary_function().apply(query, key, positions, sections, base, style == "interleaved")
+    return tuple(_turn((query, key), positions, sections, base, style == "interleaved", False))
 
 
 # ---- softmax cross entropy of a linear head ------------------------------------------------------------------------------
@@ -144,15 +146,13 @@ def _loss_function():
 
     def follow(d, x, weight, bias, target, state):
         """The descriptor's tensors (in the backward pass: as they come back from where they were kept)."""
-        n, at = d.n, state.data_ptr()
         d.x, d.w, d.bias, d.target = x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), target.data_ptr()
-        d.counted, d.idx, d.place, d.tgt, d.lse2 = at, at + 16, at + 16 + 4 * n, at + 16 + 8 * n, at + 16 + 12 * n
-        d.ld_x, d.ld_w = x.stride(0), weight.stride(0)
+        d.ld_x, d.ld_w, d.state = x.stride(0), weight.stride(0), 0 if state is None else state.data_ptr()
 
-    def workspace(lib, d, backward, device):
-        size = lib.r3d_linear_ce_workspace_bytes(C.byref(d), backward)
+    def space(lib, d, which, device):
+        size = lib.r3d_linear_ce_bytes(C.byref(d), which)
         if size == 0:
-            _lib.check(_lib.E_ARG, "r3d_linear_ce_workspace_bytes")
+            _lib.check(_lib.E_ARG, "r3d_linear_ce_bytes")
         return torch.empty(size, dtype=torch.uint8, device=device), size
 
     class LinearCrossEntropy(torch.autograd.Function):
@@ -161,13 +161,14 @@ def _loss_function():
             n = x.shape[0]
             with on_device_of("linear_cross_entropy", x):
                 lib = _lib.load()
-                state = torch.empty(4 + 4 * n, dtype=torch.int32, device=x.device)
                 loss = torch.empty(n if how[1] == _lib.CE_NONE else (), dtype=torch.float32, device=x.device)
                 types = _types()
                 d = _lib.LinearCE(n=n, v=weight.shape[0], d=x.shape[1], ignore_index=how[0], reduction=how[1], piece=how[2],
                                   type=types[0][x.dtype], target_type=types[1][target.dtype], loss=loss.data_ptr())
-                follow(d, x, weight, bias, target, state)
-                ws, size = workspace(lib, d, 0, x.device)
+                follow(d, x, weight, bias, target, None)
+                state, _ = space(lib, d, _lib.CE_BYTES_STATE, x.device)
+                d.state = state.data_ptr()
+                ws, size = space(lib, d, _lib.CE_BYTES_FORWARD, x.device)
                 _lib.check(lib.r3d_linear_ce_forward(C.byref(d), ws.data_ptr(), size, _lib.raw_stream(x.get_device())), "r3d_linear_ce_forward")
             ctx.save_for_backward(x, weight, bias, target, state)
             ctx.descriptor = d
@@ -181,13 +182,15 @@ def _loss_function():
             with on_device_of("linear_cross_entropy", x):
                 lib = _lib.load()
                 d = _lib.LinearCE.from_buffer_copy(ctx.descriptor)      # (two backward passes may run at once)
+                # what was multiplied in place still has to be fit for it, wherever it was kept in the meantime
+                x, weight = (t.clone() if t.data_ptr() % 16 and not at % 16 else t for t, at in ((x, d.x), (weight, d.w)))
                 follow(d, x, weight, bias, target, state)
                 grad = grad.to(torch.float32).contiguous()
                 d.grad = grad.data_ptr()
                 new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
                 dx, dw, db = (new(x) if need[0] else None, new(weight) if need[1] else None, new(bias) if need[2] else None)
                 d.dx, d.dw, d.db = (0 if o is None else o.data_ptr() for o in (dx, dw, db))
-                ws, size = workspace(lib, d, 1, x.device)
+                ws, size = space(lib, d, _lib.CE_BYTES_BACKWARD, x.device)
                 _lib.check(lib.r3d_linear_ce_backward(C.byref(d), ws.data_ptr(), size, _lib.raw_stream(x.get_device())), "r3d_linear_ce_backward")
             return dx, dw, db, None, None
 

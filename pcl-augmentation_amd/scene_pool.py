@@ -6,6 +6,7 @@ the pages it needs.  Tensors on the GPU in and out, on the current stream, no ho
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import NamedTuple
 
 from . import _lib
@@ -111,9 +112,7 @@ def _move(what, sources, dests, src_slots, dst_slots, n):
     arrays = (_lib.Rows * len(sources))()
     for a, s, t in zip(arrays, sources, dests):
         size = s.element_size()
-        width = size
-        for e in s.shape[1:]:
-            width *= e
+        width = size * math.prod(s.shape[1:])
         a.src, a.dst, a.row_bytes = s.data_ptr(), t.data_ptr(), width
         a.src_stride, a.dst_stride = (s.stride(0) * size if s.shape[0] > 1 else width), (t.stride(0) * size if t.shape[0] > 1 else width)
     _lib.check(_lib.load().r3d_move_rows(arrays, len(sources), 0 if src_slots is None else src_slots.data_ptr(),
@@ -131,6 +130,8 @@ def _rows_of(what, name, tensors, like=None):
             raise ValueError(f"{what}: {name} must have the same number of rows")
         if t.requires_grad:
             raise ValueError(f"{what}: no gradient passes through moved rows (detach them)")
+        if t.is_contiguous() and t.numel():
+            continue
         width = 1
         for e, s in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
             if e != 1 and s != width:

@@ -40,13 +40,14 @@ def test_c_entries_refuse_without_a_gpu(pkg):
     d.sections[0], d.base = 4, -1.0
     assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG
     e = L.LinearCE(n=4, v=3, d=8, ld_x=8, ld_w=8, type=L.T_F32, target_type=L.T_I64, reduction=L.CE_MEAN)
-    assert lib.r3d_linear_ce_workspace_bytes(C.byref(e), 0) > 0 and lib.r3d_linear_ce_workspace_bytes(C.byref(e), 1) > 0
+    assert all(lib.r3d_linear_ce_bytes(C.byref(e), which) > 0 for which in (0, 1, 2))
+    assert lib.r3d_linear_ce_bytes(C.byref(e), 3) == 0 and lib.r3d_linear_ce_bytes(C.byref(e), -1) == 0
     assert lib.r3d_linear_ce_forward(C.byref(e), None, 0, None) == L.E_ARG
     assert lib.r3d_linear_ce_backward(C.byref(e), None, 0, None) == L.E_ARG
     for name, value in (("n", 0), ("v", 0), ("d", 0), ("ld_x", 7), ("type", L.T_F64), ("target_type", L.T_F32), ("reduction", 3), ("piece", -1)):
         old = getattr(e, name)
         setattr(e, name, value)
-        assert lib.r3d_linear_ce_workspace_bytes(C.byref(e), 0) == 0, name
+        assert lib.r3d_linear_ce_bytes(C.byref(e), 0) == 0, name
         setattr(e, name, old)
 
 
@@ -54,7 +55,7 @@ def test_descriptors_match_the_header(pkg):
     L = pkg._lib
     assert C.sizeof(L.Rows) == 2 * 8 + 3 * 8
     assert C.sizeof(L.Rotary) == 4 * 8 + 4 * 8 + 8 + 2 * 4 + 4 * 4 + 4 + 8 * 4 + 4 + 8 + 2 * 8 + 8
-    assert C.sizeof(L.LinearCE) == 4 * 8 + 7 * 8 + 4 * 4 + 10 * 8
+    assert C.sizeof(L.LinearCE) == 4 * 8 + 7 * 8 + 4 * 4 + 6 * 8
 
 
 def test_block_tables_refuses(pkg):
