@@ -90,9 +90,13 @@ __device__ __forceinline__ void store_piece(T *to, int plane, uint4 piece) {
   }
 }
 
+// Waves a SIMD the registers are cut for: what the tile's LDS lets stand beside each other anyway.  480 000 x 20 x 96 bf16,
+// backward: 68 us with one, 57 with three; 200 000 x 20 x 256: 114 with one, 69 with two; 512 features: 218 with one, 270 with two.
+constexpr int few_waves(int planes, int vt, int nb) { return planes == 3 ? (vt * nb == 1 ? 2 : 1) : vt * nb == 1 ? 3 : vt * nb == 2 ? 2 : 1; }
+
 // kVT: blocks of 32 classes; kNB: blocks of 32 features of dW a wave keeps (dp <= 128 kNB); kTP: points of a tile.
 template <class V, class T, int kPlanes, int kVT, int kNB, int kTP, bool kGrad>
-__global__ __launch_bounds__(kThreads, 1) void k_few(FewArgs a) {
+__global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(FewArgs a) {
   constexpr int kEach = 16 / sizeof(V), kPer = kTP * kNB * 128 / kEach / kThreads, kPv = kVT * 32 + 8;
   constexpr int kPairCount = kPlanes == 3 ? kPairs : 1;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -457,7 +461,7 @@ bool few_plan(const r3d_linear_ce_t &d, FewPlan &p) {
   p.vt = d.v <= 32 ? 1 : d.v <= 64 ? 2 : 4;
   p.nb = p.dp <= 128 ? 1 : p.dp <= 256 ? 2 : 4;
   if (p.vt * p.nb > 8 || (planes == 3 && (p.vt == 4 || p.nb == 4))) return false;
-  p.tp = p.nb == 4 || p.vt * p.nb == 8 || (planes == 3 && (p.nb == 2 || p.vt == 2)) ? 64 : 128;
+  p.tp = p.nb >= 2 || planes == 3 ? 64 : 128;      // (two workgroups a CU beat one with the longer tile: 200 000 x 20 x 256 forward 58 -> 38 us)
   const size_t pitch = p.dp + 8;
   p.lds_forward = (size_t)planes * 2 * (p.tp + p.vt * 32) * pitch + p.vt * 32 * 4 + (size_t)p.tp * 16;
   p.lds_backward = p.lds_forward + (size_t)planes * 2 * p.tp * (p.vt * 32 + 8);
@@ -502,7 +506,7 @@ int dispatch(const FewArgs &a, const FewPlan &p, hipStream_t st) {
   const int key = p.vt * 10 + p.nb;
   if constexpr (kPlanes == 3) {
     switch (key) {
-      case 11: return launch<V, T, 3, 1, 1, 128, kGrad>(a, p, st);
+      case 11: return launch<V, T, 3, 1, 1, 64, kGrad>(a, p, st);
       case 12: return launch<V, T, 3, 1, 2, 64, kGrad>(a, p, st);
       case 21: return launch<V, T, 3, 2, 1, 64, kGrad>(a, p, st);
       default: return launch<V, T, 3, 2, 2, 64, kGrad>(a, p, st);
@@ -510,10 +514,10 @@ int dispatch(const FewArgs &a, const FewPlan &p, hipStream_t st) {
   } else {
     switch (key) {
       case 11: return launch<V, T, 1, 1, 1, 128, kGrad>(a, p, st);
-      case 12: return launch<V, T, 1, 1, 2, 128, kGrad>(a, p, st);
+      case 12: return launch<V, T, 1, 1, 2, 64, kGrad>(a, p, st);
       case 14: return launch<V, T, 1, 1, 4, 64, kGrad>(a, p, st);
       case 21: return launch<V, T, 1, 2, 1, 128, kGrad>(a, p, st);
-      case 22: return launch<V, T, 1, 2, 2, 128, kGrad>(a, p, st);
+      case 22: return launch<V, T, 1, 2, 2, 64, kGrad>(a, p, st);
       case 24: return launch<V, T, 1, 2, 4, 64, kGrad>(a, p, st);
       case 41: return launch<V, T, 1, 4, 1, 128, kGrad>(a, p, st);
       default: return launch<V, T, 1, 4, 2, 64, kGrad>(a, p, st);

@@ -5,7 +5,6 @@ the pages it needs.  Tensors on the GPU in and out, on the current stream, no ho
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
 from typing import NamedTuple
 
