@@ -673,10 +673,175 @@ __global__ __launch_bounds__(256) void k_ce_finish(FinishArgs all) {
   }
 }
 
+// ---- a head that fits LDS ------------------------------------------------------------------------------------------------------
+// Up to 288 classes of the 16-bit types: the head stands in LDS once a workgroup, and a wave goes its way alone, 32 points a
+// time, without a barrier.  Their features come from memory as the fragments that the product takes (two lanes share a row: 32
+// bytes each time, the rest of the cache line with the next k-steps), all classes' logits are in its registers, and in the
+// backward pass dx = dl W is multiplied from there: the classes of a k-step are taken in the order in which the lanes have them.
+constexpr int kHeadThreads = 512, kHeadBlocks = 9;
+
+struct HeadArgs {
+  Operand w, x;
+  int64_t v, d;
+  int32_t dp, ldo;
+  const float *bias2;
+  const int32_t *tgt, *idx;
+  const Counted *counted;
+  float *part_m, *part_l, *hit;      // forward
+  // backward
+  const float *lse2, *weight, *scale;
+  float held, unheld;
+  void *dl, *dx;                     // dl: pieces of 8 classes, or null
+  int64_t n_pad;
+  int32_t vector_out;
+};
+
+template <class T, int kVB, bool kGrad>
+__global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
+  typedef typename Mma<T>::v8 v8;
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int pitch = a.dp + 8;      // an odd number of 16 bytes: rows begin on different banks
+  T *ws = reinterpret_cast<T *>(smem);
+  float *bias2 = reinterpret_cast<float *>(ws + kVB * 32 * pitch);
+  const int lane = threadIdx.x & 63, half = lane >> 5, low = lane & 31, group = lane >> 4, sub = lane & 15;
+  const int nc = a.counted->n, cols = a.dp / 8;
+  if (blockIdx.x * 32 >= nc) return;
+  for (int i0 = threadIdx.x; i0 < kVB * 32 * cols; i0 += 6 * kHeadThreads) {      // (six loads on their way: 147 KB are 18 a thread)
+    v8 v[6];
+    int to[6];
+#pragma unroll
+    for (int e = 0; e < 6; ++e) {
+      const int i = i0 + e * kHeadThreads, r = (unsigned)i / (unsigned)cols, c = (i - r * cols) * 8;
+      to[e] = r < kVB * 32 ? r * pitch + c : -1;
+      const int from = r < a.v ? r : (int)a.v - 1;      // (classes behind the last one: probability 0 by their bias)
+      v[e] = *reinterpret_cast<const v8 *>(static_cast<const T *>(a.w.p) + from * a.w.ld + c);
+    }
+#pragma unroll
+    for (int e = 0; e < 6; ++e)
+      if (to[e] >= 0) *reinterpret_cast<v8 *>(ws + to[e]) = v[e];
+  }
+  for (int i = threadIdx.x; i < kVB * 32; i += kHeadThreads) bias2[i] = a.bias2[i];
+  __syncthreads();
+  const float out_scale = kGrad && a.dx ? *a.scale * a.unheld : 1.0f;
+  // neighbouring tiles go to different workgroups, so that a few tiles are a few workgroups' too
+  for (int64_t tile = blockIdx.x + (int64_t)gridDim.x * (threadIdx.x >> 6); tile * 32 < nc; tile += (int64_t)gridDim.x * (kHeadThreads / 64)) {
+    const int64_t point = tile * 32 + low;
+    const bool in = point < nc;
+    const int64_t row = a.idx[in ? point : nc - 1];
+    const T *x = static_cast<const T *>(a.x.p) + row * a.x.ld + half * 8;
+    f32x16 acc[kVB];
+#pragma unroll
+    for (int v = 0; v < kVB; ++v)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[v][r] = 0.0f;
+    v8 f[2][4];
+    auto features = [&](int k, int into) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[into][e] = *reinterpret_cast<const v8 *>(x + k + e * 16);
+    };
+    auto multiply = [&](int k, int of) {
+      const T *w = ws + low * pitch + half * 8 + k;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int v = 0; v < kVB; ++v) acc[v] = Mma<T>::mma(*reinterpret_cast<const v8 *>(w + v * 32 * pitch + e * 16), f[of][e], acc[v]);
+    };
+    features(0, 0);
+    int k = 0;
+    for (; k + 128 <= a.dp; k += 128) {      // (dp is a multiple of 64)
+      features(k + 64, 1);
+      multiply(k, 0);
+      if (k + 128 < a.dp) features(k + 128, 0);
+      multiply(k + 64, 1);
+    }
+    if (k < a.dp) multiply(k, 0);
+    const int t = in ? a.tgt[point] : -1;
+    if constexpr (!kGrad) {
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kVB; ++v)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          acc[v][r] = __builtin_fmaf(acc[v][r], kLog2e, bias2[v * 32 + mma_row(r)]);
+          top = fmaxf(top, acc[v][r]);
+          if (t == v * 32 + mma_row(r)) a.hit[point] = acc[v][r];
+        }
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int v = 0; v < kVB; ++v)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(acc[v][r] - base);
+      sum += __shfl_xor(sum, 32);
+      if (in && half == 0) {
+        a.part_m[point] = top;
+        a.part_l[point] = sum;
+      }
+    } else {
+      typedef unsigned u2 __attribute__((ext_vector_type(2)));
+      typedef unsigned u4 __attribute__((ext_vector_type(4)));
+      const float lse2 = in ? a.lse2[point] : 0.0f, by = in ? a.weight[point] * a.held : 0.0f;
+      t4 q[kVB][4];
+#pragma unroll
+      for (int v = 0; v < kVB; ++v) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v][r], kLog2e, bias2[v * 32 + mma_row(r)]) - lse2);
+          p -= t == v * 32 + mma_row(r) ? 1.0f : 0.0f;
+          q[v][r >> 2][r & 3] = (T)(in ? p * by : 0.0f);
+        }
+        __builtin_amdgcn_sched_barrier(0);      // (a block at a time: all blocks' addresses and biases at once spill)
+      }
+      if (a.dl) {
+#pragma unroll
+        for (int v = 0; v < kVB; ++v)
+#pragma unroll
+          for (int h = 0; h < 4; h += 2) {
+            const u2 even = __builtin_bit_cast(u2, q[v][h]), odd = __builtin_bit_cast(u2, q[v][h + 1]);
+            const auto s0 = __builtin_amdgcn_permlane32_swap(even[0], odd[0], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(even[1], odd[1], false, false);
+            const u4 out = {s0[0], s1[0], s0[1], s1[1]};
+            *reinterpret_cast<u4 *>(static_cast<T *>(a.dl) + ((int64_t)(v * 4 + h + half) * a.n_pad + point) * 8) = out;
+          }
+      }
+      if (a.dx) {
+        const T *wt = ws + (4 * half + (sub >> 2)) * pitch + (group & 1) * 16 + (sub & 3) * 4;
+        T *out = static_cast<T *>(a.dx) + row * a.d;
+        for (int f0 = 0; f0 < a.d; f0 += 32) {
+          f32x16 g;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) g[r] = 0.0f;
+#pragma unroll
+          for (int v = 0; v < kVB; ++v) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+              g = Mma<T>::mma(turned<T>(wt + (v * 32 + 16 * s) * pitch + f0, wt + (v * 32 + 16 * s + 8) * pitch + f0),
+                              __builtin_shufflevector(q[v][2 * s], q[v][2 * s + 1], 0, 1, 2, 3, 4, 5, 6, 7), g);
+            if (v % 3 == 2) __builtin_amdgcn_sched_barrier(0);
+          }
+          if (!in) continue;
+          if (a.vector_out && f0 + 32 <= a.d) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const t4 o = {(T)(g[4 * h] * out_scale), (T)(g[4 * h + 1] * out_scale), (T)(g[4 * h + 2] * out_scale), (T)(g[4 * h + 3] * out_scale)};
+              *reinterpret_cast<t4 *>(out + f0 + 8 * h + 4 * half) = o;
+            }
+          } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              if (f0 + mma_row(r) < a.d) out[f0 + mma_row(r)] = (T)(g[r] * out_scale);
+          }
+        }
+      }
+    }
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------------------------------------
 // What a piece's dl may take.  8192 points x 161280 classes x 512: 8.8 ms with 64 MB, 7.1 with 256, 6.7 with 512, 6.4 with all 2.6 GB.
 constexpr int64_t kPieceBytes = 512ll << 20;
-constexpr int kCus = 256;
+constexpr int kCus = 256, kHeadLds = 160 * 1024;
 constexpr int kPadK = 64;      // operands are padded to whole cache lines along k
 
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
@@ -712,6 +877,8 @@ struct Plan {
   int64_t dp, n_pad, v_pad, piece;
   bool lse_big, dl_big, dx_big, dw_big;
   int lse_splits, dx_splits, dw_splits, top_parts, groups;
+  int head;                     // blocks of 32 classes of a head that fits LDS, or 0
+  size_t head_lds;
   bool dx_final, dw_final;      // nothing to add: straight into the result
   // kept from the forward to the backward pass
   Counted *counted;
@@ -738,6 +905,8 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   p.dp = up(d.d, kPadK);
   p.n_pad = up(d.n, Big::BN);
   p.v_pad = up(d.v, Big::BM);
+  p.head_lds = (size_t)up(d.v, 32) * (p.dp + 8) * 2 + up(d.v, 32) * 4;
+  p.head = p.planes == 1 && d.v <= kHeadBlocks * 32 && p.head_lds <= (size_t)kHeadLds ? (int)(up(d.v, 32) / 32) : 0;
   p.groups = d.n <= kOneGroup ? 1 : (int)((d.n + kStartRows - 1) / kStartRows);
   Carver k(d.state);
   p.counted = k.take<Counted>(1);
@@ -755,7 +924,7 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   if (!backward) {
     p.lse_big = large_tiles(d.v, d.n, 1);
     const int64_t bm = p.lse_big ? Big::BM : Small::BM, bn = p.lse_big ? Big::BN : Small::BN;
-    p.lse_splits = cut(up(d.n, bn) / bn, kCus * (p.lse_big ? Big::per_cu : Small::per_cu), up(d.v, bm) / bm);
+    p.lse_splits = p.head ? 1 : cut(up(d.n, bn) / bn, kCus * (p.lse_big ? Big::per_cu : Small::per_cu), up(d.v, bm) / bm);
     p.part = c.take<int32_t>(p.groups);
     p.part_m = c.take<float>((size_t)p.lse_splits * p.n_pad);
     p.part_l = c.take<float>((size_t)p.lse_splits * p.n_pad);
@@ -767,7 +936,7 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     if (piece < Small::BM) piece = Small::BM;
     p.piece = piece < v64 ? piece : v64;
     if (d.piece == 0) p.piece = up((v64 + (v64 + p.piece - 1) / p.piece - 1) / ((v64 + p.piece - 1) / p.piece), Big::BM);      // pieces of one size
-    if (p.piece > v64) p.piece = v64;
+    if (p.piece > v64 || p.head) p.piece = v64;
     p.dl_big = large_tiles(p.piece, d.n, 1);
     const int64_t kx = p.piece / 256, kw = p.n_pad / 256;
     p.dx_big = large_tiles(d.n, p.dp, kx);
@@ -775,7 +944,7 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     auto tiles = [&](int64_t m, int64_t n, bool big) { return big ? tiles_of(m, n, Big::BM, Big::BN) : tiles_of(m, n, Small::BM, Small::BN); };
     p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus * (p.dx_big ? Big::per_cu : Small::per_cu), kx);
     p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus * (p.dw_big ? Big::per_cu : Small::per_cu), kw);
-    p.dx_final = p.dx_splits == 1 && p.piece >= d.v;
+    p.dx_final = p.head || (p.dx_splits == 1 && p.piece >= d.v);
     p.dw_final = p.dw_splits == 1;
     p.top_parts = (int)(d.n < 256 * 256 ? (d.n + 255) / 256 : 256);
     p.top = c.take<float>(p.top_parts);
@@ -819,6 +988,57 @@ void lse(LseArgs a, const Plan &p, int64_t n, int64_t v, hipStream_t st) {
   hipLaunchKernelGGL((k_ce_lse<T, S>), dim3((unsigned)(a.ntiles * p.lse_splits)), dim3(S::threads), 0, st, a);
 }
 
+void join(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
+  JoinArgs ja{p.part_m, p.part_l, p.hit, p.tgt, p.place, p.counted, p.lse2, d.reduction == R3D_CE_NONE ? d.loss : nullptr, d.loss, p.sums, d.n, p.n_pad,
+              p.lse_splits, d.reduction == R3D_CE_MEAN};
+  hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((d.n + 255) / 256)), dim3(256), 0, st, ja);
+}
+
+HeadArgs head_args(const r3d_linear_ce_t &d, const Plan &p) {
+  HeadArgs a{};
+  operands(d, p, a.x, a.w);
+  a.v = d.v;
+  a.d = d.d;
+  a.dp = (int)p.dp;
+  a.bias2 = p.bias2;
+  a.tgt = p.tgt;
+  a.idx = p.idx;
+  a.counted = p.counted;
+  a.part_m = p.part_m;
+  a.part_l = p.part_l;
+  a.hit = p.hit;
+  a.lse2 = p.lse2;
+  a.weight = p.weight;
+  a.scale = p.scale;
+  a.dl = p.dl;
+  a.dx = d.dx;
+  a.n_pad = p.n_pad;
+  a.vector_out = d.d % 4 == 0 && aligned16(d.dx);
+  return a;
+}
+
+template <class T, bool kGrad>
+int head(const HeadArgs &a, const Plan &p, int64_t n, hipStream_t st) {
+  const int64_t tiles = (n + 31) / 32;
+  auto run = [&](auto *kernel) {
+    if (p.head_lds > 64 * 1024)
+      R3D_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.head_lds));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles < kCus ? tiles : kCus)), dim3(kHeadThreads), p.head_lds, st, a);
+    return R3D_OK;
+  };
+  switch (p.head) {
+    case 1: return run(&k_ce_head<T, 1, kGrad>);
+    case 2: return run(&k_ce_head<T, 2, kGrad>);
+    case 3: return run(&k_ce_head<T, 3, kGrad>);
+    case 4: return run(&k_ce_head<T, 4, kGrad>);
+    case 5: return run(&k_ce_head<T, 5, kGrad>);
+    case 6: return run(&k_ce_head<T, 6, kGrad>);
+    case 7: return run(&k_ce_head<T, 7, kGrad>);
+    case 8: return run(&k_ce_head<T, 8, kGrad>);
+    default: return run(&k_ce_head<T, 9, kGrad>);
+  }
+}
+
 template <class S, class T, int kPlanes>
 void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   const bool mean = d.reduction == R3D_CE_MEAN;
@@ -845,6 +1065,11 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   }
   hipLaunchKernelGGL((k_ce_start<S, T, kPlanes>), dim3(sa.groups + sa.bias_blocks + sa.pack[0].blocks + sa.pack[1].blocks), dim3(kStartThreads), 0, st, sa);
   if (p.groups > 1) hipLaunchKernelGGL(k_ce_index, dim3(p.groups), dim3(kStartThreads), 0, st, sa);
+  if (p.head) {
+    if constexpr (kPlanes == 1) head<T, false>(head_args(d, p), p, d.n, st);
+    join(d, p, st);
+    return;
+  }
   LseArgs la{};
   operands(d, p, la.p.b, la.p.a);
   la.p.planes = kPlanes;
@@ -860,9 +1085,7 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   la.n_pad = p.n_pad;
   if (p.lse_big) lse<T, Big>(la, p, d.n, d.v, st);
   else lse<T, Small>(la, p, d.n, d.v, st);
-  JoinArgs ja{p.part_m, p.part_l, p.hit, p.tgt, p.place, p.counted, p.lse2, d.reduction == R3D_CE_NONE ? d.loss : nullptr, d.loss, p.sums, d.n, p.n_pad,
-              p.lse_splits, mean};
-  hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((d.n + 255) / 256)), dim3(256), 0, st, ja);
+  join(d, p, st);
 }
 
 template <class T, class S, int kPlanes>
@@ -929,10 +1152,21 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     da.tgt = p.tgt;
     da.counted = p.counted;
     da.dl = p.dl;
-    if (p.dl_big) dl_piece<T, Big, kPlanes>(da, d.n, st);
-    else dl_piece<T, Small, kPlanes>(da, d.n, st);
+    if (p.head) {
+      if constexpr (kPlanes == 1) {
+        HeadArgs ha = head_args(d, p);
+        ha.held = held;
+        ha.unheld = unheld;
+        if (!d.dw && !d.db) ha.dl = nullptr;
+        head<T, true>(ha, p, d.n, st);
+      }
+    } else if (p.dl_big) {
+      dl_piece<T, Big, kPlanes>(da, d.n, st);
+    } else {
+      dl_piece<T, Small, kPlanes>(da, d.n, st);
+    }
     const Operand dl{p.dl, p.n_pad, p.n_pad * p.piece, nullptr};
-    if (d.dx) {
+    if (d.dx && !p.head) {
       Operand wv = w;      // the rows of this piece
       wv.p = static_cast<const char *>(w.p) + v0 * w.ld * 2;
       OutArgs oa{};

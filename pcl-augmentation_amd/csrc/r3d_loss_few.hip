@@ -17,6 +17,8 @@ using namespace r3d;
 
 constexpr int kThreads = 256, kLdsMost = 160 * 1024, kTopParts = 256;
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 struct FewArgs {
   const void *x, *w, *bias, *target;
   int64_t ld_x, ld_w, n, ignore;
@@ -45,32 +47,24 @@ __device__ __forceinline__ float taken_out(const FewArgs &a) {
   return top > 0.0f && top < INFINITY ? top : 1.0f;
 }
 
-template <class T>
-__device__ __forceinline__ typename Mma<T>::v8 turned(const T *lo_at, const T *hi_at) {
-  typedef short s4 __attribute__((ext_vector_type(4)));
-  const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)lo_at);
-  const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)hi_at);
-  return __builtin_bit_cast(typename Mma<T>::v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
 template <class V>
-__device__ __forceinline__ uint4 load_piece(const FewArgs &a, int64_t row, int col) {
+__device__ __forceinline__ u32x4 load_piece(const FewArgs &a, int64_t row, int col) {
   constexpr int kEach = 16 / sizeof(V);
-  uint4 r = make_uint4(0, 0, 0, 0);
+  u32x4 r = {0, 0, 0, 0};
   if (row >= a.n) return r;
   const V *at = static_cast<const V *>(a.x) + row * a.ld_x + col;
-  if (a.vector && col + kEach <= a.d) return *reinterpret_cast<const uint4 *>(at);
+  if (a.vector && col + kEach <= a.d) return *reinterpret_cast<const u32x4 *>(at);
   alignas(16) V v[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) v[e] = col + e < a.d ? at[e] : (V)0.0f;
-  return *reinterpret_cast<const uint4 *>(v);
+  return *reinterpret_cast<const u32x4 *>(v);
 }
 
 // 16 bytes of a row into the LDS planes.
 template <class V, class T, int kPlanes>
-__device__ __forceinline__ void store_piece(T *to, int plane, uint4 piece) {
+__device__ __forceinline__ void store_piece(T *to, int plane, u32x4 piece) {
   if constexpr (kPlanes == 1) {
-    *reinterpret_cast<uint4 *>(to) = piece;
+    *reinterpret_cast<u32x4 *>(to) = piece;
   } else {
     typedef float f4 __attribute__((ext_vector_type(4)));
     typedef T t4 __attribute__((ext_vector_type(4)));
@@ -91,7 +85,7 @@ __device__ __forceinline__ void store_piece(T *to, int plane, uint4 piece) {
 }
 
 // Waves a SIMD the registers are cut for: what the tile's LDS lets stand beside each other anyway.  480 000 x 20 x 96 bf16,
-// backward: 68 us with one, 57 with three; 200 000 x 20 x 256: 114 with one, 69 with two; 512 features: 218 with one, 270 with two.
+// backward: 68 us with one, 57 with three; 200 000 x 20 x 256: 114 with one, 69 with two.
 constexpr int few_waves(int planes, int vt, int nb) { return planes == 3 ? (vt * nb == 1 ? 2 : 1) : vt * nb == 1 ? 3 : vt * nb == 2 ? 2 : 1; }
 
 // kVT: blocks of 32 classes; kNB: blocks of 32 features of dW a wave keeps (dp <= 128 kNB); kTP: points of a tile.
@@ -116,12 +110,12 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
     alignas(16) V v[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) v[e] = r < a.v && col + e < a.d ? static_cast<const V *>(a.w)[r * a.ld_w + col + e] : (V)0.0f;
-    store_piece<V, T, kPlanes>(ws + r * pitch + col, w_plane, *reinterpret_cast<const uint4 *>(v));
+    store_piece<V, T, kPlanes>(ws + r * pitch + col, w_plane, *reinterpret_cast<const u32x4 *>(v));
   }
   for (int c = threadIdx.x; c < kVT * 32; c += kThreads)
     bias2[c] = c >= a.v ? -INFINITY : a.bias ? (float)static_cast<const V *>(a.bias)[c] * kLog2e : 0.0f;
 
-  uint4 reg[kPer];
+  u32x4 reg[kPer];
   auto fetch = [&](int64_t tile) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -170,7 +164,7 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
       if (c < pieces) {
         const int r = (int)(((unsigned)c * (unsigned)a.magic) >> 20);
         const bool counts = tgt[r] != -2;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
+        const u32x4 zero = {0, 0, 0, 0};
         store_piece<V, T, kPlanes>(xs + r * pitch + (c - r * cols) * kEach, x_plane, counts ? reg[i] : zero);
       }
     }
@@ -422,10 +416,10 @@ __global__ __launch_bounds__(256) void k_few_top(FewArgs a, float *top_out) {
   if (threadIdx.x == 0) top_out[blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
 }
 
-// dW and db: the workgroups' sums joined, 64 values by four slices of the workgroups a time.
+// dW and db: the workgroups' sums joined, 64 values by sixteen slices of the workgroups a time.
 template <class V>
-__global__ __launch_bounds__(256) void k_few_join(FewArgs a, int groups, int vp, V *dw, V *db) {
-  __shared__ float s[4][64];
+__global__ __launch_bounds__(1024) void k_few_join(FewArgs a, int groups, int vp, V *dw, V *db) {
+  __shared__ float s[16][64];
   const int v = a.v, d = a.d, dp = a.dp;
   const float scale = taken_out(a) * a.unheld;
   const int64_t stride = (int64_t)vp * (dp + 1);
@@ -434,12 +428,15 @@ __global__ __launch_bounds__(256) void k_few_join(FewArgs a, int groups, int vp,
   if (i < all) {
     const float *from = a.part + (i < v * d ? (int64_t)(i / d) * dp + i % d : (int64_t)vp * dp + (i - v * d));
 #pragma unroll 8
-    for (int g = slice; g < groups; g += 4) sum += from[g * stride];
+    for (int g = slice; g < groups; g += 16) sum += from[g * stride];
   }
   s[slice][lane] = sum;
   __syncthreads();
   if (slice == 0 && i < all) {
-    sum = (s[0][lane] + s[1][lane] + s[2][lane] + s[3][lane]) * scale;
+    sum = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) sum += s[g][lane];
+    sum *= scale;
     if (i < v * d) {
       if (dw) dw[i] = (V)sum;
     } else if (db) {
@@ -456,11 +453,13 @@ struct FewPlan {
 // Whether the head is this file's: its classes and features beside a tile of points in LDS, dW in registers.
 bool few_plan(const r3d_linear_ce_t &d, FewPlan &p) {
   const int planes = d.type == R3D_T_F32 ? 3 : 1;
-  if (d.v > 128 || d.d > 512) return false;
+  if (d.v > 128 || d.d > 256) return false;
   p.dp = (int)((d.d + 31) / 32 * 32);
   p.vt = d.v <= 32 ? 1 : d.v <= 64 ? 2 : 4;
-  p.nb = p.dp <= 128 ? 1 : p.dp <= 256 ? 2 : 4;
-  if (p.vt * p.nb > 8 || (planes == 3 && (p.vt == 4 || p.nb == 4))) return false;
+  p.nb = p.dp <= 128 ? 1 : 2;
+  // beyond that, a head in LDS and a product for dW are faster (r3d_loss.hip; bf16, 200 000 points, us here / there:
+  // 20 x 256 116 / 175, 50 x 256 190 / 179, 100 x 96 129 / 157, 100 x 256 284 / 193, 20 x 512 372 / 282)
+  if (p.vt * p.nb > 4 || p.nb > 2 || (planes == 3 && p.vt == 4)) return false;
   p.tp = p.nb >= 2 || planes == 3 ? 64 : 128;      // (two workgroups a CU beat one with the longer tile: 200 000 x 20 x 256 forward 58 -> 38 us)
   const size_t pitch = p.dp + 8;
   p.lds_forward = (size_t)planes * 2 * (p.tp + p.vt * 32) * pitch + p.vt * 32 * 4 + (size_t)p.tp * 16;
@@ -515,12 +514,9 @@ int dispatch(const FewArgs &a, const FewPlan &p, hipStream_t st) {
     switch (key) {
       case 11: return launch<V, T, 1, 1, 1, 128, kGrad>(a, p, st);
       case 12: return launch<V, T, 1, 1, 2, 64, kGrad>(a, p, st);
-      case 14: return launch<V, T, 1, 1, 4, 64, kGrad>(a, p, st);
       case 21: return launch<V, T, 1, 2, 1, 128, kGrad>(a, p, st);
       case 22: return launch<V, T, 1, 2, 2, 64, kGrad>(a, p, st);
-      case 24: return launch<V, T, 1, 2, 4, 64, kGrad>(a, p, st);
-      case 41: return launch<V, T, 1, 4, 1, 128, kGrad>(a, p, st);
-      default: return launch<V, T, 1, 4, 2, 64, kGrad>(a, p, st);
+      default: return launch<V, T, 1, 4, 1, 128, kGrad>(a, p, st);
     }
   }
 }
@@ -602,11 +598,11 @@ int few_backward(const r3d_linear_ce_t &d, void *workspace, hipStream_t st) {
   if (rc != R3D_OK || !a.want_w) return rc;
   const dim3 blocks((unsigned)((d.v * d.d + d.v + 63) / 64));
   if (d.type == R3D_T_F32)
-    hipLaunchKernelGGL(k_few_join<float>, blocks, dim3(256), 0, st, a, p.groups, p.vt * 32, static_cast<float *>(d.dw), static_cast<float *>(d.db));
+    hipLaunchKernelGGL(k_few_join<float>, blocks, dim3(1024), 0, st, a, p.groups, p.vt * 32, static_cast<float *>(d.dw), static_cast<float *>(d.db));
   else if (d.type == R3D_T_BF16)
-    hipLaunchKernelGGL(k_few_join<__bf16>, blocks, dim3(256), 0, st, a, p.groups, p.vt * 32, static_cast<__bf16 *>(d.dw), static_cast<__bf16 *>(d.db));
+    hipLaunchKernelGGL(k_few_join<__bf16>, blocks, dim3(1024), 0, st, a, p.groups, p.vt * 32, static_cast<__bf16 *>(d.dw), static_cast<__bf16 *>(d.db));
   else
-    hipLaunchKernelGGL(k_few_join<_Float16>, blocks, dim3(256), 0, st, a, p.groups, p.vt * 32, static_cast<_Float16 *>(d.dw), static_cast<_Float16 *>(d.db));
+    hipLaunchKernelGGL(k_few_join<_Float16>, blocks, dim3(1024), 0, st, a, p.groups, p.vt * 32, static_cast<_Float16 *>(d.dw), static_cast<_Float16 *>(d.db));
   return R3D_OK;
 }
 

@@ -140,6 +140,15 @@ struct Loader {
   }
 };
 
+// Eight k of a lane's column, from two rows of fours (each lane's address: its row's, see above).
+template <class T>
+__device__ __forceinline__ typename Mma<T>::v8 turned(const T *lo_at, const T *hi_at) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)lo_at);
+  const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)hi_at);
+  return __builtin_bit_cast(typename Mma<T>::v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 // Fragment of the 32 rows (columns) from r0, k-step kk of 16: lane holds row lane & 31, k = (lane >> 5) * 8 + 0..7.
 template <class T, Lies L, int R>
 __device__ __forceinline__ typename Mma<T>::v8 fragment(const T *lds, int r0, int kk) {
@@ -149,7 +158,6 @@ __device__ __forceinline__ typename Mma<T>::v8 fragment(const T *lds, int r0, in
     const T *at = L == Lies::Rows ? lds + r * kTileK + ((q ^ ((r >> 2) & 3)) << 3) : lds + (q * R + r) * 8;
     return *reinterpret_cast<const typename Mma<T>::v8 *>(at);
   } else {
-    typedef short s4 __attribute__((ext_vector_type(4)));
     const int group = lane >> 4, p = lane & 15;
     const int c = r0 + (group & 1) * 16 + (p & 3) * 4, k = kk * 16 + (group >> 1) * 8 + (p >> 2), q = c >> 3;
     const T *lo_at, *hi_at;
@@ -160,9 +168,7 @@ __device__ __forceinline__ typename Mma<T>::v8 fragment(const T *lds, int r0, in
       lo_at = lds + (q * kTileK + (k ^ ((q & 3) << 2))) * 8 + (c & 7);
       hi_at = lds + (q * kTileK + ((k + 4) ^ ((q & 3) << 2))) * 8 + (c & 7);
     }
-    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)lo_at);
-    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4 *)hi_at);
-    return __builtin_bit_cast(typename Mma<T>::v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    return turned<T>(lo_at, hi_at);
   }
 }
 

@@ -191,7 +191,8 @@ def check_loss(pkg, n, v, d, dtype, bias=True, ignore=-100, reduction="mean", pi
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("n,v,d", [(1, 1, 1), (1, 2, 8), (3, 20, 64), (127, 129, 67), (128, 128, 64), (129, 20, 96), (257, 260, 128), (500, 33, 30),
                                    (64, 1000, 192), (40, 3001, 16), (2, 700, 513),
-                                   (300, 32, 128), (1000, 64, 250), (77, 128, 100), (200, 100, 256), (150, 31, 511), (64, 7, 512), (333, 40, 33), (129, 65, 129)])
+                                   (300, 32, 128), (1000, 64, 250), (77, 128, 100), (200, 100, 256), (150, 31, 511), (64, 7, 512), (333, 40, 33), (129, 65, 129), (65, 129, 32), (200, 160, 256),
+                                   (64, 200, 255), (1000, 224, 100), (63, 288, 256), (130, 261, 8), (1, 289, 64)])
 def test_loss_sizes(pkg, dtype, n, v, d):
     check_loss(pkg, n, v, d, dtype)
 
@@ -217,7 +218,7 @@ def test_loss_large_logits(pkg, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n,v,d,share", [(5000, 20, 32, 0.1), (70000, 20, 96, 0.1), (9000, 50, 300, 0.3), (40000, 90, 64, 0.0), (3000, 260, 128, 0.85), (1500, 5000, 64, 0.0), (20, 20000, 128, 0.2)])
+@pytest.mark.parametrize("n,v,d,share", [(5000, 20, 32, 0.1), (70000, 20, 96, 0.1), (9000, 50, 300, 0.3), (20000, 260, 256, 0.1), (17000, 150, 96, 0.1), (40000, 90, 64, 0.0), (3000, 260, 128, 0.85), (1500, 5000, 64, 0.0), (20, 20000, 128, 0.2)])
 def test_loss_larger(pkg, dtype, n, v, d, share):
     check_loss(pkg, n, v, d, dtype, share=share)
 
