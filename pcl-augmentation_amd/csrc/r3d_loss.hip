@@ -560,15 +560,17 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
 #pragma unroll
   for (int i = 0; i < S::FM; ++i) row_sum[i] = 0.0f;
   const int64_t kb0 = kb * split / a.splits, kb1 = kb * (split + 1) / a.splits;
+  constexpr bool kGather = LA == Lies::PiecesCols;      // x by the points' numbers
+  __shared__ int32_t numbers[Stream<T, S, LA, Lies::Cols, kGather>::number_words];
   if (kb1 > kb0) {
-    Stream<T, S, LA, Lies::Cols> st;
+    Stream<T, S, LA, Lies::Cols, kGather> st;
     st.a = a.p.a;
     st.b = a.p.b;
     st.rows_b = (int)(a.points == 2 ? nc : a.rows_b);
     st.la.tile(st.a, m0, a.points == 1 ? nc : a.limit_a);
     st.lb.tile(st.b, n0, a.limit_b);
     auto more = [] { return false; };
-    st.begin(lds, (int)kb0, (int)kb1, a.p.planes, more);
+    st.begin(lds, (int)kb0, (int)kb1, a.p.planes, more, numbers);
     st.template run<kSums>(lds, acc, row_sum, sums, more);
     st.end();
   }
@@ -740,12 +742,19 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[into][e] = *reinterpret_cast<const v8 *>(x + k + e * 16);
     };
+    // the head's fragments three products ahead (left alone, the compiler reads one, waits, multiplies)
     auto multiply = [&](int k, int of) {
       const T *w = ws + low * pitch + half * 8 + k;
+      v8 fa[4];
+      auto read = [&](int i) { fa[i & 3] = *reinterpret_cast<const v8 *>(w + (i % kVB) * 32 * pitch + (i / kVB) * 16); };
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int i = 0; i < 3; ++i) read(i);
 #pragma unroll
-        for (int v = 0; v < kVB; ++v) acc[v] = Mma<T>::mma(*reinterpret_cast<const v8 *>(w + v * 32 * pitch + e * 16), f[of][e], acc[v]);
+      for (int i = 0; i < 4 * kVB; ++i) {
+        if (i + 3 < 4 * kVB) read(i + 3);
+        acc[i % kVB] = Mma<T>::mma(fa[i & 3], f[of][i / kVB], acc[i % kVB]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
     features(0, 0);
     int k = 0;
@@ -758,15 +767,16 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
     if (k < a.dp) multiply(k, 0);
     const int t = in ? a.tgt[point] : -1;
     if constexpr (!kGrad) {
-      float top = -INFINITY, sum = 0.0f;
+      float top = -INFINITY, sum = 0.0f, hit = -INFINITY;
 #pragma unroll
       for (int v = 0; v < kVB; ++v)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           acc[v][r] = __builtin_fmaf(acc[v][r], kLog2e, bias2[v * 32 + mma_row(r)]);
           top = fmaxf(top, acc[v][r]);
-          if (t == v * 32 + mma_row(r)) a.hit[point] = acc[v][r];
+          hit = t == v * 32 + mma_row(r) ? acc[v][r] : hit;
         }
+      if (t >= 0 && (t >> 2 & 1) == half) a.hit[point] = hit;      // (the lane that holds the target's class)
       top = fmaxf(top, __shfl_xor(top, 32));
       const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll

@@ -67,7 +67,7 @@ __device__ __forceinline__ void load_lds16(const void *g, unsigned to) {
 template <class T, Lies L, int R, int kThreads>
 struct Loader {
   static constexpr int per = R * kTileK / 8 / kThreads;
-  static constexpr int row_lanes = R / 8, rows_wave = 64 / row_lanes;      // Cols: lanes to a row, rows to a wave's load
+  static constexpr int row_lanes = R / 8;      // Cols: lanes to a row
   const T *at[per];
   int col;      // Cols: first column of the thread's pieces
 
@@ -103,33 +103,21 @@ struct Loader {
   }
   // Elements from one k-block to the next.
   static __device__ __forceinline__ int64_t step(const Operand &o) {
-    return L == Lies::Rows ? kTileK : L == Lies::PiecesRows ? (kTileK / 8) * o.ld * 8 : L == Lies::PiecesCols ? kTileK * 8 : 0;
+    return L == Lies::Rows ? kTileK : L == Lies::PiecesRows ? (kTileK / 8) * o.ld * 8 : L == Lies::PiecesCols ? kTileK * 8 : kTileK * o.ld;
   }
   __device__ __forceinline__ void move(int64_t elements) {
-    if constexpr (L != Lies::Cols) {
 #pragma unroll
-      for (int i = 0; i < per; ++i) at[i] += elements;
-    }
+    for (int i = 0; i < per; ++i) at[i] += elements;
   }
-  // Cols: the rows of k-block kb.  Their numbers come by scalar loads -- a vector load would have to wait for every load to LDS
-  // that was issued before it.
-  __device__ __forceinline__ void look(const Operand &o, int kb, int rows, int64_t plane) {
+  // Cols: row of the k-block that piece i is of.
+  static __device__ __forceinline__ int row_of(int i) { return (i * kThreads + (int)threadIdx.x) / row_lanes; }
+  // Cols: k-block kb, by row numbers (`numbers`: the block's, in LDS) or in order.
+  __device__ __forceinline__ void to_block(const Operand &o, int kb, int rows, int64_t plane, const int32_t *numbers) {
     if constexpr (L == Lies::Cols) {
-      const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mine = (threadIdx.x & 63) / row_lanes;
       const T *base = static_cast<const T *>(o.p) + plane;
 #pragma unroll
       for (int i = 0; i < per; ++i) {
-        const int first = kb * kTileK + (i * (kThreads / 64) + wave) * rows_wave;
-        int row = first + mine < rows ? first + mine : rows - 1;
-        if (o.idx) {
-          const auto *idx = (const __attribute__((address_space(4))) int32_t *)o.idx;
-          int32_t n[rows_wave];
-#pragma unroll
-          for (int e = 0; e < rows_wave; ++e) n[e] = idx[first + e < rows ? first + e : rows - 1];
-          row = n[0];
-#pragma unroll
-          for (int e = 1; e < rows_wave; ++e) row = mine == e ? n[e] : row;
-        }
+        const int row = numbers ? numbers[row_of(i)] : min(kb * kTileK + row_of(i), rows - 1);
         at[i] = base + ((uint64_t)(uint32_t)row * (uint32_t)o.ld + (uint32_t)col);
       }
     }
@@ -194,21 +182,34 @@ __device__ __forceinline__ void wait_loads() {
 // A stream of k-blocks through LDS buffers: S::ahead blocks are on their way while one is multiplied.  One barrier a
 // block: behind it the block is there for all waves, and all of them are done with the one before, whose buffer the next load
 // takes.  The stream goes on over the tiles of a workgroup (`more`): their loads do not wait for a tile's end.
-template <class T, class S, Lies LA, Lies LB>
+// kGather: the rows of a Cols operand B are taken by their numbers, b.idx.  Those of a block come to LDS S::ahead blocks before its
+// own loads, with the loads of that earlier block (every wave for itself): looked up when they are wanted, by vector or by
+// scalar loads, they hold up every step (dW of 119999 x 260 x 256: 73 us by scalar loads a step, 139 a step ahead).
+template <class T, class S, Lies LA, Lies LB, bool kGather = false>
 struct Stream {
   Operand a, b;
   Loader<T, LA, S::BM, S::threads> la;
   Loader<T, LB, S::BN, S::threads> lb;
-  static constexpr int loads = Loader<T, LA, S::BM, S::threads>::per + Loader<T, LB, S::BN, S::threads>::per;
+  static constexpr int loads = Loader<T, LA, S::BM, S::threads>::per + Loader<T, LB, S::BN, S::threads>::per + (kGather ? 1 : 0);
+  static constexpr int number_words = kGather ? 64 * S::buffers * (S::threads / 64) : 1;      // LDS that `numbers` has
   int rows_b;                  // rows of a Cols operand
   int kb, kb0, kb1;
   int pair, pairs, get, put;   // buffers: the next to multiply, the next to fill
   bool dry;                    // nothing left to load
   unsigned base;               // LDS address of the wave's part of buffer 0
+  int32_t *numbers;            // [S::buffers][64] of this wave: slot put holds those of the next block to load
+
+  // The numbers of block n (of this tile; clamped behind the last row) to slot `slot`.
+  __device__ __forceinline__ void fetch_numbers(int n, int slot) {
+    const int row = n * kTileK + (threadIdx.x & 31);
+    const int32_t *from = b.idx + (row < rows_b ? row : rows_b - 1);
+    const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_void *)(numbers + slot * 64));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "m0", "memory");
+  }
 
   // k-blocks [first, end) of every tile (at least one); the loaders hold the first tile.
   template <class More>
-  __device__ __forceinline__ void begin(T *lds, int first, int end, int planes, More &&more) {
+  __device__ __forceinline__ void begin(T *lds, int first, int end, int planes, More &&more, int32_t *number_lds = nullptr) {
     kb = kb0 = first;
     kb1 = end;
     pairs = planes == 3 ? kPairs : 1;
@@ -216,7 +217,16 @@ struct Stream {
     dry = false;
     base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_void *)lds + (threadIdx.x >> 6) * 1024);
     la.move(first * la.step(a));
-    lb.move(first * lb.step(b));
+    if constexpr (kGather) {
+      numbers = number_lds + (threadIdx.x >> 6) * 64 * S::buffers;
+#pragma unroll
+      for (int i = 0; i < S::ahead; ++i) fetch_numbers(first + i % (end - first), i);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    } else if constexpr (LB == Lies::Cols) {
+      lb.to_block(b, kb, rows_b, 0, nullptr);
+    } else {
+      lb.move(first * lb.step(b));
+    }
 #pragma unroll
     for (int i = 0; i < S::ahead; ++i) issue(more);
   }
@@ -224,7 +234,11 @@ struct Stream {
   // Without one the last block is loaded again: the count of loads on their way stays what wait_loads() takes it for.
   template <class More>
   __device__ __forceinline__ void issue(More &&more) {
-    lb.look(b, kb, rows_b, kPlaneB[pair] * b.plane);
+    if constexpr (kGather) {
+      lb.to_block(b, kb, rows_b, kPlaneB[pair] * b.plane, numbers + put * 64);
+      // (the slot that was read S::buffers - S::ahead blocks ago; blocks go round within a tile)
+      fetch_numbers(kb0 + (kb - kb0 + S::ahead) % (kb1 - kb0), (put + S::ahead) % S::buffers);
+    }
     const unsigned to = base + put * (S::buffer * (unsigned)sizeof(T));
     la.issue(to);
     lb.issue(to + S::a_elems * (unsigned)sizeof(T));
@@ -232,7 +246,10 @@ struct Stream {
     if (dry) return;
     if (++kb < kb1) {
       la.move(la.step(a));
-      lb.move(lb.step(b));
+      if constexpr (!kGather) {
+        if (LB == Lies::Cols && (kb + 1) * kTileK > rows_b) lb.to_block(b, kb, rows_b, kPlaneB[pair] * b.plane, nullptr);
+        else lb.move(lb.step(b));
+      }
       return;
     }
     const int was = pair;
@@ -248,8 +265,11 @@ struct Stream {
     } else {
       la.move((kb0 + 1 - kb1) * la.step(a) + (kPlaneA[pair] - kPlaneA[was]) * a.plane);
     }
-    lb.move((kb0 + 1 - kb1) * lb.step(b) + (kPlaneB[pair] - kPlaneB[was]) * b.plane);
     kb = kb0;
+    if constexpr (!kGather) {
+      if constexpr (LB == Lies::Cols) lb.to_block(b, kb, rows_b, kPlaneB[pair] * b.plane, nullptr);
+      else lb.move((kb0 + 1 - kb1) * lb.step(b) + (kPlaneB[pair] - kPlaneB[was]) * b.plane);
+    }
   }
   // acc += all k-blocks of a tile.  kSums: row_sum += sums over k of A, where `sums`.  A fragment is read one k-step before it is
   // multiplied, over the blocks' borders too: the reads after a barrier would else hold up the matrix cores of all waves at once.
