@@ -858,7 +858,8 @@ int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t tiles_of(int64_t m, int64_t n, int64_t bm, int64_t bn) { return (up(m, bm) / bm) * (up(n, bn) / bn); }
 
 // Parts in which the long axis of a product is cut: enough workgroups for the chip, and no last round that leaves most of it
-// idle; at least four k-blocks each.
+// idle.  For dx and dW one workgroup a CU of either shape (parts are written and joined: dW of 119999 x 260 x 256 with two of
+// the small shape 64 + 13 us, with one 49 + 7).
 int cut(int64_t tiles, int64_t slots, int64_t most) {
   if (most < 1) most = 1;
   int best = 1;
@@ -952,8 +953,8 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     p.dx_big = large_tiles(d.n, p.dp, kx);
     p.dw_big = large_tiles(p.piece, p.dp, kw);
     auto tiles = [&](int64_t m, int64_t n, bool big) { return big ? tiles_of(m, n, Big::BM, Big::BN) : tiles_of(m, n, Small::BM, Small::BN); };
-    p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus * (p.dx_big ? Big::per_cu : Small::per_cu), kx);
-    p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus * (p.dw_big ? Big::per_cu : Small::per_cu), kw);
+    p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus, kx);
+    p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus, kw);
     p.dx_final = p.head || (p.dx_splits == 1 && p.piece >= d.v);
     p.dw_final = p.dw_splits == 1;
     p.top_parts = (int)(d.n < 256 * 256 ? (d.n + 255) / 256 : 256);
