@@ -261,9 +261,8 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
   if (vt1 > vt0) st.begin(lds, 0, (int)a.kb, a.p.planes, more);
   for (int vt = vt0; vt < vt1; ++vt) {
     f32x16 acc[S::FM][S::FN];
-    float none[S::FM];
     clear(acc);
-    st.template run<false>(lds, acc, none, false, more);
+    st.run(lds, acc, more);
 #pragma unroll
     for (int i = 0; i < S::FM; ++i) {
       const int vb = vt * S::BM + (wm * S::FM + i) * 32;
@@ -441,6 +440,8 @@ struct DlArgs {
   const int32_t *tgt;
   const Counted *counted;
   void *dl;        // [planes][width / 8][n_pad][8]
+  float *sums;     // [tiles of points][piece]: db of a tile's points, before dl is rounded; or null
+  int64_t piece;
 };
 
 // dl of a piece of the classes.  A lane holds 4 neighbouring classes of a point and its partner 32 lanes on the next 4: a swap
@@ -452,10 +453,12 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
   int64_t vt, nt;
   tile_of(xcd_order(blockIdx.x, gridDim.x), a.vtiles, a.ntiles, vt, nt);
   const int64_t n0 = nt * S::BN;
-  if (n0 >= nc) return;
+  if (n0 >= nc) {
+    for (int c = threadIdx.x; a.sums && c < S::BM && vt * S::BM + c < a.width; c += S::threads) a.sums[nt * a.piece + vt * S::BM + c] = 0.0f;
+    return;
+  }
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
   f32x16 acc[S::FM][S::FN];
-  float none[S::FM];
   clear(acc);
   {
     Stream<T, S, Lies::Rows, Lies::Rows> st;
@@ -466,25 +469,39 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
     st.lb.tile(st.b, n0, nc);
     auto more = [] { return false; };
     st.begin(lds, 0, (int)a.kb, a.p.planes, more);
-    st.template run<false>(lds, acc, none, false, more);
+    st.run(lds, acc, more);
     st.end();
   }
   T *dl = static_cast<T *>(a.dl);
+  float *s_sum = reinterpret_cast<float *>(lds);      // [WN][BM]
+  int64_t col[S::FN];
+  int tgt[S::FN];
+  float lse2[S::FN], weight[S::FN];
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) {
-    const int64_t col = n0 + (wn * S::FN + j) * 32 + (lane & 31);
-    const bool in = col < nc;
-    const int tgt = in ? a.tgt[col] : -1;
-    const float lse2 = in ? a.lse2[col] : 0.0f, weight = in ? a.weight[col] * a.held : 0.0f;
+    col[j] = n0 + (wn * S::FN + j) * 32 + (lane & 31);
+    const bool in = col[j] < nc;
+    tgt[j] = in ? a.tgt[col[j]] : -1;
+    lse2[j] = in ? a.lse2[col[j]] : 0.0f;
+    weight[j] = in ? a.weight[col[j]] * a.held : 0.0f;
+  }
 #pragma unroll
-    for (int i = 0; i < S::FM; ++i) {
-      const int local = (int)vt * S::BM + (wm * S::FM + i) * 32;
-      if (local >= a.width) continue;
-      const int64_t vb = a.piece0 + local;
-      const int64_t d = tgt - vb;
+  for (int i = 0; i < S::FM; ++i) {
+    const int local = (int)vt * S::BM + (wm * S::FM + i) * 32;
+    if (local >= a.width) continue;
+    const int64_t vb = a.piece0 + local;
+    float b[16], sums[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      b[r] = a.bias2[vb + mma_row(r)];
+      sums[r] = 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) {
+      const int64_t d = tgt[j] - vb;
       float p[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, a.bias2[vb + mma_row(r)]) - lse2);
+      for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, b[r]) - lse2[j]);
       if (__any(d >= 0 && d < 32)) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] -= d == mma_row(r) ? 1.0f : 0.0f;
@@ -495,7 +512,8 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
       t4 q[4][kPlanes];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float w = in ? p[r] * weight : 0.0f;
+        const float w = col[j] < nc ? p[r] * weight[j] : 0.0f;
+        sums[r] += w;
         if constexpr (kPlanes == 3) {
           T h, mm, l;
           split3(w, h, mm, l);
@@ -515,9 +533,23 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
           const auto s1 = __builtin_amdgcn_permlane32_swap(even[1], odd[1], false, false);
           const u4 out = {s0[0], s1[0], s0[1], s1[1]};
           const int64_t piece = local / 8 + h + (lane >> 5);
-          *reinterpret_cast<u4 *>(dl + k * a.dl_plane + (piece * a.n_pad + col) * 8) = out;
+          *reinterpret_cast<u4 *>(dl + k * a.dl_plane + (piece * a.n_pad + col[j]) * 8) = out;
         }
     }
+    if (a.sums) {
+      const float mine = block_sum(sums);
+      if ((lane & 15) < 8) s_sum[wn * S::BM + (wm * S::FM + i) * 32 + block_sum_row()] = mine;
+    }
+  }
+  if (!a.sums) return;
+  __syncthreads();
+  for (int c = threadIdx.x; c < S::BM; c += S::threads) {
+    const int local = (int)vt * S::BM + c;
+    if (local >= a.width) break;
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < S::WN; ++w) sum += s_sum[w * S::BM + c];
+    a.sums[nt * a.piece + local] = sum;
   }
 }
 
@@ -534,12 +566,10 @@ struct OutArgs {
   const int32_t *idx;
   const float *scale;
   float unheld;
-  float *row_sum;                        // [splits][sum_stride]: sums over k of A, or null
-  int64_t sum_stride;
 };
 
-// The products with dl: dx = dl W and dW = dl^T x (with db, the sums of dl's columns, which pass by), into 32-bit sums in the
-// workspace or, where nothing is left to add, to the result.
+// The products with dl: dx = dl W and dW = dl^T x, into 32-bit sums in the workspace or, where nothing is left to add, to the
+// result.
 template <class V, class T, class S, Lies LA>
 __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
   __shared__ __attribute__((aligned(128))) T lds[S::buffers * S::buffer];
@@ -551,14 +581,9 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
   const int64_t m0 = mt * S::BM, n0 = nt * S::BN;
   const int64_t m = a.points == 1 ? nc : a.m, kb = a.points == 2 ? (nc + kTileK - 1) / kTileK : a.kb;
   if (m0 >= m) return;
-  constexpr bool kSums = LA == Lies::PiecesCols;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-  const bool sums = kSums && a.row_sum && nt == 0 && wn == 0;
   f32x16 acc[S::FM][S::FN];
-  float row_sum[S::FM];
   clear(acc);
-#pragma unroll
-  for (int i = 0; i < S::FM; ++i) row_sum[i] = 0.0f;
   const int64_t kb0 = kb * split / a.splits, kb1 = kb * (split + 1) / a.splits;
   constexpr bool kGather = LA == Lies::PiecesCols;      // x by the points' numbers
   __shared__ int32_t numbers[Stream<T, S, LA, Lies::Cols, kGather>::number_words];
@@ -571,17 +596,12 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
     st.lb.tile(st.b, n0, a.limit_b);
     auto more = [] { return false; };
     st.begin(lds, (int)kb0, (int)kb1, a.p.planes, more, numbers);
-    st.template run<kSums>(lds, acc, row_sum, sums, more);
+    st.run(lds, acc, more);
     st.end();
   }
   const float scale = a.final_out ? *a.scale * a.unheld : 1.0f;
 #pragma unroll
   for (int i = 0; i < S::FM; ++i) {
-    if (kSums && sums) {
-      const float s = row_sum[i] + __shfl_xor(row_sum[i], 32);
-      const int64_t row = m0 + (wm * S::FM + i) * 32 + lane;
-      if (lane < 32 && row < m) a.row_sum[split * a.sum_stride + row] = s;
-    }
 #pragma unroll
     for (int j = 0; j < S::FN; ++j) {
       const int64_t n = n0 + (wn * S::FN + j) * 32 + (lane & 31), row0 = m0 + (wm * S::FM + i) * 32;
@@ -694,6 +714,7 @@ struct HeadArgs {
   const float *lse2, *weight, *scale;
   float held, unheld;
   void *dl, *dx;                     // dl: pieces of 8 classes, or null
+  float *sums;                       // [workgroups][classes padded to 32]: db of its points, or null
   int64_t n_pad;
   int32_t vector_out;
 };
@@ -708,7 +729,11 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
   float *bias2 = reinterpret_cast<float *>(ws + kVB * 32 * pitch);
   const int lane = threadIdx.x & 63, half = lane >> 5, low = lane & 31, group = lane >> 4, sub = lane & 15;
   const int nc = a.counted->n, cols = a.dp / 8;
-  if (blockIdx.x * 32 >= nc) return;
+  if (blockIdx.x * 32 >= nc) {
+    if (kGrad && a.sums)
+      for (int c = threadIdx.x; c < kVB * 32; c += kHeadThreads) a.sums[(int64_t)blockIdx.x * kVB * 32 + c] = 0.0f;
+    return;
+  }
   for (int i0 = threadIdx.x; i0 < kVB * 32 * cols; i0 += 6 * kHeadThreads) {      // (six loads on their way: 147 KB are 18 a thread)
     v8 v[6];
     int to[6];
@@ -724,7 +749,11 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
       if (to[e] >= 0) *reinterpret_cast<v8 *>(ws + to[e]) = v[e];
   }
   for (int i = threadIdx.x; i < kVB * 32; i += kHeadThreads) bias2[i] = a.bias2[i];
+  float *sums = bias2 + kVB * 32;      // [waves][classes] db of a wave's points, before dl is rounded (in registers they spill)
+  if constexpr (kGrad)
+    for (int i = threadIdx.x; i < kHeadThreads / 64 * kVB * 32; i += kHeadThreads) sums[i] = 0.0f;
   __syncthreads();
+  float *mine = sums + (threadIdx.x >> 6) * kVB * 32 + block_sum_row();
   const float out_scale = kGrad && a.dx ? *a.scale * a.unheld : 1.0f;
   // neighbouring tiles go to different workgroups, so that a few tiles are a few workgroups' too
   for (int64_t tile = blockIdx.x + (int64_t)gridDim.x * (threadIdx.x >> 6); tile * 32 < nc; tile += (int64_t)gridDim.x * (kHeadThreads / 64)) {
@@ -795,11 +824,17 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
       t4 q[kVB][4];
 #pragma unroll
       for (int v = 0; v < kVB; ++v) {
+        float w[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v][r], kLog2e, bias2[v * 32 + mma_row(r)]) - lse2);
           p -= t == v * 32 + mma_row(r) ? 1.0f : 0.0f;
-          q[v][r >> 2][r & 3] = (T)(in ? p * by : 0.0f);
+          w[r] = in ? p * by : 0.0f;
+          q[v][r >> 2][r & 3] = (T)w[r];
+        }
+        if (a.sums) {
+          const float s = block_sum(w);
+          if ((lane & 15) < 8) mine[v * 32] += s;
         }
         __builtin_amdgcn_sched_barrier(0);      // (a block at a time: all blocks' addresses and biases at once spill)
       }
@@ -846,6 +881,16 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
       }
     }
   }
+  if constexpr (kGrad) {
+    if (!a.sums) return;
+    __syncthreads();
+    for (int c = threadIdx.x; c < kVB * 32; c += kHeadThreads) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kHeadThreads / 64; ++w) sum += sums[w * kVB * 32 + c];
+      a.sums[(int64_t)blockIdx.x * kVB * 32 + c] = sum;
+    }
+  }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
@@ -887,7 +932,7 @@ struct Plan {
   int planes, type_bytes;
   int64_t dp, n_pad, v_pad, piece;
   bool lse_big, dl_big, dx_big, dw_big;
-  int lse_splits, dx_splits, dw_splits, top_parts, groups;
+  int lse_splits, dx_splits, dw_splits, db_parts, top_parts, groups;
   int head;                     // blocks of 32 classes of a head that fits LDS, or 0
   size_t head_lds;
   bool dx_final, dw_final;      // nothing to add: straight into the result
@@ -916,7 +961,7 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   p.dp = up(d.d, kPadK);
   p.n_pad = up(d.n, Big::BN);
   p.v_pad = up(d.v, Big::BM);
-  p.head_lds = (size_t)up(d.v, 32) * (p.dp + 8) * 2 + up(d.v, 32) * 4;
+  p.head_lds = (size_t)up(d.v, 32) * ((p.dp + 8) * 2 + 4 + kHeadThreads / 64 * 4);
   p.head = p.planes == 1 && d.v <= kHeadBlocks * 32 && p.head_lds <= (size_t)kHeadLds ? (int)(up(d.v, 32) / 32) : 0;
   p.groups = d.n <= kOneGroup ? 1 : (int)((d.n + kStartRows - 1) / kStartRows);
   Carver k(d.state);
@@ -963,8 +1008,10 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     p.weight = c.take<float>(p.n_pad);
     p.dl = c.take<uint16_t>((size_t)p.planes * p.n_pad * p.piece);
     if (!p.dx_final) p.accx = c.take<float>((size_t)p.dx_splits * p.n_pad * p.dp);
-    p.accw = c.take<float>((size_t)(p.dw_final && d.dw ? 0 : p.dw_splits) * p.piece * p.dp);
-    p.accb = c.take<float>((size_t)p.dw_splits * p.piece);
+    p.accw = c.take<float>((size_t)(p.dw_final || !d.dw ? 0 : p.dw_splits) * p.piece * p.dp);
+    // db: a part for every tile of points (the tiles of dl) or every workgroup of a head in LDS
+    p.db_parts = p.head ? (int)(up(d.n, 32) / 32 < kCus ? up(d.n, 32) / 32 : kCus) : (int)(up(d.n, p.dl_big ? Big::BN : Small::BN) / (p.dl_big ? Big::BN : Small::BN));
+    p.accb = c.take<float>((size_t)p.db_parts * p.piece);
   }
   p.bytes = c.off;
   return p;
@@ -1163,12 +1210,15 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     da.tgt = p.tgt;
     da.counted = p.counted;
     da.dl = p.dl;
+    da.sums = d.db ? p.accb : nullptr;
+    da.piece = p.piece;
     if (p.head) {
       if constexpr (kPlanes == 1) {
         HeadArgs ha = head_args(d, p);
         ha.held = held;
         ha.unheld = unheld;
-        if (!d.dw && !d.db) ha.dl = nullptr;
+        if (!d.dw) ha.dl = nullptr;
+        ha.sums = d.db ? p.accb : nullptr;
         head<T, true>(ha, p, d.n, st);
       }
     } else if (p.dl_big) {
@@ -1201,8 +1251,8 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       else out_product<S, T, Small, Lies::PiecesRows>(oa, d.n, p.dp, st);
       if (!p.dx_final && v0 + p.piece >= d.v) of[n_of++] = finish_of<S>(p.accx, p.dp, p.n_pad * p.dp, d.n, d.d, p.dx_splits, p.place, d.dx);
     }
-    if (d.dw || d.db) {
-      const bool straight = p.dw_final && d.dw;
+    if (d.dw) {
+      const bool straight = p.dw_final;
       OutArgs oa{};
       oa.p = Product{dl, x, kPlanes};
       oa.m = straight ? real_v : width;
@@ -1218,13 +1268,14 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       oa.final_out = straight ? static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes : nullptr;
       oa.scale = p.scale;
       oa.unheld = unheld;
-      oa.row_sum = d.db ? p.accb : nullptr;
-      oa.sum_stride = p.piece;
       if (p.dw_big) out_product<S, T, Big, Lies::PiecesCols>(oa, width, p.dp, st);
       else out_product<S, T, Small, Lies::PiecesCols>(oa, width, p.dp, st);
-      if (d.dw && !straight)
+      if (!straight)
         of[n_of++] = finish_of<S>(p.accw, p.dp, p.piece * p.dp, real_v, d.d, p.dw_splits, nullptr, static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes);
-      if (d.db) of[n_of++] = finish_of<S>(p.accb, p.piece, p.piece, 1, real_v, p.dw_splits, nullptr, static_cast<char *>(d.db) + v0 * p.type_bytes);
+    }
+    if (d.db) {
+      const int64_t stride = p.head ? up(d.v, 32) : p.piece;
+      of[n_of++] = finish_of<S>(p.accb, stride, stride, 1, real_v, p.db_parts, nullptr, static_cast<char *>(d.db) + v0 * p.type_bytes);
     }
     finish<S>(of, n_of, p, unheld, st);
   }

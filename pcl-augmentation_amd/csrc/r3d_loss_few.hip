@@ -141,10 +141,10 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
   double loss_sum = 0.0;
   int count = 0;
   f32x16 acc_w[kGrad ? kVT : 1][kGrad ? kNB : 1];
-  float row_sum[kVT];
+  float sums[kVT];      // db of the wave's points, before dl is rounded
   if constexpr (kGrad) clear(acc_w);
 #pragma unroll
-  for (int v = 0; v < kVT; ++v) row_sum[v] = 0.0f;
+  for (int v = 0; v < kVT; ++v) sums[v] = 0.0f;
 
   int64_t tile = blockIdx.x;
   int at = 0;
@@ -230,12 +230,13 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
         const float by = t == -2 ? 0.0f : s_weight[at * kTP + wave * 32 + low] * a.held;
         t4 q[kVT][4][kPlanes];
 #pragma unroll
-        for (int v = 0; v < kVT; ++v)
+        for (int v = 0; v < kVT; ++v) {
+          float w[16];
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             float p = __builtin_amdgcn_exp2f(acc[v][r] - lse2);
             p -= t == v * 32 + mma_row(r) ? 1.0f : 0.0f;
-            p = t == -2 ? 0.0f : p * by;
+            w[r] = p = t == -2 ? 0.0f : p * by;
             if constexpr (kPlanes == 3) {
               T h, m, l;
               split3(p, h, m, l);
@@ -246,6 +247,8 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
               q[v][r >> 2][0][r & 3] = (T)p;
             }
           }
+          if (a.want_w) sums[v] += block_sum(w);
+        }
 #pragma unroll
         for (int v = 0; v < kVT; ++v)
 #pragma unroll
@@ -317,7 +320,6 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
 #pragma unroll
             for (int v = 0; v < kVT; ++v) {
               fa[v] = turned<T>(dt + v * 32, dt + v * 32 + 4 * kPv);
-              if (wave == 0 && kPlaneB[pr] == 0) row_sum[v] = sum8<T>(fa[v], row_sum[v]);
             }
 #pragma unroll
             for (int b = 0; b < kNB; ++b) {
@@ -345,11 +347,14 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
 #pragma unroll
           for (int r = 0; r < 16; ++r) part[(v * 32 + mma_row(r)) * a.dp + f0 + low] = acc_w[v][b][r];
       }
-      if (wave == 0) {
-        const float s = row_sum[v] + __shfl_xor(row_sum[v], 32);
-        if (lane < 32) part[kVT * 32 * a.dp + v * 32 + lane] = s;
-      }
     }
+    float *s_sum = reinterpret_cast<float *>(smem);      // [waves][classes] (nobody reads the tile any more)
+#pragma unroll
+    for (int v = 0; v < kVT; ++v)
+      if ((lane & 15) < 8) s_sum[wave * kVT * 32 + v * 32 + block_sum_row()] = sums[v];
+    __syncthreads();
+    for (int c = threadIdx.x; c < kVT * 32; c += kThreads)
+      part[kVT * 32 * a.dp + c] = s_sum[c] + s_sum[kVT * 32 + c] + s_sum[2 * kVT * 32 + c] + s_sum[3 * kVT * 32 + c];
   } else {
     __syncthreads();
     double *s_sum = reinterpret_cast<double *>(smem);

@@ -160,13 +160,6 @@ __device__ __forceinline__ typename Mma<T>::v8 fragment(const T *lds, int r0, in
   }
 }
 
-template <class T>
-__device__ __forceinline__ float sum8(typename Mma<T>::v8 v, float s) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s += (float)v[i];
-  return s;
-}
-
 // (plane of A, plane of B) of the products of two operands in three planes of 8 bits each: what is left out is below 2^-24.
 constexpr int kPairs = 6;
 __device__ constexpr int kPlaneA[kPairs] = {0, 0, 1, 1, 0, 2}, kPlaneB[kPairs] = {0, 1, 0, 1, 2, 0};
@@ -271,13 +264,12 @@ struct Stream {
       else lb.move((kb0 + 1 - kb1) * lb.step(b) + (kPlaneB[pair] - kPlaneB[was]) * b.plane);
     }
   }
-  // acc += all k-blocks of a tile.  kSums: row_sum += sums over k of A, where `sums`.  A fragment is read one k-step before it is
-  // multiplied, over the blocks' borders too: the reads after a barrier would else hold up the matrix cores of all waves at once.
-  template <bool kSums, class More>
-  __device__ __forceinline__ void run(T *lds, f32x16 (&acc)[S::FM][S::FN], float (&row_sum)[S::FM], bool sums, More &&more) {
+  // acc += all k-blocks of a tile.  A fragment is read one k-step before it is multiplied, over the blocks' borders too: the reads
+  // after a barrier would else hold up the matrix cores of all waves at once.
+  template <class More>
+  __device__ __forceinline__ void run(T *lds, f32x16 (&acc)[S::FM][S::FN], More &&more) {
     const int wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
     const int steps = (kb1 - kb0) * pairs;
-    int at_pair = 0, pair_end = kb1 - kb0;
     typename Mma<T>::v8 fa[2][S::FM], fb[2][S::FN];
     auto read = [&](int kk, int into) {
       const T *pa = lds + get * S::buffer, *pb = pa + S::a_elems;
@@ -291,19 +283,11 @@ struct Stream {
       for (int i = 0; i < S::FM; ++i)
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) acc[i][j] = Mma<T>::mma(fa[from][i], fb[from][j], acc[i][j]);
-      if (kSums && sums && kPlaneB[at_pair] == 0) {      // (every plane of A once)
-#pragma unroll
-        for (int i = 0; i < S::FM; ++i) row_sum[i] = sum8<T>(fa[from][i], row_sum[i]);
-      }
     };
     static_assert(kTileK == 32, "two k-steps a block");
     wait_loads<(S::ahead - 1) * loads>();
     read(0, 0);
     for (int s = 0; s < steps; ++s) {
-      if (s == pair_end) {
-        ++at_pair;
-        pair_end += kb1 - kb0;
-      }
       read(1, 1);
       __builtin_amdgcn_sched_barrier(0);
       multiply(0);
@@ -334,6 +318,25 @@ __device__ __forceinline__ void clear(f32x16 (&acc)[FM][FN]) {
 
 // Row of C in a 32 x 32 block that register j of a lane holds (its column is lane & 31).
 __device__ __forceinline__ int mma_row(int j) { return (j & 3) + 8 * (j >> 2) + 4 * ((threadIdx.x & 63) >> 5); }
+
+// The sums over the 32 columns of a block whose register r holds v[r]: lane l < 8 of every 16 gets that of the row block_sum_row(l).
+// A swap of 16 lanes and an addition make one register of two, then four rotated additions a register.
+__device__ __forceinline__ float block_sum(const float (&v)[16]) {
+  float mine = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v[k]), __builtin_bit_cast(unsigned, v[k + 8]), false, false);
+    const unsigned lo = s[0], hi = s[1];      // (a cast of an element itself takes element 0)
+    float t = __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+    t += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, t), 0x128, 0xf, 0xf, false));      // row_ror:8
+    t += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, t), 0x124, 0xf, 0xf, false));
+    t += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, t), 0x122, 0xf, 0xf, false));
+    t += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, t), 0x121, 0xf, 0xf, false));
+    mine = (threadIdx.x & 15) == k ? t : mine;
+  }
+  return mine;
+}
+__device__ __forceinline__ int block_sum_row() { return mma_row((threadIdx.x & 7) + 8 * ((threadIdx.x >> 4) & 1)); }
 
 // Work number of a block such that neighbours in number are on one XCD (blocks go round the eight) and share its L2.
 __device__ __forceinline__ int64_t xcd_order(int64_t block, int64_t blocks) {
