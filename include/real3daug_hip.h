@@ -624,7 +624,9 @@ int r3d_host_append_text_files(const char *const *src, const char *const *dst, c
  *   order), then every row with fewer pops the rest from the end of the stack.  The first row whose blocks are not there and
  *   every later growing row keep what they had, and so does a row whose length is negative or beyond its table.
  * held_out[i] = lengths[i] where served, held[i] elsewhere; status (nullable) is set to R3D_S_CAPACITY where a row was not
- * served or a block is both free and held, else to 0.  free_out is -1 from n_free_out[0] on.  Needs max_blocks * block_size < 2^31. */
+ * served or a block is both free and held, else to 0.  free_out is -1 from n_free_out[0] on.  Needs max_blocks * block_size < 2^31 and
+ * at most R3D_MAX_SCENES rows (256 rows a workgroup, and each reads the sums of all). */
+#define R3D_MAX_SCENES (1 << 24)
 size_t r3d_block_tables_workspace_bytes(int64_t n_rows);
 int r3d_block_tables(const int32_t *lengths, int64_t n_rows, int32_t block_size, int32_t max_blocks, const int32_t *tables,
                      const int32_t *held, const int32_t *free_blocks, int64_t n_blocks, const int32_t *n_free, int32_t *tables_out,
@@ -638,7 +640,7 @@ int r3d_block_tables(const int32_t *lengths, int64_t n_rows, int32_t block_size,
  *   tables null: one block a row (a batch's slabs, block_size = cap): slots[t] = row * block_size + p;
  *   sequence[t] = i.
  * -1 in both behind the last token, up to capacity; tokens beyond capacity are left out (offsets tell).  A row may be listed twice.
- * slots and sequence 16-byte aligned. */
+ * At most R3D_MAX_SCENES sequences (one workgroup sums them); slots and sequence 16-byte aligned. */
 int r3d_slot_map(const int32_t *lengths, int64_t n_lengths, const int32_t *tables, int32_t block_size, int32_t max_blocks,
                  const int32_t *rows, int64_t n_seq, int64_t capacity, int64_t *offsets, int64_t *slots, int32_t *sequence,
                  void *stream);

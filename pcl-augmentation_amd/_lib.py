@@ -87,6 +87,7 @@ class Rows(C.Structure):
 
 T_F32, T_BF16, T_F16, T_F64, T_I32, T_I64 = range(6)
 MAX_ROW_ARRAYS, ROTARY_MAX_AXES, ROTARY_MAX_PAIRS = 4, 8, 256
+MAX_SCENES = 1 << 24
 CE_NONE, CE_SUM, CE_MEAN = 0, 1, 2
 CE_BYTES_STATE, CE_BYTES_FORWARD, CE_BYTES_BACKWARD = 0, 1, 2
 

@@ -347,7 +347,7 @@ int64_t groups_of(int64_t n_rows) { return (n_rows + kGroup - 1) / kGroup; }
 }  // namespace
 
 extern "C" size_t r3d_block_tables_workspace_bytes(int64_t n_rows) {
-  if (n_rows <= 0 || n_rows > INT32_MAX) return 0;
+  if (n_rows <= 0 || n_rows > R3D_MAX_SCENES) return 0;
   return align_up((size_t)groups_of(n_rows) * 2 * sizeof(int64_t));
 }
 
@@ -357,7 +357,7 @@ extern "C" int r3d_block_tables(const int32_t *lengths, int64_t n_rows, int32_t 
                                 void *workspace, size_t workspace_bytes, void *stream) {
   if (!lengths || !tables || !held || !free_blocks || !n_free || !tables_out || !held_out || !free_out || !n_free_out || !workspace)
     return fail(R3D_E_ARG, "block_tables: null pointer");
-  if (n_rows <= 0 || n_rows > INT32_MAX || block_size <= 0 || max_blocks <= 0 || n_blocks <= 0 || n_blocks > INT32_MAX ||
+  if (n_rows <= 0 || n_rows > R3D_MAX_SCENES || block_size <= 0 || max_blocks <= 0 || n_blocks <= 0 || n_blocks > INT32_MAX ||
       (int64_t)max_blocks * block_size > INT32_MAX || n_rows * (int64_t)max_blocks > (1ll << 40))
     return fail(R3D_E_ARG, "block_tables: bad size");
   if (tables == tables_out || held == held_out || free_blocks == free_out || n_free == n_free_out)
@@ -382,7 +382,7 @@ extern "C" int r3d_slot_map(const int32_t *lengths, int64_t n_lengths, const int
                             const int32_t *rows, int64_t n_seq, int64_t capacity, int64_t *offsets, int64_t *slots,
                             int32_t *sequence, void *stream) {
   if (!lengths || !offsets || !slots || !sequence) return fail(R3D_E_ARG, "slot_map: null pointer");
-  if (n_lengths <= 0 || n_lengths > INT32_MAX || n_seq < 0 || n_seq > INT32_MAX || (!rows && n_seq > n_lengths) || capacity < 0 ||
+  if (n_lengths <= 0 || n_lengths > INT32_MAX || n_seq < 0 || n_seq > R3D_MAX_SCENES || (!rows && n_seq > n_lengths) || capacity < 0 ||
       block_size <= 0 || (tables && max_blocks <= 0) || capacity > (1ll << 42) ||
       (tables && (int64_t)max_blocks * block_size > INT32_MAX))
     return fail(R3D_E_ARG, "slot_map: bad size");

@@ -47,8 +47,8 @@ def block_tables(lengths, block_size, tables, held, free_blocks, n_free):
     rows, most = tables.shape
     if lengths.shape[0] != rows or held.shape[0] != rows or n_free.shape[0] != 1:
         raise ValueError(f"{what}: lengths and held must be [{rows}], n_free [1]")
-    if rows < 1 or most < 1 or free_blocks.shape[0] < 1:
-        raise ValueError(f"{what}: no rows or no blocks")
+    if not 1 <= rows <= _lib.MAX_SCENES or most < 1 or free_blocks.shape[0] < 1:
+        raise ValueError(f"{what}: no rows or no blocks (or more than 2^24 rows)")
     block_size = int(block_size)
     if block_size < 1 or block_size * most >= 2 ** 31:
         raise ValueError(f"{what}: block_size must be positive and block_size * max_blocks below 2^31")
@@ -83,6 +83,8 @@ def slot_map(lengths, block_size, tables=None, rows=None, capacity=None):
         raise ValueError(f"{what}: no rows, or block_size not positive, or block_size * max_blocks not below 2^31")
     if capacity is not None and int(capacity) < 0:
         raise ValueError(f"{what}: capacity must not be negative")
+    if (lengths if rows is None else rows).shape[0] > _lib.MAX_SCENES:
+        raise ValueError(f"{what}: more than 2^24 scenes")
     with on_device_of(what, lengths, *[t for t in (tables, rows) if t is not None]):
         lib = _lib.load()
         if capacity is None:
@@ -162,7 +164,8 @@ def take_rows(slots, sources):
 def put_rows(slots, rows, dests, source_slots=None):
     """The other way, in place: ``dests[k][slots[t]] = rows[k][t]`` -- or ``rows[k][source_slots[t]]`` -- for up to four pairs of
     tensors in one pass.  Nothing is written where either slot is outside (a map's -1): rows that no slot names stay as they
-    were.  The slots must be distinct; which of two equal ones wins is not defined.  Returns dests."""
+    were.  The slots must be distinct; which of two equal ones wins is not defined, nor is a row read that the same call writes.
+    Returns dests."""
     what = "put_rows"
     _slots(what, "slots", slots)
     rows, dests = _rows_of(what, "rows", rows), _rows_of(what, "dests", dests)
@@ -196,7 +199,8 @@ class ScenePool:
     """Up to ``max_scenes`` augmented scenes resident on one GPU, in ``n_blocks`` pages of ``block_size`` points.
 
     ``add(batch)`` takes the scenes of a finished ``SceneBatch`` where they stand, ``packed(scenes)`` returns the points of the
-    scenes a step asks for; neither waits for the device (but see ``packed``)."""
+    scenes a step asks for; neither waits for the device (but see ``packed``, and numbers in a tensor are read back).  All on the
+    current stream: a program that uses the pool from several orders them."""
 
     def __init__(self, max_scenes, max_points, n_blocks=None, block_size=2048, device="cuda:0"):
         torch = _lib.require_gpu()
@@ -226,6 +230,11 @@ class ScenePool:
             raise ValueError(f"ScenePool: scenes are numbered 0 to {self.max_scenes - 1}")
         return scenes
 
+    def _on_device(self, scenes):
+        """Scene numbers on the device; from pinned memory, which no call waits for."""
+        import torch
+        return torch.tensor(scenes, dtype=torch.int32, pin_memory=True).to(self.device, non_blocking=True)
+
     @property
     def lengths(self):
         """Points of every scene (int32 [max_scenes], on the device; 0: no scene)."""
@@ -254,7 +263,7 @@ class ScenePool:
         scenes = self.check_scenes(scenes, batch.B)
         if batch.device != self.device and (batch.device.type, batch.device.index or 0) != (self.device.type, self.device.index or 0):
             raise ValueError(f"ScenePool.add: the batch is on {batch.device}, the pool on {self.device}")
-        rows = torch.tensor(scenes, dtype=torch.int32, device=self.device)
+        rows = self._on_device(scenes)
         self.resize(self.blocks.held.index_copy(0, rows.long(), batch.n_out))
         taken = self.blocks.held[rows.long()] == batch.n_out
         new = torch.where(taken, batch.n_out, 0)
@@ -267,17 +276,14 @@ class ScenePool:
     @_lib.on_own_device
     def remove(self, scenes):
         """These scenes' pages are free again."""
-        import torch
-        rows = torch.tensor(self._rows(scenes), dtype=torch.int64, device=self.device)
-        self.resize(self.blocks.held.index_fill(0, rows, 0))
+        self.resize(self.blocks.held.index_fill(0, self._on_device(self._rows(scenes)).long(), 0))
 
     @_lib.on_own_device
     def packed(self, scenes, capacity=None):
         """The points and labels of these scenes (any order, repeats allowed), one scene after the other (``PackedScenes``).
         ``capacity``: room for that many points, zeros behind the last one (None: exactly as many as there are, which
         reads the lengths back)."""
-        import torch
-        rows = torch.tensor(self._rows(scenes), dtype=torch.int32, device=self.device)
+        rows = self._on_device(self._rows(scenes))
         m = slot_map(self.blocks.held, self.block_size, self.blocks.tables, rows, capacity)
         xyzi, label = take_rows(m.slots, (self.xyzi, self.label))
         return PackedScenes(xyzi, label, m.offsets, m.sequence, m.slots)

@@ -323,3 +323,48 @@ def test_from_a_batch_to_the_gradients_of_a_step(pkg, synth):
         assert (a.double() - b).norm() <= 7 * 260 * 2.0 ** -24 * max(b.norm().item(), 1e-3) * 8
     attended = own[1]
     assert torch.isfinite(attended).all() and attended.any()
+
+
+def test_rows_beyond_32_bits(pkg):
+    """A pool of 300 million points: slots, byte offsets and pages past 2^32."""
+    block, most, scenes = 2048, 64, 2300
+    points = block * most * scenes      # 4.8 GB of x y z i
+    xyzi = torch.arange(points, dtype=torch.int32, device="cuda").view(-1, 1).expand(-1, 4).to(torch.int32).contiguous()
+    tables = torch.randperm(most * scenes, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(scenes, most).cuda()
+    lengths = torch.full((scenes,), block * most - 7, dtype=torch.int32, device="cuda")
+    m = pkg.slot_map(lengths, block, tables, capacity=points)
+    n = scenes * (block * most - 7)
+    assert int(m.offsets[-1]) == n and (m.slots[n:] == -1).all() and (m.sequence[n:] == -1).all()
+    t = torch.arange(n, device="cuda")
+    seq, p = t // (block * most - 7), t % (block * most - 7)
+    assert torch.equal(m.sequence[:n], seq.int())
+    assert torch.equal(m.slots[:n], tables[seq, p // block].long() * block + p % block)
+    out, = pkg.take_rows(m.slots, (xyzi,))
+    assert torch.equal(out[:n, 3], m.slots[:n].int()) and not out[n:].any()
+    back = torch.full_like(xyzi, -5)
+    pkg.put_rows(m.slots, (out,), (back,))
+    named = torch.zeros(points, dtype=torch.bool, device="cuda")
+    named[m.slots[:n]] = True
+    assert torch.equal(back[named], xyzi[named]) and (back[~named] == -5).all()
+
+
+def test_pool_calls_do_not_wait_for_the_device(pkg, synth):
+    """Work that is still running when ``packed`` and ``remove`` are called is still running when they return."""
+    scenes, slots, need = _scenes(synth, 3)
+    pool = pkg.ScenePool(4, 8192, block_size=512)
+    want, _ = pkg.augment_batch(scenes, slots, need), pkg.augment_batch(scenes, slots, need, pool=pool)
+    pool.packed([1, 0], capacity=9000)      # (kernels loaded)
+    pool.remove([3])
+    a = torch.randn((8192, 8192), device="cuda")
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    for _ in range(12):
+        a = a @ a * 1e-4
+    done.record()
+    got = pool.packed([1, 0], capacity=9000)
+    pool.remove([0])
+    running = not done.query()
+    torch.cuda.synchronize()
+    assert running
+    n = len(want[0][1][0])
+    assert got.xyzi[:n].cpu().numpy().tobytes() == want[0][1][0].tobytes() and pool.lengths.tolist()[0] == 0
