@@ -383,7 +383,7 @@ __global__ __launch_bounds__(256) void k_ce_top(const float *grad, int64_t n, co
   __shared__ float s[4];
   float top = 0.0f;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-    if (place[i] >= 0) top = fmaxf(top, fabsf(grad[i]));      // (fmaxf passes over NaN)
+    if (place[i] >= 0 && fabsf(grad[i]) < INFINITY) top = fmaxf(top, fabsf(grad[i]));      // (what is no number or infinite is left out)
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = top;
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(256) void k_ce_weight(WeightArgs a) {
     for (int b = threadIdx.x & 63; b < a.parts; b += 64) scale = fmaxf(scale, a.part[b]);
 #pragma unroll
     for (int d = 32; d; d >>= 1) scale = fmaxf(scale, __shfl_xor(scale, d));
-    if (!(scale > 0.0f) || scale == INFINITY) scale = 1.0f;      // nothing to take out
+    if (!(scale > 0.0f)) scale = 1.0f;      // nothing to take out
   } else {
     scale = a.grad[0] * a.counted->share;
   }

@@ -44,7 +44,7 @@ __device__ __forceinline__ float taken_out(const FewArgs &a) {
   for (int i = threadIdx.x & 63; i < a.parts; i += 64) top = fmaxf(top, a.top[i]);
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  return top > 0.0f && top < INFINITY ? top : 1.0f;
+  return top > 0.0f ? top : 1.0f;
 }
 
 template <class V>
@@ -412,7 +412,7 @@ __global__ __launch_bounds__(256) void k_few_top(FewArgs a, float *top_out) {
   float top = 0.0f;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n; i += (int64_t)gridDim.x * 256) {
     const int64_t t = a.wide_target ? static_cast<const int64_t *>(a.target)[i] : static_cast<const int32_t *>(a.target)[i];
-    if (t != a.ignore) top = fmaxf(top, fabsf(a.grad[i]));      // (fmaxf passes over NaN)
+    if (t != a.ignore && fabsf(a.grad[i]) < INFINITY) top = fmaxf(top, fabsf(a.grad[i]));      // (what is no number or infinite is left out)
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));

@@ -147,7 +147,9 @@ def _loss_function():
     def follow(d, x, weight, bias, target, state):
         """The descriptor's tensors (in the backward pass: as they come back from where they were kept)."""
         d.x, d.w, d.bias, d.target = x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), target.data_ptr()
-        d.ld_x, d.ld_w, d.state = x.stride(0), weight.stride(0), 0 if state is None else state.data_ptr()
+        # (the stride of a single row means nothing)
+        d.ld_x, d.ld_w = (t.stride(0) if t.shape[0] > 1 else t.shape[1] for t in (x, weight))
+        d.state = 0 if state is None else state.data_ptr()
 
     def space(lib, d, which, device):
         size = lib.r3d_linear_ce_bytes(C.byref(d), which)
@@ -171,7 +173,7 @@ def _loss_function():
                 ws, size = space(lib, d, _lib.CE_BYTES_FORWARD, x.device)
                 _lib.check(lib.r3d_linear_ce_forward(C.byref(d), ws.data_ptr(), size, _lib.raw_stream(x.get_device())), "r3d_linear_ce_forward")
             ctx.save_for_backward(x, weight, bias, target, state)
-            ctx.descriptor = d
+            ctx.descriptor, ctx.strides = d, (x.stride(), weight.stride())
             return loss
 
         @staticmethod
@@ -182,8 +184,10 @@ def _loss_function():
             with on_device_of("linear_cross_entropy", x):
                 lib = _lib.load()
                 d = _lib.LinearCE.from_buffer_copy(ctx.descriptor)      # (two backward passes may run at once)
-                # what was multiplied in place still has to be fit for it, wherever it was kept in the meantime
+                # what was multiplied in place still has to be fit for it, wherever and however it was kept in the meantime
+                x, weight = (t if t.stride() == ctx.strides[i] else t.contiguous() for i, t in enumerate((x, weight)))
                 x, weight = (t.clone() if t.data_ptr() % 16 and not at % 16 else t for t, at in ((x, d.x), (weight, d.w)))
+                bias, target = None if bias is None else bias.contiguous(), target.contiguous()
                 follow(d, x, weight, bias, target, state)
                 grad = grad.to(torch.float32).contiguous()
                 d.grad = grad.data_ptr()
@@ -199,7 +203,7 @@ def _loss_function():
 
 def _rows_dense(t):
     """[n, d] with the last axis dense and rows that do not overlap."""
-    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+    return t if t.stride(1) == 1 and (t.shape[0] == 1 or t.shape[1] <= t.stride(0) < 2 ** 31) else t.contiguous()
 
 
 def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduction="mean", piece=0):

@@ -105,6 +105,31 @@ def test_rotary_takes_strides(pkg, dtype):
     near(pkg.rotary_positions(wide, rows[:, :1], (12,))[0], *rotate64(wide, rows[:, :1], (12,), 10000.0, "half"))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("heads,kv,dim,sections", [(4, 2, 48, (8, 8, 8)), (3, 3, 34, (5, 5, 7)), (1, 0, 6, (3,)), (50, 7, 512, (100, 100, 56)), (5, 1, 2, (1,))])
+def test_rotary_layouts_give_the_dense_result(pkg, dtype, heads, kv, dim, sections):
+    """Slices of one projection, heads in front of tokens, one token for all, one head for all, rows that begin anywhere."""
+    g = gen(heads * dim)
+    tokens = 37
+    pos = torch.randn((tokens, len(sections)), generator=g).cuda() * 50
+    both = torch.randn((tokens, heads + 2 * kv + 1, dim + 2), generator=g).to(dtype).cuda()
+    front = torch.randn((heads + kv, tokens, dim), generator=g).to(dtype).cuda().transpose(0, 1)
+    whole = torch.randn((tokens, (heads + 2 * kv) * dim + 1), generator=g).to(dtype).cuda()[:, 1:].view(tokens, -1, dim) if dim > 2 else front
+    for x in (both[:, 1:, :dim], both[:, 1:, 2:], both[:, :, 1:dim + 1], front, whole, both[:1, 1:, :dim].expand(tokens, -1, -1),
+              both[:, :1, :dim].expand(-1, heads + kv, -1)):
+        q, k = x[:, :heads], x[:, heads:heads + kv] if kv else None
+        got = pkg.rotary_positions(q, pos, sections, key=k)
+        want = pkg.rotary_positions(q.contiguous(), pos, sections, key=None if k is None else k.contiguous())
+        assert torch.equal(got[0], want[0]) and (k is None or torch.equal(got[1], want[1]))
+    if kv:      # the gradient of a view goes where the view's elements are
+        x = both[:, 1:, :dim].detach().clone().requires_grad_()
+        y, z = pkg.rotary_positions(x[:, :heads], pos, sections, key=x[:, heads:heads + kv])
+        gy, gz = (torch.randn(t.shape, generator=g).to(dtype).cuda().transpose(0, 1).contiguous().transpose(0, 1) for t in (y, z))
+        dx, = torch.autograd.grad((y, z), x, (gy, gz))
+        turned = pkg.rotary_positions(torch.cat([gy, gz], 1).contiguous(), -pos, sections)[0]
+        assert (dx[:, :heads + kv].float() - turned.float()).abs().max() <= 1e-6 and not dx[:, heads + kv:].any()
+
+
 def test_rotary_of_nothing_and_not_a_number(pkg):
     q = torch.zeros((0, 2, 8), device="cuda", requires_grad=True)
     y, k = pkg.rotary_positions(q, torch.zeros((0, 1), device="cuda"), (4,))
@@ -275,6 +300,59 @@ def test_loss_targets_that_are_no_class(pkg):
     assert torch.isfinite(dx[0]).all() and torch.isnan(dx[1:]).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("v,d", [(20, 64), (260, 64), (400, 96)])
+def test_loss_infinite_gradients_stay_with_their_points(pkg, dtype, v, d):
+    """The gradient of point 3 is infinite, that of point 5 no number: their rows of dx say so, the others are what they are alone."""
+    g = gen(v)
+    x, w = (torch.randn(s, generator=g).to(dtype).cuda() for s in ((300, d), (v, d)))
+    target, up = torch.randint(0, v, (300,), generator=g).cuda(), (torch.rand((300,), generator=g) + 1).cuda() * 40
+    target[7] = -100
+    bad = up.clone()
+    bad[3], bad[5], bad[7], up[3], up[5] = math.inf, math.nan, math.inf, 0, 0
+
+    def dx(u):
+        a = x.clone().requires_grad_()
+        return torch.autograd.grad(pkg.linear_cross_entropy(a, w, target, reduction="none"), a, u)[0]
+
+    got, want = dx(bad), dx(up)
+    assert not torch.isfinite(got[[3, 5]]).any()
+    got[[3, 5]] = 0
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("v,d", [(20, 64), (260, 64), (400, 128), (400, 50)])
+def test_loss_tensors_that_were_kept_elsewhere(pkg, dtype, v, d):
+    """What the backward pass gets back need not lie as it lay: other strides, other addresses, a single row of any stride."""
+    g = gen(v + d)
+    x, w, b = (torch.randn(s, generator=g).to(dtype).cuda() for s in ((90, d), (v, d), (v,)))
+    target = torch.randint(0, v, (90,), generator=g).cuda()
+    turned = lambda t: t.t().contiguous().t() if t.dim() == 2 else t.clone()  # noqa: E731
+
+    def moved(t):
+        out = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:].view(t.shape)
+        return out.copy_(t)
+
+    def wide(t):
+        return torch.empty(t.shape[:-1] + (t.shape[-1] + 3,), dtype=t.dtype, device=t.device)[..., :t.shape[-1]].copy_(t)
+
+    def step(x, w, back=None):
+        ins = [t.detach().requires_grad_() for t in (x, w, b)]
+        if back is None:
+            loss = pkg.linear_cross_entropy(ins[0], ins[1], target[:len(x)], bias=ins[2])
+        else:
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: back(t) if t.is_floating_point() else t):
+                loss = pkg.linear_cross_entropy(ins[0], ins[1], target[:len(x)], bias=ins[2])
+        return (loss.detach(), *torch.autograd.grad(loss, ins))
+
+    want = step(x, w)
+    for back in (turned, moved, wide):
+        assert all(torch.equal(p, q) for p, q in zip(step(x, w, back), want))
+    one = torch.as_strided(x, (1, d), (1, 1))
+    assert all(torch.equal(p, q) for p, q in zip(step(one, w), step(x[:1].clone(), w)))
+
+
 def test_loss_layouts(pkg):
     g = gen(4)
     for dtype in (BF16, F32):
@@ -381,3 +459,117 @@ def test_operators_on_another_stream_and_in_a_graph(pkg):
             graph.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(x, y) for x, y in zip(out, eager(a, b))), k
+
+
+@pytest.mark.parametrize("dtype,v,d,reduction", [(BF16, 260, 64, "none"), (F16, 260, 128, "none"), (BF16, 400, 96, "mean"), (F32, 400, 64, "sum"), (F32, 50, 64, "none")])
+def test_loss_of_many_classes_in_a_graph(pkg, dtype, v, d, reduction):
+    """Forward and backward of every way the head is taken, captured; replayed with new points, labels and gradients."""
+    g = gen(v)
+    n = 700
+    x, w, up = torch.randn((n, d), generator=g).to(dtype).cuda(), torch.randn((v, d), generator=g).to(dtype).cuda(), torch.rand((n,), generator=g).cuda()
+    b, target = torch.randn((v,), generator=g).to(dtype).cuda(), torch.randint(-1, v, (n,), generator=g).cuda()
+
+    def step(x, w, b):
+        loss = pkg.linear_cross_entropy(x, w, target, bias=b, ignore_index=-1, reduction=reduction)
+        return (loss, *torch.autograd.grad(loss, (x, w, b), up if reduction == "none" else up[0]))
+
+    def eager():
+        return [t.detach().clone() for t in step(*(t.detach().clone().requires_grad_() for t in (x, w, b)))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    with torch.cuda.stream(side):
+        step(*leaves)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*leaves)
+    for k in range(4):
+        share = (0.0, 0.3, 1.0, 0.9)[k]
+        x.normal_()
+        up.uniform_(-1, 1)
+        target.copy_(torch.where(torch.rand((n,), generator=g) < share, -1, torch.randint(0, v, (n,), generator=g)))
+        with torch.no_grad():
+            leaves[0].copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, eager())), k
+
+
+def test_two_losses_at_once_on_two_streams(pkg):
+    g = gen(12)
+    work = []
+    for v, d, n, dtype in ((20, 96, 60000, BF16), (260, 128, 30000, F16), (700, 64, 20000, BF16), (30, 64, 20000, F32)):
+        x, w = (torch.randn(s, generator=g).to(dtype).cuda().requires_grad_() for s in ((n, d), (v, d)))
+        work.append((x, w, torch.randint(-1, v, (n,), generator=g).cuda()))
+
+    def step(x, w, t):
+        loss = pkg.linear_cross_entropy(x, w, t, ignore_index=-1)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+
+    want = [step(*p) for p in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for turn in range(3):
+        got = []
+        for s, p in zip(streams, work[turn:] + work[:turn]):
+            with torch.cuda.stream(s):
+                got.append(step(*p))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want[turn:] + want[:turn]):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+# ---- beyond 32 bits ------------------------------------------------------------------------------------------------------------
+def test_rotary_beyond_32_bits(pkg):
+    tokens, heads, dim = 4_300_001, 8, 64      # 2.2e9 elements
+    q = torch.empty((tokens, heads, dim), dtype=BF16, device="cuda").normal_()
+    pos = torch.empty((tokens, 3), device="cuda").uniform_(-50, 50)
+    y, _ = pkg.rotary_positions(q, pos, (10, 10, 10))
+    at = torch.tensor([0, 1, 2 ** 21, 4_194_303, 4_194_304, 4_194_305, tokens - 2, tokens - 1])
+    near(y[at.cuda()], *rotate64(q[at.cuda()], pos[at.cuda()], (10, 10, 10), 10000.0, "half"))
+
+
+@pytest.mark.parametrize("n,v,d", [(9_000_001, 20, 256), (8_500_001, 200, 256), (4_300_001, 300, 512)])
+def test_loss_beyond_32_bits(pkg, n, v, d):
+    """More than 2^31 features: loss and dx at points along the way, db of all (against the definition in 32 bits, in parts)."""
+    x = torch.empty((n, d), dtype=BF16, device="cuda").normal_().requires_grad_()
+    w = (torch.randn((v, d), generator=gen(v)) / math.sqrt(d)).to(BF16).cuda().requires_grad_()
+    b = torch.zeros((v,), dtype=BF16, device="cuda").requires_grad_()
+    target = torch.randint(0, v, (n,), device="cuda")
+    target[torch.rand((n,), device="cuda") < 0.1] = -100
+    loss = pkg.linear_cross_entropy(x, w, target, bias=b, reduction="none")
+    up = torch.rand((n,), device="cuda")
+    dx, dw, db = torch.autograd.grad(loss, (x, w, b), up)
+    at = torch.cat([torch.arange(0, n, n // 200, device="cuda"), torch.tensor([n - 1, 2 ** 31 // d, 2 ** 31 // d - 1, 2 ** 32 // d - 1], device="cuda").clamp(max=n - 1)])
+    x64, w64, t = x.detach()[at].double().cpu(), w.detach().double().cpu(), target[at].cpu()
+    keep = (t != -100).double()
+    logits = x64 @ w64.t()
+    lse = torch.logsumexp(logits, 1)
+    each = (lse - logits[torch.arange(len(at)), t.clamp(min=0)]) * keep
+    e_l = (d + 16) * E * ((x64.abs() @ w64.abs().t()).amax(1) + 1)
+    near(loss[at], each, 2 * e_l + 8 * E * (lse.abs() + each.abs()))
+    dl = torch.exp(logits - lse[:, None])
+    p = dl.clone()
+    dl[torch.arange(len(at)), t.clamp(min=0)] -= 1
+    by = (up[at].double().cpu() * keep)[:, None]
+    tol = (p * (2 * e_l[:, None] + 2.0 ** -20) + 2.0 ** -8 * dl.abs()) * by + 2.0 ** -126
+    size = (dl * by).abs() @ w64.abs()
+    near(dx[at], (dl * by) @ w64, (tol @ w64.abs() + (v + 64) * E * size) * (1 + 2.0 ** -8) + 2.0 ** -8 * ((dl * by) @ w64).abs() + 2.0 ** -126)
+    want, total = torch.zeros((v,), dtype=torch.float64, device="cuda"), torch.zeros((v,), dtype=torch.float64, device="cuda")
+    want_w, total_w = torch.zeros((v, d), dtype=torch.float64, device="cuda"), torch.zeros((v, d), dtype=torch.float64, device="cuda")
+    for part in range(0, n, 200_000):
+        xs, ts, us = x.detach()[part:part + 200_000].double(), target[part:part + 200_000], up[part:part + 200_000].double()
+        g = torch.softmax(xs @ w.detach().double().t(), 1)
+        g[torch.arange(len(ts), device="cuda"), ts.clamp(min=0)] -= 1
+        g *= (us * (ts != -100))[:, None]
+        want += g.sum(0)
+        total += g.abs().sum(0)
+        want_w += g.t().contiguous() @ xs
+        total_w += g.abs().t().contiguous() @ xs.abs()
+    # a probability is off by 2 e_l + 2^-20 of itself, dl of dW by half a step of bfloat16; additions in 32 bits, in chains of at
+    # most 2^14 (a chain's rounding is off by its length times E of what it has summed)
+    rel = 2 * float(e_l.max()) * 2 + 2.0 ** -20 + 2.0 ** 14 * E
+    assert ((db.double() - want).abs() <= rel * total + 2.0 ** -8 * want.abs()).all()
+    assert ((dw.double() - want_w).abs() <= (rel + 2.0 ** -8) * total_w + 2.0 ** -8 * want_w.abs()).all()

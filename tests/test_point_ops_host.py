@@ -138,3 +138,19 @@ def test_linear_cross_entropy_refuses(pkg):
     if not torch.cuda.is_available():
         with pytest.raises(pkg.R3DError):
             pkg.linear_cross_entropy(x, w, t)
+
+
+def test_limits_refuse_without_a_gpu(pkg):
+    L, lib = pkg._lib, pkg._lib.load()
+    p = C.cast(C.create_string_buffer(64), C.c_void_p).value // 16 * 16
+    assert lib.r3d_block_tables_workspace_bytes(L.MAX_SCENES) > 0 and lib.r3d_block_tables_workspace_bytes(L.MAX_SCENES + 1) == 0
+    assert lib.r3d_block_tables(p, L.MAX_SCENES + 1, 16, 2, p, p, p, 8, p, p + 16, p + 16, p + 16, p + 16, None, p, 1 << 40, None) == L.E_ARG
+    assert lib.r3d_slot_map(p, 4, None, 16, 1, p, L.MAX_SCENES + 1, 10, p, p, p, None) == L.E_ARG
+    d = L.Rotary(tokens=4, dim=8, axes=1, base=10.0, pos_type=L.T_F32, type=L.T_F32, pos=p, pos_token_stride=1, pos_axis_stride=1)
+    d.sections[0], d.heads[0], d.token_stride[0], d.head_stride[0], d.x[0], d.y[0] = 4, 1, 8, 8, p + 2, p + 16
+    assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG and b"aligned" in lib.r3d_last_error()
+    d.dim, d.heads[0], d.head_stride[0], d.token_stride[0], d.x[0] = 4096, 65536, 4096, 4096 << 16, p + 32
+    d.heads[1], d.head_stride[1], d.token_stride[1], d.x[1], d.y[1] = 65536, 4096, 4096 << 16, p + 32, p + 16
+    assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG and b"heads" in lib.r3d_last_error()
+    e = L.LinearCE(n=4, v=3, d=8, ld_x=1 << 31, ld_w=8, type=L.T_F32, target_type=L.T_I64, reduction=L.CE_MEAN)
+    assert lib.r3d_linear_ce_bytes(C.byref(e), 0) == 0
