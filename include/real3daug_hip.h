@@ -686,7 +686,8 @@ int r3d_rotary(const r3d_rotary_t *d, void *stream);
  * loss NaN.  loss: float [n] (R3D_CE_NONE) or [1] (sum, mean over the points that count; 0 where none does).
  * The forward call fills `state` (R3D_CE_BYTES_STATE bytes: which points count, their statistics, what had to be packed), which
  * the backward call of the same descriptor reads and leaves as it is.  backward: grad = float [n] or [1]; dx [n][d], dw [v][d],
- * db [v] dense, of `type`, each nullable.  piece: classes whose logit gradients are held at a time (0: as many as 512 MB take).
+ * db [v] dense, of `type`, each nullable.  piece: classes whose logit gradients are held at a time (0: as many as 512 MB take;
+ * with at most 128 features none are).
  * r3d_linear_ce_bytes: of the state and of the two calls' workspaces, for the descriptor as it will be passed (0: bad descriptor). */
 #define R3D_CE_NONE 0
 #define R3D_CE_SUM 1

@@ -348,37 +348,40 @@ __global__ __launch_bounds__(256) void k_ce_join(JoinArgs a) {
   __shared__ int s_last;
   __shared__ float s_top[256], s_sum[256];
   const int points = a.points, slices = 256 / points, p = (int)threadIdx.x % points, slice = (int)threadIdx.x / points;
-  const int64_t i = (int64_t)blockIdx.x * points + p;
-  const int at = i < a.n ? a.place[i] : -1;
-  float top = -INFINITY, sum = 0.0f;
-  if (at >= 0) {
+  double losses = 0.0;
+  for (int64_t block = blockIdx.x; block * points < a.n; block += gridDim.x) {
+    const int64_t i = block * points + p;
+    const int at = i < a.n ? a.place[i] : -1;
+    float top = -INFINITY, sum = 0.0f;
+    if (at >= 0) {
 #pragma unroll 4
-    for (int k = slice; k < a.splits; k += slices) top = fmaxf(top, a.part_m[k * a.n_pad + at]);
-    const float base = top == -INFINITY ? 0.0f : top;
+      for (int k = slice; k < a.splits; k += slices) top = fmaxf(top, a.part_m[k * a.n_pad + at]);
+      const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll 4
-    for (int k = slice; k < a.splits; k += slices) sum += a.part_l[k * a.n_pad + at] * __builtin_amdgcn_exp2f(a.part_m[k * a.n_pad + at] - base);
+      for (int k = slice; k < a.splits; k += slices) sum += a.part_l[k * a.n_pad + at] * __builtin_amdgcn_exp2f(a.part_m[k * a.n_pad + at] - base);
+    }
+    if (slices > 1) {
+      __syncthreads();
+      s_top[threadIdx.x] = top;
+      s_sum[threadIdx.x] = sum;
+      __syncthreads();
+      sum = 0.0f;
+      for (int k = 0; k < slices; ++k) top = fmaxf(top, s_top[k * points + p]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      for (int k = 0; k < slices; ++k) sum += s_sum[k * points + p] * __builtin_amdgcn_exp2f(s_top[k * points + p] - base);
+    }
+    float loss = 0.0f;
+    if (at >= 0 && slice == 0) {
+      const bool fine = a.tgt[at] >= 0;      // a target that is no class: NaN, and so are its gradients
+      const float lse2 = fine ? top + __builtin_amdgcn_logf(sum) : NAN;
+      a.lse2[at] = lse2;
+      loss = fine ? (lse2 - a.hit[at]) * kLn2 : NAN;
+    }
+    losses += loss;
+    if (a.each && i < a.n && slice == 0) a.each[i] = loss;
   }
-  if (slices > 1) {
-    s_top[threadIdx.x] = top;
-    s_sum[threadIdx.x] = sum;
-    __syncthreads();
-    sum = 0.0f;
-    for (int k = 0; k < slices; ++k) top = fmaxf(top, s_top[k * points + p]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    for (int k = 0; k < slices; ++k) sum += s_sum[k * points + p] * __builtin_amdgcn_exp2f(s_top[k * points + p] - base);
-  }
-  float loss = 0.0f;
-  if (at >= 0 && slice == 0) {
-    const bool fine = a.tgt[at] >= 0;      // a target that is no class: NaN, and so are its gradients
-    const float lse2 = fine ? top + __builtin_amdgcn_logf(sum) : NAN;
-    a.lse2[at] = lse2;
-    loss = fine ? (lse2 - a.hit[at]) * kLn2 : NAN;
-  }
-  if (a.each) {
-    if (i < a.n && slice == 0) a.each[i] = loss;
-    return;
-  }
-  const double mine = group_sum(loss, s);
+  if (a.each) return;
+  const double mine = group_sum(losses, s);
   if (threadIdx.x == 0) {
     a.sums[blockIdx.x] = mine;
     __threadfence();
@@ -941,6 +944,24 @@ int cut(int64_t tiles, int64_t slots, int64_t most) {
   return best;
 }
 
+// Parts in which the rows that meet are cut (r3d_loss_narrow.hip): rounds of workgroups times 2.5 us for every 64 rows of a part
+// (417 824 points x 3114 classes x 64: 2.3), and what parts cost that have to be added, written and read at 4.7 TB/s.
+int narrow_splits(int64_t kept, int64_t rows, int64_t slots, int64_t met, int64_t bytes) {
+  const int64_t tiles = (kept + rows - 1) / rows, chunks = (met + 63) / 64;
+  int64_t best = 1;
+  double best_us = 0.0;
+  for (int k = 0; k < 4; ++k) {
+    int64_t s = k ? k * slots / tiles : 1;
+    s = s < 1 ? 1 : s > chunks ? chunks : s;
+    const double us = (double)((tiles * s + slots - 1) / slots * ((chunks + s - 1) / s)) * 2.5 + (s > 1 ? (double)(s * kept * bytes) * 2.0 / 4.7e6 : 0.0);
+    if (k == 0 || us < best_us) {
+      best = s;
+      best_us = us;
+    }
+  }
+  return (int)best;
+}
+
 // A product's tiles: large ones where they fill the chip and waste no more than a quarter over small ones at the edges.
 bool large_tiles(int64_t m, int64_t n, int64_t most_splits) {
   const int64_t big = tiles_of(m, n, Big::BM, Big::BN), small = tiles_of(m, n, Small::BM, Small::BN);
@@ -952,6 +973,7 @@ struct Plan {
   int planes, type_bytes;
   int64_t dp, n_pad, v_pad, piece;
   bool lse_big, dl_big, dx_big, dw_big;
+  bool narrow;      // dl stays in registers (r3d_loss_narrow.hip)
   int lse_splits, dx_splits, dw_splits, db_parts, top_parts, groups;
   int head;                     // blocks of 32 classes of a head that fits LDS, or 0
   size_t head_lds;
@@ -983,6 +1005,12 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   p.v_pad = up(d.v, Big::BM);
   p.head_lds = (size_t)up(d.v, 32) * ((p.dp + 8) * 2 + 4 + kHeadThreads / 64 * 4);
   p.head = p.planes == 1 && d.v <= kHeadBlocks * 32 && p.head_lds <= (size_t)kHeadLds ? (int)(up(d.v, 32) / 32) : 0;
+  // Few features: logits are made again rather than their gradients stored.  Stored / made again, us, forward and backward: bf16
+  // 417 824 x 3114 x 9 4350 / 1400, 200 000 x 1000 x 64 630 / 350, 20 000 x 20 000 x 128 1050 / 690, 2000 x 161 280 x 128 920 / 600;
+  // fp32 199 334 x 878 x 10 2010 / 610, 5000 x 5000 x 128 330 / 240.  A head in LDS with 128 features stores: 100 000 x 150 x 128
+  // 106 / 117, 126 403 x 260 x 128 160 / 157; with 64 it does not: 270 597 x 260 x 64 237 / 214, 200 000 x 150 x 64 142 / 143.
+  p.narrow = p.dp <= 128 && !(p.head && p.dp > 64);
+  const int64_t slots = p.planes == 3 && p.dp > 64 ? kCus : 2 * kCus;      // workgroups of r3d_loss_narrow.hip that the chip holds
   p.groups = d.n <= kOneGroup ? 1 : (int)((d.n + kStartRows - 1) / kStartRows);
   Carver k(d.state);
   p.counted = k.take<Counted>(1);
@@ -1000,14 +1028,32 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   if (!backward) {
     p.lse_big = large_tiles(d.v, d.n, 1);
     const int64_t bm = p.lse_big ? Big::BM : Small::BM, bn = p.lse_big ? Big::BN : Small::BN;
-    p.lse_splits = p.head ? 1 : cut(up(d.n, bn) / bn, kCus * (p.lse_big ? Big::per_cu : Small::per_cu), up(d.v, bm) / bm);
+    const int64_t of_points = p.narrow ? narrow_rows(Narrow::Lse, p.planes, (int)p.dp) : 0;
+    p.lse_splits = p.head ? 1 : p.narrow ? narrow_splits(d.n, of_points, slots, d.v, 8) : cut(up(d.n, bn) / bn, kCus * (p.lse_big ? Big::per_cu : Small::per_cu), up(d.v, bm) / bm);
     p.part = c.take<int32_t>(p.groups);
     p.part_m = c.take<float>((size_t)p.lse_splits * p.n_pad);
     p.part_l = c.take<float>((size_t)p.lse_splits * p.n_pad);
     p.hit = c.take<float>(p.n_pad);
-    p.sums = c.take<double>((d.n + join_points(p.lse_splits) - 1) / join_points(p.lse_splits));
+    p.sums = c.take<double>(kCus);
   } else {
     const int64_t v64 = up(d.v, kPadK);
+    p.top_parts = (int)(d.n < 256 * 256 ? (d.n + 255) / 256 : 256);
+    p.top = c.take<float>(p.top_parts);
+    p.scale = c.take<float>(1);
+    p.weight = c.take<float>(p.n_pad);
+    if (p.narrow) {
+      const int64_t of_points = narrow_rows(Narrow::Dx, p.planes, (int)p.dp), of_classes = narrow_rows(Narrow::Dw, p.planes, (int)p.dp);
+      p.piece = v64;
+      p.dx_splits = narrow_splits(d.n, of_points, slots, d.v, p.dp * 4);
+      p.dw_splits = p.db_parts = narrow_splits(d.v, of_classes, slots, d.n, p.dp * 4);
+      p.dx_final = p.dx_splits == 1;
+      p.dw_final = p.dw_splits == 1;
+      if (!p.dx_final && d.dx) p.accx = c.take<float>((size_t)p.dx_splits * p.n_pad * p.dp);
+      if (!p.dw_final && d.dw) p.accw = c.take<float>((size_t)p.dw_splits * v64 * p.dp);
+      if (d.db) p.accb = c.take<float>((size_t)p.db_parts * v64);
+      p.bytes = c.off;
+      return p;
+    }
     int64_t piece = d.piece > 0 ? up(d.piece, kPadK) : kPieceBytes / (p.n_pad * 2 * p.planes) / Big::BM * Big::BM;
     if (piece < Small::BM) piece = Small::BM;
     p.piece = piece < v64 ? piece : v64;
@@ -1022,10 +1068,6 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus, kw);
     p.dx_final = p.head || (p.dx_splits == 1 && p.piece >= d.v);
     p.dw_final = p.dw_splits == 1;
-    p.top_parts = (int)(d.n < 256 * 256 ? (d.n + 255) / 256 : 256);
-    p.top = c.take<float>(p.top_parts);
-    p.scale = c.take<float>(1);
-    p.weight = c.take<float>(p.n_pad);
     p.dl = c.take<uint16_t>((size_t)p.planes * p.n_pad * p.piece);
     if (!p.dx_final) p.accx = c.take<float>((size_t)p.dx_splits * p.n_pad * p.dp);
     p.accw = c.take<float>((size_t)(p.dw_final || !d.dw ? 0 : p.dw_splits) * p.piece * p.dp);
@@ -1070,7 +1112,8 @@ void join(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   JoinArgs ja{p.part_m, p.part_l, p.hit, p.tgt, p.place, p.counted, p.lse2, d.reduction == R3D_CE_NONE ? d.loss : nullptr, d.loss, p.sums, d.n, p.n_pad,
               p.lse_splits, d.reduction == R3D_CE_MEAN};
   ja.points = join_points(p.lse_splits);
-  hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((d.n + ja.points - 1) / ja.points)), dim3(256), 0, st, ja);
+  // a sum: a workgroup a CU, each raises the one counter (270 597 points: 39 us with one for every 256 points, 17 so)
+  hipLaunchKernelGGL(k_ce_join, dim3(blocks_for(d.n, ja.points, d.reduction == R3D_CE_NONE ? INT32_MAX : kCus)), dim3(256), 0, st, ja);
 }
 
 HeadArgs head_args(const r3d_linear_ce_t &d, const Plan &p) {
@@ -1149,6 +1192,24 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     join(d, p, st);
     return;
   }
+  if (p.narrow) {
+    NarrowArgs na{};
+    operands(d, p, na.kept, na.met);
+    const int64_t of_points = narrow_rows(Narrow::Lse, kPlanes, (int)p.dp);
+    na.v = d.v;
+    na.bias2 = p.bias2;
+    na.tgt = p.tgt;
+    na.counted = p.counted;
+    na.tiles = (int)((d.n + of_points - 1) / of_points);
+    na.splits = p.lse_splits;
+    na.split_stride = p.n_pad;
+    na.part_m = p.part_m;
+    na.part_l = p.part_l;
+    na.hit = p.hit;
+    narrow(Narrow::Lse, na, d.type, (int)p.dp, st);
+    join(d, p, st);
+    return;
+  }
   LseArgs la{};
   operands(d, p, la.p.b, la.p.a);
   la.p.planes = kPlanes;
@@ -1212,6 +1273,52 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   Operand x, w;
   operands(d, p, x, w);
   const float held = d.type == R3D_T_F16 ? 32768.0f : 1.0f, unheld = 1.0f / held;
+  if (p.narrow) {
+    Finish of[3];
+    int n_of = 0;
+    NarrowArgs na{};
+    na.v = d.v;
+    na.bias2 = p.bias2;
+    na.lse2 = p.lse2;
+    na.weight = p.weight;
+    na.tgt = p.tgt;
+    na.counted = p.counted;
+    na.held = held;
+    na.d = d.d;
+    na.scale = p.scale;
+    na.unheld = unheld;
+    const int64_t of_points = narrow_rows(Narrow::Dx, kPlanes, (int)p.dp), of_classes = narrow_rows(Narrow::Dw, kPlanes, (int)p.dp);
+    auto vector = [&](const void *out) { return d.d % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(S)) == 0; };
+    if (d.dx) {
+      na.kept = x;
+      na.met = w;
+      na.tiles = (int)((d.n + of_points - 1) / of_points);
+      na.splits = p.dx_splits;
+      na.out = p.accx;
+      na.split_stride = p.n_pad * p.dp;
+      na.final_out = p.dx_final ? d.dx : nullptr;
+      na.vector_out = vector(d.dx);
+      narrow(Narrow::Dx, na, d.type, (int)p.dp, st);
+      if (!p.dx_final) of[n_of++] = finish_of<S>(p.accx, p.dp, p.n_pad * p.dp, d.n, d.d, p.dx_splits, p.place, d.dx);
+    }
+    if (d.dw || d.db) {
+      na.kept = w;
+      na.met = x;
+      na.tiles = (int)((d.v + of_classes - 1) / of_classes);
+      na.splits = p.dw_splits;
+      na.out = p.accw;
+      na.split_stride = p.piece * p.dp;
+      na.final_out = p.dw_final ? d.dw : nullptr;
+      na.vector_out = vector(d.dw);
+      na.sums = p.accb;
+      na.sums_stride = p.piece;
+      narrow(Narrow::Dw, na, d.type, (int)p.dp, st);
+      if (!p.dw_final && d.dw) of[n_of++] = finish_of<S>(p.accw, p.dp, p.piece * p.dp, d.v, d.d, p.dw_splits, nullptr, d.dw);
+      if (d.db) of[n_of++] = finish_of<S>(p.accb, p.piece, p.piece, 1, d.v, p.db_parts, nullptr, d.db);
+    }
+    finish<S>(of, n_of, p, unheld, st);
+    return;
+  }
   for (int64_t v0 = 0; v0 < d.v; v0 += p.piece) {
     const int64_t real_v = p.piece < d.v - v0 ? p.piece : d.v - v0, width = up(real_v, kPadK);
     Finish of[3];

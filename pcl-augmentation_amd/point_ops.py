@@ -213,7 +213,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     Points whose target is ``ignore_index`` have loss and gradient 0, whatever their features are; a target that is no class makes
     the loss NaN.  reduction: "mean" over the points that count (0 where none does), "sum" or "none" ([...]); the loss is
     float32.  Differentiable once in x, weight and bias; the backward pass makes the logits' gradients ``piece`` classes at a time
-    (0: as many as 512 MB hold).  The same inputs give the same bits."""
+    (0: as many as 512 MB hold; with at most 128 features none are held).  The same inputs give the same bits."""
     import torch
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise ValueError(f"linear_cross_entropy: x [..., features] and weight [classes, features], got {tuple(x.shape)} and {tuple(weight.shape)}")
