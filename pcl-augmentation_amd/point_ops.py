@@ -144,34 +144,37 @@ def _loss_function():
     import torch
     from torch.autograd.function import once_differentiable
 
+    # Every line here is on the way of each step, forward on the caller's thread and backward on the engine's: what a small call
+    # costs beyond its kernels is these lines (and the engine itself, 70 us).
+    empty, f32, u8 = torch.empty, torch.float32, torch.uint8
+    values, targets = _types()
+
     def follow(d, x, weight, bias, target, state):
         """The descriptor's tensors (in the backward pass: as they come back from where they were kept)."""
         d.x, d.w, d.bias, d.target = x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), target.data_ptr()
         # (the stride of a single row means nothing)
         d.ld_x, d.ld_w = (t.stride(0) if t.shape[0] > 1 else t.shape[1] for t in (x, weight))
-        d.state = 0 if state is None else state.data_ptr()
+        d.state = state.data_ptr()
 
     def space(lib, d, which, device):
         size = lib.r3d_linear_ce_bytes(C.byref(d), which)
         if size == 0:
             _lib.check(_lib.E_ARG, "r3d_linear_ce_bytes")
-        return torch.empty(size, dtype=torch.uint8, device=device), size
+        return empty(size, dtype=u8, device=device)
 
     class LinearCrossEntropy(torch.autograd.Function):
         @staticmethod
-        def forward(ctx, x, weight, bias, target, how):
-            n = x.shape[0]
-            with on_device_of("linear_cross_entropy", x):
-                lib = _lib.load()
-                loss = torch.empty(n if how[1] == _lib.CE_NONE else (), dtype=torch.float32, device=x.device)
-                types = _types()
-                d = _lib.LinearCE(n=n, v=weight.shape[0], d=x.shape[1], ignore_index=how[0], reduction=how[1], piece=how[2],
-                                  type=types[0][x.dtype], target_type=types[1][target.dtype], loss=loss.data_ptr())
-                follow(d, x, weight, bias, target, None)
-                state, _ = space(lib, d, _lib.CE_BYTES_STATE, x.device)
-                d.state = state.data_ptr()
-                ws, size = space(lib, d, _lib.CE_BYTES_FORWARD, x.device)
-                _lib.check(lib.r3d_linear_ce_forward(C.byref(d), ws.data_ptr(), size, _lib.raw_stream(x.get_device())), "r3d_linear_ce_forward")
+        def forward(ctx, x, weight, bias, target, how):      # (the tensors' device is the current one)
+            lib, device = _lib.load(), x.device
+            (n, width), (v, _) = x.shape, weight.shape
+            loss = empty(n if how[1] == _lib.CE_NONE else (), dtype=f32, device=device)
+            d = _lib.LinearCE(x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), target.data_ptr(),
+                              x.stride(0) if n > 1 else width, weight.stride(0) if v > 1 else width, n, v, width, how[0], how[2],
+                              values[x.dtype], targets[target.dtype], how[1], 0, 0, loss.data_ptr())
+            state = space(lib, d, _lib.CE_BYTES_STATE, device)
+            d.state = state.data_ptr()
+            ws = space(lib, d, _lib.CE_BYTES_FORWARD, device)
+            _lib.check(lib.r3d_linear_ce_forward(C.byref(d), ws.data_ptr(), ws.numel(), _lib.raw_stream(x.get_device())), "r3d_linear_ce_forward")
             ctx.save_for_backward(x, weight, bias, target, state)
             ctx.descriptor, ctx.strides = d, (x.stride(), weight.stride())
             return loss
@@ -180,22 +183,32 @@ def _loss_function():
         @once_differentiable
         def backward(ctx, grad):
             x, weight, bias, target, state = ctx.saved_tensors
-            need = ctx.needs_input_grad
             with on_device_of("linear_cross_entropy", x):
-                lib = _lib.load()
+                lib, device = _lib.load(), x.device
                 d = _lib.LinearCE.from_buffer_copy(ctx.descriptor)      # (two backward passes may run at once)
-                # what was multiplied in place still has to be fit for it, wherever and however it was kept in the meantime
-                x, weight = (t if t.stride() == ctx.strides[i] else t.contiguous() for i, t in enumerate((x, weight)))
-                x, weight = (t.clone() if t.data_ptr() % 16 and not at % 16 else t for t, at in ((x, d.x), (weight, d.w)))
-                bias, target = None if bias is None else bias.contiguous(), target.contiguous()
-                follow(d, x, weight, bias, target, state)
-                grad = grad.to(torch.float32).contiguous()
+                if (x.data_ptr(), weight.data_ptr(), target.data_ptr(), state.data_ptr(), x.stride(), weight.stride()) != (d.x, d.w, d.target, d.state, *ctx.strides) \
+                        or (bias is not None and bias.data_ptr() != d.bias):
+                    # what was multiplied in place still has to be fit for it, wherever and however it was kept in the meantime
+                    x, weight = (t if t.stride() == ctx.strides[i] else t.contiguous() for i, t in enumerate((x, weight)))
+                    x, weight = (t.clone() if t.data_ptr() % 16 and not at % 16 else t for t, at in ((x, d.x), (weight, d.w)))
+                    bias, target = None if bias is None else bias.contiguous(), target.contiguous()
+                    follow(d, x, weight, bias, target, state)
+                if grad.dtype is not f32 or not grad.is_contiguous():
+                    grad = grad.to(f32).contiguous()
                 d.grad = grad.data_ptr()
-                new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-                dx, dw, db = (new(x) if need[0] else None, new(weight) if need[1] else None, new(bias) if need[2] else None)
-                d.dx, d.dw, d.db = (0 if o is None else o.data_ptr() for o in (dx, dw, db))
-                ws, size = space(lib, d, _lib.CE_BYTES_BACKWARD, x.device)
-                _lib.check(lib.r3d_linear_ce_backward(C.byref(d), ws.data_ptr(), size, _lib.raw_stream(x.get_device())), "r3d_linear_ce_backward")
+                need_x, need_w, need_b, _, _ = ctx.needs_input_grad
+                dx = dw = db = None
+                if need_x:
+                    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+                    d.dx = dx.data_ptr()
+                if need_w:
+                    dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
+                    d.dw = dw.data_ptr()
+                if need_b:
+                    db = torch.empty_like(bias, memory_format=torch.contiguous_format)
+                    d.db = db.data_ptr()
+                ws = space(lib, d, _lib.CE_BYTES_BACKWARD, device)
+                _lib.check(lib.r3d_linear_ce_backward(C.byref(d), ws.data_ptr(), ws.numel(), _lib.raw_stream(x.get_device())), "r3d_linear_ce_backward")
             return dx, dw, db, None, None
 
     return LinearCrossEntropy
@@ -215,29 +228,31 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     float32.  Differentiable once in x, weight and bias; the backward pass makes the logits' gradients ``piece`` classes at a time
     (0: as many as 512 MB hold; with at most 128 features none are held).  The same inputs give the same bits."""
     import torch
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise ValueError(f"linear_cross_entropy: x [..., features] and weight [classes, features], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    shape, dtype, wide = x.shape, x.dtype, weight.shape
+    if len(shape) < 1 or len(wide) != 2 or shape[-1] != wide[1] or wide[0] < 1 or wide[1] < 1:
+        raise ValueError(f"linear_cross_entropy: x [..., features] and weight [classes, features], got {tuple(shape)} and {tuple(wide)}")
     _value_type("linear_cross_entropy", x)
-    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+    if weight.dtype != dtype or (bias is not None and bias.dtype != dtype):
         raise TypeError("linear_cross_entropy: x, weight and bias must have one type")
-    if bias is not None and bias.shape != weight.shape[:1]:
-        raise ValueError(f"linear_cross_entropy: bias must be [{weight.shape[0]}], got {tuple(bias.shape)}")
-    if target.shape != x.shape[:-1]:
-        raise ValueError(f"linear_cross_entropy: target must be {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    if bias is not None and bias.shape != wide[:1]:
+        raise ValueError(f"linear_cross_entropy: bias must be [{wide[0]}], got {tuple(bias.shape)}")
+    if target.shape != shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: target must be {tuple(shape[:-1])}, got {tuple(target.shape)}")
     if target.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"linear_cross_entropy: target is int32 or int64, got {target.dtype}")
     if reduction not in _REDUCTIONS:
         raise ValueError("linear_cross_entropy: reduction is 'none', 'sum' or 'mean'")
     if int(piece) < 0:
         raise ValueError("linear_cross_entropy: piece must not be negative")
-    if target.numel() > 2 ** 31 - 1025 or weight.shape[0] > 2 ** 31 - 1025 or weight.shape[1] > 1 << 20:
+    points = target.numel()
+    if points > 2 ** 31 - 1025 or wide[0] > 2 ** 31 - 1025 or wide[1] > 1 << 20:
         raise ValueError("linear_cross_entropy: too large (2^31 points, 2^31 classes, 2^20 features)")
-    on_device_of("linear_cross_entropy", x, weight, target, *(() if bias is None else (bias,)))
-    if target.numel() == 0:      # nothing to sum; the gradients are zeros
+    here = on_device_of("linear_cross_entropy", x, weight, target, *(() if bias is None else (bias,)))
+    if points == 0:      # nothing to sum; the gradients are zeros
         none = (x.sum() + weight.sum() * 0 + (0 if bias is None else bias.sum() * 0)).float() * 0
         return none if reduction != "none" else none.expand(target.shape) + torch.zeros(target.shape, device=x.device)
-    how = (int(ignore_index), _REDUCTIONS[reduction], int(piece))
-    flat = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    loss = _loss_function().apply(_rows_dense(flat), _rows_dense(weight), None if bias is None else bias.contiguous(),
-                                  (target if target.dim() == 1 else target.reshape(-1)).contiguous(), how)
-    return loss.reshape(target.shape) if reduction == "none" else loss
+    with here:
+        loss = _loss_function().apply(_rows_dense(x if len(shape) == 2 else x.reshape(-1, shape[-1])), _rows_dense(weight),
+                                      None if bias is None else bias.contiguous(),
+                                      (target if len(shape) == 2 else target.reshape(-1)).contiguous(), (int(ignore_index), _REDUCTIONS[reduction], int(piece)))
+    return loss.reshape(target.shape) if reduction == "none" and len(shape) != 2 else loss
