@@ -45,31 +45,33 @@ def _value_type(what, t):
 
 # ---- rotary positions -------------------------------------------------------------------------------------------------
 def _turn(tensors, positions, sections, base, interleaved, backward):
-    """One launch over up to two [tokens, heads, dim] tensors (None: none); returns dense ones."""
+    """One launch over up to two [tokens, heads, dim] tensors (None: none), on the current device; returns dense ones."""
     import torch
-    d = _lib.Rotary()
-    outs = []
-    for w, x in enumerate(tensors):
-        if x is None or x.shape[1] == 0:
-            d.heads[w] = 0
-            outs.append(None if x is None else torch.empty_like(x))
+    values, whole = _types()
+    first = tensors[0] if tensors[0] is not None else tensors[1]
+    if first is None:
+        return [None, None]
+    tokens, _, dim = first.shape
+    outs, x, y, token_stride, head_stride, heads = [], [0, 0], [0, 0], [0, 0], [0, 0], [0, 0]
+    kept = []
+    for w, t in enumerate(tensors):
+        if t is None:
+            outs.append(None)
             continue
-        if x.stride(2) != 1:
-            x = x.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        outs.append(y)
-        d.x[w], d.y[w] = x.data_ptr(), y.data_ptr()
-        d.token_stride[w], d.head_stride[w] = x.stride(0), x.stride(1)
-        d.heads[w], d.tokens, d.dim, d.type = x.shape[1], x.shape[0], x.shape[2], _types()[0][x.dtype]
-        tensors = tensors[:w] + (x,) + tensors[w + 1:]      # (kept until the launch)
-    if d.heads[0] + d.heads[1] == 0 or d.tokens == 0:
+        outs.append(torch.empty_like(t, memory_format=torch.contiguous_format))
+        if t.shape[1] == 0:
+            continue
+        if t.stride(2) != 1:
+            t = t.contiguous()
+            kept.append(t)      # (until the launch)
+        x[w], y[w] = t.data_ptr(), outs[w].data_ptr()
+        token_stride[w], head_stride[w], _ = t.stride()
+        heads[w] = t.shape[1]
+    if heads == [0, 0] or tokens == 0:
         return outs
-    d.interleaved, d.backward, d.axes, d.base = int(interleaved), int(backward), len(sections), base
-    d.sections[:len(sections)] = sections
-    d.pos_type, d.pos = _types()[1][positions.dtype], positions.data_ptr()
-    d.pos_token_stride, d.pos_axis_stride = positions.stride()
-    with on_device_of("rotary_positions", positions):
-        _lib.check(_lib.load().r3d_rotary(C.byref(d), _lib.raw_stream(positions.get_device())), "r3d_rotary")
+    d = _lib.Rotary(tuple(x), tuple(y), tuple(token_stride), tuple(head_stride), tokens, tuple(heads), dim, values[first.dtype], interleaved, backward,
+                    len(sections), sections, whole[positions.dtype], positions.data_ptr(), *positions.stride(), base)
+    _lib.check(_lib.load().r3d_rotary(C.byref(d), _lib.raw_stream(positions.get_device())), "r3d_rotary")
     return outs
 
 
@@ -89,8 +91,10 @@ def _rotary_function():
         @once_differentiable
         def backward(ctx, grad_query, grad_key):
             # a rotation: the gradient is turned back
-            need = [g if n else None for g, n in zip((grad_query, grad_key), ctx.needs_input_grad)]
-            got = _turn(tuple(need), ctx.saved_tensors[0], *ctx.how, True)
+            positions, = ctx.saved_tensors
+            need = ctx.needs_input_grad
+            with on_device_of("rotary_positions", positions):
+                got = _turn((grad_query if need[0] else None, grad_key if need[1] else None), positions, *ctx.how, True)
             return got[0], got[1], None, None, None, None
 
     return RotaryPositions
@@ -132,10 +136,10 @@ def rotary_positions(query, positions, sections, key=None, base=10000.0, style="
     base = float(base)
     if not base > 0.0 or base == float("inf"):
         raise ValueError("rotary_positions: base must be positive and finite")
-    on_device_of("rotary_positions", query, positions, *(() if key is None else (key,)))
-    if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
-        return _rotary_function().apply(query, key, positions, sections, base, style == "interleaved")
-    return tuple(_turn((query, key), positions, sections, base, style == "interleaved", False))
+    with on_device_of("rotary_positions", query, positions, *(() if key is None else (key,))):
+        if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+            return _rotary_function().apply(query, key, positions, sections, base, style == "interleaved")
+        return tuple(_turn((query, key), positions, sections, base, style == "interleaved", False))
 
 
 # ---- softmax cross entropy of a linear head ------------------------------------------------------------------------------
