@@ -262,7 +262,7 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
   for (int vt = vt0; vt < vt1; ++vt) {
     f32x16 acc[S::FM][S::FN];
     clear(acc);
-    st.run(lds, acc, more);
+    st.run(lds, acc, more, a.v - (int64_t)vt * S::BM);
 #pragma unroll
     for (int i = 0; i < S::FM; ++i) {
       const int vb = vt * S::BM + (wm * S::FM + i) * 32;
@@ -492,7 +492,7 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
     st.lb.tile(st.b, n0, nc);
     auto more = [] { return false; };
     st.begin(lds, 0, (int)a.kb, a.p.planes, more);
-    st.run(lds, acc, more);
+    st.run(lds, acc, more, (a.v - a.piece0 < a.width ? a.v - a.piece0 : a.width) - vt * S::BM);
     st.end();
   }
   T *dl = static_cast<T *>(a.dl);
@@ -619,7 +619,7 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
     st.lb.tile(st.b, n0, a.limit_b);
     auto more = [] { return false; };
     st.begin(lds, (int)kb0, (int)kb1, a.p.planes, more, numbers);
-    st.run(lds, acc, more);
+    st.run(lds, acc, more, m - m0);
     st.end();
   }
   const float scale = a.final_out ? *a.scale * a.unheld : 1.0f;
@@ -920,7 +920,7 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
 // What a piece's dl may take.  8192 points x 161280 classes x 512: 8.8 ms with 64 MB, 7.1 with 256, 6.7 with 512, 6.4 with all 2.6 GB.
 constexpr int64_t kPieceBytes = 512ll << 20;
 constexpr int kCus = 256, kHeadLds = 160 * 1024;
-constexpr int kPadK = 64;      // operands are padded to whole cache lines along k
+constexpr int kPadK = 64;      // a head in LDS and few features: padded to whole cache lines; pieces of the classes
 
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t tiles_of(int64_t m, int64_t n, int64_t bm, int64_t bn) { return (up(m, bm) / bm) * (up(n, bn) / bn); }
@@ -999,7 +999,6 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   Plan p{};
   p.planes = d.type == R3D_T_F32 ? 3 : 1;
   p.type_bytes = d.type == R3D_T_F32 ? 4 : 2;
-  p.direct = p.planes == 1 && d.d % kPadK == 0 && d.ld_x % 8 == 0 && d.ld_w % 8 == 0 && aligned16(d.x) && aligned16(d.w);
   p.dp = up(d.d, kPadK);
   p.n_pad = up(d.n, Big::BN);
   p.v_pad = up(d.v, Big::BM);
@@ -1010,6 +1009,8 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   // fp32 199 334 x 878 x 10 2010 / 610, 5000 x 5000 x 128 330 / 240.  A head in LDS with 128 features stores: 100 000 x 150 x 128
   // 106 / 117, 126 403 x 260 x 128 160 / 157; with 64 it does not: 270 597 x 260 x 64 237 / 214, 200 000 x 150 x 64 142 / 143.
   p.narrow = p.dp <= 128 && !(p.head && p.dp > 64);
+  if (!p.head && !p.narrow) p.dp = up(d.d, kTileK);      // (13 421 x 80 469 x 139 bf16: padded to 160 3370 us, to 192 3500)
+  p.direct = p.planes == 1 && d.d == p.dp && d.ld_x % 8 == 0 && d.ld_w % 8 == 0 && aligned16(d.x) && aligned16(d.w);
   const int64_t slots = p.planes == 3 && p.dp > 64 ? kCus : 2 * kCus;      // workgroups of r3d_loss_narrow.hip that the chip holds
   p.groups = d.n <= kOneGroup ? 1 : (int)((d.n + kStartRows - 1) / kStartRows);
   Carver k(d.state);

@@ -264,25 +264,36 @@ struct Stream {
       else lb.move((kb0 + 1 - kb1) * lb.step(b) + (kPlaneB[pair] - kPlaneB[was]) * b.plane);
     }
   }
-  // acc += all k-blocks of a tile.  A fragment is read one k-step before it is multiplied, over the blocks' borders too: the reads
-  // after a barrier would else hold up the matrix cores of all waves at once.
+  // acc += all k-blocks of a tile whose rows from `rows` on are not there: a wave leaves out its blocks of 32 behind them.
+  // (Waves w and w + 4 of the large shape share a SIMD and have different halves of the rows: what one leaves out the other gains.)
   template <class More>
-  __device__ __forceinline__ void run(T *lds, f32x16 (&acc)[S::FM][S::FN], More &&more) {
+  __device__ __forceinline__ void run(T *lds, f32x16 (&acc)[S::FM][S::FN], More &&more, int64_t rows) {
+    const int64_t mine = (rows + 31) / 32 - (int)(threadIdx.x >> 6) / S::WN * S::FM;
+    const int blocks = __builtin_amdgcn_readfirstlane((int)(mine < 0 ? 0 : mine < S::FM ? mine : S::FM));
+    if (blocks == S::FM) run_blocks<true>(lds, acc, more, S::FM);
+    else run_blocks<false>(lds, acc, more, blocks);
+  }
+  // A fragment is read one k-step before it is multiplied, over the blocks' borders too: the reads after a barrier would else hold
+  // up the matrix cores of all waves at once.
+  template <bool kAll, class More>
+  __device__ __forceinline__ void run_blocks(T *lds, f32x16 (&acc)[S::FM][S::FN], More &&more, int blocks) {
     const int wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
     const int steps = (kb1 - kb0) * pairs;
     typename Mma<T>::v8 fa[2][S::FM], fb[2][S::FN];
     auto read = [&](int kk, int into) {
       const T *pa = lds + get * S::buffer, *pb = pa + S::a_elems;
 #pragma unroll
-      for (int i = 0; i < S::FM; ++i) fa[into][i] = fragment<T, LA, S::BM>(pa, (wm * S::FM + i) * 32, kk);
+      for (int i = 0; i < S::FM; ++i)
+        if (kAll || i < blocks) fa[into][i] = fragment<T, LA, S::BM>(pa, (wm * S::FM + i) * 32, kk);
 #pragma unroll
       for (int j = 0; j < S::FN; ++j) fb[into][j] = fragment<T, LB, S::BN>(pb, (wn * S::FN + j) * 32, kk);
     };
     auto multiply = [&](int from) {
 #pragma unroll
       for (int i = 0; i < S::FM; ++i)
+        if (kAll || i < blocks)
 #pragma unroll
-        for (int j = 0; j < S::FN; ++j) acc[i][j] = Mma<T>::mma(fa[from][i], fb[from][j], acc[i][j]);
+          for (int j = 0; j < S::FN; ++j) acc[i][j] = Mma<T>::mma(fa[from][i], fb[from][j], acc[i][j]);
     };
     static_assert(kTileK == 32, "two k-steps a block");
     wait_loads<(S::ahead - 1) * loads>();
