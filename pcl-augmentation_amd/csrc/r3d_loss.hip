@@ -925,23 +925,23 @@ constexpr int kPadK = 64;      // a head in LDS and few features: padded to whol
 int64_t up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 int64_t tiles_of(int64_t m, int64_t n, int64_t bm, int64_t bn) { return (up(m, bm) / bm) * (up(n, bn) / bn); }
 
-// Parts in which the long axis of a product is cut: enough workgroups for the chip, and no last round that leaves most of it
-// idle.  For dx and dW one workgroup a CU of either shape (parts are written and joined: dW of 119999 x 260 x 256 with two of
-// the small shape 64 + 13 us, with one 49 + 7).
+// Parts in which the long axis of a product is cut: enough workgroups for the chip (two of the small shape a CU: dW of 119 999 x
+// 260 x 256 takes 58 us with one, 45 with two), and no last round that leaves most of it idle.
 int cut(int64_t tiles, int64_t slots, int64_t most) {
-  if (most < 1) most = 1;
-  int best = 1;
+  int64_t best = 1;
   double best_share = 0.0;
-  for (int64_t s = 1; s <= most && s <= 1024; ++s) {
+  for (int k = 0; k <= 4; ++k) {      // one part, and what fills one to four rounds
+    int64_t s = k ? k * slots / tiles : 1;
+    s = s > most ? most : s > 1024 ? 1024 : s;
+    if (s < 1) s = 1;
     const int64_t all = tiles * s, rounds = (all + slots - 1) / slots;
     const double share = (double)all / (double)(rounds * slots);
     if (share > best_share * 1.05) {
-      best = (int)s;
+      best = s;
       best_share = share;
     }
-    if (all >= 4 * slots) break;
   }
-  return best;
+  return (int)best;
 }
 
 // Parts in which the rows that meet are cut (r3d_loss_narrow.hip): rounds of workgroups times 2.5 us for every 64 rows of a part
@@ -962,10 +962,18 @@ int narrow_splits(int64_t kept, int64_t rows, int64_t slots, int64_t met, int64_
   return (int)best;
 }
 
-// A product's tiles: large ones where they fill the chip and waste no more than a quarter over small ones at the edges.
+// A product's tiles: the large ones where their rounds take less time than those of the small ones.  A large tile is four times the
+// work; the small one loses a fifth to LDS (each number that it holds is multiplied half as often).  A large tile with rows behind
+// the last one takes its loads, 0.3 of it, and the blocks of 32 that are there.  70 657 points x 152 classes x 586 fp32, logits: 183
+// us in large tiles, 214 in small; 35 061 x 260 x 256 fp32, dx: 80 and 69.
 bool large_tiles(int64_t m, int64_t n, int64_t most_splits) {
-  const int64_t big = tiles_of(m, n, Big::BM, Big::BN), small = tiles_of(m, n, Small::BM, Small::BN);
-  return big * most_splits >= kCus && big * 4 * 4 <= small * 5;
+  auto rounds = [&](int64_t tiles) {
+    const int64_t s = cut(tiles, kCus, most_splits);
+    return (double)((tiles * s + kCus - 1) / kCus) / (double)s;
+  };
+  const int64_t down = up(m, Big::BM) / Big::BM;
+  const double full = (double)(m / Big::BM) + (m % Big::BM ? 0.3 + 0.7 * (double)up(m % Big::BM, 32) / Big::BM : 0.0);
+  return rounds(tiles_of(m, n, Big::BM, Big::BN)) * 4 * full / (double)down <= rounds(tiles_of(m, n, Small::BM, Small::BN)) * 1.2;
 }
 
 struct Plan {
@@ -1027,7 +1035,7 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   p.state_bytes = k.off;
   Carver c(workspace);
   if (!backward) {
-    p.lse_big = large_tiles(d.v, d.n, 1);
+    p.lse_big = large_tiles(d.v, d.n, up(d.v, Big::BM) / Big::BM);
     const int64_t bm = p.lse_big ? Big::BM : Small::BM, bn = p.lse_big ? Big::BN : Small::BN;
     const int64_t of_points = p.narrow ? narrow_rows(Narrow::Lse, p.planes, (int)p.dp) : 0;
     p.lse_splits = p.head ? 1 : p.narrow ? narrow_splits(d.n, of_points, slots, d.v, 8) : cut(up(d.n, bn) / bn, kCus * (p.lse_big ? Big::per_cu : Small::per_cu), up(d.v, bm) / bm);
@@ -1065,8 +1073,8 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     p.dx_big = large_tiles(d.n, p.dp, kx);
     p.dw_big = large_tiles(p.piece, p.dp, kw);
     auto tiles = [&](int64_t m, int64_t n, bool big) { return big ? tiles_of(m, n, Big::BM, Big::BN) : tiles_of(m, n, Small::BM, Small::BN); };
-    p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus, kx);
-    p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus, kw);
+    p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus * (p.dx_big ? Big::per_cu : Small::per_cu), kx);
+    p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus * (p.dw_big ? Big::per_cu : Small::per_cu), kw);
     p.dx_final = p.head || (p.dx_splits == 1 && p.piece >= d.v);
     p.dw_final = p.dw_splits == 1;
     p.dl = c.take<uint16_t>((size_t)p.planes * p.n_pad * p.piece);
