@@ -248,6 +248,20 @@ def test_loss_larger(pkg, dtype, n, v, d, share):
     check_loss(pkg, n, v, d, dtype, share=share)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,v,d,reduction", [(9000, 1500, 64, "mean"), (2500, 2900, 128, "none"), (70000, 100, 128, "sum"), (33000, 50, 64, "none"),
+                                             (600, 40000, 30, "mean"), (7, 30000, 100, "none"), (1, 65, 1, "sum"), (257, 129, 65, "none"), (64, 64, 200, "mean")])
+def test_loss_few_features(pkg, dtype, n, v, d, reduction):
+    """Logits that are made again: points and classes that end anywhere in what a wave keeps and in what it meets."""
+    check_loss(pkg, n, v, d, dtype, reduction=reduction, share=0.15)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,v,d", [(33000, 152, 586), (35000, 260, 160), (2000, 5600, 310), (5, 9000, 290), (300, 1100, 512)])
+def test_loss_many_features(pkg, dtype, n, v, d):
+    check_loss(pkg, n, v, d, dtype, share=0.1)
+
+
 @pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
 def test_loss_where_no_point_counts(pkg, reduction):
     loss, got = check_loss(pkg, 150, 20, 64, BF16, target=torch.full((150,), -100), reduction=reduction)
