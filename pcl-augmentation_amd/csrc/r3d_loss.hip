@@ -203,7 +203,6 @@ __global__ __launch_bounds__(kStartThreads) void k_ce_index(StartArgs a) {
 // ---- products --------------------------------------------------------------------------------------------------------------
 struct Product {
   Operand a, b;
-  int32_t planes;
 };
 
 // Tiles in groups of 8 in n, so that the workgroups that run at a time share their rows of both operands.
@@ -227,7 +226,7 @@ struct LseArgs {
 // Maximum and sum of 2^(logit * log2 e) over a split of the classes for the points of a tile.  The classes are the rows of C, so
 // a lane holds 16 FM classes of each of its FN points: the statistics of a tile stay in its registers, lanes and waves are
 // joined once at the end.
-template <class T, class S>
+template <class T, class S, int kPlanes>
 __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
   __shared__ __attribute__((aligned(128))) T lds[S::buffers * S::buffer];
   const int nc = a.counted->n;
@@ -246,7 +245,7 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
     tgt[j] = col < nc ? a.tgt[col] : -1;
   }
   const int vt0 = (int)((int64_t)a.vtiles * split / a.splits), vt1 = (int)((int64_t)a.vtiles * (split + 1) / a.splits);
-  Stream<T, S, Lies::Rows, Lies::Rows> st;
+  Stream<T, S, Lies::Rows, Lies::Rows, kPlanes> st;
   st.a = a.p.a;
   st.b = a.p.b;
   st.rows_b = 0;
@@ -258,7 +257,7 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
     st.la.tile(st.a, (int64_t)ahead * S::BM, a.v);
     return true;
   };
-  if (vt1 > vt0) st.begin(lds, 0, (int)a.kb, a.p.planes, more);
+  if (vt1 > vt0) st.begin(lds, 0, (int)a.kb, more);
   for (int vt = vt0; vt < vt1; ++vt) {
     f32x16 acc[S::FM][S::FN];
     clear(acc);
@@ -484,14 +483,14 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
   f32x16 acc[S::FM][S::FN];
   clear(acc);
   {
-    Stream<T, S, Lies::Rows, Lies::Rows> st;
+    Stream<T, S, Lies::Rows, Lies::Rows, kPlanes> st;
     st.a = a.p.a;
     st.b = a.p.b;
     st.rows_b = 0;
     st.la.tile(st.a, a.piece0 + vt * S::BM, a.v);
     st.lb.tile(st.b, n0, nc);
     auto more = [] { return false; };
-    st.begin(lds, 0, (int)a.kb, a.p.planes, more);
+    st.begin(lds, 0, (int)a.kb, more);
     st.run(lds, acc, more, (a.v - a.piece0 < a.width ? a.v - a.piece0 : a.width) - vt * S::BM);
     st.end();
   }
@@ -609,16 +608,17 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
   clear(acc);
   const int64_t kb0 = kb * split / a.splits, kb1 = kb * (split + 1) / a.splits;
   constexpr bool kGather = LA == Lies::PiecesCols;      // x by the points' numbers
-  __shared__ int32_t numbers[Stream<T, S, LA, Lies::Cols, kGather>::number_words];
+  constexpr int kPlanes = sizeof(V) == 4 ? 3 : 1;
+  __shared__ int32_t numbers[Stream<T, S, LA, Lies::Cols, kPlanes, kGather>::number_words];
   if (kb1 > kb0) {
-    Stream<T, S, LA, Lies::Cols, kGather> st;
+    Stream<T, S, LA, Lies::Cols, kPlanes, kGather> st;
     st.a = a.p.a;
     st.b = a.p.b;
     st.rows_b = (int)(a.points == 2 ? nc : a.rows_b);
     st.la.tile(st.a, m0, a.points == 1 ? nc : a.limit_a);
     st.lb.tile(st.b, n0, a.limit_b);
     auto more = [] { return false; };
-    st.begin(lds, (int)kb0, (int)kb1, a.p.planes, more, numbers);
+    st.begin(lds, (int)kb0, (int)kb1, more, numbers);
     st.run(lds, acc, more, m - m0);
     st.end();
   }
@@ -1035,7 +1035,7 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   p.state_bytes = k.off;
   Carver c(workspace);
   if (!backward) {
-    p.lse_big = large_tiles(d.v, d.n, up(d.v, Big::BM) / Big::BM);
+    p.lse_big = p.planes == 1 && large_tiles(d.v, d.n, up(d.v, Big::BM) / Big::BM);
     const int64_t bm = p.lse_big ? Big::BM : Small::BM, bn = p.lse_big ? Big::BN : Small::BN;
     const int64_t of_points = p.narrow ? narrow_rows(Narrow::Lse, p.planes, (int)p.dp) : 0;
     p.lse_splits = p.head ? 1 : p.narrow ? narrow_splits(d.n, of_points, slots, d.v, 8) : cut(up(d.n, bn) / bn, kCus * (p.lse_big ? Big::per_cu : Small::per_cu), up(d.v, bm) / bm);
@@ -1068,10 +1068,10 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     p.piece = piece < v64 ? piece : v64;
     if (d.piece == 0) p.piece = up((v64 + (v64 + p.piece - 1) / p.piece - 1) / ((v64 + p.piece - 1) / p.piece), Big::BM);      // pieces of one size
     if (p.piece > v64 || p.head) p.piece = v64;
-    p.dl_big = large_tiles(p.piece, d.n, 1);
+    p.dl_big = p.planes == 1 && large_tiles(p.piece, d.n, 1);
     const int64_t kx = p.piece / 256, kw = p.n_pad / 256;
-    p.dx_big = large_tiles(d.n, p.dp, kx);
-    p.dw_big = large_tiles(p.piece, p.dp, kw);
+    p.dx_big = p.planes == 1 && large_tiles(d.n, p.dp, kx);
+    p.dw_big = p.planes == 1 && large_tiles(p.piece, p.dp, kw);
     auto tiles = [&](int64_t m, int64_t n, bool big) { return big ? tiles_of(m, n, Big::BM, Big::BN) : tiles_of(m, n, Small::BM, Small::BN); };
     p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus * (p.dx_big ? Big::per_cu : Small::per_cu), kx);
     p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus * (p.dw_big ? Big::per_cu : Small::per_cu), kw);
@@ -1110,11 +1110,22 @@ PackArgs pack_args(const Plan &p, const void *src, void *dst, int64_t ld, int64_
   return PackArgs{src, dst, ld, rows, width, p.dp, rows * p.dp, vector, blocks_for(rows * p.dp / 8, kStartThreads * 2, 1024)};
 }
 
-template <class T, class S>
+// Three planes take the small tiles alone: plane 0 beside the others' fragments and the sums of a large one are more than 256
+// registers, and six products for three planes' loads are enough for the matrix cores (6 x 512 cycles of them a k-block and CU,
+// 2300 of LDS).
+template <int kPlanes, class F>
+void with_shape(bool big, F &&f) {
+  if constexpr (kPlanes == 1) {
+    if (big) return f(Big{});
+  }
+  f(Small{});
+}
+
+template <class T, class S, int kPlanes>
 void lse(LseArgs a, const Plan &p, int64_t n, int64_t v, hipStream_t st) {
   a.ntiles = up(n, S::BN) / S::BN;
   a.vtiles = (int)(up(v, S::BM) / S::BM);
-  hipLaunchKernelGGL((k_ce_lse<T, S>), dim3((unsigned)(a.ntiles * p.lse_splits)), dim3(S::threads), 0, st, a);
+  hipLaunchKernelGGL((k_ce_lse<T, S, kPlanes>), dim3((unsigned)(a.ntiles * p.lse_splits)), dim3(S::threads), 0, st, a);
 }
 
 void join(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
@@ -1221,7 +1232,6 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   }
   LseArgs la{};
   operands(d, p, la.p.b, la.p.a);
-  la.p.planes = kPlanes;
   la.v = d.v;
   la.kb = p.dp / kTileK;
   la.splits = p.lse_splits;
@@ -1232,8 +1242,7 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   la.part_l = p.part_l;
   la.hit = p.hit;
   la.n_pad = p.n_pad;
-  if (p.lse_big) lse<T, Big>(la, p, d.n, d.v, st);
-  else lse<T, Small>(la, p, d.n, d.v, st);
+  with_shape<kPlanes>(p.lse_big, [&](auto shape) { lse<T, decltype(shape), kPlanes>(la, p, d.n, d.v, st); });
   join(d, p, st);
 }
 
@@ -1333,7 +1342,7 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     Finish of[3];
     int n_of = 0;
     DlArgs da{};
-    da.p = Product{w, x, kPlanes};
+    da.p = Product{w, x};
     da.v = d.v;
     da.kb = p.dp / kTileK;
     da.piece0 = v0;
@@ -1358,17 +1367,15 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
         ha.sums = d.db ? p.accb : nullptr;
         head<T, true>(ha, p, d.n, st);
       }
-    } else if (p.dl_big) {
-      dl_piece<T, Big, kPlanes>(da, d.n, st);
     } else {
-      dl_piece<T, Small, kPlanes>(da, d.n, st);
+      with_shape<kPlanes>(p.dl_big, [&](auto shape) { dl_piece<T, decltype(shape), kPlanes>(da, d.n, st); });
     }
     const Operand dl{p.dl, p.n_pad, p.n_pad * p.piece, nullptr};
     if (d.dx && !p.head) {
       Operand wv = w;      // the rows of this piece
       wv.p = static_cast<const char *>(w.p) + v0 * w.ld * 2;
       OutArgs oa{};
-      oa.p = Product{dl, wv, kPlanes};
+      oa.p = Product{dl, wv};
       oa.n = p.dx_final ? d.d : p.dp;
       oa.kb = width / kTileK;
       oa.limit_b = p.dp;
@@ -1384,14 +1391,13 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       oa.idx = p.idx;
       oa.scale = p.scale;
       oa.unheld = unheld;
-      if (p.dx_big) out_product<S, T, Big, Lies::PiecesRows>(oa, d.n, p.dp, st);
-      else out_product<S, T, Small, Lies::PiecesRows>(oa, d.n, p.dp, st);
+      with_shape<kPlanes>(p.dx_big, [&](auto shape) { out_product<S, T, decltype(shape), Lies::PiecesRows>(oa, d.n, p.dp, st); });
       if (!p.dx_final && v0 + p.piece >= d.v) of[n_of++] = finish_of<S>(p.accx, p.dp, p.n_pad * p.dp, d.n, d.d, p.dx_splits, p.place, d.dx);
     }
     if (d.dw) {
       const bool straight = p.dw_final;
       OutArgs oa{};
-      oa.p = Product{dl, x, kPlanes};
+      oa.p = Product{dl, x};
       oa.m = straight ? real_v : width;
       oa.n = straight ? d.d : p.dp;
       oa.limit_a = width;
@@ -1405,8 +1411,7 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       oa.final_out = straight ? static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes : nullptr;
       oa.scale = p.scale;
       oa.unheld = unheld;
-      if (p.dw_big) out_product<S, T, Big, Lies::PiecesCols>(oa, width, p.dp, st);
-      else out_product<S, T, Small, Lies::PiecesCols>(oa, width, p.dp, st);
+      with_shape<kPlanes>(p.dw_big, [&](auto shape) { out_product<S, T, decltype(shape), Lies::PiecesCols>(oa, width, p.dp, st); });
       if (!straight)
         of[n_of++] = finish_of<S>(p.accw, p.dp, p.piece * p.dp, real_v, d.d, p.dw_splits, nullptr, static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes);
     }

@@ -178,7 +178,8 @@ __device__ __forceinline__ void wait_loads() {
 // kGather: the rows of a Cols operand B are taken by their numbers, b.idx.  Those of a block come to LDS S::ahead blocks before its
 // own loads, with the loads of that earlier block (every wave for itself): looked up when they are wanted, by vector or by
 // scalar loads, they hold up every step (dW of 119999 x 260 x 256: 73 us by scalar loads a step, 139 a step ahead).
-template <class T, class S, Lies LA, Lies LB, bool kGather = false>
+// kPlanes = 3: operands of three planes; a block comes plane by plane, plane 0 stays in registers for the products of the other two.
+template <class T, class S, Lies LA, Lies LB, int kPlanes, bool kGather = false>
 struct Stream {
   Operand a, b;
   Loader<T, LA, S::BM, S::threads> la;
@@ -186,34 +187,37 @@ struct Stream {
   static constexpr int loads = Loader<T, LA, S::BM, S::threads>::per + Loader<T, LB, S::BN, S::threads>::per + (kGather ? 1 : 0);
   static constexpr int number_words = kGather ? 64 * S::buffers * (S::threads / 64) : 1;      // LDS that `numbers` has
   int rows_b;                  // rows of a Cols operand
-  int kb, kb0, kb1;
-  int pair, pairs, get, put;   // buffers: the next to multiply, the next to fill
+  int kb, kb0, kb1, plane;     // the next to load
+  int get, put;                // buffers: the next to multiply, the next to fill
+  int number_kb, number_plane; // the next whose numbers are fetched
   bool dry;                    // nothing left to load
   unsigned base;               // LDS address of the wave's part of buffer 0
   int32_t *numbers;            // [S::buffers][64] of this wave: slot put holds those of the next block to load
 
-  // The numbers of block n (of this tile; clamped behind the last row) to slot `slot`.
-  __device__ __forceinline__ void fetch_numbers(int n, int slot) {
-    const int row = n * kTileK + (threadIdx.x & 31);
+  // The numbers of the block after those that have them (they go round within a tile; clamped behind the last row) to slot `slot`.
+  __device__ __forceinline__ void fetch_numbers(int slot) {
+    const int row = number_kb * kTileK + (threadIdx.x & 31);
     const int32_t *from = b.idx + (row < rows_b ? row : rows_b - 1);
     const unsigned to = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_void *)(numbers + slot * 64));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(from) : "m0", "memory");
+    if (++number_plane < kPlanes) return;
+    number_plane = 0;
+    if (++number_kb == kb1) number_kb = kb0;
   }
 
   // k-blocks [first, end) of every tile (at least one); the loaders hold the first tile.
   template <class More>
-  __device__ __forceinline__ void begin(T *lds, int first, int end, int planes, More &&more, int32_t *number_lds = nullptr) {
-    kb = kb0 = first;
+  __device__ __forceinline__ void begin(T *lds, int first, int end, More &&more, int32_t *number_lds = nullptr) {
+    kb = kb0 = number_kb = first;
     kb1 = end;
-    pairs = planes == 3 ? kPairs : 1;
-    get = put = pair = 0;
+    get = put = plane = number_plane = 0;
     dry = false;
     base = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_void *)lds + (threadIdx.x >> 6) * 1024);
     la.move(first * la.step(a));
     if constexpr (kGather) {
       numbers = number_lds + (threadIdx.x >> 6) * 64 * S::buffers;
 #pragma unroll
-      for (int i = 0; i < S::ahead; ++i) fetch_numbers(first + i % (end - first), i);
+      for (int i = 0; i < S::ahead; ++i) fetch_numbers(i);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     } else if constexpr (LB == Lies::Cols) {
       lb.to_block(b, kb, rows_b, 0, nullptr);
@@ -228,40 +232,40 @@ struct Stream {
   template <class More>
   __device__ __forceinline__ void issue(More &&more) {
     if constexpr (kGather) {
-      lb.to_block(b, kb, rows_b, kPlaneB[pair] * b.plane, numbers + put * 64);
-      // (the slot that was read S::buffers - S::ahead blocks ago; blocks go round within a tile)
-      fetch_numbers(kb0 + (kb - kb0 + S::ahead) % (kb1 - kb0), (put + S::ahead) % S::buffers);
+      lb.to_block(b, kb, rows_b, plane * b.plane, numbers + put * 64);
+      fetch_numbers((put + S::ahead) % S::buffers);      // (the slot that was read S::buffers - S::ahead blocks ago)
     }
     const unsigned to = base + put * (S::buffer * (unsigned)sizeof(T));
     la.issue(to);
     lb.issue(to + S::a_elems * (unsigned)sizeof(T));
     put = (put + 1) % S::buffers;
     if (dry) return;
+    if (kPlanes > 1 && ++plane < kPlanes) {
+      la.move(a.plane);
+      if constexpr (!kGather) lb.move(b.plane);
+      return;
+    }
+    plane = 0;
+    const int64_t back_a = (kPlanes - 1) * a.plane, back_b = (kPlanes - 1) * b.plane;
     if (++kb < kb1) {
-      la.move(la.step(a));
+      la.move(la.step(a) - back_a);
       if constexpr (!kGather) {
-        if (LB == Lies::Cols && (kb + 1) * kTileK > rows_b) lb.to_block(b, kb, rows_b, kPlaneB[pair] * b.plane, nullptr);
-        else lb.move(lb.step(b));
+        if (LB == Lies::Cols && (kb + 1) * kTileK > rows_b) lb.to_block(b, kb, rows_b, 0, nullptr);
+        else lb.move(lb.step(b) - back_b);
       }
       return;
     }
-    const int was = pair;
-    if (++pair == pairs) {
-      pair = 0;
-      if (!more()) {
-        dry = true;
-        pair = was;
-        kb = kb1 - 1;
-        return;
-      }
-      la.move(kb0 * la.step(a));
-    } else {
-      la.move((kb0 + 1 - kb1) * la.step(a) + (kPlaneA[pair] - kPlaneA[was]) * a.plane);
+    if (!more()) {
+      dry = true;
+      kb = kb1 - 1;
+      plane = kPlanes - 1;
+      return;
     }
     kb = kb0;
+    la.move(kb0 * la.step(a));
     if constexpr (!kGather) {
-      if constexpr (LB == Lies::Cols) lb.to_block(b, kb, rows_b, kPlaneB[pair] * b.plane, nullptr);
-      else lb.move((kb0 + 1 - kb1) * lb.step(b) + (kPlaneB[pair] - kPlaneB[was]) * b.plane);
+      if constexpr (LB == Lies::Cols) lb.to_block(b, kb, rows_b, 0, nullptr);
+      else lb.move((kb0 + 1 - kb1) * lb.step(b) - back_b);
     }
   }
   // acc += all k-blocks of a tile whose rows from `rows` on are not there: a wave leaves out its blocks of 32 behind them.
@@ -273,44 +277,96 @@ struct Stream {
     if (blocks == S::FM) run_blocks<true>(lds, acc, more, S::FM);
     else run_blocks<false>(lds, acc, more, blocks);
   }
+  typedef typename Mma<T>::v8 v8;
+  template <bool kAll>
+  __device__ __forceinline__ void read(const T *lds, int kk, v8 (&fa)[S::FM], v8 (&fb)[S::FN], int blocks) const {
+    const int wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
+    const T *pa = lds + get * S::buffer, *pb = pa + S::a_elems;
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+      if (kAll || i < blocks) fa[i] = fragment<T, LA, S::BM>(pa, (wm * S::FM + i) * 32, kk);
+#pragma unroll
+    for (int j = 0; j < S::FN; ++j) fb[j] = fragment<T, LB, S::BN>(pb, (wn * S::FN + j) * 32, kk);
+  }
+  template <bool kAll>
+  static __device__ __forceinline__ void multiply(const v8 (&fa)[S::FM], const v8 (&fb)[S::FN], f32x16 (&acc)[S::FM][S::FN], int blocks) {
+#pragma unroll
+    for (int i = 0; i < S::FM; ++i)
+      if (kAll || i < blocks)
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) acc[i][j] = Mma<T>::mma(fa[i], fb[j], acc[i][j]);
+  }
   // A fragment is read one k-step before it is multiplied, over the blocks' borders too: the reads after a barrier would else hold
   // up the matrix cores of all waves at once.
   template <bool kAll, class More>
   __device__ __forceinline__ void run_blocks(T *lds, f32x16 (&acc)[S::FM][S::FN], More &&more, int blocks) {
-    const int wave = threadIdx.x >> 6, wm = wave / S::WN, wn = wave % S::WN;
-    const int steps = (kb1 - kb0) * pairs;
-    typename Mma<T>::v8 fa[2][S::FM], fb[2][S::FN];
-    auto read = [&](int kk, int into) {
-      const T *pa = lds + get * S::buffer, *pb = pa + S::a_elems;
-#pragma unroll
-      for (int i = 0; i < S::FM; ++i)
-        if (kAll || i < blocks) fa[into][i] = fragment<T, LA, S::BM>(pa, (wm * S::FM + i) * 32, kk);
-#pragma unroll
-      for (int j = 0; j < S::FN; ++j) fb[into][j] = fragment<T, LB, S::BN>(pb, (wn * S::FN + j) * 32, kk);
-    };
-    auto multiply = [&](int from) {
-#pragma unroll
-      for (int i = 0; i < S::FM; ++i)
-        if (kAll || i < blocks)
-#pragma unroll
-          for (int j = 0; j < S::FN; ++j) acc[i][j] = Mma<T>::mma(fa[from][i], fb[from][j], acc[i][j]);
-    };
     static_assert(kTileK == 32, "two k-steps a block");
-    wait_loads<(S::ahead - 1) * loads>();
-    read(0, 0);
-    for (int s = 0; s < steps; ++s) {
-      read(1, 1);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(0);
-      __builtin_amdgcn_sched_barrier(0);
-      // the next block is there, and all waves are done with the one before this one: its buffer is filled
-      wait_loads<(S::ahead - 2) * loads>();
-      issue(more);
-      get = (get + 1) % S::buffers;
-      if (s + 1 < steps) read(0, 0);
-      __builtin_amdgcn_sched_barrier(0);
-      multiply(1);
-      __builtin_amdgcn_sched_barrier(0);
+    const int steps = kb1 - kb0;
+    v8 fa[2][S::FM], fb[2][S::FN];
+    auto next = [&] { get = (get + 1) % S::buffers; };
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+    if constexpr (kPlanes == 1) {
+      wait_loads<(S::ahead - 1) * loads>();
+      read<kAll>(lds, 0, fa[0], fb[0], blocks);
+      for (int s = 0; s < steps; ++s) {
+        read<kAll>(lds, 1, fa[1], fb[1], blocks);
+        fence();
+        multiply<kAll>(fa[0], fb[0], acc, blocks);
+        fence();
+        // the next block is there, and all waves are done with the one before this one: its buffer is filled
+        wait_loads<(S::ahead - 2) * loads>();
+        issue(more);
+        next();
+        if (s + 1 < steps) read<kAll>(lds, 0, fa[0], fb[0], blocks);
+        fence();
+        multiply<kAll>(fa[1], fb[1], acc, blocks);
+        fence();
+      }
+    } else {
+      // the products of planes 00, 01 10 11, 02 20; behind a barrier the buffer of the plane before is filled, so its reads are
+      // waited for (their first product stands between)
+      auto turn = [&] {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wait_loads<(S::ahead - 1) * loads>();
+      };
+      v8 fa0[2][S::FM], fb0[2][S::FN];
+      for (int s = 0; s < steps; ++s) {
+        turn();
+        read<kAll>(lds, 0, fa0[0], fb0[0], blocks);
+        if (s) multiply<kAll>(fa[1], fb0[1], acc, blocks);      // (20 of the block before)
+        read<kAll>(lds, 1, fa0[1], fb0[1], blocks);
+        issue(more);
+        next();
+        fence();
+        multiply<kAll>(fa0[0], fb0[0], acc, blocks);
+        turn();
+        read<kAll>(lds, 0, fa[0], fb[0], blocks);
+        issue(more);
+        fence();
+        multiply<kAll>(fa0[1], fb0[1], acc, blocks);
+        fence();
+        read<kAll>(lds, 1, fa[1], fb[1], blocks);
+        next();
+        fence();
+        multiply<kAll>(fa0[0], fb[0], acc, blocks);
+        multiply<kAll>(fa[0], fb0[0], acc, blocks);
+        multiply<kAll>(fa[0], fb[0], acc, blocks);
+        multiply<kAll>(fa0[1], fb[1], acc, blocks);
+        multiply<kAll>(fa[1], fb0[1], acc, blocks);
+        turn();
+        read<kAll>(lds, 0, fa[0], fb[0], blocks);
+        issue(more);
+        fence();
+        multiply<kAll>(fa[1], fb[1], acc, blocks);
+        fence();
+        read<kAll>(lds, 1, fa[1], fb[1], blocks);
+        next();
+        fence();
+        multiply<kAll>(fa0[0], fb[0], acc, blocks);
+        multiply<kAll>(fa[0], fb0[0], acc, blocks);
+        multiply<kAll>(fa0[1], fb[1], acc, blocks);
+      }
+      multiply<kAll>(fa[1], fb0[1], acc, blocks);
     }
   }
   // Before LDS is used for anything else, and before the workgroup ends: nothing on its way to it.
