@@ -160,7 +160,8 @@ __device__ __forceinline__ typename Mma<T>::v8 fragment(const T *lds, int r0, in
   }
 }
 
-// (plane of A, plane of B) of the products of two operands in three planes of 8 bits each: what is left out is below 2^-24.
+// (plane of A, plane of B) of the products of two operands in three planes of 8 bits each: what is left out is below 2^-24.  (Heads
+// that stand in LDS; a stream takes them plane by plane.)
 constexpr int kPairs = 6;
 __device__ constexpr int kPlaneA[kPairs] = {0, 0, 1, 1, 0, 2}, kPlaneB[kPairs] = {0, 1, 0, 1, 2, 0};
 
@@ -178,7 +179,8 @@ __device__ __forceinline__ void wait_loads() {
 // kGather: the rows of a Cols operand B are taken by their numbers, b.idx.  Those of a block come to LDS S::ahead blocks before its
 // own loads, with the loads of that earlier block (every wave for itself): looked up when they are wanted, by vector or by
 // scalar loads, they hold up every step (dW of 119999 x 260 x 256: 73 us by scalar loads a step, 139 a step ahead).
-// kPlanes = 3: operands of three planes; a block comes plane by plane, plane 0 stays in registers for the products of the other two.
+// kPlanes = 3: operands of three planes; a block comes plane by plane, plane 0 stays in registers for the products of the other two
+// (13 777 points x 20 244 classes x 512, all products: 6.5 ms, with two planes loaded for each product 7.5).
 template <class T, class S, Lies LA, Lies LB, int kPlanes, bool kGather = false>
 struct Stream {
   Operand a, b;
