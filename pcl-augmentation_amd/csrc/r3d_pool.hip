@@ -106,27 +106,41 @@ __device__ __forceinline__ int64_t clamp_free(const TablesArgs &a) {
 // the launch: workgroup g copies its part of the stack, and pushes what the rows of group g give back.
 __global__ __launch_bounds__(kGroup) void k_tables_release(TablesArgs a) {
   __shared__ int64_t s[4];
-  __shared__ int64_t s_at[kGroup];
-  __shared__ int32_t s_from[kGroup], s_to[kGroup];
   const int group = blockIdx.x;
+  const int64_t row = (int64_t)group * kGroup + threadIdx.x;
+  const RowWant w = group < a.groups ? row_want(a, row) : RowWant{0, 0, true};
   const Sums sum = sums_before(a, group, s);
   const int64_t n_free = clamp_free(a), n_all = n_free + sum.back_all;
   for (int64_t i = (int64_t)blockIdx.x * kGroup + threadIdx.x; i < a.n_blocks; i += (int64_t)gridDim.x * kGroup)
     if (i < n_free || i >= n_all) a.free_out[i] = i < n_free ? a.free_blocks[i] : -1;
   if (group >= a.groups) return;
-  const int64_t row = (int64_t)group * kGroup + threadIdx.x;
-  const RowWant w = row_want(a, row);
   const int32_t back = w.have > w.want ? w.have - w.want : 0;
-  s_at[threadIdx.x] = n_free + sum.back_before + group_scan(back, s) - back;
-  s_from[threadIdx.x] = w.want;
-  s_to[threadIdx.x] = back ? w.have : w.want;
-  __syncthreads();
+  const int64_t mine = n_free + sum.back_before + group_scan(back, s) - back;
+  // a wave's rows that give something back, four at a time, 64 of their blocks each time
   const int lane = threadIdx.x & 63;
-  for (int r = threadIdx.x >> 6; r < kGroup; r += kGroup / 64)      // a wave per row
-    for (int c = s_from[r] + lane; c < s_to[r]; c += 64) {
-      const int64_t at = s_at[r] + (c - s_from[r]);
-      if (at < a.n_blocks) a.free_out[at] = a.tables[((int64_t)group * kGroup + r) * a.most + c];
+  uint64_t rows = __ballot(back > 0);
+  while (rows) {
+    int64_t at[4];
+    const int32_t *from[4];
+    int n[4], most = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = rows ? __builtin_ctzll(rows) : 0;
+      n[k] = rows ? __shfl(back, r) : 0;
+      at[k] = __shfl(mine, r);
+      from[k] = a.tables + (row - lane + r) * a.most + __shfl(w.want, r);
+      most = n[k] > most ? n[k] : most;
+      rows &= rows - 1;
     }
+    for (int c = lane; c < most; c += 64) {
+      int32_t v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = c < n[k] ? from[k][c] : 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c < n[k] && at[k] + c < a.n_blocks) a.free_out[at[k] + c] = v[k];
+    }
+  }
 }
 
 // The new tables.  A growing row pops its blocks from the end of the stack; the cell that takes an entry is the only one
@@ -162,8 +176,9 @@ __global__ __launch_bounds__(kGroup) void k_tables_write(TablesArgs a) {
   __syncthreads();
   const int64_t rows = min((int64_t)kGroup, a.n_rows - (int64_t)group * kGroup);
   const int64_t cells = rows * a.most, first = (int64_t)group * kGroup * a.most;
+  const bool few = cells <= UINT32_MAX;
   for (int64_t i = (int64_t)blockIdx.y * kGroup + threadIdx.x; i < cells; i += (int64_t)gridDim.y * kGroup) {
-    const int r = (int)(i / a.most), c = (int)(i - (int64_t)r * a.most);
+    const int r = few ? (int)((unsigned)i / (unsigned)a.most) : (int)(i / a.most), c = (int)(i - (int64_t)r * a.most);
     int32_t v = -1;
     if (c < s_want[r]) {
       if (c < s_have[r]) {
@@ -372,10 +387,11 @@ extern "C" int r3d_block_tables(const int32_t *lengths, int64_t n_rows, int32_t 
   hipLaunchKernelGGL(k_tables_count, dim3(a.groups), dim3(kGroup), 0, st, a);
   const int copies = blocks_for(n_blocks, kGroup * 8, 1024);
   hipLaunchKernelGGL(k_tables_release, dim3(a.groups > copies ? a.groups : copies), dim3(kGroup), 0, st, a);
-  // slices: about eight cells a thread, no more than fill the chip
+  // slices: two cells a thread (256 x 74: 7.8 us with eight, 6.0 with two), four workgroups a CU at most (23 201 x 74: 11 us, with
+  // 3400 workgroups, each of which sums the groups before it, 20)
   const int64_t cells = (n_rows < kGroup ? n_rows : kGroup) * max_blocks;
-  int slices = blocks_for(cells, kGroup * 8, 1024);
-  while (slices > 1 && (int64_t)slices * a.groups > 4096) slices /= 2;
+  int slices = blocks_for(cells, kGroup * 2, 1024);
+  while (slices > 1 && (int64_t)slices * a.groups > 1024) slices /= 2;
   hipLaunchKernelGGL(k_tables_write, dim3(a.groups, slices), dim3(kGroup), 0, st, a);
   R3D_LAUNCHED("block_tables kernels");
   return R3D_OK;

@@ -27,7 +27,7 @@ class SlotMap(NamedTuple):
 
 
 def _whole(what, name, t, dtype, dims):
-    if t.dtype != dtype or t.dim() != dims or not t.is_contiguous():
+    if t.dtype is not dtype or t.dim() != dims or not t.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous {dtype} tensor of {dims} axes, got {t.dtype} {tuple(t.shape)}")
 
 
@@ -44,23 +44,22 @@ def block_tables(lengths, block_size, tables, held, free_blocks, n_free):
     what = "block_tables"
     for name, t, dims in (("lengths", lengths, 1), ("tables", tables, 2), ("held", held, 1), ("free_blocks", free_blocks, 1), ("n_free", n_free, 1)):
         _whole(what, name, t, torch.int32, dims)
-    rows, most = tables.shape
+    (rows, most), blocks = tables.shape, free_blocks.shape[0]
     if lengths.shape[0] != rows or held.shape[0] != rows or n_free.shape[0] != 1:
         raise ValueError(f"{what}: lengths and held must be [{rows}], n_free [1]")
-    if not 1 <= rows <= _lib.MAX_SCENES or most < 1 or free_blocks.shape[0] < 1:
+    if not 1 <= rows <= _lib.MAX_SCENES or most < 1 or blocks < 1:
         raise ValueError(f"{what}: no rows or no blocks (or more than 2^24 rows)")
     block_size = int(block_size)
     if block_size < 1 or block_size * most >= 2 ** 31:
         raise ValueError(f"{what}: block_size must be positive and block_size * max_blocks below 2^31")
     with on_device_of(what, lengths, tables, held, free_blocks, n_free):
         lib = _lib.load()
-        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=lengths.device)  # noqa: E731
-        out = BlockTables(new(rows, most), new(rows), new(free_blocks.shape[0]), new(1), new(1))
+        new = torch.empty_like      # (all dense)
+        out = BlockTables(new(tables), new(held), new(free_blocks), new(n_free), new(n_free))
         ws = torch.empty(lib.r3d_block_tables_workspace_bytes(rows), dtype=torch.uint8, device=lengths.device)
         _lib.check(lib.r3d_block_tables(lengths.data_ptr(), rows, block_size, most, tables.data_ptr(), held.data_ptr(), free_blocks.data_ptr(),
-                                        free_blocks.shape[0], n_free.data_ptr(), out.tables.data_ptr(), out.held.data_ptr(),
-                                        out.free_blocks.data_ptr(), out.n_free.data_ptr(), out.status.data_ptr(), ws.data_ptr(), ws.numel(),
-                                        _lib.raw_stream(lengths.get_device())), "r3d_block_tables")
+                                        blocks, n_free.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), out[3].data_ptr(),
+                                        out[4].data_ptr(), ws.data_ptr(), ws.numel(), _lib.raw_stream(lengths.get_device())), "r3d_block_tables")
     return out
 
 
