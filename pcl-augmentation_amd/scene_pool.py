@@ -109,13 +109,13 @@ def _slots(what, name, slots):
 
 
 def _move(what, sources, dests, src_slots, dst_slots, n):
-    arrays = (_lib.Rows * len(sources))()
-    for a, s, t in zip(arrays, sources, dests):
+    rows = []
+    for s, t in zip(sources, dests):
         size = s.element_size()
-        width = size * math.prod(s.shape[1:])
-        a.src, a.dst, a.row_bytes = s.data_ptr(), t.data_ptr(), width
-        a.src_stride, a.dst_stride = (s.stride(0) * size if s.shape[0] > 1 else width), (t.stride(0) * size if t.shape[0] > 1 else width)
-    _lib.check(_lib.load().r3d_move_rows(arrays, len(sources), 0 if src_slots is None else src_slots.data_ptr(),
+        shape = s.shape
+        width = size * (shape[1] if len(shape) == 2 else math.prod(shape[1:]))
+        rows.append((s.data_ptr(), t.data_ptr(), s.stride(0) * size if shape[0] > 1 else width, t.stride(0) * size if t.shape[0] > 1 else width, width))
+    _lib.check(_lib.load().r3d_move_rows((_lib.Rows * len(rows))(*rows), len(rows), 0 if src_slots is None else src_slots.data_ptr(),
                                          0 if dst_slots is None else dst_slots.data_ptr(), n, sources[0].shape[0], dests[0].shape[0],
                                          _lib.raw_stream(sources[0].get_device())), "r3d_move_rows")
 
@@ -152,7 +152,7 @@ def take_rows(slots, sources):
     sources = _rows_of(what, "sources", sources)
     n = slots.shape[0]
     with on_device_of(what, slots, *sources):
-        outs = tuple(torch.empty((n,) + t.shape[1:], dtype=t.dtype, device=t.device) for t in sources)
+        outs = tuple([t.new_empty((n, *t.shape[1:])) for t in sources])
         if n:
             if sources[0].shape[0] == 0:
                 return tuple(o.zero_() for o in outs)
