@@ -2,6 +2,9 @@
 //
 //   l = x W^T + b,  loss_n = log sum_v exp l_nv - l_n,target;   dl = g_n (softmax(l) - onehot),  dx = dl W,  dW = dl^T x,  db = sum_n dl.
 //
+// This file: any sizes, and heads of up to 288 classes that stand in LDS; r3d_loss_few.hip: few classes and not many features;
+// r3d_loss_narrow.hip: at most 128 features.  few_plan() and plan() choose.
+//
 // Forward: one product x W^T whose tiles end in a running maximum and sum per point (base 2), joined over the waves and over
 // the splits of the classes.  Backward: for one piece of the classes at a time the logits once more, their gradient rounded to
 // 16 bits into the workspace, and the two products with it.  Points whose target is ignored are left out at the start: the
@@ -917,7 +920,7 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
-// What a piece's dl may take.  8192 points x 161280 classes x 512: 8.8 ms with 64 MB, 7.1 with 256, 6.7 with 512, 6.4 with all 2.6 GB.
+// What a piece's dl may take.  8192 points x 161280 classes x 512: 8.4 ms with 64 MB, 6.6 with 256, 6.3 with 512 and with all 2.6 GB.
 constexpr int64_t kPieceBytes = 512ll << 20;
 constexpr int kCus = 256, kHeadLds = 160 * 1024;
 constexpr int kPadK = 64;      // a head in LDS and few features: padded to whole cache lines; pieces of the classes

@@ -462,9 +462,9 @@ bool few_plan(const r3d_linear_ce_t &d, FewPlan &p) {
   p.dp = (int)((d.d + 31) / 32 * 32);
   p.vt = d.v <= 32 ? 1 : d.v <= 64 ? 2 : 4;
   p.nb = p.dp <= 128 ? 1 : 2;
-  // Beyond that, and for many points near it, the other kernels are faster.  200 000 points, us here / there: bf16 20 x 256 116 / 175,
-  // 50 x 96 72 / 128, 100 x 96 128 / 140, but 50 x 200 211 / 185, 100 x 128 146 / 131, 100 x 256 284 / 193, 20 x 512 372 / 282; fp32 20 x 64
-  // 94 / 172, 50 x 96 294 / 318, but 50 x 64 243 / 174.  4000 points: 50 x 200 42 / 49, 100 x 128 41 / 49, fp32 50 x 64 37 / 47.
+  // Beyond that, and for many points near it, the other kernels are faster.  200 000 points, us here / there: bf16 20 x 256 119 / 148,
+  // 50 x 96 73 / 130, 100 x 96 128 / 138, but 50 x 200 211 / 186, 100 x 128 146 / 130, 100 x 256 284 / 170, 20 x 512 372 / 242; fp32 20 x 64
+  // 94 / 175, 50 x 96 291 / 321, but 50 x 64 243 / 173.  4000 points: 50 x 200 42 / 49, 100 x 128 41 / 49, fp32 50 x 64 37 / 47.
   if (p.vt * p.nb > 4 || p.nb > 2 || (planes == 3 && p.vt == 4)) return false;
   if (planes == 1 ? p.vt * p.nb == 4 && p.dp > 96 && d.n > 65536 : p.vt == 2 && p.dp <= 64 && d.n > 32768) return false;
   p.tp = p.nb >= 2 || planes == 3 ? 64 : 128;      // (two workgroups a CU beat one with the longer tile: 200 000 x 20 x 256 forward 58 -> 38 us)
