@@ -43,6 +43,33 @@ def _value_type(what, t):
     return kind
 
 
+@functools.lru_cache(maxsize=None)
+def _once():
+    """Decorator of a backward pass that has none of its own: under ``create_graph`` its results raise where they are differentiated
+    (torch's own lets them pass as constants where the incoming gradient needs none)."""
+    import torch
+
+    class Once(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, gradient, _):
+            return gradient.view_as(gradient)
+
+        @staticmethod
+        def backward(ctx, *_):
+            raise RuntimeError("rotary_positions and linear_cross_entropy are differentiable once")
+
+    def decorate(backward):
+        def run(ctx, *gradients):
+            if not torch.is_grad_enabled():
+                return backward(ctx, *gradients)
+            with torch.no_grad():
+                got = backward(ctx, *gradients)
+            return tuple(None if g is None else Once.apply(g, torch.empty(0, requires_grad=True)) for g in got)
+        return run
+
+    return decorate
+
+
 # ---- rotary positions -------------------------------------------------------------------------------------------------
 def _turn(tensors, positions, sections, base, interleaved, backward):
     """One launch over up to two [tokens, heads, dim] tensors (None: none), on the current device; returns dense ones."""
@@ -78,7 +105,6 @@ def _turn(tensors, positions, sections, base, interleaved, backward):
 @functools.lru_cache(maxsize=None)
 def _rotary_function():
     import torch
-    from torch.autograd.function import once_differentiable
 
     class RotaryPositions(torch.autograd.Function):
         @staticmethod
@@ -88,7 +114,7 @@ def _rotary_function():
             return tuple(_turn((query, key), positions, sections, base, interleaved, False))
 
         @staticmethod
-        @once_differentiable
+        @_once()
         def backward(ctx, grad_query, grad_key):
             # a rotation: the gradient is turned back
             positions, = ctx.saved_tensors
@@ -146,7 +172,6 @@ def rotary_positions(query, positions, sections, key=None, base=10000.0, style="
 @functools.lru_cache(maxsize=None)
 def _loss_function():
     import torch
-    from torch.autograd.function import once_differentiable
 
     # Every line here is on the way of each step, forward on the caller's thread and backward on the engine's: what a small call
     # costs beyond its kernels is these lines (and the engine itself, 70 us).
@@ -184,7 +209,7 @@ def _loss_function():
             return loss
 
         @staticmethod
-        @once_differentiable
+        @_once()
         def backward(ctx, grad):
             x, weight, bias, target, state = ctx.saved_tensors
             with on_device_of("linear_cross_entropy", x):

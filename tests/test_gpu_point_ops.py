@@ -407,6 +407,20 @@ def test_loss_parts_of_the_gradient(pkg):
         assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(loss, ins, retain_graph=True), want))
 
 
+def test_second_derivatives_are_refused(pkg):
+    x, w = torch.randn((40, 64), generator=gen(1)).cuda().requires_grad_(), torch.randn((30, 64), generator=gen(2)).cuda().requires_grad_()
+    t = torch.randint(0, 30, (40,), generator=gen(3)).cuda()
+    plain, = torch.autograd.grad(pkg.linear_cross_entropy(x, w, t), x)
+    dx, = torch.autograd.grad(pkg.linear_cross_entropy(x, w, t), x, create_graph=True)      # (harmless as long as nobody follows it)
+    assert torch.equal(dx, plain)
+    with pytest.raises(RuntimeError, match="once"):
+        (dx ** 2).sum().backward()
+    q, pos = torch.randn((40, 2, 8), generator=gen(4)).cuda().requires_grad_(), torch.randn((40, 1), generator=gen(5)).cuda()
+    dq, = torch.autograd.grad((pkg.rotary_positions(q, pos, (4,))[0] ** 3).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        dq.sum().backward()
+
+
 def test_loss_of_no_points(pkg):
     w = torch.randn((30, 64), device="cuda").requires_grad_()
     x = torch.zeros((0, 64), device="cuda").requires_grad_()
