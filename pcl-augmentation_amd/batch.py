@@ -639,6 +639,7 @@ def augment_batch(scenes, candidates, min_points, rows=_lib.NUMROW, cols=_lib.NU
         raise ValueError("augment_batch: a pool takes scenes from the batched path only, which this range image is not for")
     if pool is not None:
         pool.check_scenes(pool_scenes, B)
+        pool.check_device(device)
     if not level2_takes(rows, cols):
         # a range image the batched kernels are not built for (columns that are no multiple of 32: the bit images are rows of
         # 32-pixel words; 2^24 pixels and more; edge tables beyond the projection kernel's LDS): every frame through the

@@ -253,6 +253,13 @@ class ScenePool:
             raise ValueError(f"ScenePool: {n} distinct scene numbers below {self.max_scenes}")
         return scenes
 
+    def check_device(self, device):
+        """Raises where scenes on this device cannot go into the pool."""
+        import torch
+        device = torch.device(device)
+        if (device.type, device.index or 0) != (self.device.type, self.device.index or 0):
+            raise ValueError(f"ScenePool: the batch is on {device}, the pool on {self.device}")
+
     @_lib.on_own_device
     def add(self, batch, scenes=None):
         """The merged clouds of a finished batch (``SceneBatch.finish``) become scenes ``scenes`` (distinct numbers, one per scene of
@@ -260,8 +267,7 @@ class ScenePool:
         Returns an int32 tensor [B] on the device: 1 where the scene was taken."""
         import torch
         scenes = self.check_scenes(scenes, batch.B)
-        if batch.device != self.device and (batch.device.type, batch.device.index or 0) != (self.device.type, self.device.index or 0):
-            raise ValueError(f"ScenePool.add: the batch is on {batch.device}, the pool on {self.device}")
+        self.check_device(batch.device)
         rows = self._on_device(scenes)
         self.resize(self.blocks.held.index_copy(0, rows.long(), batch.n_out))
         taken = self.blocks.held[rows.long()] == batch.n_out

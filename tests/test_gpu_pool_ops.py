@@ -368,3 +368,11 @@ def test_pool_calls_do_not_wait_for_the_device(pkg, synth):
     assert running
     n = len(want[0][1][0])
     assert got.xyzi[:n].cpu().numpy().tobytes() == want[0][1][0].tobytes() and pool.lengths.tolist()[0] == 0
+
+
+def test_pool_of_another_device_is_refused_before_the_work(pkg, synth):
+    scenes, slots, need = _scenes(synth, 1)
+    pool = pkg.ScenePool(1, 8192)
+    with pytest.raises(ValueError, match="cuda:1"):
+        pkg.augment_batch(scenes, slots, need, device="cuda:1", pool=pool)
+    assert pool.lengths.tolist() == [0]
