@@ -3,7 +3,7 @@
 // A finished batch stands in HBM with a length per scene that only the device knows (r3d_batch_t.n_out).  These kernels
 // give every scene its blocks, number the points of the scenes a training step asks for and move the points, without a
 // word to the host.  All of it is copying and prefix sums: the large calls are bound by HBM, the small ones by the launch.
-// Measured: tables of 256 scenes x 74 blocks 19 us (three launches), of 23 201 scenes 30; the map of 30.7 million points 92 us, 461 MB
+// Measured: tables of 256 scenes x 74 blocks 10 us (two launches), of 23 201 scenes 29; the map of 30.7 million points 92 us, 461 MB
 // written at 5.0 TB/s; 480 000 rows of 20 bytes taken in 6.3 us, 7.7 million put in 86 us, 5.3 TB/s.
 #include "r3d_host.hpp"
 
@@ -73,7 +73,6 @@ __global__ __launch_bounds__(kGroup) void k_tables_count(TablesArgs a) {
   if (threadIdx.x == 0) {
     a.part[blockIdx.x] = back;
     a.part[a.groups + blockIdx.x] = grow;
-    if (blockIdx.x == 0 && a.status) *a.status = 0;      // (k_tables_write adds what it finds)
   }
 }
 
@@ -81,6 +80,10 @@ struct Sums {
   int64_t back_before, back_all, grow_before;
 };
 __device__ __forceinline__ Sums sums_before(const TablesArgs &a, int group, int64_t *s) {
+  if (a.groups == 1) {      // (no launch for the sums of a single group)
+    const RowWant w = row_want(a, threadIdx.x);
+    return Sums{0, group_sum(w.have > w.want ? w.have - w.want : 0, s), 0};
+  }
   int64_t before = 0, all = 0, grow = 0;
   for (int g = threadIdx.x; g < a.groups; g += kGroup) {
     const int64_t b = a.part[g];
@@ -110,6 +113,7 @@ __global__ __launch_bounds__(kGroup) void k_tables_release(TablesArgs a) {
   const int64_t row = (int64_t)group * kGroup + threadIdx.x;
   const RowWant w = group < a.groups ? row_want(a, row) : RowWant{0, 0, true};
   const Sums sum = sums_before(a, group, s);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && a.status) *a.status = 0;      // (k_tables_write adds what it finds)
   const int64_t n_free = clamp_free(a), n_all = n_free + sum.back_all;
   for (int64_t i = (int64_t)blockIdx.x * kGroup + threadIdx.x; i < a.n_blocks; i += (int64_t)gridDim.x * kGroup)
     if (i < n_free || i >= n_all) a.free_out[i] = i < n_free ? a.free_blocks[i] : -1;
@@ -247,13 +251,31 @@ __device__ __forceinline__ int64_t find_sequence(const int64_t *off, int64_t bas
   return lo;
 }
 
+// kSums: the offsets are made here, by every workgroup for itself (n_seq <= kMapLds), and there is no k_map_offsets before.
+template <bool kSums>
 __global__ __launch_bounds__(256) void k_map_slots(MapArgs a) {
   __shared__ int64_t s_off[kMapLds + 1];
-  const int64_t first = (int64_t)blockIdx.x * kMapTokens, total = a.offsets[a.n_seq];
-  const int64_t last = min(first + kMapTokens, a.capacity);
-  int64_t lo = 0, hi = 0;
+  const int64_t first = (int64_t)blockIdx.x * kMapTokens, last = min(first + kMapTokens, a.capacity);
+  int64_t lo = 0, hi = 0, total;
   bool near = false;
-  if (first < total) {
+  if constexpr (kSums) {
+    static_assert(kMapLds == 512, "two sequences a thread");
+    __shared__ int64_t s[4];
+    const int64_t i = threadIdx.x * 2, l0 = i < a.n_seq ? seq_length(a, i) : 0, l1 = i + 1 < a.n_seq ? seq_length(a, i + 1) : 0;
+    const int64_t run = group_scan(l0 + l1, s);
+    if (i < a.n_seq) s_off[i] = run - l0 - l1;
+    if (i + 1 < a.n_seq) s_off[i + 1] = run - l1;
+    if (threadIdx.x == 255) s_off[a.n_seq] = run;
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int64_t k = threadIdx.x; k <= a.n_seq; k += 256) a.offsets[k] = s_off[k];
+    total = s_off[a.n_seq];
+    hi = a.n_seq;
+    near = true;
+  } else {
+    total = a.offsets[a.n_seq];
+  }
+  if (!kSums && first < total) {
     // the sequences this part of the tokens touches; short ranges are searched in LDS from then on
     lo = find_sequence(a.offsets, 0, 0, a.n_seq, first);
     hi = find_sequence(a.offsets, 0, lo, a.n_seq, min(last, total) - 1) + 1;
@@ -384,7 +406,7 @@ extern "C" int r3d_block_tables(const int32_t *lengths, int64_t n_rows, int32_t 
   hipStream_t st = static_cast<hipStream_t>(stream);
   TablesArgs a{lengths, tables, held, free_blocks, n_free, tables_out, held_out, free_out, n_free_out, status, n_rows, n_blocks,
                block_size, max_blocks, static_cast<int64_t *>(workspace), (int32_t)groups_of(n_rows)};
-  hipLaunchKernelGGL(k_tables_count, dim3(a.groups), dim3(kGroup), 0, st, a);
+  if (a.groups > 1) hipLaunchKernelGGL(k_tables_count, dim3(a.groups), dim3(kGroup), 0, st, a);
   const int copies = blocks_for(n_blocks, kGroup * 8, 1024);
   hipLaunchKernelGGL(k_tables_release, dim3(a.groups > copies ? a.groups : copies), dim3(kGroup), 0, st, a);
   // slices: two cells a thread (256 x 74: 7.8 us with eight, 6.0 with two), four workgroups a CU at most (23 201 x 74: 11 us, with
@@ -410,10 +432,14 @@ extern "C" int r3d_slot_map(const int32_t *lengths, int64_t n_lengths, const int
   hipStream_t st = static_cast<hipStream_t>(stream);
   MapArgs a{lengths, tables, rows, n_lengths, n_seq, capacity, block_size, tables ? max_blocks : 1, -1, offsets, slots, sequence};
   if ((block_size & (block_size - 1)) == 0) a.shift = __builtin_ctz((unsigned)block_size);
-  hipLaunchKernelGGL(k_map_offsets, dim3(1), dim3(1024), 0, st, a);
-  if (capacity > 0) {
-    const int64_t blocks = (capacity + kMapTokens - 1) / kMapTokens;
-    hipLaunchKernelGGL(k_map_slots, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  // few sequences and points: one launch (8 scenes, 64 000 points: 8.4 us and a launch, 2.4 + 8.2 and two), else every
+  // workgroup would make the sums again
+  const int64_t blocks = (capacity + kMapTokens - 1) / kMapTokens;
+  if (blocks > 0 && blocks <= 512 && n_seq <= kMapLds) {
+    hipLaunchKernelGGL(k_map_slots<true>, dim3((unsigned)blocks), dim3(256), 0, st, a);
+  } else {
+    hipLaunchKernelGGL(k_map_offsets, dim3(1), dim3(1024), 0, st, a);
+    if (blocks > 0) hipLaunchKernelGGL(k_map_slots<false>, dim3((unsigned)blocks), dim3(256), 0, st, a);
   }
   R3D_LAUNCHED("slot_map kernels");
   return R3D_OK;

@@ -175,11 +175,12 @@ extern "C" int r3d_rotary(const r3d_rotary_t *d, void *stream) {
     return fail(R3D_E_ARG, "rotary: type of the positions");
   if (!(d->base > 0.0)) return fail(R3D_E_ARG, "rotary: base must be positive");
   RotArgs a{};
+  const double octaves = std::log2(d->base);
   for (int x = 0; x < d->axes; ++x) {
     const int s = d->sections[x];
     if (s < 0 || a.pairs + s > kMaxPairs) return fail(R3D_E_ARG, "rotary: sections (at most 256 pairs)");
     for (int j = 0; j < s; ++j) {
-      a.turns[a.pairs] = std::exp2(-(double)j / s * std::log2(d->base)) / (2.0 * M_PI);
+      a.turns[a.pairs] = std::exp2(-(double)j / s * octaves) / (2.0 * M_PI);
       a.axis[a.pairs++] = (uint8_t)x;
     }
   }

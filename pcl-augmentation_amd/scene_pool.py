@@ -93,8 +93,8 @@ def slot_map(lengths, block_size, tables=None, rows=None, capacity=None):
                 each = torch.where(there, each[rows.clamp(0, lengths.shape[0] - 1).long()], 0)
             capacity = int(each.sum(dtype=torch.int64))
         n, capacity = lengths.shape[0] if rows is None else rows.shape[0], int(capacity)
-        out = SlotMap(torch.empty(n + 1, dtype=torch.int64, device=lengths.device), torch.empty(capacity, dtype=torch.int64, device=lengths.device),
-                      torch.empty(capacity, dtype=torch.int32, device=lengths.device))
+        device, empty = lengths.device, torch.empty
+        out = SlotMap(empty(n + 1, dtype=torch.int64, device=device), empty(capacity, dtype=torch.int64, device=device), lengths.new_empty(capacity))
         # (an empty tensor has no address; nothing is written where capacity is 0)
         slots, sequence = (t.data_ptr() if capacity else out.offsets.data_ptr() for t in out[1:])
         _lib.check(lib.r3d_slot_map(lengths.data_ptr(), lengths.shape[0], 0 if tables is None else tables.data_ptr(), block_size, most,
@@ -108,14 +108,16 @@ def _slots(what, name, slots):
     _whole(what, name, slots, torch.int64, 1)
 
 
+_ROWS = [_lib.Rows * n for n in range(_lib.MAX_ROW_ARRAYS + 1)]
+
+
 def _move(what, sources, dests, src_slots, dst_slots, n):
     rows = []
     for s, t in zip(sources, dests):
-        size = s.element_size()
-        shape = s.shape
-        width = size * (shape[1] if len(shape) == 2 else math.prod(shape[1:]))
+        size, shape = s.element_size(), s.shape
+        width = size * (1 if len(shape) == 1 else shape[1] if len(shape) == 2 else math.prod(shape[1:]))
         rows.append((s.data_ptr(), t.data_ptr(), s.stride(0) * size if shape[0] > 1 else width, t.stride(0) * size if t.shape[0] > 1 else width, width))
-    _lib.check(_lib.load().r3d_move_rows((_lib.Rows * len(rows))(*rows), len(rows), 0 if src_slots is None else src_slots.data_ptr(),
+    _lib.check(_lib.load().r3d_move_rows(_ROWS[len(rows)](*rows), len(rows), 0 if src_slots is None else src_slots.data_ptr(),
                                          0 if dst_slots is None else dst_slots.data_ptr(), n, sources[0].shape[0], dests[0].shape[0],
                                          _lib.raw_stream(sources[0].get_device())), "r3d_move_rows")
 
@@ -125,8 +127,9 @@ def _rows_of(what, name, tensors, like=None):
     tensors = tuple(tensors)
     if not 1 <= len(tensors) <= _lib.MAX_ROW_ARRAYS:
         raise ValueError(f"{what}: 1 to {_lib.MAX_ROW_ARRAYS} {name}")
+    n = tensors[0].shape[:1]
     for t in tensors:
-        if t.dim() < 1 or t.shape[0] != tensors[0].shape[0]:
+        if not n or t.shape[:1] != n:
             raise ValueError(f"{what}: {name} must have the same number of rows")
         if t.requires_grad:
             raise ValueError(f"{what}: no gradient passes through moved rows (detach them)")
