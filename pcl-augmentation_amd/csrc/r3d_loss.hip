@@ -331,26 +331,30 @@ struct JoinArgs {
   int32_t splits, mean, points;      // points: of a workgroup
 };
 
+constexpr int kJoinThreads = 1024, kJoinSlices = 16;
+
 __device__ __forceinline__ double group_sum(double d, double *s) {
 #pragma unroll
   for (int k = 32; k; k >>= 1) d += __shfl_xor(d, k);
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = d;
   __syncthreads();
-  return s[0] + s[1] + s[2] + s[3];
+  d = 0.0;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 64; ++w) d += s[w];
+  return d;
 }
 
 // The splits joined; the loss of every point (each), or their sum: every workgroup leaves that of its points, the last one adds them
-// up, always in the same order.  Over the points as the caller numbers them.  Few points have many splits: a workgroup takes 16 of
-// them then and 16 threads share the splits of each (24 points x 38 322 classes, 300 splits: 140 us with one thread a point, 9 so;
+// up, always in the same order.  Over the points as the caller numbers them.  Few points have many splits: a workgroup takes 64 of
+// them then and 16 threads share the splits of each (24 points x 38 322 classes, 300 splits: 140 us with one thread a point, 11 so;
 // 8192 points of 8 splits: 10 and 22, every workgroup raises the one counter that tells which is the last).
-constexpr int kJoinSlices = 16;
-int join_points(int splits) { return splits >= 16 ? 256 / kJoinSlices : 256; }
+int join_points(int splits) { return splits >= 16 ? kJoinThreads / kJoinSlices : kJoinThreads; }
 
-__global__ __launch_bounds__(256) void k_ce_join(JoinArgs a) {
-  __shared__ double s[4];
+__global__ __launch_bounds__(kJoinThreads) void k_ce_join(JoinArgs a) {
+  __shared__ double s[kJoinThreads / 64];
   __shared__ int s_last;
-  __shared__ float s_top[256], s_sum[256];
-  const int points = a.points, slices = 256 / points, p = (int)threadIdx.x % points, slice = (int)threadIdx.x / points;
+  __shared__ float s_top[kJoinThreads], s_sum[kJoinThreads];
+  const int points = a.points, slices = kJoinThreads / points, p = (int)threadIdx.x % points, slice = (int)threadIdx.x / points;
   double losses = 0.0;
   for (int64_t block = blockIdx.x; block * points < a.n; block += gridDim.x) {
     const int64_t i = block * points + p;
@@ -394,7 +398,7 @@ __global__ __launch_bounds__(256) void k_ce_join(JoinArgs a) {
   __syncthreads();
   if (!s_last) return;
   double d = 0.0;
-  for (int64_t b = threadIdx.x; b < gridDim.x; b += 256) d += __hip_atomic_load(&a.sums[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int64_t b = threadIdx.x; b < gridDim.x; b += kJoinThreads) d += __hip_atomic_load(&a.sums[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   d = group_sum(d, s);
   if (threadIdx.x == 0) {
@@ -1140,8 +1144,8 @@ void join(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   JoinArgs ja{p.part_m, p.part_l, p.hit, p.tgt, p.place, p.counted, p.lse2, d.reduction == R3D_CE_NONE ? d.loss : nullptr, d.loss, p.sums, d.n, p.n_pad,
               p.lse_splits, d.reduction == R3D_CE_MEAN};
   ja.points = join_points(p.lse_splits);
-  // a sum: a workgroup a CU, each raises the one counter (270 597 points: 39 us with one for every 256 points, 17 so)
-  hipLaunchKernelGGL(k_ce_join, dim3(blocks_for(d.n, ja.points, d.reduction == R3D_CE_NONE ? INT32_MAX : kCus)), dim3(256), 0, st, ja);
+  // a sum: a workgroup a CU, each raises the one counter (270 597 points: 39 us with one for every 256 points, 13 so)
+  hipLaunchKernelGGL(k_ce_join, dim3(blocks_for(d.n, ja.points, d.reduction == R3D_CE_NONE ? INT32_MAX : kCus)), dim3(kJoinThreads), 0, st, ja);
 }
 
 HeadArgs head_args(const r3d_linear_ce_t &d, const Plan &p) {
