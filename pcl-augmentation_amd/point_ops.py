@@ -85,15 +85,15 @@ def _turn(tensors, positions, sections, base, interleaved, backward):
         if t is None:
             outs.append(None)
             continue
-        outs.append(torch.empty_like(t, memory_format=torch.contiguous_format))
-        if t.shape[1] == 0:
-            continue
-        if t.stride(2) != 1:
+        out = torch.empty_like(t, memory_format=torch.contiguous_format)
+        outs.append(out)
+        strides = t.stride()
+        if strides[2] != 1:
             t = t.contiguous()
             kept.append(t)      # (until the launch)
-        x[w], y[w] = t.data_ptr(), outs[w].data_ptr()
-        token_stride[w], head_stride[w], _ = t.stride()
-        heads[w] = t.shape[1]
+            strides = t.stride()
+        x[w], y[w], heads[w] = t.data_ptr(), out.data_ptr(), t.shape[1]
+        token_stride[w], head_stride[w], _ = strides
     if heads == [0, 0] or tokens == 0:
         return outs
     d = _lib.Rotary(tuple(x), tuple(y), tuple(token_stride), tuple(head_stride), tokens, tuple(heads), dim, values[first.dtype], interleaved, backward,
@@ -137,27 +137,30 @@ def rotary_positions(query, positions, sections, key=None, base=10000.0, style="
     (``"interleaved"``), elements from 2 R on stay.  Angles are taken in double, products in 32 bits, one rounding.
     Returns (query, key), key None where none was given; differentiable in both, once."""
     import torch
-    if query.dim() != 3 or (key is not None and key.dim() != 3):
+    shape, like, where = query.shape, None if key is None else key.shape, positions.shape
+    if len(shape) != 3 or (like is not None and len(like) != 3):
         raise ValueError("rotary_positions: query and key must be [tokens, heads, dim]")
     if style not in ("half", "interleaved"):
         raise ValueError("rotary_positions: style is 'half' or 'interleaved'")
-    sections = tuple(int(s) for s in sections)
-    if not 1 <= len(sections) <= _lib.ROTARY_MAX_AXES or min(sections) < 0:
+    sections = tuple([int(s) for s in sections])
+    axes, pairs = len(sections), sum(sections)
+    if not 1 <= axes <= _lib.ROTARY_MAX_AXES or min(sections) < 0:
         raise ValueError(f"rotary_positions: 1 to {_lib.ROTARY_MAX_AXES} sections of zero or more pairs")
-    if positions.dim() != 2 or positions.shape != (query.shape[0], len(sections)):
-        raise ValueError(f"rotary_positions: positions must be [{query.shape[0]}, {len(sections)}], got {tuple(positions.shape)}")
+    tokens, heads, dim = shape
+    if len(where) != 2 or where[0] != tokens or where[1] != axes:
+        raise ValueError(f"rotary_positions: positions must be [{tokens}, {axes}], got {tuple(where)}")
     if positions.dtype not in _types()[1]:
         raise TypeError(f"rotary_positions: positions are int32, int64, float32 or float64, got {positions.dtype}")
     if positions.requires_grad:
         raise ValueError("rotary_positions: positions have no gradient here (detach them)")
     _value_type("rotary_positions", query)
-    if key is not None and (key.dtype != query.dtype or key.shape[0] != query.shape[0] or key.shape[2] != query.shape[2]):
+    if like is not None and (key.dtype is not query.dtype or like[0] != tokens or like[2] != dim):
         raise ValueError("rotary_positions: key must have query's tokens, dim and type")
-    if sum(sections) > _lib.ROTARY_MAX_PAIRS or 2 * sum(sections) > query.shape[2]:
-        raise ValueError(f"rotary_positions: {sum(sections)} pairs do not fit a head of {query.shape[2]} (at most {_lib.ROTARY_MAX_PAIRS} pairs)")
-    if query.shape[2] % 2 or query.shape[2] > 4096:
+    if pairs > _lib.ROTARY_MAX_PAIRS or 2 * pairs > dim:
+        raise ValueError(f"rotary_positions: {pairs} pairs do not fit a head of {dim} (at most {_lib.ROTARY_MAX_PAIRS} pairs)")
+    if dim % 2 or dim > 4096:
         raise ValueError("rotary_positions: the size of a head must be even and at most 4096")
-    if max(query.shape[1], 0 if key is None else key.shape[1]) > 65536:
+    if heads > 65536 or (like is not None and like[1] > 65536):
         raise ValueError("rotary_positions: at most 65536 heads")
     base = float(base)
     if not base > 0.0 or base == float("inf"):
