@@ -3,8 +3,8 @@
 // A finished batch stands in HBM with a length per scene that only the device knows (r3d_batch_t.n_out).  These kernels
 // give every scene its blocks, number the points of the scenes a training step asks for and move the points, without a
 // word to the host.  All of it is copying and prefix sums: the large calls are bound by HBM, the small ones by the launch.
-// Measured: tables of 256 scenes x 74 blocks 10 us (two launches), of 23 201 scenes 29; the map of 30.7 million points 92 us, 461 MB
-// written at 5.0 TB/s; 480 000 rows of 20 bytes taken in 6.3 us, 7.7 million put in 86 us, 5.3 TB/s.
+// Measured: tables of 256 scenes x 74 blocks 10 us (two launches), of 23 201 scenes 29; the map of 30.7 million points (38 million slots)
+// 81 us, 461 MB written at 5.7 TB/s; 480 000 rows of 20 bytes taken in 6.3 us, 7.7 million put in 86 us, 5.3 TB/s.
 #include "r3d_host.hpp"
 
 namespace {
@@ -240,7 +240,9 @@ __global__ __launch_bounds__(1024) void k_map_offsets(MapArgs a) {
   if (threadIdx.x == 1023) a.offsets[a.n_seq] = run;
 }
 
-constexpr int kMapTokens = 4096, kMapLds = 512;
+// kMapAhead: pairs of tokens of a thread.  All of a workgroup's are on their way together (38 million slots: 86 us in two turns of four
+// pairs, 81 in one of four, 81 in one of eight, 99 in one of two).
+constexpr int kMapLds = 512, kMapAhead = 4, kMapTokens = kMapAhead * 512;
 
 // Last sequence i in [lo, hi) with off[i - base] <= t, i.e. the one token t falls in (empty sequences are passed over).
 __device__ __forceinline__ int64_t find_sequence(const int64_t *off, int64_t base, int64_t lo, int64_t hi, int64_t t) {
@@ -284,43 +286,50 @@ __global__ __launch_bounds__(256) void k_map_slots(MapArgs a) {
       for (int64_t i = threadIdx.x; i <= hi - lo; i += 256) s_off[i] = a.offsets[lo + i];
   }
   __syncthreads();
-  for (int64_t t0 = first + threadIdx.x * 4; t0 < last; t0 += 1024) {
-    int64_t slot[4];
-    int32_t seq[4];
-    int64_t i = -1, end = t0, row = 0, at = 0, blk = 0, in = 0, page = 0;
+  // a thread's tokens two by two, so that the lanes of a store lie in one line: 1 KB of slots, 512 bytes of numbers
+  int64_t i = -1, start = 0, end = first, row = 0;      // the sequence that a token before this one fell in
+  const int64_t t0 = first + threadIdx.x * 2;
+  int64_t slot[kMapAhead][2];
+  int32_t seq[kMapAhead][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t t = t0 + j;
-      slot[j] = -1;
-      seq[j] = -1;
-      if (t < total) {
-        if (t >= end) {                      // the next sequence that has points
-          const int64_t from = i < 0 ? lo : i + 1;
-          i = near ? find_sequence(s_off, lo, from, hi, t) : find_sequence(a.offsets, 0, from, a.n_seq, t);
-          const int64_t start = near ? s_off[i - lo] : a.offsets[i];
-          end = near ? s_off[i - lo + 1] : a.offsets[i + 1];
-          row = seq_row(a, i);
-          at = t - start;
-          blk = a.shift >= 0 ? at >> a.shift : (int64_t)((uint32_t)at / (uint32_t)a.block);
-          in = at - blk * a.block;
-          page = a.tables ? a.tables[row * a.most + blk] : row;
-        } else if (++in == a.block) {
-          in = 0;
-          page = a.tables ? a.tables[row * a.most + ++blk] : row;
-        }
-        slot[j] = page < 0 ? -1 : page * a.block + in;
-        seq[j] = (int32_t)i;
+  for (int u = 0; u < kMapAhead; ++u) {
+    int64_t blk = 0, in = -1, page = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int64_t t = t0 + u * 512 + j;
+      slot[u][j] = -1;
+      seq[u][j] = -1;
+      if (t >= total) continue;
+      if (t >= end) {                      // the next sequence that has points
+        const int64_t from = i < 0 ? lo : i + 1;
+        i = near ? find_sequence(s_off, lo, from, hi, t) : find_sequence(a.offsets, 0, from, a.n_seq, t);
+        start = near ? s_off[i - lo] : a.offsets[i];
+        end = near ? s_off[i - lo + 1] : a.offsets[i + 1];
+        row = seq_row(a, i);
+        in = -1;
       }
+      if (in < 0) {
+        const int64_t at = t - start;
+        blk = a.shift >= 0 ? at >> a.shift : (int64_t)((uint32_t)at / (uint32_t)a.block);
+        in = at - blk * a.block;
+        page = a.tables ? a.tables[row * a.most + blk] : row;
+      } else if (++in == a.block) {
+        in = 0;
+        page = a.tables ? a.tables[row * a.most + ++blk] : row;
+      }
+      slot[u][j] = page < 0 ? -1 : page * a.block + in;
+      seq[u][j] = (int32_t)i;
     }
-    if (t0 + 4 <= last) {
-      reinterpret_cast<longlong2 *>(a.slots + t0)[0] = make_longlong2(slot[0], slot[1]);
-      reinterpret_cast<longlong2 *>(a.slots + t0)[1] = make_longlong2(slot[2], slot[3]);
-      *reinterpret_cast<int4 *>(a.sequence + t0) = make_int4(seq[0], seq[1], seq[2], seq[3]);
-    } else {
-      for (int j = 0; t0 + j < last; ++j) {
-        a.slots[t0 + j] = slot[j];
-        a.sequence[t0 + j] = seq[j];
-      }
+  }
+#pragma unroll
+  for (int u = 0; u < kMapAhead; ++u) {
+    const int64_t t = t0 + u * 512;
+    if (t + 2 <= last) {
+      *reinterpret_cast<longlong2 *>(a.slots + t) = make_longlong2(slot[u][0], slot[u][1]);
+      *reinterpret_cast<int2 *>(a.sequence + t) = make_int2(seq[u][0], seq[u][1]);
+    } else if (t < last) {
+      a.slots[t] = slot[u][0];
+      a.sequence[t] = seq[u][0];
     }
   }
 }
@@ -424,7 +433,7 @@ extern "C" int r3d_slot_map(const int32_t *lengths, int64_t n_lengths, const int
                             int32_t *sequence, void *stream) {
   if (!lengths || !offsets || !slots || !sequence) return fail(R3D_E_ARG, "slot_map: null pointer");
   if (n_lengths <= 0 || n_lengths > INT32_MAX || n_seq < 0 || n_seq > R3D_MAX_SCENES || (!rows && n_seq > n_lengths) || capacity < 0 ||
-      block_size <= 0 || (tables && max_blocks <= 0) || capacity > (1ll << 42) ||
+      block_size <= 0 || (tables && max_blocks <= 0) || capacity > (1ll << 40) ||
       (tables && (int64_t)max_blocks * block_size > INT32_MAX))
     return fail(R3D_E_ARG, "slot_map: bad size");
   if ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(sequence)) & 15)
@@ -432,10 +441,10 @@ extern "C" int r3d_slot_map(const int32_t *lengths, int64_t n_lengths, const int
   hipStream_t st = static_cast<hipStream_t>(stream);
   MapArgs a{lengths, tables, rows, n_lengths, n_seq, capacity, block_size, tables ? max_blocks : 1, -1, offsets, slots, sequence};
   if ((block_size & (block_size - 1)) == 0) a.shift = __builtin_ctz((unsigned)block_size);
-  // few sequences and points: one launch (8 scenes, 64 000 points: 8.4 us and a launch, 2.4 + 8.2 and two), else every
-  // workgroup would make the sums again
+  // few sequences: one launch, in which every workgroup makes the sums (256 scenes, 38 million slots: one microsecond less
+  // than without, and 5 and a launch of k_map_offsets; 8 scenes, 64 000 points: 6.3 us)
   const int64_t blocks = (capacity + kMapTokens - 1) / kMapTokens;
-  if (blocks > 0 && blocks <= 512 && n_seq <= kMapLds) {
+  if (blocks > 0 && n_seq <= kMapLds) {
     hipLaunchKernelGGL(k_map_slots<true>, dim3((unsigned)blocks), dim3(256), 0, st, a);
   } else {
     hipLaunchKernelGGL(k_map_offsets, dim3(1), dim3(1024), 0, st, a);
