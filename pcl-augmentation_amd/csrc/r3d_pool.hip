@@ -6,6 +6,7 @@
 // Measured: tables of 256 scenes x 74 blocks 10 us (two launches), of 23 201 scenes 29; the map of 30.7 million points (38 million slots)
 // 81 us, 461 MB written at 5.7 TB/s; 480 000 rows of 20 bytes taken in 6.3 us, 7.7 million put in 86 us, 5.3 TB/s.
 #include "r3d_host.hpp"
+#include "r3d_map_core.hpp"
 
 namespace {
 using namespace r3d;
@@ -240,26 +241,13 @@ __global__ __launch_bounds__(1024) void k_map_offsets(MapArgs a) {
   if (threadIdx.x == 1023) a.offsets[a.n_seq] = run;
 }
 
-// kMapAhead: pairs of tokens of a thread.  All of a workgroup's are on their way together (38 million slots: 86 us in two turns of four
-// pairs, 81 in one of four, 81 in one of eight, 99 in one of two).
-constexpr int kMapLds = 512, kMapAhead = 4, kMapTokens = kMapAhead * 512;
-
-// Last sequence i in [lo, hi) with off[i - base] <= t, i.e. the one token t falls in (empty sequences are passed over).
-__device__ __forceinline__ int64_t find_sequence(const int64_t *off, int64_t base, int64_t lo, int64_t hi, int64_t t) {
-  while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (off[mid - base] <= t) lo = mid; else hi = mid;
-  }
-  return lo;
-}
-
 // kSums: the offsets are made here, by every workgroup for itself (n_seq <= kMapLds), and there is no k_map_offsets before.
 template <bool kSums>
 __global__ __launch_bounds__(256) void k_map_slots(MapArgs a) {
   __shared__ int64_t s_off[kMapLds + 1];
   const int64_t first = (int64_t)blockIdx.x * kMapTokens, last = min(first + kMapTokens, a.capacity);
-  int64_t lo = 0, hi = 0, total;
-  bool near = false;
+  MapPart part{0, 0, false};
+  int64_t total;
   if constexpr (kSums) {
     static_assert(kMapLds == 512, "two sequences a thread");
     __shared__ int64_t s[4];
@@ -272,55 +260,23 @@ __global__ __launch_bounds__(256) void k_map_slots(MapArgs a) {
     if (blockIdx.x == 0)
       for (int64_t k = threadIdx.x; k <= a.n_seq; k += 256) a.offsets[k] = s_off[k];
     total = s_off[a.n_seq];
-    hi = a.n_seq;
-    near = true;
+    part = MapPart{0, a.n_seq, true};
   } else {
     total = a.offsets[a.n_seq];
   }
-  if (!kSums && first < total) {
+  const int64_t stop = min(last, total);      // tokens beyond the capacity are left out: what is looked up here ends before them
+  if (!kSums && first < stop) {
     // the sequences this part of the tokens touches; short ranges are searched in LDS from then on
-    lo = find_sequence(a.offsets, 0, 0, a.n_seq, first);
-    hi = find_sequence(a.offsets, 0, lo, a.n_seq, min(last, total) - 1) + 1;
-    near = hi - lo <= kMapLds;
-    if (near)
-      for (int64_t i = threadIdx.x; i <= hi - lo; i += 256) s_off[i] = a.offsets[lo + i];
+    part = map_part(a.offsets, a.n_seq, first, stop);
+    if (part.near)
+      for (int64_t i = threadIdx.x; i <= part.hi - part.lo; i += 256) s_off[i] = a.offsets[part.lo + i];
   }
   __syncthreads();
   // a thread's tokens two by two, so that the lanes of a store lie in one line: 1 KB of slots, 512 bytes of numbers
-  int64_t i = -1, start = 0, end = first, row = 0;      // the sequence that a token before this one fell in
   const int64_t t0 = first + threadIdx.x * 2;
   int64_t slot[kMapAhead][2];
   int32_t seq[kMapAhead][2];
-#pragma unroll
-  for (int u = 0; u < kMapAhead; ++u) {
-    int64_t blk = 0, in = -1, page = 0;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int64_t t = t0 + u * 512 + j;
-      slot[u][j] = -1;
-      seq[u][j] = -1;
-      if (t >= total) continue;
-      if (t >= end) {                      // the next sequence that has points
-        const int64_t from = i < 0 ? lo : i + 1;
-        i = near ? find_sequence(s_off, lo, from, hi, t) : find_sequence(a.offsets, 0, from, a.n_seq, t);
-        start = near ? s_off[i - lo] : a.offsets[i];
-        end = near ? s_off[i - lo + 1] : a.offsets[i + 1];
-        row = seq_row(a, i);
-        in = -1;
-      }
-      if (in < 0) {
-        const int64_t at = t - start;
-        blk = a.shift >= 0 ? at >> a.shift : (int64_t)((uint32_t)at / (uint32_t)a.block);
-        in = at - blk * a.block;
-        page = a.tables ? a.tables[row * a.most + blk] : row;
-      } else if (++in == a.block) {
-        in = 0;
-        page = a.tables ? a.tables[row * a.most + ++blk] : row;
-      }
-      slot[u][j] = page < 0 ? -1 : page * a.block + in;
-      seq[u][j] = (int32_t)i;
-    }
-  }
+  map_walk(a, s_off, part, t0, stop, slot, seq);
 #pragma unroll
   for (int u = 0; u < kMapAhead; ++u) {
     const int64_t t = t0 + u * 512;

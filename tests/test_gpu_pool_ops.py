@@ -376,3 +376,20 @@ def test_pool_of_another_device_is_refused_before_the_work(pkg, synth):
     with pytest.raises(ValueError, match="cuda:1"):
         pkg.augment_batch(scenes, slots, need, device="cuda:1", pool=pool)
     assert pool.lengths.tolist() == [0]
+
+
+@pytest.mark.parametrize("scenes,points,block,empty", [(600, 10, 16, 0.0), (700, 3, 2, 0.0), (5000, 9, 4, 0.8), (900, 700, 64, 0.3), (512, 10, 16, 0.0), (513, 40, 7, 0.1)])
+def test_slot_map_of_many_sequences_with_little_room(pkg, scenes, points, block, empty):
+    """Capacities far below the number of tokens, and ends in the middle of what a workgroup takes."""
+    rng = np.random.default_rng(scenes)
+    lengths = np.full(scenes, points) if not empty else rng.integers(1, points + 1, scenes)
+    lengths[rng.random(scenes) < empty] = 0
+    most = -(-points // block)
+    tables, rows = rng.permutation(scenes * most).reshape(scenes, most), rng.permutation(scenes)
+    total = int(lengths.sum())
+    offsets, slots, seq = map_by_tokens(lengths.tolist(), block, tables.tolist(), rows.tolist(), total)
+    for capacity in (1, 2, 511, 2047, 2048, 2049, 2100, total // 2, total - 1):
+        if capacity >= total:
+            continue
+        got = pkg.slot_map(i32(lengths), block, i32(tables), i32(rows), capacity)
+        assert got.offsets.tolist() == offsets and got.slots.tolist() == slots[:capacity] and got.sequence.tolist() == seq[:capacity], capacity
