@@ -280,8 +280,8 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     if points > 2 ** 31 - 1025 or wide[0] > 2 ** 31 - 1025 or wide[1] > 1 << 20:
         raise ValueError("linear_cross_entropy: too large (2^31 points, 2^31 classes, 2^20 features)")
     here = on_device_of("linear_cross_entropy", x, weight, target, *(() if bias is None else (bias,)))
-    if points == 0:      # nothing to sum; the gradients are zeros
-        none = (x.sum() + weight.sum() * 0 + (0 if bias is None else bias.sum() * 0)).float() * 0
+    if points == 0:      # nothing to sum, whatever the head holds; the gradients are zeros
+        none = (x.sum() + weight[:0].sum() + (0 if bias is None else bias[:0].sum())).float()
         return none if reduction != "none" else none.expand(target.shape) + torch.zeros(target.shape, device=x.device)
     with here:
         loss = _loss_function().apply(_rows_dense(x if len(shape) == 2 else x.reshape(-1, shape[-1])), _rows_dense(weight),

@@ -660,3 +660,17 @@ def test_loss_repeats_its_bits_every_way(pkg, v, d, dtype):
         for _ in range(4):
             noise = noise @ noise * 1e-3
             assert all(torch.equal(p, q) for p, q in zip(step(reduction), want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_loss_of_no_points_whatever_the_head_holds(pkg, dtype):
+    w = torch.ones((2000, 64), dtype=dtype, device="cuda")
+    b = torch.zeros(2000, dtype=dtype, device="cuda")
+    w[3, 5], b[7] = float("inf"), float("-inf")
+    for head, bias in ((w, b), (torch.ones_like(w), None), (torch.full_like(w, torch.finfo(dtype).max), b)):
+        ins = [t.clone().requires_grad_() for t in (torch.zeros((0, 64), dtype=dtype, device="cuda"), head) + (() if bias is None else (bias,))]
+        for reduction in ("mean", "sum", "none"):
+            loss = pkg.linear_cross_entropy(ins[0], ins[1], torch.zeros(0, dtype=torch.int64, device="cuda"), bias=None if bias is None else ins[2], reduction=reduction)
+            assert loss.dtype == F32 and loss.shape == ((0,) if reduction == "none" else ()) and (loss == 0).all()
+            got = torch.autograd.grad(loss.sum(), ins)
+            assert all(g.shape == t.shape and g.dtype == dtype and not g.any() for g, t in zip(got, ins))
