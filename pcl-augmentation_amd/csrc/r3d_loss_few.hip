@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
         if (a.dx) {
           // dx = dl W: features are the rows of C.  The classes of a k-step are taken in the order in which the lanes have
           // them (fours of a lane, then of the next block of 8), from both operands alike.
-          const float out_scale = scale * a.unheld;
+          const float out_scale = t == -2 ? 0.0f : scale * a.unheld;      // (a factor that is infinite or no number makes 0 NaN)
           const int64_t i = tile * kTP + wave * 32 + low;
           V *out = static_cast<V *>(a.dx) + i * a.d;
           const T *wt = ws + (4 * half + (sub >> 2)) * pitch + (group & 1) * 16 + (sub & 3) * 4;

@@ -674,3 +674,21 @@ def test_loss_of_no_points_whatever_the_head_holds(pkg, dtype):
             assert loss.dtype == F32 and loss.shape == ((0,) if reduction == "none" else ()) and (loss == 0).all()
             got = torch.autograd.grad(loss.sum(), ins)
             assert all(g.shape == t.shape and g.dtype == dtype and not g.any() for g, t in zip(got, ins))
+
+
+FEW = [(20, 64, F16), (20, 64, F32), (100, 96, BF16), (40, 200, F16)]      # flavours of the few classes' way that WAYS leaves out
+
+
+@pytest.mark.parametrize("v,d,dtype", WAYS + FEW)
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_loss_points_that_do_not_count_have_no_gradient_whatever_comes_in(pkg, v, d, dtype, reduction):
+    g = gen(v + d)
+    n = 301
+    x, w = (torch.randn(s, generator=g).to(dtype).cuda().requires_grad_() for s in ((n, d), (v, d)))
+    target = torch.randint(0, v, (n,), generator=g)
+    out = torch.rand((n,), generator=g) < 0.4
+    target[out] = -100
+    loss = pkg.linear_cross_entropy(x, w, target.cuda(), reduction=reduction)
+    for up in (math.inf, -math.inf, math.nan):
+        dx, = torch.autograd.grad(loss, x, torch.tensor(up).cuda(), retain_graph=True)
+        assert (dx[out.cuda()] == 0).all() and not torch.isfinite(dx[~out.cuda()]).any()
