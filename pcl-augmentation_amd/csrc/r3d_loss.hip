@@ -443,7 +443,7 @@ __global__ __launch_bounds__(256) void k_ce_weight(WeightArgs a) {
     for (int d = 32; d; d >>= 1) scale = fmaxf(scale, __shfl_xor(scale, d));
     if (!(scale > 0.0f)) scale = 1.0f;      // nothing to take out
   } else {
-    scale = a.grad[0] * a.counted->share;
+    scale = nc ? a.grad[0] * a.counted->share : 0.0f;      // (of no point: 0, whatever comes in)
   }
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i < a.n_pad) a.weight[i] = i >= nc ? 0.0f : a.each ? a.grad[a.idx[i]] / scale : 1.0f;

@@ -39,7 +39,7 @@ struct FewArgs {
 
 // The factor that is taken out of dl: the one weight of a sum or a mean; for float16 the largest weight of single points.
 __device__ __forceinline__ float taken_out(const FewArgs &a) {
-  if (!a.grad_each) return a.grad[0] * a.counted->share;
+  if (!a.grad_each) return a.counted->n ? a.grad[0] * a.counted->share : 0.0f;      // (of no point: 0, whatever comes in)
   float top = 0.0f;
   for (int i = threadIdx.x & 63; i < a.parts; i += 64) top = fmaxf(top, a.top[i]);
 #pragma unroll

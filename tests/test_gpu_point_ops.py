@@ -692,3 +692,15 @@ def test_loss_points_that_do_not_count_have_no_gradient_whatever_comes_in(pkg, v
     for up in (math.inf, -math.inf, math.nan):
         dx, = torch.autograd.grad(loss, x, torch.tensor(up).cuda(), retain_graph=True)
         assert (dx[out.cuda()] == 0).all() and not torch.isfinite(dx[~out.cuda()]).any()
+
+
+@pytest.mark.parametrize("v,d,dtype", WAYS + FEW)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_loss_without_points_that_count_has_no_gradient_whatever_comes_in(pkg, v, d, dtype, reduction):
+    g = gen(v + d)
+    n = 150
+    ins = [torch.randn(s, generator=g).to(dtype).cuda().requires_grad_() for s in ((n, d), (v, d), (v,))]
+    loss = pkg.linear_cross_entropy(ins[0], ins[1], torch.full((n,), -100).cuda(), bias=ins[2], reduction=reduction)
+    for up in (math.inf, math.nan):
+        got = torch.autograd.grad(loss, ins, torch.full(loss.shape, up, device="cuda"), retain_graph=True)
+        assert all((t == 0).all() for t in got)
