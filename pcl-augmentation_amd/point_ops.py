@@ -36,6 +36,12 @@ def on_device_of(what, *tensors):
     return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
+def forward_mode():
+    """Inside of a level of forward-mode differentiation (``torch.autograd.forward_ad``, ``torch.func.jvp``)?"""
+    import torch
+    return torch.autograd.forward_ad._current_level >= 0
+
+
 def _value_type(what, t):
     kind = _types()[0].get(t.dtype)
     if kind is None:
@@ -60,6 +66,8 @@ def _once():
 
     def decorate(backward):
         def run(ctx, *gradients):
+            if forward_mode() and any(g is not None and torch.autograd.forward_ad.unpack_dual(g).tangent is not None for g in gradients):
+                raise RuntimeError("rotary_positions and linear_cross_entropy have no forward-mode derivative of their gradients")
             if not torch.is_grad_enabled():
                 return backward(ctx, *gradients)
             with torch.no_grad():
@@ -135,7 +143,7 @@ def rotary_positions(query, positions, sections, key=None, base=10000.0, style="
     axis with s pairs turns by ``position * base ** (-j / s)``; the pairs of the axes stand one after the other, R in all
     (at most 256, 2 R <= dim): pair i is the elements (i, i + R) of a head (``style="half"``) or (2i, 2i + 1)
     (``"interleaved"``), elements from 2 R on stay.  Angles are taken in double, products in 32 bits, one rounding.
-    Returns (query, key), key None where none was given; differentiable in both, once."""
+    Returns (query, key), key None where none was given; differentiable in both, once and backwards (forward mode raises)."""
     import torch
     shape, like, where = query.shape, None if key is None else key.shape, positions.shape
     if len(shape) != 3 or (like is not None and len(like) != 3):
@@ -166,7 +174,8 @@ def rotary_positions(query, positions, sections, key=None, base=10000.0, style="
     if not base > 0.0 or base == float("inf"):
         raise ValueError("rotary_positions: base must be positive and finite")
     with on_device_of("rotary_positions", query, positions, *(() if key is None else (key,))):
-        if torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad)):
+        # (a tangent of forward-mode differentiation shows in no flag of its tensor: inside of a level torch looks, and raises)
+        if forward_mode() or (torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))):
             return _rotary_function().apply(query, key, positions, sections, base, style == "interleaved")
         return tuple(_turn((query, key), positions, sections, base, style == "interleaved", False))
 
@@ -257,7 +266,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
 
     Points whose target is ``ignore_index`` have loss and gradient 0, whatever their features are; a target that is no class makes
     the loss NaN.  reduction: "mean" over the points that count (0 where none does), "sum" or "none" ([...]); the loss is
-    float32.  Differentiable once in x, weight and bias; the backward pass makes the logits' gradients ``piece`` classes at a time
+    float32.  Differentiable once in x, weight and bias (forward mode raises); the backward pass makes the logits' gradients ``piece`` classes at a time
     (0: as many as 512 MB hold; with at most 128 features none are held).  The same inputs give the same bits."""
     import torch
     shape, dtype, wide = x.shape, x.dtype, weight.shape

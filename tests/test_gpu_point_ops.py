@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -704,3 +705,45 @@ def test_loss_without_points_that_count_has_no_gradient_whatever_comes_in(pkg, v
     for up in (math.inf, math.nan):
         got = torch.autograd.grad(loss, ins, torch.full(loss.shape, up, device="cuda"), retain_graph=True)
         assert all((t == 0).all() for t in got)
+
+
+def test_rotary_refuses_forward_mode(pkg):
+    q, k, pos = torch.randn((5, 2, 8)).cuda(), torch.randn((5, 1, 8)).cuda(), torch.randn((5, 1)).cuda()
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for a, p, b in ((dual(q), pos, k), (q, pos, dual(k)), (q, dual(pos), k), (dual(q), pos, None)):
+            with pytest.raises(RuntimeError):
+                pkg.rotary_positions(a, p, (4,), key=b)
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                pkg.rotary_positions(a, p, (4,), key=b)
+        plain = pkg.rotary_positions(q, pos, (4,), key=k)
+    want = pkg.rotary_positions(q, pos, (4,), key=k)
+    assert all(torch.equal(a, b) for a, b in zip(plain, want))
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: pkg.rotary_positions(t, pos, (4,))[0], (q,), (q,))
+
+
+def test_loss_refuses_forward_mode(pkg):
+    x, w, t = torch.randn((5, 8)).cuda(), torch.randn((3, 8)).cuda(), torch.zeros(5, dtype=torch.int64).cuda()
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError):
+            pkg.linear_cross_entropy(dual, w, t)
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            pkg.linear_cross_entropy(dual, w, t)
+        wd = fwd.make_dual(w, torch.ones_like(w))
+        with pytest.raises(RuntimeError):
+            pkg.linear_cross_entropy(x, wd, t)
+
+
+def test_gradients_refuse_forward_mode(pkg):
+    q, pos = torch.randn((5, 2, 8)).cuda().requires_grad_(), torch.randn((5, 1)).cuda()
+    x, w, t = torch.randn((5, 8)).cuda().requires_grad_(), torch.randn((3, 8)).cuda(), torch.zeros(5, dtype=torch.int64).cuda()
+    y, loss = pkg.rotary_positions(q, pos, (4,))[0], pkg.linear_cross_entropy(x, w, t)
+    with fwd.dual_level():
+        for out, leaf in ((y, q), (loss, x)):
+            up = torch.ones_like(out).detach()
+            want, = torch.autograd.grad(out, leaf, up, retain_graph=True)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(out, leaf, fwd.make_dual(up, torch.ones_like(up)), retain_graph=True)
+            assert torch.equal(torch.autograd.grad(out, leaf, up, retain_graph=True)[0], want)
