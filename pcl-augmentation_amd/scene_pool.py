@@ -9,7 +9,7 @@ import math
 from typing import NamedTuple
 
 from . import _lib
-from .point_ops import on_device_of
+from .point_ops import forward_mode, on_device_of
 
 
 class BlockTables(NamedTuple):
@@ -124,14 +124,15 @@ def _move(what, sources, dests, src_slots, dst_slots, n):
 
 def _rows_of(what, name, tensors, like=None):
     """Tensors [rows, ...] with a row in one piece, the same number of rows each."""
-    tensors = tuple(tensors)
+    import torch
+    tensors, forward = tuple(tensors), forward_mode()
     if not 1 <= len(tensors) <= _lib.MAX_ROW_ARRAYS:
         raise ValueError(f"{what}: 1 to {_lib.MAX_ROW_ARRAYS} {name}")
     n = tensors[0].shape[:1]
     for t in tensors:
         if not n or t.shape[:1] != n:
             raise ValueError(f"{what}: {name} must have the same number of rows")
-        if t.requires_grad:
+        if t.requires_grad or (forward and torch.autograd.forward_ad.unpack_dual(t).tangent is not None):
             raise ValueError(f"{what}: no gradient passes through moved rows (detach them)")
         if t.is_contiguous() and t.numel():
             continue

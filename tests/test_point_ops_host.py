@@ -154,3 +154,13 @@ def test_limits_refuse_without_a_gpu(pkg):
     assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG and b"heads" in lib.r3d_last_error()
     e = L.LinearCE(n=4, v=3, d=8, ld_x=1 << 31, ld_w=8, type=L.T_F32, target_type=L.T_I64, reduction=L.CE_MEAN)
     assert lib.r3d_linear_ce_bytes(C.byref(e), 0) == 0
+
+
+def test_rows_refuse_forward_mode(pkg):
+    import torch.autograd.forward_ad as fwd
+    s, x = torch.zeros(3, dtype=torch.int64), torch.zeros((5, 4))
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: pkg.take_rows(s, (dual,)), lambda: pkg.put_rows(s, (dual,), (x,)), lambda: pkg.put_rows(s, (x,), (dual,))):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
