@@ -169,6 +169,7 @@ def put_rows(slots, rows, dests, source_slots=None):
     tensors in one pass.  Nothing is written where either slot is outside (a map's -1): rows that no slot names stay as they
     were.  The slots must be distinct; which of two equal ones wins is not defined, nor is a row read that the same call writes.
     Returns dests."""
+    import torch
     what = "put_rows"
     _slots(what, "slots", slots)
     rows, dests = _rows_of(what, "rows", rows), _rows_of(what, "dests", dests)
@@ -187,6 +188,7 @@ def put_rows(slots, rows, dests, source_slots=None):
     with on_device_of(what, slots, *rows, *dests, *(() if source_slots is None else (source_slots,))):
         if n and rows[0].shape[0] and dests[0].shape[0]:
             _move(what, rows, dests, source_slots, slots, n)
+            torch.autograd.graph.increment_version(dests)      # (autograd sees a tensor that it has kept change)
     return dests
 
 

@@ -393,3 +393,23 @@ def test_slot_map_of_many_sequences_with_little_room(pkg, scenes, points, block,
             continue
         got = pkg.slot_map(i32(lengths), block, i32(tables), i32(rows), capacity)
         assert got.offsets.tolist() == offsets and got.slots.tolist() == slots[:capacity] and got.sequence.tolist() == seq[:capacity], capacity
+
+
+def test_put_rows_is_seen_by_autograd(pkg):
+    """A tensor that a backward pass has kept and that was written in the meantime: the pass raises, as for torch's own writes."""
+    x, s = torch.randn((5, 4), device="cuda"), torch.tensor([1, 0], device="cuda")
+    w = torch.ones((5, 4), device="cuda", requires_grad=True)
+    y = (w * x).sum()
+    before = x._version
+    pkg.put_rows(s, (torch.zeros((2, 4), device="cuda"),), (x[:3],))      # (a view of it)
+    assert x._version > before
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    y = (w * x).sum()
+    pkg.put_rows(s[:0], (torch.zeros((2, 4), device="cuda"),), (x,))      # nothing is written
+    y.backward()
+    assert torch.equal(w.grad, x)
+    with torch.inference_mode():
+        z = torch.zeros((5, 4), device="cuda")
+        pkg.put_rows(s, (x[:2],), (z,))
+    assert torch.equal(z[:2], x[[1, 0]])
