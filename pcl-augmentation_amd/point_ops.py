@@ -24,15 +24,18 @@ def _types():
 
 
 def on_device_of(what, *tensors):
-    """The device of these tensors made current (a null context where it is already); refuses tensors that are not on one GPU."""
+    """The device of these tensors made current (a null context where it is already); refuses tensors that are not on one GPU, or not in
+    memory as they read."""
     import torch
     index = tensors[0].get_device()
     if index < 0:
         _lib.require_gpu()
         raise _lib.R3DError(f"{what}: the tensors must be on a GPU, got {tensors[0].device}")
-    for t in tensors[1:]:
+    for t in tensors:
         if t.get_device() != index:
             raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+        if t.is_neg() or t.is_conj():      # (what stands in memory is not what the tensor reads as)
+            raise ValueError(f"{what}: a tensor that is negated or conjugated when it is read (resolve_neg, resolve_conj)")
     return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
@@ -96,8 +99,8 @@ def _turn(tensors, positions, sections, base, interleaved, backward):
         out = torch.empty_like(t, memory_format=torch.contiguous_format)
         outs.append(out)
         strides = t.stride()
-        if strides[2] != 1:
-            t = t.contiguous()
+        if strides[2] != 1 or t.is_neg():      # (a gradient may come in so)
+            t = t.resolve_neg().contiguous()
             kept.append(t)      # (until the launch)
             strides = t.stride()
         x[w], y[w], heads[w] = t.data_ptr(), out.data_ptr(), t.shape[1]
@@ -234,8 +237,8 @@ def _loss_function():
                     x, weight = (t.clone() if t.data_ptr() % 16 and not at % 16 else t for t, at in ((x, d.x), (weight, d.w)))
                     bias, target = None if bias is None else bias.contiguous(), target.contiguous()
                     follow(d, x, weight, bias, target, state)
-                if grad.dtype is not f32 or not grad.is_contiguous():
-                    grad = grad.to(f32).contiguous()
+                if grad.dtype is not f32 or not grad.is_contiguous() or grad.is_neg():
+                    grad = grad.to(f32).resolve_neg().contiguous()
                 d.grad = grad.data_ptr()
                 need_x, need_w, need_b, _, _ = ctx.needs_input_grad
                 dx = dw = db = None

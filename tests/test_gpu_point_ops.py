@@ -747,3 +747,25 @@ def test_gradients_refuse_forward_mode(pkg):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 torch.autograd.grad(out, leaf, fwd.make_dual(up, torch.ones_like(up)), retain_graph=True)
             assert torch.equal(torch.autograd.grad(out, leaf, up, retain_graph=True)[0], want)
+
+
+def test_tensors_that_are_negated_when_they_are_read(pkg):
+    """Views with the bit that torch resolves at the next read: refused as inputs, right as gradients."""
+    minus = torch._neg_view
+    q, pos = torch.randn((5, 2, 8)).cuda(), torch.randn((5, 1)).cuda()
+    x, w, t = torch.randn((5, 8)).cuda(), torch.randn((3, 8)).cuda(), torch.zeros(5, dtype=torch.int64).cuda()
+    rows, s = torch.randn((5, 4), dtype=torch.complex64).cuda(), torch.tensor([1, 0]).cuda()
+    for call in (lambda: pkg.rotary_positions(minus(q), pos, (4,)), lambda: pkg.rotary_positions(q, minus(pos), (4,)),
+                 lambda: pkg.rotary_positions(q, pos, (4,), key=minus(q)), lambda: pkg.linear_cross_entropy(minus(x), w, t),
+                 lambda: pkg.linear_cross_entropy(x, minus(w), t), lambda: pkg.linear_cross_entropy(x, w, t, bias=minus(w[:, 0].contiguous())),
+                 lambda: pkg.take_rows(s, (rows.conj(),)), lambda: pkg.put_rows(s, (rows[:2],), (rows.conj(),)),
+                 lambda: pkg.take_rows(s, (minus(x),)), lambda: pkg.put_rows(s, (minus(x),), (x.clone(),))):
+        with pytest.raises(ValueError, match="resolve"):
+            call()
+    assert torch.equal(pkg.take_rows(s, (rows.conj().resolve_conj(),))[0], rows.conj()[s])
+    q.requires_grad_()
+    x.requires_grad_()
+    for out, leaf in ((pkg.rotary_positions(q, pos, (4,))[0], q), (pkg.linear_cross_entropy(x, w, t, reduction="none"), x)):
+        up = torch.randn(out.shape).cuda()
+        one, two = (torch.autograd.grad(out, leaf, g, retain_graph=True)[0] for g in (minus(up), -up))
+        assert torch.equal(one, two)
