@@ -225,6 +225,7 @@ class ScenePool:
             i32 = dict(dtype=torch.int32, device=self.device)
             self.blocks = BlockTables(torch.full((max_scenes, most), -1, **i32), torch.zeros(max_scenes, **i32),
                                       torch.arange(n_blocks - 1, -1, -1, **i32), torch.full((1,), n_blocks, **i32), torch.zeros(1, **i32))
+            self._refused = torch.zeros(1, **i32)      # bits of every ``resize`` since ``raise_on_status`` last looked
 
     def _rows(self, scenes):
         import torch
@@ -251,6 +252,7 @@ class ScenePool:
         scene's first points are stays; new ones are whatever the page held."""
         b = self.blocks
         self.blocks = block_tables(lengths, self.block_size, b.tables, b.held, b.free_blocks, b.n_free)
+        self._refused.bitwise_or_(self.blocks.status)
 
     def check_scenes(self, scenes, n):
         """The distinct scene numbers of a batch of n (None: 0 .. n-1); raises where they are not that."""
@@ -299,7 +301,10 @@ class ScenePool:
         xyzi, label = take_rows(m.slots, (self.xyzi, self.label))
         return PackedScenes(xyzi, label, m.offsets, m.sequence, m.slots)
 
+    @_lib.on_own_device
     def raise_on_status(self):
-        """Waits for the device; raises where the last ``add`` / ``resize`` did not find room for a scene."""
-        if int(self.blocks.status.item()):
+        """Waits for the device; raises where any ``add`` / ``resize`` since the last call of this did not find room for a scene
+        (and forgets it: the next call asks about what comes after)."""
+        if int(self._refused.item()):
+            self._refused.zero_()
             raise _lib.R3DError("ScenePool: no room for a scene (out of pages, or more points than max_points)")

@@ -413,3 +413,22 @@ def test_put_rows_is_seen_by_autograd(pkg):
         z = torch.zeros((5, 4), device="cuda")
         pkg.put_rows(s, (x[:2],), (z,))
     assert torch.equal(z[:2], x[[1, 0]])
+
+
+def test_pool_remembers_a_scene_without_room(pkg, synth):
+    """One call that finds no room, then one that does: the status still tells, once."""
+    scenes, slots, need = _scenes(synth, 2)
+    pool = pkg.ScenePool(3, 8192, n_blocks=1 + 8192 // 512, block_size=512)
+    pool.resize(i32([8192, 512, 1]))
+    pool.resize(i32([8192, 512, 0]))
+    assert pool.lengths.tolist() == [8192, 512, 0] and pool.blocks.status.tolist() == [0]
+    with pytest.raises(pkg.R3DError, match="no room"):
+        pool.raise_on_status()
+    pool.raise_on_status()
+    pool.resize(i32([0, 0, 0]))
+    batch = {}
+    pkg.augment_batch(scenes, slots, need, reuse=batch, pool=pool)
+    pool.resize(i32([9000, 0, 0]))      # more than max_points
+    pool.add(batch[2], [1, 2])
+    with pytest.raises(pkg.R3DError, match="no room"):
+        pool.raise_on_status()
