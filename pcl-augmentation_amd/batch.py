@@ -632,7 +632,9 @@ def augment_batch(scenes, candidates, min_points, rows=_lib.NUMROW, cols=_lib.NU
     (results, accepted) with results as ``SceneBatch.results`` and accepted[s][k] = index of the
     accepted candidate or -1.  ``reuse``: optional dict in which the ``SceneBatch`` is kept between
     calls (keyed by B) instead of being allocated every time.  ``pool``: a ``ScenePool`` of the same GPU which takes the
-    finished scenes where they stand, as scenes ``pool_scenes`` (default 0 .. B-1); nothing is downloaded then, results is None.
+    finished scenes where they stand, as scenes ``pool_scenes`` (default 0 .. B-1); results is None then, and nothing is
+    downloaded.  Where the pool has no room for a scene (its ``raise_on_status`` tells too), results is a list with that
+    scene's clouds, so that none is lost, and None for those that the pool took.
     """
     B = len(scenes)
     if pool is not None and not level2_takes(rows, cols):
@@ -693,8 +695,11 @@ def augment_batch(scenes, candidates, min_points, rows=_lib.NUMROW, cols=_lib.NU
                 batch.replace_result(s, *results[s][:2])
         batch.last_level1 = SceneBatch.last_level1 = redo
     if pool is not None:
-        pool.add(batch, pool_scenes)
-        return None, accepted
+        taken = pool.add(batch, pool_scenes).cpu().numpy()
+        if taken.all():
+            return None, accepted
+        whole = batch.results()
+        return [None if t else r or w for t, r, w in zip(taken, results, whole)], accepted
     return results, accepted
 
 

@@ -432,3 +432,23 @@ def test_pool_remembers_a_scene_without_room(pkg, synth):
     pool.add(batch[2], [1, 2])
     with pytest.raises(pkg.R3DError, match="no room"):
         pool.raise_on_status()
+
+
+def _equal(a, b):
+    return all(p.dtype == q.dtype and p.shape == q.shape and p.tobytes() == q.tobytes() for p, q in zip(a, b)) and len(a) == len(b)
+
+
+def test_scenes_without_room_come_back(pkg, synth):
+    scenes, slots, need = _scenes(synth, 4)
+    want, acc = pkg.augment_batch(scenes, slots, need)
+    blocks = [-(-len(r[0]) // 128) for r in want]
+    pool = pkg.ScenePool(6, 128 * max(blocks), n_blocks=sum(blocks[:2]), block_size=128)
+    got, acc2 = pkg.augment_batch(scenes, slots, need, pool=pool, pool_scenes=[4, 1, 0, 5])
+    served = pool.lengths.tolist()      # rows in order: 0, 1, 4, 5
+    kept = [s for s, row in enumerate([4, 1, 0, 5]) if served[row]]
+    assert acc2 == acc and 0 < len(kept) < 4
+    for s in range(4):
+        assert got[s] is None if s in kept else _equal(got[s], want[s])
+    _same(pool, [[4, 1, 0, 5][s] for s in kept], [want[s] for s in kept])
+    with pytest.raises(pkg.R3DError):
+        pool.raise_on_status()
