@@ -640,7 +640,7 @@ def augment_batch(scenes, candidates, min_points, rows=_lib.NUMROW, cols=_lib.NU
     if pool is not None and not level2_takes(rows, cols):
         raise ValueError("augment_batch: a pool takes scenes from the batched path only, which this range image is not for")
     if pool is not None:
-        pool.check_scenes(pool_scenes, B)
+        pool_scenes = pool.check_scenes(pool_scenes, B)      # (a list from here on: an iterator ends at its first reading)
         pool.check_device(device)
     if not level2_takes(rows, cols):
         # a range image the batched kernels are not built for (columns that are no multiple of 32: the bit images are rows of

@@ -452,3 +452,11 @@ def test_scenes_without_room_come_back(pkg, synth):
     _same(pool, [[4, 1, 0, 5][s] for s in kept], [want[s] for s in kept])
     with pytest.raises(pkg.R3DError):
         pool.raise_on_status()
+
+
+def test_pool_scenes_from_an_iterator(pkg, synth):
+    scenes, slots, need = _scenes(synth, 3)
+    want, _ = pkg.augment_batch(scenes, slots, need)
+    pool = pkg.ScenePool(5, 8192, block_size=512)
+    assert pkg.augment_batch(scenes, slots, need, pool=pool, pool_scenes=(4 - s for s in range(3)))[0] is None
+    _same(pool, iter([4, 3, 2]), want)
