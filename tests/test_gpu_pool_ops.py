@@ -460,3 +460,33 @@ def test_pool_scenes_from_an_iterator(pkg, synth):
     pool = pkg.ScenePool(5, 8192, block_size=512)
     assert pkg.augment_batch(scenes, slots, need, pool=pool, pool_scenes=(4 - s for s in range(3)))[0] is None
     _same(pool, iter([4, 3, 2]), want)
+
+
+def test_pool_takes_a_frame_of_the_level1_kernels(pkg, synth):
+    """A sample of more points than the batched kernels take: its frame goes through the Level-1 kernels and from there into the pool."""
+    scenes, slots, need = _scenes(synth, 3)
+    slots[1][1] = [synth.make_insert(9199, "car", points=70000, centre_range=7.0, centre_az=0.7)]
+    want, acc = pkg.augment_batch(scenes, slots, need)
+    assert pkg.SceneBatch.last_level1 == [1]
+    pool = pkg.ScenePool(4, max(len(r[0]) for r in want), block_size=512)
+    none, acc2 = pkg.augment_batch(scenes, slots, need, pool=pool, pool_scenes=[3, 1, 0])
+    assert none is None and [list(a) for a in acc2] == [list(a) for a in acc] and pkg.SceneBatch.last_level1 == [1]
+    _same(pool, [3, 1, 0], want)
+    little = pkg.ScenePool(3, pool.max_points, n_blocks=-(-len(want[0][0]) // 512), block_size=512)
+    got, _ = pkg.augment_batch(scenes, slots, need, pool=little)
+    assert [g is None for g in got] == [n > 0 for n in little.lengths.tolist()] and got[1] is not None
+    assert all(g is None or _equal(g, w) for g, w in zip(got, want))
+
+
+def test_replaced_result_refuses(pkg, synth):
+    scenes, slots, need = _scenes(synth, 2)
+    reuse = {}
+    want, _ = pkg.augment_batch(scenes, slots, need, reuse=reuse)
+    batch = reuse[2]
+    batch.replace_result(0, want[1][0], want[1][1])
+    again = batch.results()
+    assert again[0][0].tobytes() == want[1][0].tobytes() and again[0][1].tobytes() == want[1][1].tobytes() and _equal(again[1], want[1])
+    with pytest.raises(ValueError):
+        batch.replace_result(0, want[1][0], want[1][1][:-1])
+    with pytest.raises(ValueError):
+        batch.replace_result(0, np.zeros((batch.cap + 1, 4), np.float32), np.zeros(batch.cap + 1, np.uint32))
