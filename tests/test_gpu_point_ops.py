@@ -769,3 +769,23 @@ def test_tensors_that_are_negated_when_they_are_read(pkg):
         up = torch.randn(out.shape).cuda()
         one, two = (torch.autograd.grad(out, leaf, g, retain_graph=True)[0] for g in (minus(up), -up))
         assert torch.equal(one, two)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rotary_positions_that_were_kept_elsewhere(pkg, dtype):
+    g = gen(3)
+    pos = torch.randn((40, 4), generator=g).cuda() * 20
+    up = torch.randn((40, 3, 24), generator=g).to(dtype).cuda()
+
+    def step(back=None):
+        q = torch.ones((40, 3, 24), dtype=dtype, device="cuda", requires_grad=True)
+        if back is None:
+            y, _ = pkg.rotary_positions(q, pos[:, :3], (4, 4, 3))
+        else:
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+                y, _ = pkg.rotary_positions(q, pos[:, :3], (4, 4, 3))
+        return torch.autograd.grad(y, q, up)[0]
+
+    want = step()
+    for back in (lambda t: t.t().contiguous().t(), lambda t: t.clone(), lambda t: t.cpu().cuda()):
+        assert torch.equal(step(back), want)
