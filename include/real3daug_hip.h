@@ -686,8 +686,14 @@ int r3d_rotary(const r3d_rotary_t *d, void *stream);
  * loss NaN.  loss: float [n] (R3D_CE_NONE) or [1] (sum, mean over the points that count; 0 where none does).
  * The forward call fills `state` (R3D_CE_BYTES_STATE bytes: which points count, their statistics, what had to be packed), which
  * the backward call of the same descriptor reads and leaves as it is.  backward: grad = float [n] or [1]; dx [n][d], dw [v][d],
- * db [v] dense, of `type`, each nullable.  piece: classes whose logit gradients are held at a time (0: as many as 512 MB take;
- * with at most 128 features none are).
+ * db [v] dense, of `type`, each nullable.
+ * Memory.  The backward workspace holds the logit gradients of `piece` classes at a time, 2 bytes a point and class (float32: 6), 128
+ * classes at least; piece 0: what 512 MB take, 256 classes at least.  (A head that stands in LDS holds as many bytes, of all
+ * its classes and fewer points.  With few classes, or at most 64 features, none are held; with 65 to 128 features only of such a head.)
+ * Beside them 32-bit sums of dx and dw where they are made in parts: 4 bytes a value, and up to 256 MB each where they are split over
+ * workgroups.  The state holds, where few points and classes do not make all of this unnecessary, 16 bytes a point and a
+ * copy of x and w that is padded and, for float32, split: 6 bytes a value of float32, 2 of the others where rows are not whole
+ * multiples of 64 features and 16 bytes.
  * r3d_linear_ce_bytes: of the state and of the two calls' workspaces, for the descriptor as it will be passed (0: bad descriptor). */
 #define R3D_CE_NONE 0
 #define R3D_CE_SUM 1

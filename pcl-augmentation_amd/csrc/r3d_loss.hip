@@ -589,6 +589,7 @@ struct OutArgs {
   int64_t m, n, kb;                      // m: rows of the result, n: columns that are written
   int64_t limit_a, limit_b, rows_b;      // columns of the operands, rows of b
   int32_t points;                        // 0: m and the rest as given; 1: m is the points that count; 2: k is
+  int32_t first, most;                   // 2: of those, `most` from number `first` on
   int32_t mtiles, ntiles, splits, add;
   const Counted *counted;
   float *out;                            // [splits][m_pad][ld], or null:
@@ -604,7 +605,7 @@ struct OutArgs {
 template <class V, class T, class S, Lies LA>
 __global__ __launch_bounds__(S::threads, 2) void k_ce_out(OutArgs a) {
   __shared__ __attribute__((aligned(128))) T lds[S::buffers * S::buffer];
-  const int nc = a.counted->n;
+  const int nc = a.points == 2 ? min(max(a.counted->n - a.first, 0), a.most) : a.counted->n;
   const int64_t id = xcd_order(blockIdx.x, gridDim.x), tiles = (int64_t)a.mtiles * a.ntiles;
   const int split = (int)(id / tiles);
   int64_t mt, nt;
@@ -742,8 +743,9 @@ struct HeadArgs {
   int64_t v, d;
   int32_t dp;
   const float *bias2;
-  const int32_t *tgt, *idx;
+  const int32_t *tgt, *idx;          // (these, and the points' other arrays, from number `first` on)
   const Counted *counted;
+  int32_t first, most;               // the points of this launch: of those that count, `most` from number `first` on
   float *part_m, *part_l, *hit;      // forward
   // backward
   const float *lse2, *weight, *scale;
@@ -763,8 +765,8 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
   T *ws = reinterpret_cast<T *>(smem);
   float *bias2 = reinterpret_cast<float *>(ws + kVB * 32 * pitch);
   const int lane = threadIdx.x & 63, half = lane >> 5, low = lane & 31, group = lane >> 4, sub = lane & 15;
-  const int nc = a.counted->n, cols = a.dp / 8;
-  if (blockIdx.x * 32 >= nc) {
+  const int nc = min(max(a.counted->n - a.first, 0), a.most), cols = a.dp / 8;
+  if ((int)blockIdx.x * 32 >= nc) {
     if (kGrad && a.sums)
       for (int c = threadIdx.x; c < kVB * 32; c += kHeadThreads) a.sums[(int64_t)blockIdx.x * kVB * 32 + c] = 0.0f;
     return;
@@ -996,6 +998,7 @@ struct Plan {
   bool narrow;      // dl stays in registers (r3d_loss_narrow.hip)
   int lse_splits, dx_splits, dw_splits, db_parts, top_parts, groups;
   int head;                     // blocks of 32 classes of a head that fits LDS, or 0
+  int64_t head_points, head_ranges, dl_rows;      // its points whose dl is held at a time; rows of dl
   size_t head_lds;
   bool dx_final, dw_final;      // nothing to add: straight into the result
   // kept from the forward to the backward pass
@@ -1013,6 +1016,7 @@ struct Plan {
   size_t bytes;
 };
 
+int64_t head_groups(int64_t points) { return up(points, 32) / 32 < kCus ? up(points, 32) / 32 : kCus; }
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
@@ -1080,20 +1084,28 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
     p.piece = piece < v64 ? piece : v64;
     if (d.piece == 0) p.piece = up((v64 + (v64 + p.piece - 1) / p.piece - 1) / ((v64 + p.piece - 1) / p.piece), Big::BM);      // pieces of one size
     if (p.piece > v64 || p.head) p.piece = v64;
+    // A head in LDS takes all classes at a time, so it is its points that are cut where dl is too much, into what a piece takes.
+    p.dl_rows = p.head_points = p.n_pad;
+    if (p.head && d.dw) {
+      const int64_t bytes = d.piece > 0 && d.piece < d.v ? p.n_pad * up(d.piece, kPadK) * 2 : kPieceBytes;
+      const int64_t rows = bytes / (v64 * 2) / Big::BN * Big::BN;
+      p.dl_rows = p.head_points = rows < Big::BN ? Big::BN : rows < p.n_pad ? rows : p.n_pad;
+    }
+    p.head_ranges = (d.n + p.head_points - 1) / p.head_points;
     p.dl_big = p.planes == 1 && large_tiles(p.piece, d.n, 1);
-    const int64_t kx = p.piece / 256, kw = p.n_pad / 256;
+    const int64_t kx = p.piece / 256, kw = p.dl_rows / 256;
     p.dx_big = p.planes == 1 && large_tiles(d.n, p.dp, kx);
     p.dw_big = p.planes == 1 && large_tiles(p.piece, p.dp, kw);
     auto tiles = [&](int64_t m, int64_t n, bool big) { return big ? tiles_of(m, n, Big::BM, Big::BN) : tiles_of(m, n, Small::BM, Small::BN); };
     p.dx_splits = cut(tiles(d.n, p.dp, p.dx_big), kCus * (p.dx_big ? Big::per_cu : Small::per_cu), kx);
     p.dw_splits = cut(tiles(p.piece, p.dp, p.dw_big), kCus * (p.dw_big ? Big::per_cu : Small::per_cu), kw);
     p.dx_final = p.head || (p.dx_splits == 1 && p.piece >= d.v);
-    p.dw_final = p.dw_splits == 1;
-    p.dl = c.take<uint16_t>((size_t)p.planes * p.n_pad * p.piece);
+    p.dw_final = p.dw_splits == 1 && p.head_ranges == 1;
+    p.dl = c.take<uint16_t>(p.head && !d.dw ? 0 : (size_t)p.planes * p.dl_rows * p.piece);
     if (!p.dx_final) p.accx = c.take<float>((size_t)p.dx_splits * p.n_pad * p.dp);
     p.accw = c.take<float>((size_t)(p.dw_final || !d.dw ? 0 : p.dw_splits) * p.piece * p.dp);
     // db: a part for every tile of points (the tiles of dl) or every workgroup of a head in LDS
-    p.db_parts = p.head ? (int)(up(d.n, 32) / 32 < kCus ? up(d.n, 32) / 32 : kCus) : (int)(up(d.n, p.dl_big ? Big::BN : Small::BN) / (p.dl_big ? Big::BN : Small::BN));
+    p.db_parts = p.head ? (int)(p.head_ranges * head_groups(d.n < p.head_points ? d.n : p.head_points)) : (int)(up(d.n, p.dl_big ? Big::BN : Small::BN) / (p.dl_big ? Big::BN : Small::BN));
     p.accb = c.take<float>((size_t)p.db_parts * p.piece);
   }
   p.bytes = c.off;
@@ -1158,6 +1170,7 @@ HeadArgs head_args(const r3d_linear_ce_t &d, const Plan &p) {
   a.tgt = p.tgt;
   a.idx = p.idx;
   a.counted = p.counted;
+  a.most = (int32_t)d.n;
   a.part_m = p.part_m;
   a.part_l = p.part_l;
   a.hit = p.hit;
@@ -1172,12 +1185,11 @@ HeadArgs head_args(const r3d_linear_ce_t &d, const Plan &p) {
 }
 
 template <class T, bool kGrad>
-int head(const HeadArgs &a, const Plan &p, int64_t n, hipStream_t st) {
-  const int64_t tiles = (n + 31) / 32;
+int head(const HeadArgs &a, const Plan &p, int64_t points, hipStream_t st) {
   auto run = [&](auto *kernel) {
     if (p.head_lds > 64 * 1024)
       R3D_HIP(hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)p.head_lds));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles < kCus ? tiles : kCus)), dim3(kHeadThreads), p.head_lds, st, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)head_groups(points)), dim3(kHeadThreads), p.head_lds, st, a);
     return R3D_OK;
   };
   switch (p.head) {
@@ -1292,6 +1304,55 @@ void finish(const Finish *of, int n, const Plan &p, float unheld, hipStream_t st
   if (n) hipLaunchKernelGGL(k_ce_finish<V>, dim3(blocks_for(most, 256, 8192), n), dim3(256), 0, st, a);
 }
 
+// A head in LDS: head_points of the points at a time, dx from the kernel itself, dW added up over them.
+template <class S, class T>
+void backward_head(const r3d_linear_ce_t &d, const Plan &p, Operand x, float held, hipStream_t st) {
+  const int64_t each = d.n < p.head_points ? d.n : p.head_points, classes = up(d.v, 32);
+  const Operand dl{p.dl, p.dl_rows, 0, nullptr};
+  const float unheld = 1.0f / held;
+  for (int64_t first = 0; first < d.n; first += each) {
+    HeadArgs ha = head_args(d, p);
+    ha.first = (int32_t)first;
+    ha.most = (int32_t)(d.n - first < each ? d.n - first : each);
+    ha.idx += first;
+    ha.tgt += first;
+    ha.lse2 += first;
+    ha.weight += first;
+    ha.held = held;
+    ha.unheld = unheld;
+    ha.n_pad = p.dl_rows;
+    if (!d.dw) ha.dl = nullptr;
+    ha.sums = d.db ? p.accb + first / each * head_groups(each) * classes : nullptr;
+    head<T, true>(ha, p, each, st);
+    if (!d.dw) continue;
+    OutArgs oa{};
+    oa.p = Product{dl, x};
+    oa.p.b.idx += first;
+    oa.m = p.dw_final ? d.v : p.piece;
+    oa.n = p.dw_final ? d.d : p.dp;
+    oa.limit_a = p.piece;
+    oa.limit_b = p.dp;
+    oa.points = 2;
+    oa.first = ha.first;
+    oa.most = ha.most;
+    oa.splits = p.dw_splits;
+    oa.add = first > 0;
+    oa.counted = p.counted;
+    oa.out = p.accw;
+    oa.ld = p.dw_final ? d.d : p.dp;
+    oa.split_stride = p.piece * p.dp;
+    oa.final_out = p.dw_final ? d.dw : nullptr;
+    oa.scale = p.scale;
+    oa.unheld = unheld;
+    with_shape<1>(p.dw_big, [&](auto shape) { out_product<S, T, decltype(shape), Lies::PiecesCols>(oa, p.piece, p.dp, st); });
+  }
+  Finish of[2];
+  int n_of = 0;
+  if (d.dw && !p.dw_final) of[n_of++] = finish_of<S>(p.accw, p.dp, p.piece * p.dp, d.v, d.d, p.dw_splits, nullptr, d.dw);
+  if (d.db) of[n_of++] = finish_of<S>(p.accb, classes, classes, 1, d.v, p.db_parts, nullptr, d.db);
+  finish<S>(of, n_of, p, unheld, st);
+}
+
 template <class S, class T, int kPlanes>
 void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   const bool each = d.reduction == R3D_CE_NONE;
@@ -1349,6 +1410,10 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     finish<S>(of, n_of, p, unheld, st);
     return;
   }
+  if (p.head) {
+    if constexpr (kPlanes == 1) backward_head<S, T>(d, p, x, held, st);
+    return;
+  }
   for (int64_t v0 = 0; v0 < d.v; v0 += p.piece) {
     const int64_t real_v = p.piece < d.v - v0 ? p.piece : d.v - v0, width = up(real_v, kPadK);
     Finish of[3];
@@ -1370,20 +1435,9 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     da.dl = p.dl;
     da.sums = d.db ? p.accb : nullptr;
     da.piece = p.piece;
-    if (p.head) {
-      if constexpr (kPlanes == 1) {
-        HeadArgs ha = head_args(d, p);
-        ha.held = held;
-        ha.unheld = unheld;
-        if (!d.dw) ha.dl = nullptr;
-        ha.sums = d.db ? p.accb : nullptr;
-        head<T, true>(ha, p, d.n, st);
-      }
-    } else {
-      with_shape<kPlanes>(p.dl_big, [&](auto shape) { dl_piece<T, decltype(shape), kPlanes>(da, d.n, st); });
-    }
+    with_shape<kPlanes>(p.dl_big, [&](auto shape) { dl_piece<T, decltype(shape), kPlanes>(da, d.n, st); });
     const Operand dl{p.dl, p.n_pad, p.n_pad * p.piece, nullptr};
-    if (d.dx && !p.head) {
+    if (d.dx) {
       Operand wv = w;      // the rows of this piece
       wv.p = static_cast<const char *>(w.p) + v0 * w.ld * 2;
       OutArgs oa{};
@@ -1415,6 +1469,7 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       oa.limit_a = width;
       oa.limit_b = p.dp;
       oa.points = 2;
+      oa.most = (int32_t)d.n;
       oa.splits = p.dw_splits;
       oa.counted = p.counted;
       oa.out = p.accw;
@@ -1427,10 +1482,7 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       if (!straight)
         of[n_of++] = finish_of<S>(p.accw, p.dp, p.piece * p.dp, real_v, d.d, p.dw_splits, nullptr, static_cast<char *>(d.dw) + v0 * d.d * p.type_bytes);
     }
-    if (d.db) {
-      const int64_t stride = p.head ? up(d.v, 32) : p.piece;
-      of[n_of++] = finish_of<S>(p.accb, stride, stride, 1, real_v, p.db_parts, nullptr, static_cast<char *>(d.db) + v0 * p.type_bytes);
-    }
+    if (d.db) of[n_of++] = finish_of<S>(p.accb, p.piece, p.piece, 1, real_v, p.db_parts, nullptr, static_cast<char *>(d.db) + v0 * p.type_bytes);
     finish<S>(of, n_of, p, unheld, st);
   }
 }

@@ -269,8 +269,12 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
 
     Points whose target is ``ignore_index`` have loss and gradient 0, whatever their features are; a target that is no class makes
     the loss NaN.  reduction: "mean" over the points that count (0 where none does), "sum" or "none" ([...]); the loss is
-    float32.  Differentiable once in x, weight and bias (forward mode raises); the backward pass makes the logits' gradients ``piece`` classes at a time
-    (0: as many as 512 MB hold; with at most 128 features none are held).  The same inputs give the same bits."""
+    float32.  Differentiable once in x, weight and bias (forward mode raises).  The same inputs give the same bits.
+
+    Memory beside inputs, outputs and gradients: the backward pass holds the logits' gradients of ``piece`` classes at a time, 2 bytes
+    a point and class (float32: 6), at least 128 classes; 0: what 512 MB take, at least 256 classes (none with few classes or few
+    features), and 32-bit sums of dx and dweight where they are made in parts.  From forward to backward it keeps 16 bytes a
+    point and, for float32 and for rows that are no multiples of 64 features, a packed copy of x and weight (6 and 2 bytes a value)."""
     import torch
     shape, dtype, wide = x.shape, x.dtype, weight.shape
     if len(shape) < 1 or len(wide) != 2 or shape[-1] != wide[1] or wide[0] < 1 or wide[1] < 1:

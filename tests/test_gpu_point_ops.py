@@ -789,3 +789,25 @@ def test_rotary_positions_that_were_kept_elsewhere(pkg, dtype):
     want = step()
     for back in (lambda t: t.t().contiguous().t(), lambda t: t.clone(), lambda t: t.cpu().cuda()):
         assert torch.equal(step(back), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,v,d", [(3001, 260, 128), (2500, 150, 192), (1030, 288, 96), (700, 130, 256)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_loss_of_a_head_in_lds_by_points(pkg, dtype, n, v, d, reduction):
+    """Heads whose points are cut so that the gradients of `piece` classes are held at a time: the same as without, but for the order
+    in which dweight is added up; dx of a point does not depend on it."""
+    whole = check_loss(pkg, n, v, d, dtype, reduction=reduction, share=0.3)
+    for piece in (1, 128, 192):
+        loss, got = check_loss(pkg, n, v, d, dtype, reduction=reduction, share=0.3, piece=piece)
+        assert torch.equal(loss, whole[0]) and torch.equal(got[0], whole[1][0])
+
+
+def test_loss_of_a_head_in_lds_by_points_where_some_parts_count_nothing(pkg):
+    """The points that count are in front of the line: the launches behind have none."""
+    g = gen(2)
+    n, v, d = 4000, 260, 128
+    for counted in (0, 1, 256, 700):
+        target = torch.full((n,), -100)
+        target[torch.randperm(n, generator=g)[:counted]] = torch.randint(0, v, (counted,), generator=g)
+        check_loss(pkg, n, v, d, BF16, target=target, piece=64)

@@ -164,3 +164,42 @@ def test_rows_refuse_forward_mode(pkg):
         for call in (lambda: pkg.take_rows(s, (dual,)), lambda: pkg.put_rows(s, (dual,), (x,)), lambda: pkg.put_rows(s, (x,), (dual,))):
             with pytest.raises(ValueError, match="gradient"):
                 call()
+
+
+def _ce_bytes(pkg, n, v, d, kind, piece, which, **more):
+    L, p = pkg._lib, 1 << 12
+    e = L.LinearCE(x=p, w=p, target=p, bias=p, n=n, v=v, d=d, ld_x=d, ld_w=d, type=kind, target_type=L.T_I64, reduction=L.CE_NONE, piece=piece,
+                   **{**dict(dx=p, dw=p, db=p), **more})
+    size = pkg._lib.load().r3d_linear_ce_bytes(C.byref(e), which)
+    assert size > 0
+    return size
+
+
+@pytest.mark.parametrize("n,v,d", [(9_000_000, 256, 256), (9_000_000, 288, 96), (838_000, 260, 256), (845_000, 260, 256), (2_000_000, 200, 250), (3001, 260, 128),
+                                   (1_500_000, 5000, 256), (2_500_000, 5000, 160), (8192, 161280, 512), (200, 777, 160), (700, 900, 200), (20, 30000, 300),
+                                   (480_000, 20, 96), (5_000_000, 20, 256), (400_000, 3000, 64), (24, 38322, 100), (100_000, 128, 640)])
+def test_loss_holds_no_more_than_it_says(pkg, n, v, d):
+    L, mb = pkg._lib, 2 ** 20
+    up = lambda a, b: -(-a // b) * b  # noqa: E731
+    rows, width, classes = up(n, 256), up(d, 64), up(v, 256)
+    for kind, planes in ((L.T_F32, 3), (L.T_BF16, 1), (L.T_F16, 1)):
+        for piece in (0, 1, 128, 192, 1000):
+            held = rows * 2 * planes * (up(max(piece, 128), 64) if piece else 256)
+            held = max(held, 512 * mb if piece == 0 else 256 * 2 * 320)      # (of a head in LDS 256 points at least)
+            if piece == 0 and planes == 1 and v <= 288 and d <= 256:
+                held = 512 * mb      # (as such a head is cut by points, there is no least number of classes)
+            sums = 4 * width * (rows + classes) + 2 * 256 * mb
+            small = held // 32 + 16 * rows + 600 * 4 * classes + 64 * mb      # db's parts, the points' weights
+            assert _ce_bytes(pkg, n, v, d, kind, piece, L.CE_BYTES_BACKWARD) <= held + sums + small, (kind, piece)
+        packed = 0 if planes == 1 and d % 64 == 0 else 2 * planes * width * (n + v)
+        assert _ce_bytes(pkg, n, v, d, kind, 0, L.CE_BYTES_STATE) <= 16 * n + 4 * classes + packed + 4096, kind
+
+
+@pytest.mark.parametrize("n,v,d,kind", [(1_000_000, 260, 256, 1), (400_000, 288, 96, 2), (300_000, 5000, 256, 1), (100_000, 900, 200, 0)])
+def test_a_smaller_piece_holds_less(pkg, n, v, d, kind):
+    """(Which also says that these heads hold anything: the tests of pieces on the GPU are of the same ways.)"""
+    which = pkg._lib.CE_BYTES_BACKWARD
+    size = [_ce_bytes(pkg, n, v, d, kind, piece, which) for piece in (128, 256, 100000)]
+    rows = n * 2 * (3 if kind == 0 else 1)      # bytes of a class
+    assert size[0] < size[1] <= size[2] and size[1] - size[0] >= 100 * rows
+    assert _ce_bytes(pkg, n, 260, d, 1, 0, which, dw=0, dx=0) < rows * 260
