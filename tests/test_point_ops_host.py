@@ -186,9 +186,9 @@ def test_loss_holds_no_more_than_it_says(pkg, n, v, d):
         for piece in (0, 1, 128, 192, 1000):
             held = rows * 2 * planes * (up(max(piece, 128), 64) if piece else 256)
             held = max(held, 512 * mb if piece == 0 else 256 * 2 * 320)      # (of a head in LDS 256 points at least)
-            if piece == 0 and planes == 1 and v <= 288 and d <= 256:
-                held = 512 * mb      # (as such a head is cut by points, there is no least number of classes)
             sums = 4 * width * (rows + classes) + 2 * 256 * mb
+            if piece == 0 and planes == 1 and v <= 288 and 64 < d <= 256:      # (cut by points: no least number of classes, dx at once)
+                held, sums = 512 * mb, 4 * width * classes + 256 * mb
             small = held // 32 + 16 * rows + 600 * 4 * classes + 64 * mb      # db's parts, the points' weights
             assert _ce_bytes(pkg, n, v, d, kind, piece, L.CE_BYTES_BACKWARD) <= held + sums + small, (kind, piece)
         packed = 0 if planes == 1 and d % 64 == 0 else 2 * planes * width * (n + v)
