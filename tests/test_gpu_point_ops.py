@@ -811,3 +811,15 @@ def test_loss_of_a_head_in_lds_by_points_where_some_parts_count_nothing(pkg):
         target = torch.full((n,), -100)
         target[torch.randperm(n, generator=g)[:counted]] = torch.randint(0, v, (counted,), generator=g)
         check_loss(pkg, n, v, d, BF16, target=target, piece=64)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("piece", [1, 128, 192, 256, 100000])
+@pytest.mark.parametrize("n,v,d", [(200, 777, 160), (700, 900, 200), (300, 641, 130)])
+def test_loss_pieces_of_many_classes(pkg, dtype, piece, n, v, d):
+    """Heads whose gradients go through memory a piece of the classes at a time (more than 288 classes and 128 features): sums
+    that go on from piece to piece, pieces that end inside a tile, a short last one."""
+    for reduction in ("none", "mean"):
+        loss, got = check_loss(pkg, n, v, d, dtype, reduction=reduction, piece=piece)
+        again = check_loss(pkg, n, v, d, dtype, reduction=reduction, piece=piece)
+        assert torch.equal(loss, again[0]) and all(torch.equal(a, b) for a, b in zip(got, again[1]))

@@ -203,3 +203,11 @@ def test_a_smaller_piece_holds_less(pkg, n, v, d, kind):
     rows = n * 2 * (3 if kind == 0 else 1)      # bytes of a class
     assert size[0] < size[1] <= size[2] and size[1] - size[0] >= 100 * rows
     assert _ce_bytes(pkg, n, 260, d, 1, 0, which, dw=0, dx=0) < rows * 260
+
+
+@pytest.mark.parametrize("n,v,d", [(200, 777, 160), (700, 900, 200), (300, 641, 130)])
+def test_pieces_of_the_gpu_tests_are_pieces(pkg, n, v, d):
+    """The heads of test_loss_pieces_of_many_classes hold less with a smaller piece: they do go piece by piece."""
+    for kind in (0, 1, 2):
+        size = [_ce_bytes(pkg, n, v, d, kind, piece, pkg._lib.CE_BYTES_BACKWARD, dw=0, db=0) for piece in (1, 256, 100000)]
+        assert size[0] < size[1] < size[2]
