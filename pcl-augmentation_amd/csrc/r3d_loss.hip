@@ -1206,7 +1206,7 @@ int head(const HeadArgs &a, const Plan &p, int64_t points, hipStream_t st) {
 }
 
 template <class S, class T, int kPlanes>
-void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
+int forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   const bool mean = d.reduction == R3D_CE_MEAN;
   StartArgs sa{};
   sa.target = d.target;
@@ -1232,9 +1232,12 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   hipLaunchKernelGGL((k_ce_start<S, T, kPlanes>), dim3(sa.groups + sa.bias_blocks + sa.pack[0].blocks + sa.pack[1].blocks), dim3(kStartThreads), 0, st, sa);
   if (p.groups > 1) hipLaunchKernelGGL(k_ce_index, dim3(p.groups), dim3(kStartThreads), 0, st, sa);
   if (p.head) {
-    if constexpr (kPlanes == 1) head<T, false>(head_args(d, p), p, d.n, st);
+    if constexpr (kPlanes == 1) {
+      const int rc = head<T, false>(head_args(d, p), p, d.n, st);
+      if (rc != R3D_OK) return rc;
+    }
     join(d, p, st);
-    return;
+    return R3D_OK;
   }
   if (p.narrow) {
     NarrowArgs na{};
@@ -1252,7 +1255,7 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     na.hit = p.hit;
     narrow(Narrow::Lse, na, d.type, (int)p.dp, st);
     join(d, p, st);
-    return;
+    return R3D_OK;
   }
   LseArgs la{};
   operands(d, p, la.p.b, la.p.a);
@@ -1268,6 +1271,7 @@ void forward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   la.n_pad = p.n_pad;
   with_shape<kPlanes>(p.lse_big, [&](auto shape) { lse<T, decltype(shape), kPlanes>(la, p, d.n, d.v, st); });
   join(d, p, st);
+  return R3D_OK;
 }
 
 template <class T, class S, int kPlanes>
@@ -1306,7 +1310,7 @@ void finish(const Finish *of, int n, const Plan &p, float unheld, hipStream_t st
 
 // A head in LDS: head_points of the points at a time, dx from the kernel itself, dW added up over them.
 template <class S, class T>
-void backward_head(const r3d_linear_ce_t &d, const Plan &p, Operand x, float held, hipStream_t st) {
+int backward_head(const r3d_linear_ce_t &d, const Plan &p, Operand x, float held, hipStream_t st) {
   const int64_t each = d.n < p.head_points ? d.n : p.head_points, classes = up(d.v, 32);
   const Operand dl{p.dl, p.dl_rows, 0, nullptr};
   const float unheld = 1.0f / held;
@@ -1323,7 +1327,8 @@ void backward_head(const r3d_linear_ce_t &d, const Plan &p, Operand x, float hel
     ha.n_pad = p.dl_rows;
     if (!d.dw) ha.dl = nullptr;
     ha.sums = d.db ? p.accb + first / each * head_groups(each) * classes : nullptr;
-    head<T, true>(ha, p, each, st);
+    const int rc = head<T, true>(ha, p, each, st);
+    if (rc != R3D_OK) return rc;
     if (!d.dw) continue;
     OutArgs oa{};
     oa.p = Product{dl, x};
@@ -1351,10 +1356,11 @@ void backward_head(const r3d_linear_ce_t &d, const Plan &p, Operand x, float hel
   if (d.dw && !p.dw_final) of[n_of++] = finish_of<S>(p.accw, p.dp, p.piece * p.dp, d.v, d.d, p.dw_splits, nullptr, d.dw);
   if (d.db) of[n_of++] = finish_of<S>(p.accb, classes, classes, 1, d.v, p.db_parts, nullptr, d.db);
   finish<S>(of, n_of, p, unheld, st);
+  return R3D_OK;
 }
 
 template <class S, class T, int kPlanes>
-void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
+int backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
   const bool each = d.reduction == R3D_CE_NONE;
   const int parts = each && d.type == R3D_T_F16 ? p.top_parts : 0;
   if (parts) hipLaunchKernelGGL(k_ce_top, dim3(parts), dim3(256), 0, st, d.grad, d.n, p.place, p.top);
@@ -1408,11 +1414,10 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
       if (d.db) of[n_of++] = finish_of<S>(p.accb, p.piece, p.piece, 1, d.v, p.db_parts, nullptr, d.db);
     }
     finish<S>(of, n_of, p, unheld, st);
-    return;
+    return R3D_OK;
   }
-  if (p.head) {
-    if constexpr (kPlanes == 1) backward_head<S, T>(d, p, x, held, st);
-    return;
+  if constexpr (kPlanes == 1) {
+    if (p.head) return backward_head<S, T>(d, p, x, held, st);
   }
   for (int64_t v0 = 0; v0 < d.v; v0 += p.piece) {
     const int64_t real_v = p.piece < d.v - v0 ? p.piece : d.v - v0, width = up(real_v, kPadK);
@@ -1485,6 +1490,7 @@ void backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     if (d.db) of[n_of++] = finish_of<S>(p.accb, p.piece, p.piece, 1, real_v, p.db_parts, nullptr, static_cast<char *>(d.db) + v0 * p.type_bytes);
     finish<S>(of, n_of, p, unheld, st);
   }
+  return R3D_OK;
 }
 }  // namespace
 
@@ -1503,13 +1509,11 @@ extern "C" int r3d_linear_ce_forward(const r3d_linear_ce_t *d, void *workspace, 
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (few_takes(*d)) {
     rc = few_forward(*d, workspace, st);
-    if (rc != R3D_OK) return rc;
   } else {
     const Plan p = plan(*d, false, workspace);
-    if (d->type == R3D_T_F32) forward<float, __bf16, 3>(*d, p, st);
-    else if (d->type == R3D_T_BF16) forward<__bf16, __bf16, 1>(*d, p, st);
-    else forward<_Float16, _Float16, 1>(*d, p, st);
+    rc = d->type == R3D_T_F32 ? forward<float, __bf16, 3>(*d, p, st) : d->type == R3D_T_BF16 ? forward<__bf16, __bf16, 1>(*d, p, st) : forward<_Float16, _Float16, 1>(*d, p, st);
   }
+  if (rc != R3D_OK) return rc;
   R3D_LAUNCHED("linear_ce forward kernels");
   return R3D_OK;
 }
@@ -1522,13 +1526,11 @@ extern "C" int r3d_linear_ce_backward(const r3d_linear_ce_t *d, void *workspace,
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (few_takes(*d)) {
     rc = few_backward(*d, workspace, st);
-    if (rc != R3D_OK) return rc;
   } else {
     const Plan p = plan(*d, true, workspace);
-    if (d->type == R3D_T_F32) backward<float, __bf16, 3>(*d, p, st);
-    else if (d->type == R3D_T_BF16) backward<__bf16, __bf16, 1>(*d, p, st);
-    else backward<_Float16, _Float16, 1>(*d, p, st);
+    rc = d->type == R3D_T_F32 ? backward<float, __bf16, 3>(*d, p, st) : d->type == R3D_T_BF16 ? backward<__bf16, __bf16, 1>(*d, p, st) : backward<_Float16, _Float16, 1>(*d, p, st);
   }
+  if (rc != R3D_OK) return rc;
   R3D_LAUNCHED("linear_ce backward kernels");
   return R3D_OK;
 }

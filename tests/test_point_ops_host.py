@@ -211,3 +211,13 @@ def test_pieces_of_the_gpu_tests_are_pieces(pkg, n, v, d):
     for kind in (0, 1, 2):
         size = [_ce_bytes(pkg, n, v, d, kind, piece, pkg._lib.CE_BYTES_BACKWARD, dw=0, db=0) for piece in (1, 256, 100000)]
         assert size[0] < size[1] < size[2]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that no GPU may be given")
+def test_loss_stops_at_the_first_call_that_fails(pkg):
+    """A head that takes more LDS than a kernel may without asking: without a GPU the question fails, and nothing goes on."""
+    L, lib, p = pkg._lib, pkg._lib.load(), 1 << 12
+    e = L.LinearCE(x=p, w=p, target=p, bias=p, n=1000, v=260, d=256, ld_x=256, ld_w=256, type=L.T_BF16, target_type=L.T_I64, reduction=L.CE_MEAN, state=p,
+                   loss=p, grad=p, dx=p, dw=p, db=p)
+    for call in (lib.r3d_linear_ce_forward, lib.r3d_linear_ce_backward):
+        assert call(C.byref(e), p, 1 << 40, None) == L.E_HIP and b"hipFuncSetAttribute" in lib.r3d_last_error()
