@@ -186,34 +186,6 @@ __device__ __forceinline__ bool inside_box(const double *R, const double *up, co
   return in;
 }
 
-// Diagnostic builds (-DR3D_GUARD, tools/build_flavour.sh guard -DR3D_GUARD): a kernel that is about to follow the pointers of
-// a query descriptor looks at them first; one that cannot be a device address is printed with the head of the descriptor
-// and the workgroup leaves (a descriptor overwritten by a stray store shows up as a line of text, not as a queue abort).
-#ifdef R3D_GUARD
-__device__ __forceinline__ bool odd_pointer(const void *p, bool nullable = false, unsigned long long align = 4) {
-  const unsigned long long a = (unsigned long long)p;
-  if (!a) return !nullable;
-  return a < (1ull << 20) || a >= (1ull << 48) || (a & (align - 1ull));
-}
-__device__ __noinline__ bool odd_query(const r3d_place_query_t *Q, int q, int kernel, bool say) {
-  const r3d_place_query_t &d = Q[q];
-  const bool bad = odd_pointer(d.scene) || odd_pointer(d.orig) || odd_pointer(d.boxes, true) || odd_pointer(d.sample) ||
-                   odd_pointer(d.map, false, 1) || odd_pointer(d.scene_ranges, true) || odd_pointer(d.orig_ranges, true) ||
-                   d.scene_ld != 4 || d.orig_ld != 4 || d.n_scene < 0 || d.n_scene > (1 << 24) || d.n_orig < 0 ||
-                   d.n_orig > (1 << 24) || d.m <= 0 || d.m > 8192 || d.n_boxes < 0 || d.n_boxes > 4096;
-  if (bad && say) {
-    const unsigned long long *u = reinterpret_cast<const unsigned long long *>(&d);
-    printf("R3D_GUARD kernel %d query %d at %p: %016llx %016llx %016llx %016llx %016llx %016llx %016llx | n %lld %lld ld %d %d m %d boxes %d | "
-           "tail %016llx %016llx %016llx\n", kernel, q, (const void *)&d, u[0], u[1], u[2], u[3], u[4], u[5], u[6], (long long)d.n_scene,
-           (long long)d.n_orig, d.scene_ld, d.orig_ld, d.m, d.n_boxes, u[56], u[60], u[62]);
-  }
-  return bad;
-}
-#define R3D_GUARD_QUERY(kernel, say) if (odd_query(Q, q, kernel, say)) return
-#else
-#define R3D_GUARD_QUERY(kernel, say)
-#endif
-
 // What k_place_centres looks at before any kernel follows a descriptor's pointers: a descriptor that was never filled, was
 // filled for another layout of the struct or has been overwritten shows up as R3D_PS_BAD_DESCRIPTOR in the query's status
 // (no placements), not as a fault of the queue.
@@ -320,7 +292,6 @@ __global__ void k_place_boxes(const r3d_place_query_t *Q, int nq, int max_boxes,
   if (t >= nq * max_boxes) return;
   int q = t / max_boxes, j = t % max_boxes;
   if (w.bad[q]) return;
-  R3D_GUARD_QUERY(__LINE__, j == 0);
   const r3d_place_query_t &qq = Q[q];
   if (j >= qq.n_boxes) return;
   const double *b = qq.boxes + (size_t)j * 10;
@@ -525,7 +496,6 @@ __global__ __launch_bounds__(kPB) void k_place_road_min(const r3d_place_query_t 
                                                         double resolved_sq) {
   const int q = blockIdx.x, tid = threadIdx.x;        // queries of one scene are neighbours: they share the chunk in L2
   if (w.bad[q]) return;
-  R3D_GUARD_QUERY(__LINE__, threadIdx.x == 0 && blockIdx.y == 0);
   const int64_t n = Q[q].n_orig, start0 = (int64_t)blockIdx.y * kPointsPerBlock * kTurns;
   if (start0 >= n) return;
   __shared__ r3d_place_query_t qq;
@@ -648,7 +618,6 @@ __device__ __forceinline__ int last_bit_exponent(double v) {
 __global__ __launch_bounds__(kPB) void k_place_surface_gather(const r3d_place_query_t *Q, PlaceWs w, Radii rad) {
   const int q = blockIdx.x, tid = threadIdx.x;        // queries of one scene are neighbours: they share the chunk in L2
   if (w.bad[q]) return;
-  R3D_GUARD_QUERY(__LINE__, threadIdx.x == 0 && blockIdx.y == 0);
   const int64_t n = Q[q].n_orig, start0 = (int64_t)blockIdx.y * kPointsPerBlock * kTurns;
   if (start0 >= n) return;
   const double reach_sq = key_depth(w.gather_sq[q]);
@@ -785,7 +754,6 @@ __global__ __launch_bounds__(kPB) void k_place_road_level(const r3d_place_query_
 __global__ __launch_bounds__(kPB) void k_place_scene_in_box(const r3d_place_query_t *Q, PlaceWs w) {
   const int q = blockIdx.x, tid = threadIdx.x;
   if (w.bad[q]) return;
-  R3D_GUARD_QUERY(__LINE__, threadIdx.x == 0 && blockIdx.y == 0);
   const int64_t n = Q[q].n_scene, start0 = (int64_t)blockIdx.y * kPointsPerBlock * kTurns;
   if (start0 >= n) return;
   __shared__ r3d_place_query_t qq;
@@ -927,7 +895,6 @@ __device__ __forceinline__ void sample_chain(ChainLds &lds, const r3d_place_quer
                                              uint8_t *flags, int32_t *n_possible, int32_t *rot_out,
                                              double *anno_out, double *cand, int32_t first_cand, int32_t *status) {
   const int q = blockIdx.x, tid = threadIdx.x;
-  R3D_GUARD_QUERY(__LINE__, threadIdx.x == 0);
   const r3d_place_query_t &qq = Q[q];
   const int m = qq.m;
   uint32_t *s_allowed = lds.allowed;
