@@ -2,6 +2,7 @@
 import ctypes
 import os
 import re
+import subprocess
 
 import pytest
 
@@ -97,3 +98,13 @@ def test_no_cpu_fallback(pkg):
         pkg.Real3DAug.insertion.add_space_for_spherical(np.zeros((4, 5)))
     with pytest.raises(pkg.R3DError):
         pkg.SceneBatch(1, 16, 16)
+
+
+def test_flavours_are_built_of_every_source():
+    """tools/build_flavour.sh takes its sources and flags from the Makefile, and the Makefile every source that is there."""
+    csrc = os.path.join(ROOT, "pcl-augmentation_amd", "csrc")
+    there = sorted(f for f in os.listdir(csrc) if f.endswith((".hip", ".cpp")))
+    run = lambda *a: subprocess.run(a, capture_output=True, text=True, check=True).stdout  # noqa: E731
+    assert sorted(run("make", "-s", "-C", csrc, "print-SRCS").split()) == there
+    assert sorted(run("bash", os.path.join(ROOT, "tools", "build_flavour.sh"), "--sources").split()) == there
+    assert "-packed-fp32-ops" in run("make", "-s", "-C", csrc, "print-HIPFLAGS").split()

@@ -5,25 +5,28 @@
 # compile job is waited for by its own PID (a failed job fails the script, it does not surface as a link error), and
 # r3d_level1 gets the same R3D_SRC_HASH csrc/Makefile passes, so that r3d_build_info() of the flavour names the sources it
 # was built from (__graft_entry__.build() compares it with the tree when the flavour is loaded through R3D_LIB).
+# Sources, headers and flags are the Makefile's; `tools/build_flavour.sh --sources` lists the sources.
 set -e
-name=$1; shift
 cd "$(dirname "$0")/../pcl-augmentation_amd/csrc"
-SRCS="r3d_level1.hip r3d_batch.hip r3d_insert.hip r3d_places.hip r3d_richmap.hip r3d_hostpack.cpp"
-HDRS="r3d_device.hpp r3d_host.hpp r3d_batch.hpp r3d_insert_core.hpp ../../include/real3daug_hip.h"
-HASH=$(cat $SRCS $HDRS | sha256sum | cut -c1-16)
+SRCS=$(make -s print-SRCS)
+if [ "$1" = --sources ]; then echo $SRCS; exit 0; fi
+name=$1; shift
+HASH=$(make -s print-SRC_HASH)
+HIPFLAGS=$(make -s print-HIPFLAGS)
+INSERT_FLAGS=$(make -s print-INSERT_FLAGS)
 T=$(mktemp -d)
 trap 'rm -rf "$T"' EXIT
-FLAGS="--offload-arch=gfx950 -O3 -ffp-contract=off -fPIC -std=c++17 -Wno-unused-function -Wno-pass-failed"
 pids=()
-for f in r3d_level1 r3d_batch r3d_insert r3d_places r3d_richmap; do
+for f in $SRCS; do
   extra=()
-  [ $f = r3d_insert ] && extra=(-mllvm -disable-machine-licm)
-  [ $f = r3d_level1 ] && extra=("-DR3D_SRC_HASH=\"$HASH\"")
-  hipcc $FLAGS "$@" "${extra[@]}" -c $f.hip -o $T/$f.o &
+  [ $f = r3d_insert.hip ] && extra=($INSERT_FLAGS)
+  [ $f = r3d_level1.hip ] && extra=("-DR3D_SRC_HASH=\"$HASH\"")
+  case $f in
+    *.cpp) hipcc $(make -s print-FLAGS) -c $f -o $T/${f%.*}.o & ;;
+    *) hipcc $HIPFLAGS "$@" "${extra[@]}" -c $f -o $T/${f%.*}.o & ;;
+  esac
   pids+=($!)
 done
-hipcc $FLAGS -c r3d_hostpack.cpp -o $T/r3d_hostpack.o &
-pids+=($!)
 for p in "${pids[@]}"; do
   wait $p || { echo "build_flavour: a compile job failed" >&2; exit 1; }
 done

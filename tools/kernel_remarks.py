@@ -5,6 +5,7 @@
 
 Compiles with the flags of csrc/Makefile plus -Rpass-analysis=kernel-resource-usage (object to /tmp) and prints one row
 per kernel: SGPRs, VGPRs, AGPRs, scratch bytes per lane, occupancy (waves per SIMD), SGPR / VGPR spills, static LDS."""
+import os
 import re
 import subprocess
 import sys
@@ -16,9 +17,9 @@ if "--" in args:
     args = args[:args.index("--")]
 src = args[0]
 flt = args[1] if len(args) > 1 else ""
-flags = ["--offload-arch=gfx950", "-O3", "-ffp-contract=off", "-fPIC", "-std=c++17", "-Wno-unused-function", "-Wno-pass-failed"]
-if src.endswith("r3d_insert.hip"):
-    flags += ["-mllvm", "-disable-machine-licm"]
+csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pcl-augmentation_amd", "csrc")
+made = lambda name: subprocess.run(["make", "-s", "-C", csrc, "print-" + name], capture_output=True, text=True, check=True).stdout.split()  # noqa: E731
+flags = made("HIPFLAGS") + (made("INSERT_FLAGS") if src.endswith("r3d_insert.hip") else [])
 p = subprocess.run(["hipcc"] + flags + extra + ["-Rpass-analysis=kernel-resource-usage", "-c", src, "-o", "/tmp/_remarks.o"],
                    capture_output=True, text=True)
 if p.returncode:
