@@ -608,6 +608,7 @@ int r3d_host_append_text_files(const char *const *src, const char *const *dst, c
  * and what a step needs of them is made on the device from lengths that only the device knows.
  * Same conventions as above: device pointers, no allocation, no synchronisation, capturable.
  * Outputs are written whole; an output must not overlap an input unless it says so.
+ * Arrays are aligned to their elements, states and workspaces to 16 bytes; what is not is refused.
  * ===================================================================================== */
 /* types of values */
 #define R3D_T_F32 0

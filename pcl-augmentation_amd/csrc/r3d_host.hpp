@@ -36,6 +36,8 @@ inline int fail_hip(hipError_t e, const char *where) {
     if (e_ != hipSuccess) return r3d::fail_hip(e_, name);    \
   } while (0)
 
+inline bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }      // (a null pointer is)
+
 inline size_t align_up(size_t v, size_t a = 256) { return (v + a - 1) / a * a; }
 
 // Carves a caller-provided workspace into aligned pieces.

@@ -1123,6 +1123,16 @@ int check(const r3d_linear_ce_t *d) {
   return R3D_OK;
 }
 
+// What the kernels take for granted of the addresses that a call brings.
+int check_aligned(const r3d_linear_ce_t &d, const void *workspace) {
+  const size_t size = d.type == R3D_T_F32 ? 4 : 2;
+  if (!aligned(d.state, 16) || !aligned(workspace, 16)) return fail(R3D_E_ARG, "linear_ce: state and workspace must be 16-byte aligned");
+  if (!aligned(d.x, size) || !aligned(d.w, size) || !aligned(d.bias, size) || !aligned(d.dx, size) || !aligned(d.dw, size) || !aligned(d.db, size) ||
+      !aligned(d.target, d.target_type == R3D_T_I64 ? 8 : 4) || !aligned(d.loss, 4) || !aligned(d.grad, 4))
+    return fail(R3D_E_ARG, "linear_ce: an array is not aligned to its type");
+  return R3D_OK;
+}
+
 // The operands as the products take them: in place, or as the forward pass has packed them.
 void operands(const r3d_linear_ce_t &d, const Plan &p, Operand &x, Operand &w) {
   x = p.direct ? Operand{d.x, d.ld_x, 0, p.idx} : Operand{p.xp, p.dp, d.n * p.dp, p.idx};
@@ -1505,6 +1515,8 @@ extern "C" int r3d_linear_ce_forward(const r3d_linear_ce_t *d, void *workspace, 
   int rc = check(d);
   if (rc != R3D_OK) return rc;
   if (!d->x || !d->w || !d->target || !d->state || !d->loss || !workspace) return fail(R3D_E_ARG, "linear_ce_forward: null pointer");
+  rc = check_aligned(*d, workspace);
+  if (rc != R3D_OK) return rc;
   if (workspace_bytes < r3d_linear_ce_bytes(d, R3D_CE_BYTES_FORWARD)) return fail(R3D_E_WORKSPACE, "linear_ce_forward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (few_takes(*d)) {
@@ -1522,6 +1534,8 @@ extern "C" int r3d_linear_ce_backward(const r3d_linear_ce_t *d, void *workspace,
   int rc = check(d);
   if (rc != R3D_OK) return rc;
   if (!d->x || !d->w || !d->target || !d->state || !d->grad || !workspace) return fail(R3D_E_ARG, "linear_ce_backward: null pointer");
+  rc = check_aligned(*d, workspace);
+  if (rc != R3D_OK) return rc;
   if (workspace_bytes < r3d_linear_ce_bytes(d, R3D_CE_BYTES_BACKWARD)) return fail(R3D_E_WORKSPACE, "linear_ce_backward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (few_takes(*d)) {

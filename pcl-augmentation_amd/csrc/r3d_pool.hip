@@ -368,6 +368,7 @@ extern "C" int r3d_block_tables(const int32_t *lengths, int64_t n_rows, int32_t 
     return fail(R3D_E_ARG, "block_tables: bad size");
   if (tables == tables_out || held == held_out || free_blocks == free_out || n_free == n_free_out)
     return fail(R3D_E_ARG, "block_tables: an output is its input");
+  if (!aligned(workspace, 8)) return fail(R3D_E_ARG, "block_tables: workspace must be 8-byte aligned");
   if (workspace_bytes < r3d_block_tables_workspace_bytes(n_rows)) return fail(R3D_E_WORKSPACE, "block_tables: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   TablesArgs a{lengths, tables, held, free_blocks, n_free, tables_out, held_out, free_out, n_free_out, status, n_rows, n_blocks,
@@ -393,8 +394,8 @@ extern "C" int r3d_slot_map(const int32_t *lengths, int64_t n_lengths, const int
       block_size <= 0 || (tables && max_blocks <= 0) || capacity > (1ll << 40) ||
       (tables && (int64_t)max_blocks * block_size > INT32_MAX))
     return fail(R3D_E_ARG, "slot_map: bad size");
-  if ((reinterpret_cast<uintptr_t>(slots) | reinterpret_cast<uintptr_t>(sequence)) & 15)
-    return fail(R3D_E_ARG, "slot_map: slots and sequence must be 16-byte aligned");
+  if (!aligned(slots, 16) || !aligned(sequence, 16) || !aligned(offsets, 8))
+    return fail(R3D_E_ARG, "slot_map: slots and sequence must be 16-byte aligned, offsets 8");
   hipStream_t st = static_cast<hipStream_t>(stream);
   MapArgs a{lengths, tables, rows, n_lengths, n_seq, capacity, block_size, tables ? max_blocks : 1, -1, offsets, slots, sequence};
   if ((block_size & (block_size - 1)) == 0) a.shift = __builtin_ctz((unsigned)block_size);
@@ -415,6 +416,7 @@ extern "C" int r3d_move_rows(const r3d_rows_t *arrays, int32_t n_arrays, const i
                              int64_t n_src, int64_t n_dst, void *stream) {
   if (!arrays || n_arrays <= 0 || n_arrays > R3D_MAX_ROW_ARRAYS || n < 0 || n_src < 0 || n_dst < 0 || n > (1ll << 40))
     return fail(R3D_E_ARG, "move_rows: bad argument");
+  if (!aligned(src_slots, 8) || !aligned(dst_slots, 8)) return fail(R3D_E_ARG, "move_rows: slots must be 8-byte aligned");
   if ((!src_slots && n > n_src) || (!dst_slots && n > n_dst)) return fail(R3D_E_ARG, "move_rows: more rows than the side without a map has");
   RowsArgs g{};
   g.n_arrays = n_arrays;

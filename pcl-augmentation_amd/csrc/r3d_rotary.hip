@@ -187,6 +187,7 @@ extern "C" int r3d_rotary(const r3d_rotary_t *d, void *stream) {
   if (2 * a.pairs > d->dim) return fail(R3D_E_ARG, "rotary: more pairs than the head has");
   if (d->tokens == 0) return R3D_OK;
   if (!d->pos) return fail(R3D_E_ARG, "rotary: null positions");
+  if (!aligned(d->pos, d->pos_type == R3D_T_I32 || d->pos_type == R3D_T_F32 ? 4 : 8)) return fail(R3D_E_ARG, "rotary: positions not aligned to their type");
   a.tokens = d->tokens;
   a.dim = d->dim;
   a.half = d->interleaved ? 0 : 1;

@@ -221,3 +221,23 @@ def test_loss_stops_at_the_first_call_that_fails(pkg):
                    loss=p, grad=p, dx=p, dw=p, db=p)
     for call in (lib.r3d_linear_ce_forward, lib.r3d_linear_ce_backward):
         assert call(C.byref(e), p, 1 << 40, None) == L.E_HIP and b"hipFuncSetAttribute" in lib.r3d_last_error()
+
+
+def test_c_entries_refuse_what_is_not_aligned(pkg):
+    """(Addresses of host memory that nothing is launched for.)"""
+    L, lib = pkg._lib, pkg._lib.load()
+    p = C.cast(C.create_string_buffer(256), C.c_void_p).value // 64 * 64 + 64
+    assert lib.r3d_block_tables(p, 4, 16, 2, p, p, p, 8, p, p + 16, p + 16, p + 16, p + 16, None, p + 4, 1 << 20, None) == L.E_ARG
+    assert lib.r3d_slot_map(p, 4, None, 16, 1, None, 4, 10, p + 4, p, p, None) == L.E_ARG
+    rows = (L.Rows * 1)(L.Rows(p, p, 16, 16, 16))
+    assert lib.r3d_move_rows(rows, 1, p + 4, None, 1, 1, 1, None) == L.E_ARG and lib.r3d_move_rows(rows, 1, None, p + 4, 1, 1, 1, None) == L.E_ARG
+    d = L.Rotary(tokens=4, dim=8, axes=1, base=10.0, pos_type=L.T_F64, type=L.T_F32, pos=p + 4, pos_token_stride=1, pos_axis_stride=1)
+    d.sections[0], d.heads[0], d.token_stride[0], d.head_stride[0], d.x[0], d.y[0] = 4, 1, 8, 8, p, p + 16
+    assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG and b"aligned" in lib.r3d_last_error()
+    good = dict(x=p, w=p, target=p, bias=p, state=p, loss=p, grad=p, dx=p, dw=p, db=p, workspace=p)
+    for name, by in (("x", 1), ("w", 1), ("bias", 1), ("dx", 1), ("dw", 1), ("db", 1), ("target", 4), ("loss", 2), ("grad", 2), ("state", 8), ("workspace", 8)):
+        at = dict(good, **{name: p + by})
+        ws = at.pop("workspace")
+        e = L.LinearCE(n=4, v=3, d=8, ld_x=8, ld_w=8, type=L.T_BF16, target_type=L.T_I64, reduction=L.CE_MEAN, **at)
+        for call in (lib.r3d_linear_ce_forward, lib.r3d_linear_ce_backward):
+            assert call(C.byref(e), ws, 1 << 40, None) == L.E_ARG and b"aligned" in lib.r3d_last_error(), name
