@@ -173,7 +173,7 @@ extern "C" int r3d_rotary(const r3d_rotary_t *d, void *stream) {
   if (!size) return fail(R3D_E_ARG, "rotary: type");
   if (d->pos_type != R3D_T_I32 && d->pos_type != R3D_T_I64 && d->pos_type != R3D_T_F32 && d->pos_type != R3D_T_F64)
     return fail(R3D_E_ARG, "rotary: type of the positions");
-  if (!(d->base > 0.0)) return fail(R3D_E_ARG, "rotary: base must be positive");
+  if (!(d->base > 0.0) || std::isinf(d->base)) return fail(R3D_E_ARG, "rotary: base must be positive and finite");
   RotArgs a{};
   const double octaves = std::log2(d->base);
   for (int x = 0; x < d->axes; ++x) {

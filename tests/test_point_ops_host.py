@@ -241,3 +241,13 @@ def test_c_entries_refuse_what_is_not_aligned(pkg):
         e = L.LinearCE(n=4, v=3, d=8, ld_x=8, ld_w=8, type=L.T_BF16, target_type=L.T_I64, reduction=L.CE_MEAN, **at)
         for call in (lib.r3d_linear_ce_forward, lib.r3d_linear_ce_backward):
             assert call(C.byref(e), ws, 1 << 40, None) == L.E_ARG and b"aligned" in lib.r3d_last_error(), name
+
+
+def test_rotary_in_c_refuses_a_base_that_is_not_finite(pkg):
+    L, lib = pkg._lib, pkg._lib.load()
+    p = C.cast(C.create_string_buffer(256), C.c_void_p).value // 64 * 64 + 64
+    d = L.Rotary(tokens=4, dim=8, axes=1, pos_type=L.T_F32, type=L.T_F32, pos=p, pos_token_stride=1, pos_axis_stride=1)
+    d.sections[0], d.heads[0], d.token_stride[0], d.head_stride[0], d.x[0], d.y[0] = 4, 1, 8, 8, p, p + 16
+    for base in (float("inf"), float("nan"), 0.0, -2.0):
+        d.base = base
+        assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG and b"base" in lib.r3d_last_error()
