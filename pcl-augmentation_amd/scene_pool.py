@@ -200,6 +200,13 @@ class PackedScenes(NamedTuple):
     slots: object     # int64 [tokens]
 
 
+def _with_index(device):
+    """This device by its number: "cuda" is the current one, now (and stays it when another becomes current)."""
+    import torch
+    device = torch.device(device)
+    return device if device.type != "cuda" or device.index is not None else torch.device("cuda", torch.cuda.current_device())
+
+
 class ScenePool:
     """Up to ``max_scenes`` augmented scenes resident on one GPU, in ``n_blocks`` pages of ``block_size`` points.
 
@@ -218,7 +225,7 @@ class ScenePool:
         n_blocks = max_scenes * most if n_blocks is None else int(n_blocks)
         if not 1 <= n_blocks < 2 ** 31:
             raise ValueError("ScenePool: n_blocks must be positive and below 2^31")
-        self.block_size, self.max_scenes, self.max_points, self.device = block_size, max_scenes, most * block_size, torch.device(device)
+        self.block_size, self.max_scenes, self.max_points, self.device = block_size, max_scenes, most * block_size, _with_index(device)
         with _lib.on(self.device):
             self.xyzi = torch.zeros((n_blocks * block_size, 4), dtype=torch.float32, device=self.device)
             self.label = torch.zeros((n_blocks * block_size,), dtype=torch.int32, device=self.device)
@@ -263,9 +270,7 @@ class ScenePool:
 
     def check_device(self, device):
         """Raises where scenes on this device cannot go into the pool."""
-        import torch
-        device = torch.device(device)
-        if (device.type, device.index or 0) != (self.device.type, self.device.index or 0):
+        if _with_index(device) != self.device:
             raise ValueError(f"ScenePool: the batch is on {device}, the pool on {self.device}")
 
     @_lib.on_own_device

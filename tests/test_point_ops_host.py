@@ -251,3 +251,19 @@ def test_rotary_in_c_refuses_a_base_that_is_not_finite(pkg):
     for base in (float("inf"), float("nan"), 0.0, -2.0):
         d.base = base
         assert lib.r3d_rotary(C.byref(d), None) == L.E_ARG and b"base" in lib.r3d_last_error()
+
+
+def test_pool_knows_its_device_by_number(pkg, monkeypatch):
+    """"cuda" is the device that is current when the pool is made, for the pool and for the batch that is to go into it."""
+    pool = object.__new__(pkg.ScenePool)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    pool.device = pkg.scene_pool._with_index("cuda")
+    assert pool.device == torch.device("cuda:1")
+    pool.check_device("cuda")
+    pool.check_device("cuda:1")
+    for other in ("cuda:0", "cpu"):
+        with pytest.raises(ValueError, match="the pool on cuda:1"):
+            pool.check_device(other)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError):
+        pool.check_device("cuda")
