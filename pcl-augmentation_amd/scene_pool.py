@@ -257,7 +257,10 @@ class ScenePool:
     def resize(self, lengths):
         """New lengths for all scenes (int32 [max_scenes] on the device): pages given back and taken (``block_tables``).  What a
         scene's first points are stays; new ones are whatever the page held."""
-        b = self.blocks
+        import torch
+        b, stream = self.blocks, torch.cuda.current_stream()
+        for t in b:      # (made on another stream, they would be handed out there while this one still reads them)
+            t.record_stream(stream)
         self.blocks = block_tables(lengths, self.block_size, b.tables, b.held, b.free_blocks, b.n_free)
         self._refused.bitwise_or_(self.blocks.status)
 

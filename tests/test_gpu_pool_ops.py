@@ -490,3 +490,26 @@ def test_replaced_result_refuses(pkg, synth):
         batch.replace_result(0, want[1][0], want[1][1][:-1])
     with pytest.raises(ValueError):
         batch.replace_result(0, np.zeros((batch.cap + 1, 4), np.float32), np.zeros(batch.cap + 1, np.uint32))
+
+
+def test_pool_used_on_another_stream_keeps_its_tables(pkg):
+    """A resize on a side stream that still has work before it: the tables that it replaces are not handed out to the stream
+    that the pool was made on before they have been read."""
+    pool = pkg.ScenePool(2000, 64 * 16, block_size=16)
+    rng = np.random.default_rng(3)
+    first, second = rng.integers(0, 64 * 16 + 1, 2000), rng.integers(0, 64 * 16 + 1, 2000)
+    pool.resize(i32(first))
+    want = pkg.block_tables(i32(second), 16, *pool.blocks[:4])
+    lengths = i32(second)
+    a = torch.randn((4096, 4096), device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(10):
+            a = a @ a * 1e-3
+        pool.resize(lengths)
+    # what the pool let go of is of these sizes: the default stream's next tensors would stand there
+    other = [torch.full((n,), 77, dtype=torch.int32, device="cuda") for n in (2000 * 64, 2000 * 64, 2000, 1) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(pool.blocks, want)) and len(other) == 16
