@@ -823,3 +823,25 @@ def test_loss_pieces_of_many_classes(pkg, dtype, piece, n, v, d):
         loss, got = check_loss(pkg, n, v, d, dtype, reduction=reduction, piece=piece)
         again = check_loss(pkg, n, v, d, dtype, reduction=reduction, piece=piece)
         assert torch.equal(loss, again[0]) and all(torch.equal(a, b) for a, b in zip(got, again[1]))
+
+
+@pytest.mark.parametrize("v,d,dtype", WAYS + FEW)
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_loss_parts_of_the_gradient_every_way(pkg, v, d, dtype, reduction):
+    """The gradient of one of features, head and bias alone, of two, and the loss without any, also in inference mode."""
+    g = gen(v * 3 + d)
+    n = 400
+    ins = [torch.randn(s, generator=g).to(dtype).cuda() for s in ((n, d), (v, d), (v,))]
+    target, up = torch.randint(-1, v, (n,), generator=g).cuda(), torch.rand((n,), generator=g).cuda()
+
+    def step(need):
+        some = [t.clone().requires_grad_(k in need) for k, t in enumerate(ins)]
+        loss = pkg.linear_cross_entropy(some[0], some[1], target, bias=some[2], ignore_index=-1, reduction=reduction)
+        return loss, torch.autograd.grad(loss, [some[k] for k in need], up if reduction == "none" else up[0])
+
+    loss, want = step((0, 1, 2))
+    for need in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        one, got = step(need)
+        assert torch.equal(one, loss) and all(torch.equal(got[i], want[k]) for i, k in enumerate(need)), need
+    with torch.inference_mode():
+        assert torch.equal(pkg.linear_cross_entropy(ins[0], ins[1], target, bias=ins[2], ignore_index=-1, reduction=reduction), loss)
