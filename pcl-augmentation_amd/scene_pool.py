@@ -125,6 +125,8 @@ def _move(what, sources, dests, src_slots, dst_slots, n):
 def _rows_of(what, name, tensors, like=None):
     """Tensors [rows, ...] with a row in one piece, the same number of rows each."""
     import torch
+    if isinstance(tensors, torch.Tensor):      # (it would be taken for its rows)
+        raise ValueError(f"{what}: {name} are a tuple of tensors")
     tensors, forward = tuple(tensors), forward_mode()
     if not 1 <= len(tensors) <= _lib.MAX_ROW_ARRAYS:
         raise ValueError(f"{what}: 1 to {_lib.MAX_ROW_ARRAYS} {name}")

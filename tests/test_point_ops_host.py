@@ -267,3 +267,10 @@ def test_pool_knows_its_device_by_number(pkg, monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     with pytest.raises(ValueError):
         pool.check_device("cuda")
+
+
+def test_rows_refuse_a_tensor_for_a_tuple(pkg):
+    s, x = torch.zeros(3, dtype=torch.int64), torch.zeros((4, 4))
+    for call in (lambda: pkg.take_rows(s, x), lambda: pkg.put_rows(s, x, (x,)), lambda: pkg.put_rows(s, (x,), x)):
+        with pytest.raises(ValueError, match="tuple"):
+            call()
