@@ -692,7 +692,7 @@ int r3d_rotary(const r3d_rotary_t *d, void *stream);
  * classes at least; piece 0: what 512 MB take, 256 classes at least.  (A head that stands in LDS holds as many bytes, of all
  * its classes and fewer points.  With few classes, or at most 64 features, none are held; with 65 to 128 features only of such a head.)
  * Beside them 32-bit sums of dx and dw where they are made in parts: 4 bytes a value, and up to 256 MB each where they are split over
- * workgroups.  The state holds, where few points and classes do not make all of this unnecessary, 16 bytes a point and a
+ * workgroups.  The state holds, where few points and classes do not make all of this unnecessary, 20 bytes a point and a
  * copy of x and w that is padded and, for float32, split: 6 bytes a value of float32, 2 of the others where rows are not whole
  * multiples of 64 features and 16 bytes.
  * r3d_linear_ce_bytes: of the state and of the two calls' workspaces, for the descriptor as it will be passed (0: bad descriptor). */

@@ -226,7 +226,7 @@ struct LseArgs {
   int64_t n_pad;
 };
 
-// Maximum and sum of 2^(logit * log2 e) over a split of the classes for the points of a tile.  The classes are the rows of C, so
+// Maximum and sum of 2^(logit * log2 e - maximum) over a split of the classes for the points of a tile.  The classes are the rows of C, so
 // a lane holds 16 FM classes of each of its FN points: the statistics of a tile stay in its registers, lanes and waves are
 // joined once at the end.  8192 points x 161 280 classes x 512 bf16: 1.5 ms, 0.9 PFLOP/s of the 1.41 that a large library product
 // reaches here: a tile's exponentials (16 384 cycles of products, some 8000 of the vector unit) find no products to stand beside.
@@ -277,13 +277,13 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
         float t[16], top = m[j];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          t[r] = __builtin_fmaf(acc[i][j][r], kLog2e, b[r]);
+          t[r] = logit2(acc[i][j][r], b[r]);
           top = fmaxf(top, t[r]);
         }
-        const float base = top == -INFINITY ? 0.0f : top;
-        float sum = l[j] * __builtin_amdgcn_exp2f(m[j] - base);
+        const float base = base_of(top);
+        float sum = l[j] * part_of(m[j], base);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(t[r] - base);
+        for (int r = 0; r < 16; ++r) sum += part_of(t[r], base);
         m[j] = top;
         l[j] = sum;
         const int d = tgt[j] - vb;
@@ -300,8 +300,8 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
   float *s_m = reinterpret_cast<float *>(lds), *s_l = s_m + S::WM * S::BN;
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) {
-    const float om = __shfl_xor(m[j], 32), ol = __shfl_xor(l[j], 32), top = fmaxf(m[j], om), base = top == -INFINITY ? 0.0f : top;
-    const float sum = l[j] * __builtin_amdgcn_exp2f(m[j] - base) + ol * __builtin_amdgcn_exp2f(om - base);
+    const float om = __shfl_xor(m[j], 32), ol = __shfl_xor(l[j], 32), top = fmaxf(m[j], om), base = base_of(top);
+    const float sum = l[j] * part_of(m[j], base) + ol * part_of(om, base);
     if (lane < 32) {
       const int at = wm * S::BN + (wn * S::FN + j) * 32 + lane;
       s_m[at] = top;
@@ -313,9 +313,9 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_lse(LseArgs a) {
     float top = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < S::WM; ++w) top = fmaxf(top, s_m[w * S::BN + c]);
-    const float base = top == -INFINITY ? 0.0f : top;
+    const float base = base_of(top);
 #pragma unroll
-    for (int w = 0; w < S::WM; ++w) sum += s_l[w * S::BN + c] * __builtin_amdgcn_exp2f(s_m[w * S::BN + c] - base);
+    for (int w = 0; w < S::WM; ++w) sum += s_l[w * S::BN + c] * part_of(s_m[w * S::BN + c], base);
     a.part_m[split * a.n_pad + n0 + c] = top;
     a.part_l[split * a.n_pad + n0 + c] = sum;
   }
@@ -325,7 +325,7 @@ struct JoinArgs {
   const float *part_m, *part_l, *hit;
   const int32_t *tgt, *place;
   Counted *counted;
-  float *lse2, *each, *loss;
+  float *base, *sum, *each, *loss;
   double *sums;
   int64_t n, n_pad;
   int32_t splits, mean, points;      // points: of a workgroup
@@ -363,9 +363,9 @@ __global__ __launch_bounds__(kJoinThreads) void k_ce_join(JoinArgs a) {
     if (at >= 0) {
 #pragma unroll 4
       for (int k = slice; k < a.splits; k += slices) top = fmaxf(top, a.part_m[k * a.n_pad + at]);
-      const float base = top == -INFINITY ? 0.0f : top;
+      const float base = base_of(top);
 #pragma unroll 4
-      for (int k = slice; k < a.splits; k += slices) sum += a.part_l[k * a.n_pad + at] * __builtin_amdgcn_exp2f(a.part_m[k * a.n_pad + at] - base);
+      for (int k = slice; k < a.splits; k += slices) sum += a.part_l[k * a.n_pad + at] * part_of(a.part_m[k * a.n_pad + at], base);
     }
     if (slices > 1) {
       __syncthreads();
@@ -374,15 +374,15 @@ __global__ __launch_bounds__(kJoinThreads) void k_ce_join(JoinArgs a) {
       __syncthreads();
       sum = 0.0f;
       for (int k = 0; k < slices; ++k) top = fmaxf(top, s_top[k * points + p]);
-      const float base = top == -INFINITY ? 0.0f : top;
-      for (int k = 0; k < slices; ++k) sum += s_sum[k * points + p] * __builtin_amdgcn_exp2f(s_top[k * points + p] - base);
+      const float base = base_of(top);
+      for (int k = 0; k < slices; ++k) sum += s_sum[k * points + p] * part_of(s_top[k * points + p], base);
     }
     float loss = 0.0f;
     if (at >= 0 && slice == 0) {
       const bool fine = a.tgt[at] >= 0;      // a target that is no class: NaN, and so are its gradients
-      const float lse2 = fine ? top + __builtin_amdgcn_logf(sum) : NAN;
-      a.lse2[at] = lse2;
-      loss = fine ? (lse2 - a.hit[at]) * kLn2 : NAN;
+      a.base[at] = fine ? base_of(top) : NAN;
+      a.sum[at] = sum;
+      loss = fine ? point_loss(top, sum, a.hit[at]) : NAN;
     }
     losses += loss;
     if (a.each && i < a.n && slice == 0) a.each[i] = loss;
@@ -466,7 +466,7 @@ struct DlArgs {
   int64_t piece0, dl_plane, n_pad;      // first class of the piece
   int32_t vtiles, width;                // width: classes of the piece, a multiple of 64
   float held;                           // 2^15 for float16
-  const float *bias2, *lse2, *weight;
+  const float *bias2, *base, *sum, *weight;
   const int32_t *tgt;
   const Counted *counted;
   void *dl;        // [planes][width / 8][n_pad][8]
@@ -507,14 +507,15 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
   float *s_sum = reinterpret_cast<float *>(lds);      // [WN][BM]
   int64_t col[S::FN];
   int tgt[S::FN];
-  float lse2[S::FN], weight[S::FN];
+  float base[S::FN], sum[S::FN], share[S::FN];      // share: the weight over the sum of the parts
 #pragma unroll
   for (int j = 0; j < S::FN; ++j) {
     col[j] = n0 + (wn * S::FN + j) * 32 + (lane & 31);
     const bool in = col[j] < nc;
     tgt[j] = in ? a.tgt[col[j]] : -1;
-    lse2[j] = in ? a.lse2[col[j]] : 0.0f;
-    weight[j] = in ? a.weight[col[j]] * a.held : 0.0f;
+    base[j] = in ? a.base[col[j]] : 0.0f;
+    sum[j] = in ? a.sum[col[j]] : 1.0f;
+    share[j] = in ? a.weight[col[j]] * a.held / sum[j] : 0.0f;
   }
 #pragma unroll
   for (int i = 0; i < S::FM; ++i) {
@@ -532,10 +533,10 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
       const int64_t d = tgt[j] - vb;
       float p[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, b[r]) - lse2[j]);
+      for (int r = 0; r < 16; ++r) p[r] = part_of(logit2(acc[i][j][r], b[r]), base[j]);
       if (__any(d >= 0 && d < 32)) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] -= d == mma_row(r) ? 1.0f : 0.0f;
+        for (int r = 0; r < 16; ++r) p[r] -= d == mma_row(r) ? sum[j] : 0.0f;
       }
       typedef T t4 __attribute__((ext_vector_type(4)));
       typedef unsigned u2 __attribute__((ext_vector_type(2)));
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(S::threads, 2) void k_ce_dl(DlArgs a) {
       t4 q[4][kPlanes];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float w = col[j] < nc ? p[r] * weight[j] : 0.0f;
+        const float w = col[j] < nc ? p[r] * share[j] : 0.0f;
         sums[r] += w;
         if constexpr (kPlanes == 3) {
           T h, mm, l;
@@ -748,7 +749,7 @@ struct HeadArgs {
   int32_t first, most;               // the points of this launch: of those that count, `most` from number `first` on
   float *part_m, *part_l, *hit;      // forward
   // backward
-  const float *lse2, *weight, *scale;
+  const float *base, *sum, *weight, *scale;
   float held, unheld;
   void *dl, *dx;                     // dl: pieces of 8 classes, or null
   float *sums;                       // [workgroups][classes padded to 32]: db of its points, or null
@@ -838,17 +839,17 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
       for (int v = 0; v < kVB; ++v)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          acc[v][r] = __builtin_fmaf(acc[v][r], kLog2e, bias2[v * 32 + mma_row(r)]);
+          acc[v][r] = logit2(acc[v][r], bias2[v * 32 + mma_row(r)]);
           top = fmaxf(top, acc[v][r]);
           hit = t == v * 32 + mma_row(r) ? acc[v][r] : hit;
         }
       if (t >= 0 && (t >> 2 & 1) == half) a.hit[point] = hit;      // (the lane that holds the target's class)
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float base = top == -INFINITY ? 0.0f : top;
+      const float base = base_of(top);
 #pragma unroll
       for (int v = 0; v < kVB; ++v)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(acc[v][r] - base);
+        for (int r = 0; r < 16; ++r) sum += part_of(acc[v][r], base);
       sum += __shfl_xor(sum, 32);
       if (in && half == 0) {
         a.part_m[point] = top;
@@ -857,16 +858,16 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
     } else {
       typedef unsigned u2 __attribute__((ext_vector_type(2)));
       typedef unsigned u4 __attribute__((ext_vector_type(4)));
-      const float lse2 = in ? a.lse2[point] : 0.0f, by = in ? a.weight[point] * a.held : 0.0f;
+      const float base = in ? a.base[point] : 0.0f, sum = in ? a.sum[point] : 1.0f, share = in ? a.weight[point] * a.held / sum : 0.0f;
       t4 q[kVB][4];
 #pragma unroll
       for (int v = 0; v < kVB; ++v) {
         float w[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[v][r], kLog2e, bias2[v * 32 + mma_row(r)]) - lse2);
-          p -= t == v * 32 + mma_row(r) ? 1.0f : 0.0f;
-          w[r] = in ? p * by : 0.0f;
+          float p = part_of(logit2(acc[v][r], bias2[v * 32 + mma_row(r)]), base);
+          p -= t == v * 32 + mma_row(r) ? sum : 0.0f;
+          w[r] = in ? p * share : 0.0f;
           q[v][r >> 2][r & 3] = (T)w[r];
         }
         if (a.sums) {
@@ -1004,7 +1005,7 @@ struct Plan {
   // kept from the forward to the backward pass
   Counted *counted;
   int32_t *idx, *place, *tgt;
-  float *lse2, *bias2;
+  float *base, *sum, *bias2;
   void *xp, *wp;
   size_t state_bytes;
   // workspace
@@ -1042,7 +1043,8 @@ Plan plan(const r3d_linear_ce_t &d, bool backward, void *workspace) {
   p.idx = k.take<int32_t>(d.n);
   p.place = k.take<int32_t>(d.n);
   p.tgt = k.take<int32_t>(d.n);
-  p.lse2 = k.take<float>(d.n);
+  p.base = k.take<float>(d.n);
+  p.sum = k.take<float>(d.n);
   p.bias2 = k.take<float>(p.v_pad);
   if (!p.direct) {
     p.xp = k.take<uint16_t>((size_t)p.planes * d.n * p.dp);
@@ -1163,7 +1165,7 @@ void lse(LseArgs a, const Plan &p, int64_t n, int64_t v, hipStream_t st) {
 }
 
 void join(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
-  JoinArgs ja{p.part_m, p.part_l, p.hit, p.tgt, p.place, p.counted, p.lse2, d.reduction == R3D_CE_NONE ? d.loss : nullptr, d.loss, p.sums, d.n, p.n_pad,
+  JoinArgs ja{p.part_m, p.part_l, p.hit, p.tgt, p.place, p.counted, p.base, p.sum, d.reduction == R3D_CE_NONE ? d.loss : nullptr, d.loss, p.sums, d.n, p.n_pad,
               p.lse_splits, d.reduction == R3D_CE_MEAN};
   ja.points = join_points(p.lse_splits);
   // a sum: a workgroup a CU, each raises the one counter (270 597 points: 39 us with one for every 256 points, 13 so)
@@ -1184,7 +1186,8 @@ HeadArgs head_args(const r3d_linear_ce_t &d, const Plan &p) {
   a.part_m = p.part_m;
   a.part_l = p.part_l;
   a.hit = p.hit;
-  a.lse2 = p.lse2;
+  a.base = p.base;
+  a.sum = p.sum;
   a.weight = p.weight;
   a.scale = p.scale;
   a.dl = p.dl;
@@ -1330,7 +1333,8 @@ int backward_head(const r3d_linear_ce_t &d, const Plan &p, Operand x, float held
     ha.most = (int32_t)(d.n - first < each ? d.n - first : each);
     ha.idx += first;
     ha.tgt += first;
-    ha.lse2 += first;
+    ha.base += first;
+    ha.sum += first;
     ha.weight += first;
     ha.held = held;
     ha.unheld = unheld;
@@ -1386,11 +1390,13 @@ int backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     NarrowArgs na{};
     na.v = d.v;
     na.bias2 = p.bias2;
-    na.lse2 = p.lse2;
+    na.base = p.base;
+    na.sum = p.sum;
     na.weight = p.weight;
     na.tgt = p.tgt;
     na.counted = p.counted;
     na.held = held;
+    na.each = each;
     na.d = d.d;
     na.scale = p.scale;
     na.unheld = unheld;
@@ -1443,7 +1449,8 @@ int backward(const r3d_linear_ce_t &d, const Plan &p, hipStream_t st) {
     da.width = (int)width;
     da.held = held;
     da.bias2 = p.bias2;
-    da.lse2 = p.lse2;
+    da.base = p.base;
+    da.sum = p.sum;
     da.weight = p.weight;
     da.tgt = p.tgt;
     da.counted = p.counted;

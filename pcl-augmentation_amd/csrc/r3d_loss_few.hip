@@ -199,23 +199,22 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
       for (int v = 0; v < kVT; ++v)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          acc[v][r] = __builtin_fmaf(acc[v][r], kLog2e, bias2[v * 32 + mma_row(r)]);
+          acc[v][r] = logit2(acc[v][r], bias2[v * 32 + mma_row(r)]);
           top = fmaxf(top, acc[v][r]);
           hit = t == v * 32 + mma_row(r) ? acc[v][r] : hit;
         }
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float base = top == -INFINITY ? 0.0f : top;
+      const float base = base_of(top);
 #pragma unroll
       for (int v = 0; v < kVT; ++v)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(acc[v][r] - base);
+        for (int r = 0; r < 16; ++r) sum += acc[v][r] = part_of(acc[v][r], base);
       sum += __shfl_xor(sum, 32);
-      const float lse2 = t == -1 ? NAN : top + __builtin_amdgcn_logf(sum);
       if constexpr (!kGrad) {
         // (only the lane that holds the target's logit has it; the other's stays -inf)
         const float other = __shfl_xor(hit, 32);
         const float mine = t >= 0 && ((t >> 2) & 1) == half ? hit : other;
-        const float loss = t == -2 ? 0.0f : t == -1 ? NAN : (lse2 - mine) * kLn2;
+        const float loss = t == -2 ? 0.0f : t == -1 ? NAN : point_loss(top, sum, mine);
         const int64_t i = tile * kTP + wave * 32 + low;
         if (half == 0) {
           if (a.each) {
@@ -227,16 +226,15 @@ __global__ __launch_bounds__(kThreads, few_waves(kPlanes, kVT, kNB)) void k_few(
         }
       } else {
         typedef T t4 __attribute__((ext_vector_type(4)));
-        const float by = t == -2 ? 0.0f : s_weight[at * kTP + wave * 32 + low] * a.held;
+        const float share = t == -2 ? 0.0f : t == -1 ? NAN : s_weight[at * kTP + wave * 32 + low] * a.held / sum;
         t4 q[kVT][4][kPlanes];
 #pragma unroll
         for (int v = 0; v < kVT; ++v) {
           float w[16];
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            float p = __builtin_amdgcn_exp2f(acc[v][r] - lse2);
-            p -= t == v * 32 + mma_row(r) ? 1.0f : 0.0f;
-            w[r] = p = t == -2 ? 0.0f : p * by;
+            const float p = t == -2 ? 0.0f : (acc[v][r] - (t == v * 32 + mma_row(r) ? sum : 0.0f)) * share;
+            w[r] = p;
             if constexpr (kPlanes == 3) {
               T h, m, l;
               split3(p, h, m, l);

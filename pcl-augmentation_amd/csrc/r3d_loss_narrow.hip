@@ -10,7 +10,7 @@
 // what is kept, one a lane) is, as it stands, the operand of the second one, whose k are the rows in the order in which the lanes
 // have them: kept^T += met^T dl.  db is the sum of a lane's dl, before it is rounded.
 //
-// Bound by the vector unit: 417 824 points x 3114 classes x 64 fp16 take 400 / 455 / 585 us, 770 to 1100 cycles of a SIMD for every
+// Bound by the vector unit: 417 824 points x 3114 classes x 64 fp16 take 425 / 475 / 585 us (643 where weights differ), 770 to 1200 cycles of a SIMD for every
 // 32 x 32 logits, of which 16 exponentials take 256, their arguments, products and roundings some 300, the matrix cores 128 or 256
 // beside them.  Two waves a SIMD (a wave's exponentials beside the other's products) is what the registers allow.
 #include "r3d_loss.hpp"
@@ -28,7 +28,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
   constexpr bool kPoints = kWhat != Narrow::Dw, kLse = kWhat == Narrow::Lse;
   constexpr int kPitch = kDP + 8, kPlane = kRows * kPitch, kCols = kDP / 8, kPer = kRows * kCols / kThreads, kPairCount = kPlanes == 3 ? kPairs : 1;
   __shared__ __attribute__((aligned(16))) T lds[2][kPlanes * kPlane];
-  __shared__ __attribute__((aligned(16))) float s_a[2][kRows], s_weight[2][kRows];      // bias of a class, or sum and weight of a point
+  // bias of a class; or a point's base, its share (over the sum of its parts: its weight, or 1 where weights differ) and its weight
+  __shared__ __attribute__((aligned(16))) float s_a[2][kRows], s_share[2][kRows], s_weight[2][kRows];
   __shared__ __attribute__((aligned(16))) int s_tgt[2][kRows];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, low = lane & 31, group = lane >> 4, sub = lane & 15;
   const int nc = a.counted->n, kept_n = kPoints ? nc : (int)a.v, met_n = kPoints ? (int)a.v : nc;
@@ -39,7 +40,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
   const int c0 = (int)((int64_t)chunks * split / a.splits), c1 = (int)((int64_t)chunks * (split + 1) / a.splits);
 
   v8 own[kSB][kDP / 16][kPlanes];
-  float own_a[kSB], own_weight[kSB];      // a point's sum and weight; a class's bias
+  float own_a[kSB], own_sum[kSB], own_share[kSB];      // a point's base, sum and share; a class's bias
   int own_tgt[kSB];                       // a point's class
   int64_t own_row[kSB];
 #pragma unroll
@@ -51,8 +52,9 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
     for (int k = 0; k < kDP / 16; ++k)
 #pragma unroll
       for (int pl = 0; pl < kPlanes; ++pl) own[s][k][pl] = *reinterpret_cast<const v8 *>(p + pl * a.kept.plane + k * 16);
-    own_a[s] = kLse ? 0.0f : kPoints ? (at < kept_n ? a.lse2[at] : INFINITY) : a.bias2[at];
-    own_weight[s] = kPoints && !kLse && at < kept_n ? a.weight[at] * a.held : 0.0f;
+    own_a[s] = kLse ? 0.0f : kPoints ? (at < kept_n ? a.base[at] : INFINITY) : a.bias2[at];
+    own_sum[s] = kPoints && !kLse && at < kept_n ? a.sum[at] : 1.0f;
+    own_share[s] = kPoints && !kLse && at < kept_n ? a.weight[at] * a.held / own_sum[s] : 0.0f;
     own_tgt[s] = kPoints && at < kept_n ? a.tgt[at] : -1;
   }
   f32x16 sums[kLse ? 1 : kDP / 32][kSB];
@@ -67,8 +69,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
   // what is met: numbers two chunks ahead, rows one
   v8 reg[kPlanes][kPer];
   int64_t number[kPer];
-  float next_a = 0.0f, next_weight = 0.0f;
-  int next_tgt = -1;
+  float next_p = 0.0f, next_q = 1.0f;      // wave 0: a class's bias, or a point's base and class; wave 1: a point's weight and sum
   auto numbers = [&](int c) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -83,13 +84,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         reg[pl][i] = *reinterpret_cast<const v8 *>(static_cast<const T *>(a.met.p) + pl * a.met.plane + number[i] * a.met.ld + ((int)threadIdx.x % kCols) * 8);
-    if (threadIdx.x < kRows) {
-      const int r = c * kRows + threadIdx.x;
-      next_a = kPoints ? a.bias2[r] : r < nc ? a.lse2[r] : INFINITY;
-      if constexpr (!kPoints) {
-        next_weight = r < nc ? a.weight[r] * a.held : 0.0f;
-        next_tgt = r < nc ? a.tgt[r] : -1;
-      }
+    const int r = c * kRows + lane;
+    if (wave == 0) {
+      next_p = kPoints ? a.bias2[r] : r < nc ? a.base[r] : INFINITY;
+      if constexpr (!kPoints) next_q = __builtin_bit_cast(float, r < nc ? a.tgt[r] : -1);
+    } else if (!kPoints && wave == 1) {
+      next_p = r < nc ? a.weight[r] * a.held : 0.0f;
+      next_q = r < nc ? a.sum[r] : 1.0f;
     }
   };
   if (c0 < c1) {
@@ -107,12 +108,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
         const int at = i * kThreads + threadIdx.x;
         *reinterpret_cast<v8 *>(met + pl * kPlane + at / kCols * kPitch + at % kCols * 8) = reg[pl][i];
       }
-    if (threadIdx.x < kRows) {
-      s_a[buf][threadIdx.x] = next_a;
-      if constexpr (!kPoints) {
-        s_weight[buf][threadIdx.x] = next_weight;
-        s_tgt[buf][threadIdx.x] = next_tgt;
-      }
+    if (wave == 0) {
+      s_a[buf][lane] = next_p;
+      if constexpr (!kPoints) s_tgt[buf][lane] = __builtin_bit_cast(int, next_q);
+    } else if (!kPoints && wave == 1) {
+      s_share[buf][lane] = (a.each ? 1.0f : next_p) / next_q;
+      s_weight[buf][lane] = next_p;
     }
     __syncthreads();      // (whoever still multiplies reads the other buffer)
     if (c + 1 < c1) {
@@ -131,15 +132,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
       for (int pr = 0; pr < kPairCount; ++pr)
 #pragma unroll
         for (int k = 0; k < kDP / 16; ++k) {
-          const v8 f = *reinterpret_cast<const v8 *>(rows + kPlaneA[pr] * kPlane + k * 16);
+          // (classes by kPlaneA, points by kPlaneB, whichever are met: the logits of all three calls are the same bits)
+          const v8 f = *reinterpret_cast<const v8 *>(rows + (kPoints ? kPlaneA : kPlaneB)[pr] * kPlane + k * 16);
 #pragma unroll
-          for (int s = 0; s < kSB; ++s) acc[s] = Mma<T>::mma(f, own[s][k][kPlaneB[pr]], acc[s]);
+          for (int s = 0; s < kSB; ++s) acc[s] = Mma<T>::mma(f, own[s][k][(kPoints ? kPlaneB : kPlaneA)[pr]], acc[s]);
         }
       float ma[16], mw[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         ma[r] = s_a[buf][vb * 32 + mma_row(r)];
-        if constexpr (!kPoints) mw[r] = s_weight[buf][vb * 32 + mma_row(r)];
+        if constexpr (!kPoints) mw[r] = s_share[buf][vb * 32 + mma_row(r)];
       }
       if constexpr (kLse) {
 #pragma unroll
@@ -147,13 +149,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
           float t[16], now = top[s];
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            t[r] = __builtin_fmaf(acc[s][r], kLog2e, ma[r]);
+            t[r] = logit2(acc[s][r], ma[r]);
             now = fmaxf(now, t[r]);
           }
-          const float base = now == -INFINITY ? 0.0f : now;
-          sum[s] *= __builtin_amdgcn_exp2f(top[s] - base);
+          const float base = base_of(now);
+          sum[s] *= part_of(top[s], base);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sum[s] += __builtin_amdgcn_exp2f(t[r] - base);
+          for (int r = 0; r < 16; ++r) sum[s] += part_of(t[r], base);
           top[s] = now;
           const int d = own_tgt[s] - (c * kRows + vb * 32);
           if (__any(d >= 0 && d < 32)) {
@@ -170,24 +172,31 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
         float p[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          p[r] = kPoints ? __builtin_amdgcn_exp2f(__builtin_fmaf(acc[s][r], kLog2e, ma[r]) - own_a[s])
-                         : __builtin_amdgcn_exp2f(__builtin_fmaf(acc[s][r], kLog2e, own_a[s]) - ma[r]);
+          p[r] = kPoints ? part_of(logit2(acc[s][r], ma[r]), own_a[s]) : part_of(logit2(acc[s][r], own_a[s]), ma[r]);
         if constexpr (kPoints) {
           const int d = own_tgt[s] - (c * kRows + vb * 32);
           if (__any(d >= 0 && d < 32)) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] -= d == mma_row(r) ? 1.0f : 0.0f;
+            for (int r = 0; r < 16; ++r) p[r] -= d == mma_row(r) ? own_sum[s] : 0.0f;
           }
         } else {
+          // one weight for all: it is in the share already; else it is multiplied in behind the target's 1 (looked up there, row by
+          // row, weights cost registers that a wave does not have: 99 us became 143, 200 000 x 1000 x 64 bf16)
           const int first = kept0 + s * 32, d = s_tgt[buf][vb * 32 + low] - first;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) p[r] *= mw[r];
           if (__any(d >= 0 && d < 32)) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] -= s_tgt[buf][vb * 32 + mma_row(r)] - first == low ? 1.0f : 0.0f;
+            for (int r = 0; r < 16; ++r) p[r] -= s_tgt[buf][vb * 32 + mma_row(r)] - first == low ? (a.each ? 1.0f : a.held) : 0.0f;
+          }
+          if (a.each) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] *= s_weight[buf][vb * 32 + mma_row(r)];
           }
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float w = p[r] * (kPoints ? own_weight[s] : mw[r]);
+          const float w = kPoints ? p[r] * own_share[s] : p[r];
           if constexpr (!kPoints) db[s] += w;
           if constexpr (kPlanes == 3) {
             T h, m, l;
@@ -220,11 +229,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_ce_narrow(NarrowArgs a) {
     // a logit that is NaN leaves the maximum as it was and the sum NaN
 #pragma unroll
     for (int s = 0; s < kSB; ++s) {
-      const float ot = __shfl_xor(top[s], 32), os = __shfl_xor(sum[s], 32), now = fmaxf(top[s], ot), base = now == -INFINITY ? 0.0f : now;
+      const float ot = __shfl_xor(top[s], 32), os = __shfl_xor(sum[s], 32), now = fmaxf(top[s], ot), base = base_of(now);
       const int at = kept0 + s * 32 + low;
       if (half == 0 && at < kept_n) {
         a.part_m[split * a.split_stride + at] = now;
-        a.part_l[split * a.split_stride + at] = sum[s] * __builtin_amdgcn_exp2f(top[s] - base) + os * __builtin_amdgcn_exp2f(ot - base);
+        a.part_l[split * a.split_stride + at] = sum[s] * part_of(top[s], base) + os * part_of(ot, base);
       }
     }
     return;

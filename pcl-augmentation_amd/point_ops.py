@@ -273,7 +273,7 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
 
     Memory beside inputs, outputs and gradients: the backward pass holds the logits' gradients of ``piece`` classes at a time, 2 bytes
     a point and class (float32: 6), at least 128 classes; 0: what 512 MB take, at least 256 classes (none with few classes or few
-    features), and 32-bit sums of dx and dweight where they are made in parts.  From forward to backward it keeps 16 bytes a
+    features), and 32-bit sums of dx and dweight where they are made in parts.  From forward to backward it keeps 20 bytes a
     point and, for float32 and for rows that are no multiples of 64 features, a packed copy of x and weight (6 and 2 bytes a value)."""
     import torch
     shape, dtype, wide = x.shape, x.dtype, weight.shape

@@ -845,3 +845,49 @@ def test_loss_parts_of_the_gradient_every_way(pkg, v, d, dtype, reduction):
         assert torch.equal(one, loss) and all(torch.equal(got[i], want[k]) for i, k in enumerate(need)), need
     with torch.inference_mode():
         assert torch.equal(pkg.linear_cross_entropy(ins[0], ins[1], target, bias=ins[2], ignore_index=-1, reduction=reduction), loss)
+
+
+@pytest.mark.parametrize("v,d,dtype", WAYS + FEW)
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_loss_of_a_head_that_is_sure_of_itself(pkg, v, d, dtype, reduction):
+    """Large logits, one class ahead of its only rival by 8: the loss is 3e-4 beside a maximum of some 200 to 300, and so are the
+    gradients.  Logits are whole numbers and exact; in units of log 2 (t, at most T) they are rounded, off by E T each, so the rival's part is off
+    by rho = ln 2 (2 E T + 2 E |t - top|) + 2^-22 of itself, whatever the rest of the way.  Sum and target's gradient: 4 additions to a
+    number near 1 (all other parts are below 2^-30: together below a step), E each."""
+    g = gen(v + d)
+    n = 300
+    w = (torch.randint(0, 2, (v, d), generator=g) * 2 - 1).double()
+    w[:, 0] = 1
+    w[1::2] = w[::2]
+    w[1::2, 1:5] *= -1      # a class's rival differs in four features
+    target = torch.randint(0, v, (n,), generator=g)
+    x = w[target].clone()
+    x[:, 0] = 128
+    logits = x @ w.t()
+    gap = (logits.amax(1, keepdim=True) - logits).sort(1).values
+    assert (gap[:, 0] == 0).all() and (gap[:, 1] == 8).all() and (gap[:, 2] > 21).all()
+    up = torch.rand((n,), generator=g) + 0.5 if reduction == "none" else torch.tensor(1.5)
+    ins = [t.to(dtype).cuda().requires_grad_() for t in (x, w, torch.zeros(v))]
+    loss = pkg.linear_cross_entropy(ins[0], ins[1], target.cuda(), bias=ins[2], reduction=reduction)
+    dx, dw, db = torch.autograd.grad(loss, ins, up.cuda())
+    large = logits.abs().amax(1, keepdim=True) * 1.4427
+    rho = math.log(2) * (2 * E * large + 2 * E * 12) + 2.0 ** -22
+    p = torch.softmax(logits, 1)
+    rest = p.scatter(1, target[:, None], 0).sum(1, keepdim=True)      # 1 - p of the target, without the subtraction
+    each = torch.log1p(rest / (1 - rest))
+    each_tol = rho * rest + 8 * E + 4 * E * each
+    if reduction == "none":
+        near(loss, each[:, 0], each_tol[:, 0])
+    else:
+        near(loss, each.sum(), each_tol.sum())
+    u = torch.finfo(dtype).eps / 2
+    dl = p.scatter(1, target[:, None], -rest)
+    tol = (rho + 8 * E + (2.0 ** -22 if dtype == F32 else u)) * dl.abs()
+    tol = tol.scatter_add(1, target[:, None], torch.full((n, 1), 8 * E, dtype=torch.float64))
+    weight = up.double().expand(n)[:, None]
+    dl, tol = dl * weight, tol * weight
+    tol = tol + weight.max() * (2.0 ** -40 if dtype == F16 else 2.0 ** -126)
+    for got, a, b, terms in ((dx, dl, w, v), (dw, dl.t(), x, n), (db, dl.t(), torch.ones((n, 1), dtype=torch.float64), n)):
+        want, size = a @ b, a.abs() @ b.abs()
+        bound = (tol if a is dl else tol.t()) @ b.abs() + ((terms + 64) * E + (2.0 ** -22 if dtype == F32 else 0)) * size + u * want.abs() * (1 + 2.0 ** -8) + torch.finfo(dtype).smallest_normal
+        near(got.reshape(want.shape), want, bound)
