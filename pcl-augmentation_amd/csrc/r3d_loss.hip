@@ -13,7 +13,8 @@
 //
 // Sums are in 32 bits (matrix cores, softmax statistics, gradients over points and classes), the mean's sum over points in 64.
 // Rounded to fewer: dl, to the inputs' 16-bit type -- the matrix cores' operand; half a step of a term each, at random, beside
-// half a step of the rounded result.  float16 has no room for a probability of 1e-6, so dl is held times 2^15 (|dl| <= 1) and
+// half a step of the rounded result (dx of one point with few classes that matter: 2.5e-3 from 64 bits where 32-bit dl gives 1.7e-3, bfloat16).
+// Two planes of dl would double the products that follow.  float16 has no room for a probability of 1e-6, so dl is held times 2^15 (|dl| <= 1) and
 // the caller's weights of the points relative to the largest.  float32 operands are split into three bfloat16 planes (8 bits
 // each, all 24) and multiplied as the six products that reach beyond 2^-24: 2.5 PFLOP/s of bfloat16 in six are more than the
 // 0.16 of float32.
@@ -734,9 +735,10 @@ __global__ __launch_bounds__(256) void k_ce_finish(FinishArgs all) {
 // time, without a barrier.  Their features come from memory as the fragments that the product takes (two lanes share a row: 32
 // bytes each time, the rest of the cache line with the next k-steps), all classes' logits are in its registers, and in the
 // backward pass dx = dl W is multiplied from there: the classes of a k-step are taken in the order in which the lanes have them.
-// 119 999 x 260 x 256 fp16: 29 us forward (LDS: every wave reads the head, 147 KB for 32 points, 15 us; HBM 13), 71 backward (LDS
-// 30, HBM 40: x, dl and dx), then dW 43 from dl.  In tiles of r3d_mfma.hpp the whole step
-// took 300, so 213 then.
+// 119 999 x 260 x 256 fp16: 28 us forward (HBM 13; LDS 7 at 128 bytes a clock: every wave reads the head, 147 KB for 32 points), 71
+// backward (HBM 42: x, dl and dx; LDS 14 at that rate), then dW 43 from dl.  Neither bounds it: a wave has 1.8 tiles, one after the other,
+// behind a head that has to come first, and two waves a SIMD.  In tiles of r3d_mfma.hpp the whole step took 300, so 213 then.
+// Beyond 64 features its points are cut where dl of all of them is more than it may hold (plan()).
 constexpr int kHeadThreads = 512, kHeadBlocks = 9;
 
 struct HeadArgs {
@@ -874,7 +876,7 @@ __global__ __launch_bounds__(kHeadThreads, 2) void k_ce_head(HeadArgs a) {
           const float s = block_sum(w);
           if ((lane & 15) < 8) mine[v * 32] += s;
         }
-        __builtin_amdgcn_sched_barrier(0);      // (a block at a time: all blocks' addresses and biases at once spill)
+        __builtin_amdgcn_sched_barrier(0);      // (a block at a time: all blocks' addresses and biases at once spill; of nine blocks 25 registers still do)
       }
       if (a.dl) {
 #pragma unroll

@@ -85,7 +85,7 @@ __device__ __forceinline__ void store_piece(T *to, int plane, u32x4 piece) {
 }
 
 // Waves a SIMD the registers are cut for: what the tile's LDS lets stand beside each other anyway.  480 000 x 20 x 96 bf16,
-// backward: 68 us with one, 57 with three; 200 000 x 20 x 256: 114 with one, 69 with two.
+// backward: 68 us with one, 57 with three (which spill 9 vector registers and are faster all the same); 200 000 x 20 x 256: 114 with one, 69 with two.
 constexpr int few_waves(int planes, int vt, int nb) { return planes == 3 ? (vt * nb == 1 ? 2 : 1) : vt * nb == 1 ? 3 : vt * nb == 2 ? 2 : 1; }
 
 // kVT: blocks of 32 classes; kNB: blocks of 32 features of dW a wave keeps (dp <= 128 kNB); kTP: points of a tile.

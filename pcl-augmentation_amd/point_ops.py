@@ -269,7 +269,11 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
 
     Points whose target is ``ignore_index`` have loss and gradient 0, whatever their features are; a target that is no class makes
     the loss NaN.  reduction: "mean" over the points that count (0 where none does), "sum" or "none" ([...]); the loss is
-    float32.  Differentiable once in x, weight and bias (forward mode raises).  The same inputs give the same bits.
+    float32.  Differentiable once in x, weight and bias (forward mode raises).  The same inputs give the same bits.  Sums are in 32
+    bits; in the 16-bit types the logits' gradients are rounded to the type before the two products with them (half a step of
+    each, beside half a step of the result), with weights of single points (reduction "none") float16 holds them relative to the
+    largest one; float32 multiplies three planes of 8 bits, all that reaches beyond 2^-24.  A bias past 2.3e38 counts as infinite:
+    the lowest float32 or bfloat16 masks a class as -inf does.
 
     Memory beside inputs, outputs and gradients: the backward pass holds the logits' gradients of ``piece`` classes at a time, 2 bytes
     a point and class (float32: 6), at least 128 classes; 0: what 512 MB take, at least 256 classes (none with few classes or few

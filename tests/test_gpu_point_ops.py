@@ -891,3 +891,16 @@ def test_loss_of_a_head_that_is_sure_of_itself(pkg, v, d, dtype, reduction):
         want, size = a @ b, a.abs() @ b.abs()
         bound = (tol if a is dl else tol.t()) @ b.abs() + ((terms + 64) * E + (2.0 ** -22 if dtype == F32 else 0)) * size + u * want.abs() * (1 + 2.0 ** -8) + torch.finfo(dtype).smallest_normal
         near(got.reshape(want.shape), want, bound)
+
+
+@pytest.mark.parametrize("v,d,dtype", [w for w in WAYS + FEW if w[2] != F16])
+def test_loss_of_a_bias_past_the_range(pkg, v, d, dtype):
+    """The lowest float32 and bfloat16 are past the range in units of log 2: they mask a class as -inf does, its own points included."""
+    g = gen(v)
+    x, w = (torch.randn(s, generator=g).to(dtype).cuda() for s in ((90, d), (v, d)))
+    target = torch.arange(90).cuda() % v
+    for low in (torch.finfo(dtype).min, -2.5e38):
+        b, c = torch.zeros((v,), dtype=dtype, device="cuda"), torch.zeros((v,), dtype=dtype, device="cuda")
+        b[::3], c[::3] = low, -math.inf
+        got, want = (pkg.linear_cross_entropy(x, w, target, bias=t, reduction="none") for t in (b, c))
+        assert torch.equal(got, want) and torch.isinf(got[target % 3 == 0]).all() and torch.isfinite(got[target % 3 != 0]).all()
