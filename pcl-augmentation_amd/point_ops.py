@@ -24,25 +24,32 @@ def _types():
 
 
 def on_device_of(what, *tensors):
-    """The device of these tensors made current (a null context where it is already); refuses tensors that are not on one GPU, or not in
-    memory as they read."""
+    """The device of these tensors made current (a null context where it is already); refuses tensors that are not on one GPU."""
     import torch
     index = tensors[0].get_device()
     if index < 0:
         _lib.require_gpu()
         raise _lib.R3DError(f"{what}: the tensors must be on a GPU, got {tensors[0].device}")
-    for t in tensors:
+    for t in tensors[1:]:
         if t.get_device() != index:
             raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
-        if t.is_neg() or t.is_conj():      # (what stands in memory is not what the tensor reads as)
-            raise ValueError(f"{what}: a tensor that is negated or conjugated when it is read (resolve_neg, resolve_conj)")
     return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+@functools.lru_cache(maxsize=None)
+def _forward_ad():
+    import torch
+    return torch.autograd.forward_ad
 
 
 def forward_mode():
     """Inside of a level of forward-mode differentiation (``torch.autograd.forward_ad``, ``torch.func.jvp``)?"""
-    import torch
-    return torch.autograd.forward_ad._current_level >= 0
+    return _forward_ad()._current_level >= 0
+
+
+def not_as_read(what):
+    """What stands in memory is not what the tensor reads as (the kernels read memory)."""
+    return ValueError(f"{what}: a tensor that is negated or conjugated when it is read (resolve_neg, resolve_conj)")
 
 
 def _value_type(what, t):
@@ -99,7 +106,7 @@ def _turn(tensors, positions, sections, base, interleaved, backward):
         out = torch.empty_like(t, memory_format=torch.contiguous_format)
         outs.append(out)
         strides = t.stride()
-        if strides[2] != 1 or t.is_neg():      # (a gradient may come in so)
+        if strides[2] != 1 or (backward and t.is_neg()):      # (a gradient may come in so)
             t = t.resolve_neg().contiguous()
             kept.append(t)      # (until the launch)
             strides = t.stride()
@@ -165,6 +172,8 @@ def rotary_positions(query, positions, sections, key=None, base=10000.0, style="
     if positions.requires_grad:
         raise ValueError("rotary_positions: positions have no gradient here (detach them)")
     _value_type("rotary_positions", query)
+    if query.is_neg() or positions.is_neg() or (like is not None and key.is_neg()):
+        raise not_as_read("rotary_positions")
     if like is not None and (key.dtype is not query.dtype or like[0] != tokens or like[2] != dim):
         raise ValueError("rotary_positions: key must have query's tokens, dim and type")
     if pairs > _lib.ROTARY_MAX_PAIRS or 2 * pairs > dim:
@@ -284,6 +293,8 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, reduct
     if len(shape) < 1 or len(wide) != 2 or shape[-1] != wide[1] or wide[0] < 1 or wide[1] < 1:
         raise ValueError(f"linear_cross_entropy: x [..., features] and weight [classes, features], got {tuple(shape)} and {tuple(wide)}")
     _value_type("linear_cross_entropy", x)
+    if x.is_neg() or weight.is_neg() or (bias is not None and bias.is_neg()):
+        raise not_as_read("linear_cross_entropy")
     if weight.dtype != dtype or (bias is not None and bias.dtype != dtype):
         raise TypeError("linear_cross_entropy: x, weight and bias must have one type")
     if bias is not None and bias.shape != wide[:1]:

@@ -9,7 +9,7 @@ import math
 from typing import NamedTuple
 
 from . import _lib
-from .point_ops import forward_mode, on_device_of
+from .point_ops import forward_mode, not_as_read, on_device_of
 
 
 class BlockTables(NamedTuple):
@@ -136,6 +136,8 @@ def _rows_of(what, name, tensors, like=None):
             raise ValueError(f"{what}: {name} must have the same number of rows")
         if t.requires_grad or (forward and torch.autograd.forward_ad.unpack_dual(t).tangent is not None):
             raise ValueError(f"{what}: no gradient passes through moved rows (detach them)")
+        if t.is_neg() or t.is_conj():
+            raise not_as_read(what)
         if t.is_contiguous() and t.numel():
             continue
         width = 1
